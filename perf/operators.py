@@ -212,18 +212,22 @@ class _DeviceArray:
 
 
 def _caches(c, h):
-    """Key and value caches of a handle, or (h None) of the plain form: [batch][layers][seq_len][kv_dim] each, for
-    the 8-bit cache followed by their scales, [batch][layers][seq_len][kv_heads]."""
-    shape = (c["batch"], c["layers"], _seq_len(c))
+    """Key and value caches of a handle, or (h None) of the plain form: [batch][layers][seq_len][kv_dim] each; of the
+    8-bit cache each followed by its scales, which lie as [batch][layers][kv_heads][seq_len] and are seen as
+    [batch][layers][seq_len][kv_heads]."""
+    B, L, S, G = c["batch"], c["layers"], _seq_len(c), c["kv_heads"]
+    values, scales = (B, L, S, G * c["head_dim"]), (B, L, G, S)
     if c["kind"].startswith("q8"):
-        kinds = ((c["kv_heads"] * c["head_dim"], "|i1", torch.int8), (c["kv_heads"], "<f4", torch.float32)) * 2
+        kinds = ((values, "|i1", torch.int8), (scales, "<f4", torch.float32)) * 2
         ptrs = h.kv_q8_device_ptr(0, 0) if h else None
     else:
-        kinds = ((c["kv_heads"] * c["head_dim"], "<f4", torch.float32),) * 2
+        kinds = ((values, "<f4", torch.float32),) * 2
         ptrs = h.kv_device_ptr(0, 0) if h else None
     if h:
-        return [torch.as_tensor(_DeviceArray(h, p, shape + (w,), t), device=DEV) for p, (w, t, _) in zip(ptrs, kinds)]
-    return [torch.empty(shape + (w,), dtype=d, device=DEV) for w, _, d in kinds]
+        t = [torch.as_tensor(_DeviceArray(h, p, shape, typestr), device=DEV) for p, (shape, typestr, _) in zip(ptrs, kinds)]
+    else:
+        t = [torch.empty(shape, dtype=dtype, device=DEV) for shape, _, dtype in kinds]
+    return [x.transpose(2, 3) if x.shape == scales else x for x in t]
 
 
 def prepare(c, seed):
@@ -265,8 +269,7 @@ def prepare(c, seed):
         S = _seq_len(c)
         st["at"] = torch.tensor([(i * L + l) * S + pos[i] + j for l in range(L) for i in range(B) for j in range(n[i])],
                                 dtype=torch.long, device=DEV)
-        st["flat"] = [t.view(-1, t.shape[-1]) for t in st["caches"]]
-        st["got"] = [torch.empty(L * N, t.shape[-1], dtype=t.dtype, device=DEV) for t in st["caches"]]
+        st["at_scale"] = ((st["at"] // S)[:, None] * G + torch.arange(G, device=DEV)) * S + (st["at"] % S)[:, None]
     torch.cuda.synchronize()
     return st
 
@@ -275,7 +278,9 @@ def prepare(c, seed):
 
 def _new_rows(st):
     """The rows of the new tokens as the cache holds them after the call."""
-    new = st["new"] if "new" in st else [torch.index_select(t, 0, st["at"], out=to) for t, to in zip(st["flat"], st["got"])]
+    new = st["new"] if "new" in st else [
+        torch.index_select(t.view(-1, t.shape[-1]), 0, st["at"]) if t.is_contiguous()
+        else torch.take(t.transpose(2, 3), st["at_scale"]) for t in st["caches"]]
     if len(new) == 2:
         return list(new)
     hd = st["c"]["head_dim"]  # 8 bits: the values they stand for
