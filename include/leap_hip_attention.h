@@ -171,6 +171,110 @@ int leap_hip_attention_step_noalloc(const leap_hip_attention_config *cfg, int po
                                     float *k_cache, float *v_cache, const float *q, const float *k_new,
                                     const float *v_new, float *out, void *stream);
 
+/* ---- Several tokens of each sequence: prompts and drafted trees ----------- */
+
+/* The new tokens of n_seq sequences (slabs 0..n_seq-1) at one layer, packed:
+ * sequence i has the rows begin[i] <= r < begin[i+1] of q, k_new, v_new and
+ * out, and token j = r - begin[i] of it goes to cache row pos[i] + j.  The
+ * reference walks a prompt token by token through run_layer
+ * (FloatTransformer.cpp:396-662); this is that walk over all of them at once:
+ * every token is rotated for its position, its k and v are stored, and it
+ * attends causally, to the rows [0, pos[i] + j] (cached ones and those of
+ * this call).  A sequence may have no tokens; rows behind begin[n_seq] and
+ * before begin[0] are left alone.  Sizes, tile and chunk lengths move results
+ * by fp32 rounding only.  An output row that attends to a key or value row
+ * with an infinity or a NaN is NaN; rows that do not are not affected.
+ * Host pointers: begin [n_seq+1] ascending from >= 0, pos [n_seq]; returns
+ * when `out` is written.  -EINVAL, with nothing changed, if a sequence's
+ * positions leave [0, seq_len). */
+int leap_hip_attention_prompt(leap_hip_attention *h, int layer, int n_seq, const int *begin,
+                              const int *pos, const float *q, const float *k_new,
+                              const float *v_new, float *out);
+
+/* As leap_hip_attention_prompt with device pointers (begin and pos included),
+ * enqueued on `stream`.  n_tokens is the rows of the packed arrays;
+ * max_tokens and max_pos are host-side upper bounds of a sequence's tokens
+ * and of the positions that tokens take; they size the launch, which may be
+ * captured and replayed with other begins and positions within them.  A
+ * sequence that breaks them, or whose rows leave [0, n_tokens), is skipped:
+ * its cache rows are neither read nor written and its output rows are NaN;
+ * from a begin that is below the one before it on, every sequence is skipped,
+ * and the rows that no earlier one has are NaN.  q, k_new, v_new and out must
+ * be 16-byte aligned, begin and pos 4-byte aligned.  A handle's first prompt
+ * or tree call allocates its workspace (about 33 MiB at head_dim 128);
+ * -EINVAL if that one is under stream capture. */
+int leap_hip_attention_prompt_async(leap_hip_attention *h, int layer, int n_seq, const int *begin,
+                                    const int *pos, int n_tokens, int max_tokens, int max_pos,
+                                    const float *q, const float *k_new, const float *v_new,
+                                    float *out, void *stream);
+
+/* A tree of drafted tokens of each sequence (speculative decoding), packed as
+ * for leap_hip_attention_prompt, at most 64 nodes a sequence: node j hangs on
+ * the earlier node parent[begin[i] + j] of its tree, or with -1 on the cached
+ * rows.  Node j's k and v go to cache row pos[i] + j; it is rotated for
+ * position pos[i] + (number of its ancestors), and attends to the rows
+ * [0, pos[i]), its ancestors and itself.  Host pointers; -EINVAL, with
+ * nothing changed, for a parent outside [-1, j). */
+int leap_hip_attention_tree(leap_hip_attention *h, int layer, int n_seq, const int *begin,
+                            const int *pos, const int *parent, const float *q, const float *k_new,
+                            const float *v_new, float *out);
+
+/* As leap_hip_attention_tree with device pointers (as
+ * leap_hip_attention_prompt_async; max_tokens <= 64; parent 4-byte aligned).  A node whose
+ * parent lies outside [-1, j) counts as one on the cached rows for what is
+ * stored, and its output row and its descendants' are NaN. */
+int leap_hip_attention_tree_async(leap_hip_attention *h, int layer, int n_seq, const int *begin,
+                                  const int *pos, const int *parent, int n_tokens, int max_tokens,
+                                  int max_pos, const float *q, const float *k_new,
+                                  const float *v_new, float *out, void *stream);
+
+/* After a tree has been verified: the rows of the accepted nodes
+ * path[i][0] < path[i][1] < ... (a root-to-node path; path is
+ * [n_seq][max_path], ended by -1) move to the rows pos[i], pos[i] + 1, ... of
+ * sequence i, in every held layer, where the next step finds them: a path's
+ * node at depth d was rotated for position pos[i] + d.  Other rows keep what
+ * they hold.  max_path <= 64.  Host pointers; -EINVAL, with nothing changed,
+ * for a path that does not ascend or leaves the cache. */
+int leap_hip_attention_tree_keep(leap_hip_attention *h, int n_seq, const int *pos, const int *path,
+                                 int max_path);
+
+/* The same with device pointers, enqueued on `stream`.  A path ends at its
+ * first entry that does not ascend, is no node of a tree (>= 64) or leaves
+ * the cache. */
+int leap_hip_attention_tree_keep_async(leap_hip_attention *h, int n_seq, const int *pos,
+                                       const int *path, int max_path, void *stream);
+
+/* ---- An 8-bit cache -------------------------------------------------------- */
+
+/* As leap_hip_attention_create, with caches of int8 values and one fp32 scale
+ * per row and KV head: for a head row x of head_dim elements,
+ * a = max(max |x_i|, 2^-100), scale = a / 127, value_i = rint(x_i * (127 / a)),
+ * in fp32; it stands for value_i * scale.  (With an infinity or a NaN in it
+ * the scale is NaN, and so is what it stands for.)  A little over a quarter
+ * of the fp32 cache's memory and traffic.  step, step_batched, block, prompt,
+ * tree and their _async forms store quantised rows (k after its rotation) and
+ * attend to what the cache then holds, the new rows included; kv_upload and
+ * kv_write_async quantise, kv_download and kv_read_async return fp32.
+ * kv_device_ptr, kv_fill_normal, floor_async, set_split, set_products and
+ * set_fold_helper return -EINVAL. */
+int leap_hip_attention_create_q8kv(const leap_hip_attention_config *cfg, leap_hip_attention **out);
+
+/* Cache rows [pos_begin, pos_end) of (seq, layer) from and to fp32 rows in
+ * device memory ([pos][kv_dim], 16-byte aligned), enqueued on `stream`: into
+ * an 8-bit cache quantised, out of one what it stands for; an fp32 cache's
+ * rows are copied.  Either k or v may be NULL.  k is stored as it is (after
+ * rotation, as kv_upload). */
+int leap_hip_attention_kv_write_async(leap_hip_attention *h, int seq, int layer, int pos_begin,
+                                      int pos_end, const float *k, const float *v, void *stream);
+int leap_hip_attention_kv_read_async(leap_hip_attention *h, int seq, int layer, int pos_begin,
+                                     int pos_end, float *k, float *v, void *stream);
+
+/* Device addresses of an 8-bit cache's (seq, layer) slabs: values
+ * [seq_len][kv_dim], scales [n_kv_heads][seq_len rounded up to 32]; layers,
+ * then sequences, follow one another.  Any output may be NULL. */
+int leap_hip_attention_kv_q8_device_ptr(leap_hip_attention *h, int seq, int layer, int8_t **k8,
+                                        float **ks, int8_t **v8, float **vs);
+
 /* ---- The attention sub-block of run_layer on the device ----------------- */
 
 /* Weights of one held layer for leap_hip_attention_block, copied from host

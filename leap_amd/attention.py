@@ -41,6 +41,10 @@ EXPORTS = (
     "leap_hip_attention_packet_upload", "leap_hip_attention_packet_download",
     "leap_hip_attention_xcc_map", "leap_hip_attention_step_noalloc", "leap_hip_attention_floor_async",
     "leap_hip_attention_set_products", "leap_hip_attention_set_fold_helper", "leap_hip_attention_timeline",
+    "leap_hip_attention_create_q8kv", "leap_hip_attention_prompt", "leap_hip_attention_prompt_async",
+    "leap_hip_attention_tree", "leap_hip_attention_tree_async", "leap_hip_attention_tree_keep",
+    "leap_hip_attention_tree_keep_async", "leap_hip_attention_kv_write_async", "leap_hip_attention_kv_read_async",
+    "leap_hip_attention_kv_q8_device_ptr",
 )
 
 PACKET_HEADER_BYTES = 8
@@ -135,6 +139,16 @@ def _open(path: str):
     L.leap_hip_attention_set_products.argtypes = [H, _I]
     L.leap_hip_attention_set_fold_helper.argtypes = [H, _I]
     L.leap_hip_attention_step_noalloc.argtypes = [ctypes.POINTER(Config), _I] + [_P] * 8
+    L.leap_hip_attention_create_q8kv.argtypes = [ctypes.POINTER(Config), ctypes.POINTER(H)]
+    L.leap_hip_attention_prompt.argtypes = [H, _I, _I, _IP, _IP, _F, _F, _F, _F]
+    L.leap_hip_attention_prompt_async.argtypes = [H, _I, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P]
+    L.leap_hip_attention_tree.argtypes = [H, _I, _I, _IP, _IP, _IP, _F, _F, _F, _F]
+    L.leap_hip_attention_tree_async.argtypes = [H, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P]
+    L.leap_hip_attention_tree_keep.argtypes = [H, _I, _IP, _IP, _I]
+    L.leap_hip_attention_tree_keep_async.argtypes = [H, _I, _P, _P, _I, _P]
+    L.leap_hip_attention_kv_write_async.argtypes = [H, _I, _I, _I, _I, _P, _P, _P]
+    L.leap_hip_attention_kv_read_async.argtypes = [H, _I, _I, _I, _I, _P, _P, _P]
+    L.leap_hip_attention_kv_q8_device_ptr.argtypes = [H, _I, _I] + [ctypes.POINTER(_P)] * 4
     L.leap_hip_attention_timeline.argtypes = [_P, ctypes.c_size_t, ctypes.POINTER(ctypes.c_longlong)]
     for name in EXPORTS:
         fn = getattr(L, name)
@@ -148,6 +162,14 @@ def _fp(a):
         return None
     assert a.dtype == np.float32 and a.flags.c_contiguous
     return a.ctypes.data_as(_F)
+
+
+def _i32(a):
+    return np.ascontiguousarray(a, dtype=np.int32).reshape(-1)
+
+
+def _ip(a):
+    return a.ctypes.data_as(ctypes.POINTER(_I))
 
 
 def _f32(a, n=None):
@@ -200,10 +222,14 @@ def packet_header(packet: bytes, dim):
 
 
 class HipAttention:
-    """One handle of the MI355X attention library (see the C header)."""
+    """One handle of the MI355X attention library (see the C header).
+    cache: "f32", the engine's cache, or "q8", int8 values with a scale per
+    row and KV head."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, seq_len, n_layers=1, layer_begin=0,
-                 layer_end=None, rope_theta=500000.0, max_batch=1, device=0, lib=None):
+                 layer_end=None, rope_theta=500000.0, max_batch=1, device=0, lib=None, cache="f32"):
+        if cache not in ("f32", "q8"):
+            raise ValueError(f"cache {cache!r} is not 'f32' or 'q8'")
         self.lib = lib if lib is not None else load_library()
         self.cfg = Config(n_layers, layer_begin, n_layers if layer_end is None else layer_end,
                           n_heads, n_kv_heads, head_dim, seq_len, rope_theta, max_batch, device)
@@ -211,7 +237,8 @@ class HipAttention:
         self.seq_len, self.max_batch = seq_len, max_batch
         self.q_dim, self.kv_dim = n_heads * head_dim, n_kv_heads * head_dim
         h = _P()
-        rc = self.lib.leap_hip_attention_create(ctypes.byref(self.cfg), ctypes.byref(h))
+        create = self.lib.leap_hip_attention_create_q8kv if cache == "q8" else self.lib.leap_hip_attention_create
+        rc = create(ctypes.byref(self.cfg), ctypes.byref(h))
         if rc != 0:
             raise LeapError(rc, self.lib.leap_hip_attention_last_error(None).decode())
         self.h = h
@@ -267,6 +294,60 @@ class HipAttention:
         self._check(self.lib.leap_hip_attention_step_batched_async(
             self.h, layer, n_seq, pos_ptr, max_pos, total_rows, q_ptr, k_ptr, v_ptr, out_ptr,
             stream))
+
+    # -- several tokens of each sequence ------------------------------------
+    def _many_in(self, begin, pos, q, k_new, v_new):
+        begin, pos = _i32(begin), _i32(pos)
+        if begin.size != pos.size + 1:
+            raise ValueError(f"{pos.size} positions need {pos.size + 1} begins, got {begin.size}")
+        n = max(0, int(begin[-1]))
+        return begin, pos, n, _f32(q, n * self.q_dim), _f32(k_new, n * self.kv_dim), _f32(v_new, n * self.kv_dim)
+
+    def prompt(self, layer, begin, pos, q, k_new, v_new):
+        """New tokens of each sequence, causal over its cache: sequence i has the rows
+        begin[i]:begin[i + 1] of q, k_new and v_new, from position pos[i] on.  Rows ahead
+        of begin[0] come back as zeros."""
+        begin, pos, n, q, k, v = self._many_in(begin, pos, q, k_new, v_new)
+        out = np.zeros(n * self.q_dim, np.float32)
+        self._check(self.lib.leap_hip_attention_prompt(self.h, layer, pos.size, _ip(begin), _ip(pos), _fp(q), _fp(k),
+                                                       _fp(v), _fp(out)))
+        return out.reshape(n, self.q_dim)
+
+    def prompt_async(self, layer, n_seq, begin_ptr, pos_ptr, n_tokens, max_tokens, max_pos, q_ptr, k_ptr, v_ptr,
+                     out_ptr, stream=0):
+        """n_tokens: rows of the packed arrays; max_tokens, max_pos: upper bounds of a
+        sequence's tokens and of the positions they take."""
+        self._check(self.lib.leap_hip_attention_prompt_async(
+            self.h, layer, n_seq, begin_ptr, pos_ptr, n_tokens, max_tokens, max_pos, q_ptr, k_ptr, v_ptr, out_ptr,
+            stream))
+
+    def tree(self, layer, begin, pos, parent, q, k_new, v_new):
+        """A tree of drafted tokens of each sequence: node j (row begin[i] + j) hangs on
+        node parent[begin[i] + j] < j, or on the cached rows (-1)."""
+        begin, pos, n, q, k, v = self._many_in(begin, pos, q, k_new, v_new)
+        parent = _i32(parent)
+        if parent.size != n:
+            raise ValueError(f"expected {n} parents, got {parent.size}")
+        out = np.zeros(n * self.q_dim, np.float32)
+        self._check(self.lib.leap_hip_attention_tree(self.h, layer, pos.size, _ip(begin), _ip(pos), _ip(parent), _fp(q),
+                                                     _fp(k), _fp(v), _fp(out)))
+        return out.reshape(n, self.q_dim)
+
+    def tree_async(self, layer, n_seq, begin_ptr, pos_ptr, parent_ptr, n_tokens, max_tokens, max_pos, q_ptr, k_ptr,
+                   v_ptr, out_ptr, stream=0):
+        self._check(self.lib.leap_hip_attention_tree_async(
+            self.h, layer, n_seq, begin_ptr, pos_ptr, parent_ptr, n_tokens, max_tokens, max_pos, q_ptr, k_ptr, v_ptr,
+            out_ptr, stream))
+
+    def tree_keep(self, pos, path):
+        """Move the rows of each sequence's accepted nodes path[i] (ascending, ended by
+        -1) to the rows from pos[i] on, in every held layer."""
+        pos = _i32(pos)
+        path = np.ascontiguousarray(path, np.int32).reshape(pos.size, -1)
+        self._check(self.lib.leap_hip_attention_tree_keep(self.h, pos.size, _ip(pos), _ip(path), path.shape[1]))
+
+    def tree_keep_async(self, n_seq, pos_ptr, path_ptr, max_path, stream=0):
+        self._check(self.lib.leap_hip_attention_tree_keep_async(self.h, n_seq, pos_ptr, path_ptr, max_path, stream))
 
     # -- the attention sub-block (rmsnorm, q/k/v, attention, wo, residual) ---
     def set_layer_weights(self, layer, rms_att, wq, wk, wv, wo):
@@ -350,6 +431,22 @@ class HipAttention:
         self._check(self.lib.leap_hip_attention_kv_download(self.h, seq, layer, pos_begin,
                                                             pos_end, _fp(k), _fp(v)))
         return k, v
+
+    def kv_write_async(self, seq, layer, pos_begin, pos_end, k_ptr, v_ptr, stream=0):
+        """fp32 rows in device memory into the cache (an 8-bit one: quantised); either may be 0."""
+        self._check(self.lib.leap_hip_attention_kv_write_async(self.h, seq, layer, pos_begin, pos_end, k_ptr, v_ptr,
+                                                               stream))
+
+    def kv_read_async(self, seq, layer, pos_begin, pos_end, k_ptr, v_ptr, stream=0):
+        """The cache's rows as fp32 into device memory; either may be 0."""
+        self._check(self.lib.leap_hip_attention_kv_read_async(self.h, seq, layer, pos_begin, pos_end, k_ptr, v_ptr,
+                                                              stream))
+
+    def kv_q8_device_ptr(self, seq, layer):
+        """Device addresses of an 8-bit cache: key values and scales, value values and scales."""
+        p = [_P() for _ in range(4)]
+        self._check(self.lib.leap_hip_attention_kv_q8_device_ptr(self.h, seq, layer, *(ctypes.byref(x) for x in p)))
+        return tuple(x.value for x in p)
 
     def kv_fill_normal(self, seed, scale):
         self._check(self.lib.leap_hip_attention_kv_fill_normal(self.h, seed, scale))

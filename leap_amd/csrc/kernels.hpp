@@ -6,7 +6,8 @@
 //     kernels_decode_{64,128}f.hip: the flat kernels (batches) by head_dim;
 //   - kernels_gemv.hip: the fp32 projection GEMVs by model width;
 //   - kernels_q8.hip: the int8 W8A8 projection GEMVs by width, group size,
-//     rows per workgroup and input kind.
+//     rows per workgroup and input kind;
+//   - kernels_many_{64,128}.hip: prompts, trees and the 8-bit cache by head_dim.
 // leap_hip_attention.hip holds the host side and picks kernels through these
 // functions only.
 #pragma once
@@ -14,6 +15,7 @@
 #include "decode_attention.hpp"
 #include "gemv.hpp"
 #include "gemv_q8.hpp"
+#include "many_attention.hpp"
 
 namespace leap_kernels {
 
@@ -106,5 +108,33 @@ bool q8_supported(int dim, int gs);
 // the fewest workgroups per CU that the compiled sizes allow, of equally many
 // rows each, by the smallest such size; false for a shape without kernels.
 bool pick_q8(int dim, int gs, int kind, int rows, int n_cu, Q8Launch *out);
+
+// Prompts, trees and the 8-bit cache: the append of the new rows and the
+// attention over tiles of 16 nb rows, on an fp32 or 8-bit cache.
+using ManyFn = void (*)(leap::ManyArgs);
+struct ManyKernels {
+    ManyFn append, attention;
+};
+// The quantising write of an 8-bit cache's rows, and their reading back.
+using RowsFn = void (*)(leap::RowsArgs);
+struct RowsKernels {
+    RowsFn write, read;
+};
+template <int HD>
+ManyKernels pick_many_hd(int nb, bool q8);
+template <int HD>
+RowsKernels pick_rows_hd();
+extern template ManyKernels pick_many_hd<64>(int, bool);
+extern template ManyKernels pick_many_hd<128>(int, bool);
+extern template RowsKernels pick_rows_hd<64>();
+extern template RowsKernels pick_rows_hd<128>();
+inline ManyKernels pick_many(int hd, int nb, bool q8)
+{
+    return hd == 64 ? pick_many_hd<64>(nb, q8) : hd == 128 ? pick_many_hd<128>(nb, q8) : ManyKernels{nullptr, nullptr};
+}
+inline RowsKernels pick_rows(int hd) { return hd == 64 ? pick_rows_hd<64>() : pick_rows_hd<128>(); }
+// The accepted paths' rows moved together, in an fp32 or 8-bit cache.
+using KeepFn = void (*)(leap::KeepArgs);
+KeepFn pick_keep(bool q8);
 
 }  // namespace leap_kernels

@@ -76,6 +76,19 @@ struct leap_hip_attention {
     int n_cu = 256;  // compute units of the device
     int max_chunks = 1;  // chunks per sequence the workspace holds records for
     int max_flat = 0;    // workgroups per XCD of a flat launch it holds records for
+    // 8-bit cache (create_q8kv; k_cache and v_cache are then NULL): values in
+    // the fp32 cache's layout, scales [seq][layer][n_kv_heads][scale_rows]
+    bool q8kv = false;
+    int8_t *k8 = nullptr, *v8 = nullptr;
+    float *ks = nullptr, *vs = nullptr;
+    int scale_rows = 0;          // seq_len rounded up to kTileKeys
+    size_t scale_layer = 0;      // n_kv_heads * scale_rows
+    // prompts, trees and the 8-bit step: records of split tiles and their
+    // counters (many_reserve), and the host-pointer calls' staging (grown)
+    float *many_o = nullptr, *many_lse = nullptr;
+    int *many_counters = nullptr;
+    char *many_in = nullptr;
+    size_t many_in_bytes = 0;
     bool valu = false;   // score and weighted-V products on the VALU (measurement knob)
     int fold_helper = 1; // 1: two workgroups share a one-level merge's final fold; 0: the last alone; 2: test of the fallback
     std::string err;
@@ -732,20 +745,6 @@ hipError_t launch_attention(const LaunchShape &shape, const LaunchBuffers &b, in
     return launch_k(mf, dim3((unsigned)n_groups), dim3((unsigned)(s.group * hd / 4)), stream, a);
 }
 
-int launch(leap_hip_attention *h, int layer, int n_seq, const int *pos_dev, int pos_scalar,
-           int max_pos, long long total_rows, const float *q, const float *k, const float *v,
-           float *out, hipStream_t stream, int kind = kDecode)
-{
-    if (!shape_supported(h->cfg.head_dim, h->group))
-        return set_err(h, -EINVAL, "unsupported head_dim %d / group %d", h->cfg.head_dim, h->group);
-    const size_t loff = (size_t)(layer - h->cfg.layer_begin) * h->layer_floats;
-    const LaunchBuffers b{h->k_cache + loff, h->v_cache + loff, (long long)h->slab_floats, h->rope,
-                          h->ws_o,           h->ws_ml,          h->counters,          h->ws_po, h->ws_pml};
-    HIP_TRY(h, launch_attention(shape_of(h), b, n_seq, pos_dev, pos_scalar, max_pos, total_rows, q, k, v, out,
-                                stream, kind));
-    return 0;
-}
-
 // Allocate every (pointer, bytes) pair or none of them: on a failure the
 // ones already made are freed and the pointers stay null, so a later call
 // starts over instead of finding half a set.
@@ -765,6 +764,177 @@ int alloc_all(leap_hip_attention *h, std::initializer_list<std::pair<void **, si
     }
     size_t i = 0;
     for (const auto &b : bufs) *b.first = made[i++];
+    return 0;
+}
+
+// The kernels' table for prompts, trees and the 8-bit cache (see
+// load_kernel_tables), for a handle that launches them.
+hipError_t load_many_table(int head_dim)
+{
+    hipFuncAttributes attr;
+    return hipFuncGetAttributes(&attr, reinterpret_cast<const void *>(pick_many(head_dim, 1, false).attention));
+}
+
+// ---- prompts, trees and the 8-bit cache ----------------------------------
+
+// Records and counters of split tiles that a handle holds (32 MiB of outputs
+// at head_dim 128): a launch whose tiles and chunks would leave more takes
+// longer chunks.
+constexpr size_t kManyRecords = 65536;
+constexpr size_t kManyCounters = 4096;
+
+// What one launch of many_attention_kernel is cut into.
+struct ManyPlan {
+    int nb;        // rows of a tile / 16
+    int slots;     // tiles of the batch, at most
+    int chunk, splits;
+    long long wgs;
+};
+ManyPlan many_plan(const leap_hip_attention *h, int n_seq, int n_tokens, int max_tokens, int max_pos,
+                   long long total_rows)
+{
+    const int group = h->group, n_kv = h->cfg.n_kv_heads;
+    const long long rows_max = (long long)max_tokens * group;
+    ManyPlan p{};
+    p.nb = rows_max <= 16 ? 1 : rows_max <= 32 ? 2 : 4;
+    const int bm = 16 * p.nb;
+    p.slots = (int)std::min((long long)n_tokens * group / bm + n_seq, n_seq * ((rows_max + bm - 1) / bm));
+    const long long groups = (long long)p.slots * n_kv;
+    const int total = max_pos + 1;
+    const long long want = (long long)h->n_cu * (p.nb == 4 ? 1 : 2);
+    const int s = (int)std::max<long long>(1, std::min<long long>(64, want / groups));
+    (void)total_rows;
+    p.chunk = std::max(leap::kPassKeys, round_up((total + s - 1) / s, leap::kPassKeys));
+    p.splits = (total + p.chunk - 1) / p.chunk;
+    while (p.splits > 1 && ((size_t)groups * p.splits * bm > kManyRecords || (size_t)groups > kManyCounters)) {
+        p.chunk *= 2;
+        p.splits = (total + p.chunk - 1) / p.chunk;
+    }
+    p.wgs = groups >= leap::kXcds ? (groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * p.splits : groups * p.splits;
+    return p;
+}
+
+// The records' memory, on the first call that needs it.
+int many_reserve(leap_hip_attention *h, hipStream_t stream)
+{
+    if (h->many_o) return 0;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIP_TRY(h, hipStreamIsCapturing(stream, &cap));
+    if (cap != hipStreamCaptureStatusNone)
+        return set_err(h, -EINVAL, "a handle's first prompt or tree call allocates its workspace: make one before capturing");
+    HIP_TRY(h, load_many_table(h->cfg.head_dim));
+    if (int rc = alloc_all(h, {{(void **)&h->many_o, kManyRecords * h->cfg.head_dim * sizeof(float)},
+                               {(void **)&h->many_lse, kManyRecords * sizeof(float)},
+                               {(void **)&h->many_counters, kManyCounters * sizeof(int)}}))
+        return rc;
+    HIP_TRY(h, hipMemsetAsync(h->many_counters, 0, kManyCounters * sizeof(int), h->stream));
+    HIP_TRY(h, hipStreamSynchronize(h->stream));
+    return 0;
+}
+
+// Enqueue the append of the new tokens' rows and their attention.  begin
+// NULL: one token of each of n_seq sequences (pos_dev, or pos_scalar).
+int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos_dev, int pos_scalar,
+                const int *parent, int n_tokens, int max_tokens, int max_pos, long long total_rows, const float *q,
+                const float *k, const float *v, float *out, hipStream_t stream)
+{
+    if (int rc = many_reserve(h, stream)) return rc;
+    const size_t li = (size_t)(layer - h->cfg.layer_begin);
+    const size_t loff = li * h->layer_floats;
+    const ManyPlan p = many_plan(h, n_seq, n_tokens, max_tokens, max_pos, total_rows);
+    leap::ManyArgs a{};
+    a.q = q;
+    a.k_new = k;
+    a.v_new = v;
+    a.out = out;
+    if (h->q8kv) {
+        a.k8 = h->k8 + loff;
+        a.v8 = h->v8 + loff;
+        a.ks = h->ks + li * h->scale_layer;
+        a.vs = h->vs + li * h->scale_layer;
+    } else {
+        a.k_cache = h->k_cache + loff;
+        a.v_cache = h->v_cache + loff;
+    }
+    a.rope = h->rope;
+    a.begin = begin;
+    a.pos = pos_dev;
+    a.parent = parent;
+    a.ws_o = h->many_o;
+    a.ws_lse = h->many_lse;
+    a.counters = h->many_counters;
+    a.seq_stride = (long long)h->slab_floats;
+    a.scale_stride = (long long)(h->scale_layer * h->n_local);
+    a.scale_rows = h->scale_rows;
+    a.n_seq = n_seq;
+    a.n_tokens = n_tokens;
+    a.max_tokens = max_tokens;
+    a.max_pos = max_pos;
+    a.pos_scalar = pos_scalar;
+    a.n_heads = h->cfg.n_heads;
+    a.n_kv_heads = h->cfg.n_kv_heads;
+    a.group = h->group;
+    a.slots = p.slots;
+    a.chunk = p.chunk;
+    a.splits = p.splits;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)h->cfg.head_dim));
+    a.by_group = leap::make_fastdiv((uint32_t)h->group);
+    a.by_kv_heads = leap::make_fastdiv((uint32_t)h->cfg.n_kv_heads);
+    a.by_splits = leap::make_fastdiv((uint32_t)p.splits);
+    if (p.wgs > 0x7fffffffLL) return set_err(h, -EINVAL, "%lld workgroups in one launch", p.wgs);
+    const ManyKernels fn = pick_many(h->cfg.head_dim, p.nb, h->q8kv);
+    if (!fn.attention) return set_err(h, -EINVAL, "unsupported head_dim %d", h->cfg.head_dim);
+    HIP_TRY(h, launch_k(fn.append, dim3((unsigned)((n_tokens + leap::kManyWaves - 1) / leap::kManyWaves)),
+                        dim3(leap::kManyThreads), stream, a));
+    HIP_TRY(h, launch_k(fn.attention, dim3((unsigned)p.wgs), dim3(leap::kManyThreads), stream, a));
+    return 0;
+}
+
+// The host-pointer calls' device staging of at least `bytes`.
+int many_staging(leap_hip_attention *h, size_t bytes)
+{
+    if (bytes <= h->many_in_bytes) return 0;
+    char *p = nullptr;
+    if (int rc = alloc_all(h, {{(void **)&p, bytes}})) return rc;
+    if (h->many_in) (void)hipFree(h->many_in);
+    h->many_in = p;
+    h->many_in_bytes = bytes;
+    return 0;
+}
+
+// Enqueue the quantising write, or the reading back, of rows [pos_begin,
+// pos_begin + n) of an 8-bit cache; either of k and v may be NULL.
+int launch_rows_q8(leap_hip_attention *h, int seq, int layer, int pos_begin, int n, const float *k_in, const float *v_in,
+                   float *k_out, float *v_out, hipStream_t stream)
+{
+    const size_t li = (size_t)(layer - h->cfg.layer_begin);
+    const size_t at = (size_t)seq * h->slab_floats + li * h->layer_floats + (size_t)pos_begin * h->kv_dim;
+    const size_t sat = ((size_t)seq * h->n_local + li) * h->scale_layer + (size_t)pos_begin;
+    leap::RowsArgs a{k_in, v_in, k_out, v_out, h->k8 + at, h->v8 + at, h->ks + sat, h->vs + sat,
+                     h->scale_rows, h->cfg.n_kv_heads, n};
+    const RowsKernels fn = pick_rows(h->cfg.head_dim);
+    const long long words = (long long)n * h->kv_dim / 4;
+    const unsigned grid = (unsigned)std::min<long long>((words + 255) / 256, 8ll * h->n_cu);
+    HIP_TRY(h, launch_k(k_in || v_in ? fn.write : fn.read, dim3(grid, 2), dim3(256), stream, a));
+    return 0;
+}
+
+int launch(leap_hip_attention *h, int layer, int n_seq, const int *pos_dev, int pos_scalar,
+           int max_pos, long long total_rows, const float *q, const float *k, const float *v,
+           float *out, hipStream_t stream, int kind = kDecode)
+{
+    if (h->q8kv) {
+        if (kind != kDecode) return set_err(h, -EINVAL, "the floor launches read fp32 caches; this handle's holds 8 bits");
+        return launch_many(h, layer, n_seq, nullptr, pos_dev, pos_scalar, nullptr, n_seq, 1, max_pos, total_rows, q, k, v,
+                           out, stream);
+    }
+    if (!shape_supported(h->cfg.head_dim, h->group))
+        return set_err(h, -EINVAL, "unsupported head_dim %d / group %d", h->cfg.head_dim, h->group);
+    const size_t loff = (size_t)(layer - h->cfg.layer_begin) * h->layer_floats;
+    const LaunchBuffers b{h->k_cache + loff, h->v_cache + loff, (long long)h->slab_floats, h->rope,
+                          h->ws_o,           h->ws_ml,          h->counters,          h->ws_po, h->ws_pml};
+    HIP_TRY(h, launch_attention(shape_of(h), b, n_seq, pos_dev, pos_scalar, max_pos, total_rows, q, k, v, out,
+                                stream, kind));
     return 0;
 }
 
@@ -923,6 +1093,23 @@ hipError_t load_flat_table(int head_dim)
     return hipFuncGetAttributes(&attr, reinterpret_cast<const void *>(head_dim == 64 ? pick_flat<64>(4, 0) : pick_flat<128>(4, 0)));
 }
 
+// Enqueue zeros over both caches on the handle's stream.
+int clear_cache(leap_hip_attention *h)
+{
+    const size_t n = (size_t)h->cfg.max_batch * h->slab_floats;
+    if (h->q8kv) {
+        const size_t scale_bytes = (size_t)h->cfg.max_batch * h->n_local * h->scale_layer * sizeof(float);
+        HIP_TRY(h, hipMemsetAsync(h->k8, 0, n, h->stream));
+        HIP_TRY(h, hipMemsetAsync(h->v8, 0, n, h->stream));
+        HIP_TRY(h, hipMemsetAsync(h->ks, 0, scale_bytes, h->stream));
+        HIP_TRY(h, hipMemsetAsync(h->vs, 0, scale_bytes, h->stream));
+        return 0;
+    }
+    HIP_TRY(h, hipMemsetAsync(h->k_cache, 0, n * sizeof(float), h->stream));
+    HIP_TRY(h, hipMemsetAsync(h->v_cache, 0, n * sizeof(float), h->stream));
+    return 0;
+}
+
 // Run the XCC probe over n_wg workgroups of the decode kernel's block size
 // on `device` and copy the XCC id of each to xcc_host[n_wg].
 int xcc_map(leap_hip_attention *h, int device, int n_wg, int *xcc_host)
@@ -969,7 +1156,7 @@ int leap_hip_attention_xcc_map(int device, int n_wg, int *xcc_out)
     return xcc_map(nullptr, device, n_wg, xcc_out);
 }
 
-int leap_hip_attention_create(const leap_hip_attention_config *cfg, leap_hip_attention **out)
+static int create(const leap_hip_attention_config *cfg, leap_hip_attention **out, bool q8kv)
 {
     if (!out) return set_err(nullptr, -EINVAL, "out is NULL");
     *out = nullptr;
@@ -1013,6 +1200,9 @@ int leap_hip_attention_create(const leap_hip_attention_config *cfg, leap_hip_att
     h->group = c.n_heads / c.n_kv_heads;
     h->layer_floats = (size_t)c.seq_len * h->kv_dim;
     h->slab_floats = (size_t)h->n_local * h->layer_floats;
+    h->q8kv = q8kv;
+    h->scale_rows = round_up(c.seq_len, leap::kTileKeys);
+    h->scale_layer = (size_t)c.n_kv_heads * h->scale_rows;
 
     auto fail = [&](int rc) {
         std::snprintf(g_create_error, sizeof g_create_error, "%s", h->err.c_str());
@@ -1034,11 +1224,18 @@ int leap_hip_attention_create(const leap_hip_attention_config *cfg, leap_hip_att
     CREATE_TRY(hipStreamCreate(&h->stream));
     CREATE_TRY(load_kernel_tables());
     if (int prc = check_placement(h, c.device, 2 * h->n_cu)) return fail(prc);
-    const size_t cache_bytes = (size_t)c.max_batch * h->slab_floats * sizeof(float);
-    CREATE_TRY(hipMalloc(&h->k_cache, cache_bytes));
-    CREATE_TRY(hipMalloc(&h->v_cache, cache_bytes));
-    CREATE_TRY(hipMemsetAsync(h->k_cache, 0, cache_bytes, h->stream));
-    CREATE_TRY(hipMemsetAsync(h->v_cache, 0, cache_bytes, h->stream));
+    const size_t cache_bytes = (size_t)c.max_batch * h->slab_floats * (q8kv ? 1 : sizeof(float));
+    if (q8kv) {
+        const size_t scale_bytes = (size_t)c.max_batch * h->n_local * h->scale_layer * sizeof(float);
+        CREATE_TRY(hipMalloc(&h->k8, cache_bytes));
+        CREATE_TRY(hipMalloc(&h->v8, cache_bytes));
+        CREATE_TRY(hipMalloc(&h->ks, scale_bytes));
+        CREATE_TRY(hipMalloc(&h->vs, scale_bytes));
+    } else {
+        CREATE_TRY(hipMalloc(&h->k_cache, cache_bytes));
+        CREATE_TRY(hipMalloc(&h->v_cache, cache_bytes));
+    }
+    if (int crc = clear_cache(h)) return fail(crc);
 
     const size_t rope_n = (size_t)c.seq_len * (c.head_dim / 2);
     std::vector<float> cs(rope_n), sn(rope_n);
@@ -1072,6 +1269,8 @@ int leap_hip_attention_create(const leap_hip_attention_config *cfg, leap_hip_att
     CREATE_TRY(hipMalloc(&h->out_dev, (size_t)c.max_batch * h->q_dim * sizeof(float)));
     CREATE_TRY(hipMalloc(&h->blk, (size_t)(3 * h->q_dim + 2 * h->kv_dim) * sizeof(float)));
     h->w_set.assign(h->n_local, 0);
+    if (q8kv)
+        if (int mrc = many_reserve(h, h->stream)) return fail(mrc);
 #ifdef LEAP_TIMELINE
     if (!g_tl_ring) {
         CREATE_TRY(hipMalloc(&g_tl_ring, kTlRingWords * sizeof(unsigned long long)));
@@ -1084,6 +1283,16 @@ int leap_hip_attention_create(const leap_hip_attention_config *cfg, leap_hip_att
     return 0;
 }
 
+int leap_hip_attention_create(const leap_hip_attention_config *cfg, leap_hip_attention **out)
+{
+    return create(cfg, out, false);
+}
+
+int leap_hip_attention_create_q8kv(const leap_hip_attention_config *cfg, leap_hip_attention **out)
+{
+    return create(cfg, out, true);
+}
+
 int leap_hip_attention_destroy(leap_hip_attention *h)
 {
     if (!h) return 0;
@@ -1092,7 +1301,8 @@ int leap_hip_attention_destroy(leap_hip_attention *h)
     void *bufs[] = {h->ws_po,   h->ws_pml,
                     h->k_cache, h->v_cache, h->rope,  h->ws_o,  h->ws_ml, h->counters, h->in_dev,
                     h->out_dev, h->blk,     h->w_qkv, h->w_o,   h->w_rms, h->w8_qkv,   h->s8_qkv,
-                    h->w8_o,    h->s8_o,    h->q8_act, h->q8_act_s};
+                    h->w8_o,    h->s8_o,    h->q8_act, h->q8_act_s, h->k8, h->v8, h->ks, h->vs,
+                    h->many_o,  h->many_lse, h->many_counters, h->many_in};
     for (void *p : bufs)
         if (p) (void)hipFree(p);
     for (void *p : {(void *)h->in_host, (void *)h->out_host})
@@ -1566,9 +1776,8 @@ int leap_hip_attention_clear(leap_hip_attention *h)
 {
     if (!h) return -EINVAL;
     HIP_TRY(h, hipSetDevice(h->cfg.device));
-    const size_t bytes = (size_t)h->cfg.max_batch * h->slab_floats * sizeof(float);
-    HIP_TRY(h, hipMemsetAsync(h->k_cache, 0, bytes, h->stream));
-    HIP_TRY(h, hipMemsetAsync(h->v_cache, 0, bytes, h->stream));
+    if (int rc = clear_cache(h)) return rc;
+    if (h->many_counters) HIP_TRY(h, hipMemsetAsync(h->many_counters, 0, kManyCounters * sizeof(int), h->stream));
     // The merge's arrival counters too: they are zero between launches, and
     // clearing them lets a handle recover after launches that overlapped on
     // two streams.
@@ -1600,6 +1809,18 @@ int leap_hip_attention_kv_upload(leap_hip_attention *h, int seq, int layer, int 
     if (int rc = kv_range(h, seq, layer, pos_begin, pos_end, &off, &n)) return rc;
     HIP_TRY(h, hipSetDevice(h->cfg.device));
     if (n == 0) return 0;
+    if (h->q8kv) {
+        if (!k && !v) return 0;
+        if (int rc = many_staging(h, 2 * n * sizeof(float))) return rc;
+        float *kd = reinterpret_cast<float *>(h->many_in), *vd = kd + n;
+        if (k) HIP_TRY(h, hipMemcpyAsync(kd, k, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
+        if (v) HIP_TRY(h, hipMemcpyAsync(vd, v, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
+        if (int rc = launch_rows_q8(h, seq, layer, pos_begin, pos_end - pos_begin, k ? kd : nullptr, v ? vd : nullptr,
+                                    nullptr, nullptr, h->stream))
+            return rc;
+        HIP_TRY(h, hipStreamSynchronize(h->stream));
+        return 0;
+    }
     if (k) HIP_TRY(h, hipMemcpyAsync(h->k_cache + off, k, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
     if (v) HIP_TRY(h, hipMemcpyAsync(h->v_cache + off, v, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
     HIP_TRY(h, hipStreamSynchronize(h->stream));
@@ -1613,6 +1834,18 @@ int leap_hip_attention_kv_download(leap_hip_attention *h, int seq, int layer, in
     if (int rc = kv_range(h, seq, layer, pos_begin, pos_end, &off, &n)) return rc;
     HIP_TRY(h, hipSetDevice(h->cfg.device));
     if (n == 0) return 0;
+    if (h->q8kv) {
+        if (!k && !v) return 0;
+        if (int rc = many_staging(h, 2 * n * sizeof(float))) return rc;
+        float *kd = reinterpret_cast<float *>(h->many_in), *vd = kd + n;
+        if (int rc = launch_rows_q8(h, seq, layer, pos_begin, pos_end - pos_begin, nullptr, nullptr, k ? kd : nullptr,
+                                    v ? vd : nullptr, h->stream))
+            return rc;
+        if (k) HIP_TRY(h, hipMemcpyAsync(k, kd, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
+        if (v) HIP_TRY(h, hipMemcpyAsync(v, vd, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
+        HIP_TRY(h, hipStreamSynchronize(h->stream));
+        return 0;
+    }
     if (k) HIP_TRY(h, hipMemcpyAsync(k, h->k_cache + off, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
     if (v) HIP_TRY(h, hipMemcpyAsync(v, h->v_cache + off, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
     HIP_TRY(h, hipStreamSynchronize(h->stream));
@@ -1622,6 +1855,7 @@ int leap_hip_attention_kv_download(leap_hip_attention *h, int seq, int layer, in
 int leap_hip_attention_kv_fill_normal(leap_hip_attention *h, uint64_t seed, float scale)
 {
     if (!h) return -EINVAL;
+    if (h->q8kv) return set_err(h, -EINVAL, "kv_fill_normal fills fp32 caches; this handle's holds 8 bits");
     HIP_TRY(h, hipSetDevice(h->cfg.device));
     const size_t n = (size_t)h->cfg.max_batch * h->slab_floats;
     const int blocks = 256 * 16;
@@ -1670,6 +1904,7 @@ int leap_hip_attention_floor_async(leap_hip_attention *h, int kind, int layer, i
     if (total_rows <= 0 || total_rows > (long long)n_seq * (max_pos + 1))
         return set_err(h, -EINVAL, "total_rows %lld outside [1, %lld]", total_rows, (long long)n_seq * (max_pos + 1));
     if (reinterpret_cast<uintptr_t>(pos) % 4) return set_err(h, -EINVAL, "pos must be 4-byte aligned");
+    if (h->q8kv) return set_err(h, -EINVAL, "the floor launches read fp32 caches; this handle's holds 8 bits");
     if (kind == kFloorBlock) {
         if (n_seq != 1 || pos || total_rows != (long long)max_pos + 1)
             return set_err(h, -EINVAL, "the sub-block floor takes one sequence at max_pos (pos NULL)");
@@ -1690,6 +1925,7 @@ int leap_hip_attention_floor_async(leap_hip_attention *h, int kind, int layer, i
 int leap_hip_attention_set_products(leap_hip_attention *h, int valu)
 {
     if (!h) return -EINVAL;
+    if (h->q8kv) return set_err(h, -EINVAL, "set_products is a knob of the fp32 cache's step");
     if (valu != 0 && valu != 1) return set_err(h, -EINVAL, "products mode %d is not 0 (MFMA) or 1 (VALU)", valu);
     h->valu = valu == 1;
     return 0;
@@ -1698,6 +1934,7 @@ int leap_hip_attention_set_products(leap_hip_attention *h, int valu)
 int leap_hip_attention_set_fold_helper(leap_hip_attention *h, int mode)
 {
     if (!h) return -EINVAL;
+    if (h->q8kv) return set_err(h, -EINVAL, "set_fold_helper is a knob of the fp32 cache's step");
     if (mode < 0 || mode > 2) return set_err(h, -EINVAL, "fold helper mode %d is not 0, 1 or 2", mode);
     h->fold_helper = mode;
     return 0;
@@ -1706,6 +1943,7 @@ int leap_hip_attention_set_fold_helper(leap_hip_attention *h, int mode)
 int leap_hip_attention_set_split(leap_hip_attention *h, int chunk_positions)
 {
     if (!h) return -EINVAL;
+    if (h->q8kv) return set_err(h, -EINVAL, "set_split is a knob of the fp32 cache's step");
     if (chunk_positions < 0 || chunk_positions % 8 != 0)
         return set_err(h, -EINVAL, "chunk %d is not a non-negative multiple of 8",
                        chunk_positions);
@@ -1784,9 +2022,235 @@ int leap_hip_attention_kv_device_ptr(leap_hip_attention *h, int seq, int layer, 
 {
     size_t off, n;
     if (int rc = kv_range(h, seq, layer, 0, 0, &off, &n)) return rc;
+    if (h->q8kv) return set_err(h, -EINVAL, "this handle's cache holds 8 bits: kv_q8_device_ptr gives its addresses");
     if (k) *k = h->k_cache + off;
     if (v) *v = h->v_cache + off;
     return 0;
+}
+
+int leap_hip_attention_kv_q8_device_ptr(leap_hip_attention *h, int seq, int layer, int8_t **k8, float **ks, int8_t **v8,
+                                        float **vs)
+{
+    size_t off, n;
+    if (int rc = kv_range(h, seq, layer, 0, 0, &off, &n)) return rc;
+    if (!h->q8kv) return set_err(h, -EINVAL, "this handle's cache holds fp32: kv_device_ptr gives its addresses");
+    const size_t soff = ((size_t)seq * h->n_local + (size_t)(layer - h->cfg.layer_begin)) * h->scale_layer;
+    if (k8) *k8 = h->k8 + off;
+    if (ks) *ks = h->ks + soff;
+    if (v8) *v8 = h->v8 + off;
+    if (vs) *vs = h->vs + soff;
+    return 0;
+}
+
+// ---- prompts and trees -----------------------------------------------------
+
+static inline bool aligned4(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
+static int many_async(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos, const int *parent,
+                      bool tree, int n_tokens, int max_tokens, int max_pos, const float *q, const float *k_new,
+                      const float *v_new, float *out, void *stream)
+{
+    if (!h) return -EINVAL;
+    if (int rc = check_layer(h, layer)) return rc;
+    if (n_seq <= 0 || n_seq > h->cfg.max_batch)
+        return set_err(h, -EINVAL, "n_seq %d outside [1, %d]", n_seq, h->cfg.max_batch);
+    if (n_tokens < 0) return set_err(h, -EINVAL, "n_tokens %d is negative", n_tokens);
+    if (max_tokens < 0 || max_tokens > n_tokens)
+        return set_err(h, -EINVAL, "max_tokens %d outside [0, %d]", max_tokens, n_tokens);
+    if (tree && max_tokens > leap::kTreeMax)
+        return set_err(h, -EINVAL, "max_tokens %d: a tree has at most %d nodes", max_tokens, leap::kTreeMax);
+    if (max_pos < 0 || max_pos >= h->cfg.seq_len)
+        return set_err(h, -EINVAL, "max_pos %d outside [0, %d)", max_pos, h->cfg.seq_len);
+    if (max_tokens > max_pos + 1)
+        return set_err(h, -EINVAL, "max_tokens %d do not fit positions up to %d", max_tokens, max_pos);
+    if (!begin || !pos || (tree && !parent)) return set_err(h, -EINVAL, "NULL buffer");
+    if (max_tokens == 0) return 0;
+    if (!q || !k_new || !v_new || !out) return set_err(h, -EINVAL, "NULL buffer");
+    if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(out) || !aligned4(begin) || !aligned4(pos) ||
+        !aligned4(parent))
+        return set_err(h, -EINVAL, "q, k_new, v_new and out must be 16-byte aligned, the int arrays 4-byte aligned");
+    HIP_TRY(h, hipSetDevice(h->cfg.device));
+    return launch_many(h, layer, n_seq, begin, pos, 0, tree ? parent : nullptr, n_tokens, max_tokens, max_pos, 0, q, k_new,
+                       v_new, out, (hipStream_t)stream);
+}
+
+// The same with host pointers: everything is checked, staged in, run and
+// copied back on the handle's stream.
+static int many_host(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos, const int *parent,
+                     bool tree, const float *q, const float *k_new, const float *v_new, float *out)
+{
+    if (!h) return -EINVAL;
+    if (int rc = check_layer(h, layer)) return rc;
+    if (n_seq <= 0 || n_seq > h->cfg.max_batch)
+        return set_err(h, -EINVAL, "n_seq %d outside [1, %d]", n_seq, h->cfg.max_batch);
+    if (!begin || !pos || (tree && !parent)) return set_err(h, -EINVAL, "NULL buffer");
+    if (begin[0] < 0) return set_err(h, -EINVAL, "begin[0] = %d is negative", begin[0]);
+    int max_tokens = 0, max_pos = 0;
+    for (int i = 0; i < n_seq; i++) {
+        if (begin[i + 1] < begin[i])
+            return set_err(h, -EINVAL, "begin[%d] = %d is below begin[%d] = %d", i + 1, begin[i + 1], i, begin[i]);
+        const int n = begin[i + 1] - begin[i];
+        if (n == 0) continue;
+        if (tree && n > leap::kTreeMax)
+            return set_err(h, -EINVAL, "sequence %d: %d nodes, a tree has at most %d", i, n, leap::kTreeMax);
+        if (pos[i] < 0 || n > h->cfg.seq_len || pos[i] > h->cfg.seq_len - n)
+            return set_err(h, -EINVAL, "sequence %d: positions [%d, %lld) outside [0, %d)", i, pos[i],
+                           (long long)pos[i] + n, h->cfg.seq_len);
+        if (tree)
+            for (int j = 0; j < n; j++)
+                if (parent[begin[i] + j] < -1 || parent[begin[i] + j] >= j)
+                    return set_err(h, -EINVAL, "sequence %d: parent %d of node %d outside [-1, %d)", i,
+                                   parent[begin[i] + j], j, j);
+        max_tokens = std::max(max_tokens, n);
+        max_pos = std::max(max_pos, pos[i] + n - 1);
+    }
+    const size_t n_tokens = (size_t)begin[n_seq], first = (size_t)begin[0];
+    if (max_tokens == 0) return 0;
+    if (!q || !k_new || !v_new || !out) return set_err(h, -EINVAL, "NULL buffer");
+    HIP_TRY(h, hipSetDevice(h->cfg.device));
+    // q | k | v | out rows, then begin, pos and parent
+    const size_t qn = n_tokens * h->q_dim, kn = n_tokens * h->kv_dim;
+    const size_t ints = (size_t)(2 * n_seq + 1) + (tree ? n_tokens : 0);
+    if (int rc = many_staging(h, (2 * qn + 2 * kn) * sizeof(float) + ints * sizeof(int))) return rc;
+    float *qd = reinterpret_cast<float *>(h->many_in), *kd = qd + qn, *vd = kd + kn, *od = vd + kn;
+    int *bd = reinterpret_cast<int *>(od + qn), *pd = bd + n_seq + 1, *td = pd + n_seq;
+    hipStream_t s = h->stream;
+    HIP_TRY(h, hipMemcpyAsync(qd, q, qn * sizeof(float), hipMemcpyHostToDevice, s));
+    HIP_TRY(h, hipMemcpyAsync(kd, k_new, kn * sizeof(float), hipMemcpyHostToDevice, s));
+    HIP_TRY(h, hipMemcpyAsync(vd, v_new, kn * sizeof(float), hipMemcpyHostToDevice, s));
+    HIP_TRY(h, hipMemcpyAsync(bd, begin, (n_seq + 1) * sizeof(int), hipMemcpyHostToDevice, s));
+    HIP_TRY(h, hipMemcpyAsync(pd, pos, n_seq * sizeof(int), hipMemcpyHostToDevice, s));
+    if (tree) HIP_TRY(h, hipMemcpyAsync(td, parent, n_tokens * sizeof(int), hipMemcpyHostToDevice, s));
+    if (int rc = launch_many(h, layer, n_seq, bd, pd, 0, tree ? td : nullptr, (int)n_tokens, max_tokens, max_pos, 0, qd,
+                             kd, vd, od, s))
+        return rc;
+    HIP_TRY(h, hipMemcpyAsync(out + first * h->q_dim, od + first * h->q_dim, (n_tokens - first) * h->q_dim * sizeof(float),
+                              hipMemcpyDeviceToHost, s));
+    HIP_TRY(h, hipStreamSynchronize(s));
+    return 0;
+}
+
+int leap_hip_attention_prompt_async(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos,
+                                    int n_tokens, int max_tokens, int max_pos, const float *q, const float *k_new,
+                                    const float *v_new, float *out, void *stream)
+{
+    return many_async(h, layer, n_seq, begin, pos, nullptr, false, n_tokens, max_tokens, max_pos, q, k_new, v_new, out,
+                      stream);
+}
+
+int leap_hip_attention_prompt(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos, const float *q,
+                              const float *k_new, const float *v_new, float *out)
+{
+    return many_host(h, layer, n_seq, begin, pos, nullptr, false, q, k_new, v_new, out);
+}
+
+int leap_hip_attention_tree_async(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos,
+                                  const int *parent, int n_tokens, int max_tokens, int max_pos, const float *q,
+                                  const float *k_new, const float *v_new, float *out, void *stream)
+{
+    return many_async(h, layer, n_seq, begin, pos, parent, true, n_tokens, max_tokens, max_pos, q, k_new, v_new, out, stream);
+}
+
+int leap_hip_attention_tree(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos, const int *parent,
+                            const float *q, const float *k_new, const float *v_new, float *out)
+{
+    return many_host(h, layer, n_seq, begin, pos, parent, true, q, k_new, v_new, out);
+}
+
+int leap_hip_attention_tree_keep_async(leap_hip_attention *h, int n_seq, const int *pos, const int *path, int max_path,
+                                       void *stream)
+{
+    if (!h) return -EINVAL;
+    if (n_seq <= 0 || n_seq > h->cfg.max_batch)
+        return set_err(h, -EINVAL, "n_seq %d outside [1, %d]", n_seq, h->cfg.max_batch);
+    if (max_path < 0 || max_path > leap::kTreeMax)
+        return set_err(h, -EINVAL, "max_path %d outside [0, %d]", max_path, leap::kTreeMax);
+    if (max_path == 0) return 0;
+    if (!pos || !path) return set_err(h, -EINVAL, "NULL buffer");
+    if (!aligned4(pos) || !aligned4(path)) return set_err(h, -EINVAL, "pos and path must be 4-byte aligned");
+    HIP_TRY(h, hipSetDevice(h->cfg.device));
+    const int size = h->q8kv ? 1 : (int)sizeof(float);
+    leap::KeepArgs a{};
+    a.k = h->q8kv ? reinterpret_cast<char *>(h->k8) : reinterpret_cast<char *>(h->k_cache);
+    a.v = h->q8kv ? reinterpret_cast<char *>(h->v8) : reinterpret_cast<char *>(h->v_cache);
+    a.ks = h->ks;
+    a.vs = h->vs;
+    a.pos = pos;
+    a.path = path;
+    a.seq_bytes = (long long)h->slab_floats * size;
+    a.layer_bytes = (long long)h->layer_floats * size;
+    a.scale_seq = (long long)(h->scale_layer * h->n_local);
+    a.scale_layer = (long long)h->scale_layer;
+    a.row_bytes = h->kv_dim * size;
+    a.scale_rows = h->scale_rows;
+    a.n_kv_heads = h->cfg.n_kv_heads;
+    a.n_layers = h->n_local;
+    a.max_path = max_path;
+    a.seq_len = h->cfg.seq_len;
+    a.columns = a.row_bytes / 16;
+    const long long columns = (long long)h->n_local * (2 * a.columns + (h->q8kv ? 2 * h->cfg.n_kv_heads : 0));
+    const dim3 grid((unsigned)((columns + leap::kKeepThreads - 1) / leap::kKeepThreads), (unsigned)n_seq);
+    HIP_TRY(h, launch_k(pick_keep(h->q8kv), grid, dim3(leap::kKeepThreads), (hipStream_t)stream, a));
+    return 0;
+}
+
+int leap_hip_attention_tree_keep(leap_hip_attention *h, int n_seq, const int *pos, const int *path, int max_path)
+{
+    if (!h) return -EINVAL;
+    if (n_seq <= 0 || n_seq > h->cfg.max_batch)
+        return set_err(h, -EINVAL, "n_seq %d outside [1, %d]", n_seq, h->cfg.max_batch);
+    if (max_path < 0 || max_path > leap::kTreeMax)
+        return set_err(h, -EINVAL, "max_path %d outside [0, %d]", max_path, leap::kTreeMax);
+    if (max_path == 0) return 0;
+    if (!pos || !path) return set_err(h, -EINVAL, "NULL buffer");
+    for (int i = 0; i < n_seq; i++) {
+        const int *p = path + (size_t)i * max_path;
+        for (int t = 0; t < max_path && p[t] != -1; t++)
+            if (p[t] <= (t ? p[t - 1] : -1) || p[t] >= leap::kTreeMax || pos[i] < 0 || pos[i] >= h->cfg.seq_len - p[t])
+                return set_err(h, -EINVAL, "sequence %d: path[%d] = %d at pos %d: a path ascends within the cache", i, t,
+                               p[t], pos[i]);
+    }
+    HIP_TRY(h, hipSetDevice(h->cfg.device));
+    const size_t np = (size_t)n_seq * max_path;
+    if (int rc = many_staging(h, (np + n_seq) * sizeof(int))) return rc;
+    int *pd = reinterpret_cast<int *>(h->many_in), *xd = pd + n_seq;
+    HIP_TRY(h, hipMemcpyAsync(pd, pos, n_seq * sizeof(int), hipMemcpyHostToDevice, h->stream));
+    HIP_TRY(h, hipMemcpyAsync(xd, path, np * sizeof(int), hipMemcpyHostToDevice, h->stream));
+    if (int rc = leap_hip_attention_tree_keep_async(h, n_seq, pd, xd, max_path, h->stream)) return rc;
+    HIP_TRY(h, hipStreamSynchronize(h->stream));
+    return 0;
+}
+
+static int rows_async(leap_hip_attention *h, int seq, int layer, int pos_begin, int pos_end, const float *k_in,
+                      const float *v_in, float *k_out, float *v_out, void *stream)
+{
+    size_t off, n;
+    if (int rc = kv_range(h, seq, layer, pos_begin, pos_end, &off, &n)) return rc;
+    for (const void *p : {(const void *)k_in, (const void *)v_in, (const void *)k_out, (const void *)v_out})
+        if (!aligned16(p)) return set_err(h, -EINVAL, "k and v must be 16-byte aligned");
+    const bool writes = k_in || v_in;
+    if (n == 0 || (!writes && !k_out && !v_out)) return 0;
+    HIP_TRY(h, hipSetDevice(h->cfg.device));
+    hipStream_t s = (hipStream_t)stream;
+    if (h->q8kv) return launch_rows_q8(h, seq, layer, pos_begin, pos_end - pos_begin, k_in, v_in, k_out, v_out, s);
+    const size_t bytes = n * sizeof(float);
+    if (k_in) HIP_TRY(h, hipMemcpyAsync(h->k_cache + off, k_in, bytes, hipMemcpyDeviceToDevice, s));
+    if (v_in) HIP_TRY(h, hipMemcpyAsync(h->v_cache + off, v_in, bytes, hipMemcpyDeviceToDevice, s));
+    if (k_out) HIP_TRY(h, hipMemcpyAsync(k_out, h->k_cache + off, bytes, hipMemcpyDeviceToDevice, s));
+    if (v_out) HIP_TRY(h, hipMemcpyAsync(v_out, h->v_cache + off, bytes, hipMemcpyDeviceToDevice, s));
+    return 0;
+}
+
+int leap_hip_attention_kv_write_async(leap_hip_attention *h, int seq, int layer, int pos_begin, int pos_end, const float *k,
+                                      const float *v, void *stream)
+{
+    return rows_async(h, seq, layer, pos_begin, pos_end, k, v, nullptr, nullptr, stream);
+}
+
+int leap_hip_attention_kv_read_async(leap_hip_attention *h, int seq, int layer, int pos_begin, int pos_end, float *k,
+                                     float *v, void *stream)
+{
+    return rows_async(h, seq, layer, pos_begin, pos_end, nullptr, nullptr, k, v, stream);
 }
 
 }  // extern "C"

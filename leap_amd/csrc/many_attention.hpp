@@ -1,0 +1,959 @@
+// Attention of several new tokens of each sequence over its cache (prompts,
+// trees of drafted tokens), and of any number of them over an 8-bit cache.
+//
+// For the q heads that share a KV head, the (token, head) pairs of a
+// sequence are the rows r = token * group + head of one product: tiles of
+// 16 NB rows of Q against the cache's rows, so that a K or V row is read
+// once for all of a tile's rows.  A workgroup takes one tile and one chunk of
+// positions; its four waves take 32 positions each in turn and keep an online
+// softmax of their own, combined at the end.  Chunks of one tile leave records
+// (output, log2 of the sum) that the last one to arrive adds up.
+//
+// Products.  S^T = K Q^T and O^T = V^T P^T as 16x16x32 MFMAs in fp16, with a
+// lane holding one row of Q throughout: S^T's column is the lane's row, its
+// four registers per block are positions 4 (lane / 16) + i, and with the
+// contraction over positions taken in that same order (slot (g, 4 b + i) is
+// position 16 b + 4 g + i) those registers are O^T's B operand as they are.
+// No score leaves its lane.
+//
+// fp32 operands in fp16 products: x = 2^e (h + l), h = fp16(x 2^-e) and
+// l = fp16(x 2^-e - h), both rounded to nearest, with e such that the
+// largest of x's tile is in [2^13, 2^14).  h and l together hold x to 2^-22
+// relative (elements below 2^-28 of the tile's largest to 2^-39 of that,
+// fp16's subnormals), and h h' + h l' + l h' leaves out l l' < 2^-22 |x x'|,
+// of either sign: on sums of 128 terms and more that is fp32's own error.
+// Three fp16 MFMAs take 3/16 of the time of the fp32 MFMAs of the product.
+// The probabilities are split the same way, with 2^14 folded into their
+// exponent.  8-bit values are exact in fp16 and take two products.
+//
+// Rows with infinities or NaN: such a key or value makes NaN of the output
+// rows that see it, and of those only: its elements are replaced by zero in
+// the products and its scores by NaN where they are not masked.
+#pragma once
+
+#include "decode_attention.hpp"
+
+namespace leap {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+
+constexpr int kManyWaves = 4;
+constexpr int kManyThreads = kManyWaves * kWave;
+constexpr int kTileKeys = 32;                          // positions a wave takes at a time
+constexpr int kPassKeys = kManyWaves * kTileKeys;      // positions a workgroup takes at a time
+constexpr int kTreeMax = 64;                           // nodes of a sequence's tree
+constexpr float kAmaxFloor = 7.888609052210118e-31f;   // 2^-100: the least largest magnitude of an 8-bit head row
+
+// One launch over one layer.  begin NULL: one token a sequence, row i of
+// sequence i (then pos NULL: position pos_scalar).
+struct ManyArgs {
+    const float *q, *k_new, *v_new;  // rows of [n_heads*HD], [n_kv_heads*HD]
+    float *out;
+    float *k_cache, *v_cache;        // fp32 cache: sequence 0's rows of this layer
+    int8_t *k8, *v8;                 // 8-bit cache: the same, values
+    float *ks, *vs;                  // and scales, [n_kv_heads][scale_rows]
+    const float4 *rope;
+    const int *begin, *pos, *parent;
+    float *ws_o, *ws_lse;            // records of split tiles: [group][split][rows][HD], [group][split][rows]
+    int *counters;                   // [group], zero between launches
+    long long seq_stride;            // elements between sequences
+    long long scale_stride;          // floats between sequences
+    int scale_rows;
+    int n_seq, n_tokens, max_tokens, max_pos, pos_scalar;
+    int n_heads, n_kv_heads, group;
+    int slots;                       // tiles of all sequences, at most
+    int chunk, splits;               // positions of a chunk, chunks of the longest sequence
+    float scale_log2;
+    FastDiv by_group, by_kv_heads, by_splits;
+};
+
+__device__ __forceinline__ int wave_scan_add(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
+}
+
+// Lane i's sequence base + i of the packed batch: its first token row, its
+// tokens (0 where there is none) and its first position.  A sequence is
+// skipped (n = -1) where its rows leave [0, n_tokens) or go backwards, as are
+// all after it, and where it has more than max_tokens tokens or positions
+// outside [0, max_pos].  *stop: the sequences behind these are skipped too.
+struct SeqLane {
+    int first, n, p0;
+};
+__device__ __forceinline__ SeqLane seq_lane(const ManyArgs &a, int base, int lane, bool *stop)
+{
+    const int i = base + lane;
+    SeqLane s{0, 0, 0};
+    bool ok = true;
+    if (i < a.n_seq) {
+        s.first = a.begin[i];
+        const int end = a.begin[i + 1];
+        s.p0 = a.pos[i];
+        ok = s.first >= 0 && end >= s.first && end <= a.n_tokens;
+        s.n = end - s.first;
+    }
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(!ok);
+    *stop = bad != 0;
+    if (bad && lane >= __builtin_ctzll(bad)) s.n = i < a.n_seq ? -1 : 0;
+    if (s.n > 0 && (s.n > a.max_tokens || s.p0 < 0 || s.p0 > a.max_pos + 1 - s.n)) s.n = -1;
+    return s;
+}
+
+// The tile `slot` of the batch (tiles of BM rows, a sequence's last first:
+// with causal masks they see the most positions): seq < 0 where there is none.
+struct Place {
+    int seq, tile, first, n, p0;
+};
+template <int BM>
+__device__ __forceinline__ Place find_place(const ManyArgs &a, int slot, int lane)
+{
+    Place p{-1, 0, 0, 0, 0};
+    if (!a.begin) {
+        const int per = (a.group + BM - 1) / BM;
+        const int seq = slot / per;
+        if (seq >= a.n_seq) return p;
+        const int p0 = a.pos ? a.pos[seq] : a.pos_scalar;
+        if (p0 < 0 || p0 > a.max_pos) return p;
+        return Place{seq, slot - seq * per, seq, 1, p0};
+    }
+    int before = 0;
+    bool stop = false;
+    for (int base = 0; base < a.n_seq && !stop; base += kWave) {
+        const SeqLane s = seq_lane(a, base, lane, &stop);
+        const int tiles = s.n > 0 ? (s.n * a.group + BM - 1) / BM : 0;
+        const int upto = wave_scan_add(tiles);
+        const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+        if (slot - before < total) {
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > slot - before));
+            p.seq = base + l;
+            p.tile = __builtin_amdgcn_readlane(upto, l) - 1 - (slot - before);
+            p.first = __builtin_amdgcn_readlane(s.first, l);
+            p.n = __builtin_amdgcn_readlane(s.n, l);
+            p.p0 = __builtin_amdgcn_readlane(s.p0, l);
+            return p;
+        }
+        before += total;
+    }
+    return p;
+}
+
+// Lane j's node j of a tree of n <= 64 nodes: the bits of its ancestors and
+// itself, by six doublings of the steps upwards.  A parent outside [-1, j)
+// marks the node and its descendants bad.
+struct TreeLane {
+    uint64_t sees;
+    bool bad;
+};
+__device__ __forceinline__ TreeLane tree_lane(const int *parent, int n, int lane)
+{
+    int up = lane < n ? parent[lane] : -1;
+    int bad = up < -1 || up >= lane;
+    if (bad) up = -1;
+    unsigned lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+    for (int k = 0; k < 6; k++) {
+        const int from = max(up, 0);
+        const unsigned lo2 = __shfl(lo, from), hi2 = __shfl(hi, from);
+        const int up2 = __shfl(up, from), bad2 = __shfl(bad, from);
+        if (up >= 0) {
+            lo |= lo2;
+            hi |= hi2;
+            bad |= bad2;
+            up = up2;
+        }
+    }
+    return TreeLane{((uint64_t)hi << 32) | lo, bad != 0};
+}
+
+__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ bool finite_bits(unsigned b) { return b < 0x7f800000u; }
+__device__ __forceinline__ unsigned max4_bits(unsigned m, float4 x)
+{
+    return max(max(max(m, abs_bits(x.x)), max(abs_bits(x.y), abs_bits(x.z))), abs_bits(x.w));
+}
+__device__ __forceinline__ unsigned dpp_max16(unsigned x)
+{
+    // over the 16 lanes of a row, in every lane (row_ror)
+    x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x121, 0xF, 0xF, true));
+    x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x122, 0xF, 0xF, true));
+    x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xF, 0xF, true));
+    x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, true));
+    return x;
+}
+__device__ __forceinline__ unsigned wave_max_bits(unsigned x)
+{
+    x = dpp_max16(x);
+    const unsigned a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+    const unsigned c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+    return max(max(a, b), max(c, d));
+}
+
+// The exponent that a tile of largest magnitude `bits` is scaled by: in
+// [-100, 127], and 2^(13 - e), 2^(e - 13) as floats.
+__device__ __forceinline__ int tile_exp(unsigned bits) { return max((int)(bits >> 23), 27) - 127; }
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// x = h + l in fp16, to 2^-22 relative (see above), x already scaled.
+__device__ __forceinline__ void split2(float x, float y, half2v &h, half2v &l)
+{
+    h = half2v{(_Float16)x, (_Float16)y};
+    asm("" : "+v"(h));  // (the packed pair is what the remainders are taken from)
+    l = half2v{(_Float16)(x - (float)h.x), (_Float16)(y - (float)h.y)};
+}
+union Half8 {
+    half8v v;
+    half2v h[4];
+};
+__device__ __forceinline__ void split8(float4 a, float4 b, float sc, half8v &hi, half8v &lo)
+{
+    Half8 h, l;
+    split2(a.x * sc, a.y * sc, h.h[0], l.h[0]);
+    split2(a.z * sc, a.w * sc, h.h[1], l.h[1]);
+    split2(b.x * sc, b.y * sc, h.h[2], l.h[2]);
+    split2(b.z * sc, b.w * sc, h.h[3], l.h[3]);
+    hi = h.v;
+    lo = l.v;
+}
+
+// Infinities and NaN replaced by zero; whether there were any.
+__device__ __forceinline__ bool zero_bad(float4 &x)
+{
+    const bool a = finite_bits(abs_bits(x.x)), b = finite_bits(abs_bits(x.y));
+    const bool c = finite_bits(abs_bits(x.z)), d = finite_bits(abs_bits(x.w));
+    x = make_float4(a ? x.x : 0.0f, b ? x.y : 0.0f, c ? x.z : 0.0f, d ? x.w : 0.0f);
+    return !(a && b && c && d);
+}
+
+// int8 values to fp16, exactly: with the sign bit flipped a byte u = x + 128
+// placed under 0x64 is the fp16 number 1024 + u.
+__device__ __forceinline__ half2v bytes_half(unsigned two)
+{
+    return __builtin_bit_cast(half2v, two) - half2v{(_Float16)1152.0f, (_Float16)1152.0f};
+}
+__device__ __forceinline__ half8v bytes_half8(unsigned a, unsigned b)
+{
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    Half8 r;
+    r.h[0] = bytes_half(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u));
+    r.h[1] = bytes_half(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u));
+    r.h[2] = bytes_half(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u));
+    r.h[3] = bytes_half(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u));
+    return r.v;
+}
+
+__device__ __forceinline__ f32x4 mfma16(half8v a, half8v b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// ---- the rows of the new tokens into the cache -------------------------------
+
+// One head row of HD elements over HD / 4 lanes as int8 values and a scale:
+// a = max(largest magnitude, 2^-100), scale a / 127, value rint(x (127 / a)),
+// in fp32.  With an infinity or a NaN the scale is NaN, which is what the
+// row then stands for.  Every lane returns its four values and the scale.
+template <int HD>
+__device__ __forceinline__ int quantize_row(float4 x, float *scale)
+{
+    unsigned m = dpp_max16(max4_bits(0u, x));
+    if (HD == 128) m = max(m, (unsigned)__shfl_xor((int)m, 16));
+    const bool fin = finite_bits(m);
+    const float a = fmaxf(__uint_as_float(m), kAmaxFloor);
+    const float r = 127.0f / a;
+    *scale = fin ? a / 127.0f : __uint_as_float(0x7fc00000u);
+    const int q = ((int)rintf(x.x * r) & 255) | (((int)rintf(x.y * r) & 255) << 8) |
+                  (((int)rintf(x.z * r) & 255) << 16) | ((int)rintf(x.w * r) << 24);
+    return fin ? q : 0;
+}
+
+// A wave per token: its K rows rotated and its V rows as they are, into
+// cache row p0 + j of its sequence; NaN into the output rows of skipped
+// sequences.  Rows behind the last sequence are left alone.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(kManyThreads) void many_append_kernel(ManyArgs a)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    const int r = blockIdx.x * kManyWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (r >= a.n_tokens) return;
+    int seq = -1, row = 0, at = 0;
+    bool skip = false;
+    if (!a.begin) {
+        seq = r;
+        row = at = a.pos ? a.pos[r] : a.pos_scalar;
+        skip = row < 0 || row > a.max_pos;
+    } else {
+        bool stop = false;
+        for (int base = 0; base < a.n_seq && !stop && seq < 0; base += kWave) {
+            const SeqLane s = seq_lane(a, base, lane, &stop);
+            const int i = base + lane;
+            // (a skipped sequence's rows by its own two bounds)
+            const bool has = i < a.n_seq && s.first <= r && r < a.begin[i + 1];
+            const uint64_t who = __builtin_amdgcn_ballot_w64(has);
+            if (!who) continue;
+            const int l = __builtin_ctzll(who);
+            seq = base + l;
+            skip = __builtin_amdgcn_readlane(s.n, l) < 0;
+            const int j = r - __builtin_amdgcn_readlane(s.first, l);
+            row = at = __builtin_amdgcn_readlane(s.p0, l) + j;
+            if (a.parent && !skip) {
+                const TreeLane t = tree_lane(a.parent + (r - j), __builtin_amdgcn_readlane(s.n, l), lane);
+                const int depth = (int)__popcll(t.sees);
+                at = row - j + __builtin_amdgcn_readlane(depth, j) - 1;
+            }
+        }
+        if (seq < 0 && !stop) return;
+        if (seq < 0) skip = true;
+    }
+    if (skip) {
+        const float nan = __uint_as_float(0x7fc00000u);
+        float4 *o = reinterpret_cast<float4 *>(a.out + (size_t)r * a.n_heads * HD);
+        for (int i = lane; i < a.n_heads * (HD / 4); i += kWave) o[i] = make_float4(nan, nan, nan, nan);
+        return;
+    }
+    constexpr int LR = HD / 4;  // lanes of a head row
+    const int kv_dim = a.n_kv_heads * HD;
+    const float4 turn = a.rope[(size_t)at * LR + (lane & (LR - 1))];
+    const float4 *kn = reinterpret_cast<const float4 *>(a.k_new + (size_t)r * kv_dim);
+    const float4 *vn = reinterpret_cast<const float4 *>(a.v_new + (size_t)r * kv_dim);
+    const size_t to = (size_t)seq * a.seq_stride + (size_t)row * kv_dim;
+    for (int i = lane; i < kv_dim / 4; i += kWave) {
+        const float4 k = rope4(kn[i], turn), v = vn[i];
+        if constexpr (Q8) {
+            float sk, sv;
+            const int qk = quantize_row<HD>(k, &sk), qv = quantize_row<HD>(v, &sv);
+            reinterpret_cast<int *>(a.k8 + to)[i] = qk;
+            reinterpret_cast<int *>(a.v8 + to)[i] = qv;
+            if ((lane & (LR - 1)) == 0) {
+                const size_t s = (size_t)seq * a.scale_stride + (size_t)(i / LR) * a.scale_rows + row;
+                a.ks[s] = sk;
+                a.vs[s] = sv;
+            }
+        } else {
+            reinterpret_cast<float4 *>(a.k_cache + to)[i] = k;
+            reinterpret_cast<float4 *>(a.v_cache + to)[i] = v;
+        }
+    }
+}
+
+// ---- the attention kernel -----------------------------------------------------
+
+template <int HD, int NB>
+struct ManyShared {
+    static constexpr int BM = 16 * NB;
+    static constexpr int kOStride = HD + 4;  // floats between rows of a wave's output (16 rows on 16 banks' groups)
+    union {
+        half8v q[NB][HD / 32][2][kWave];     // Q's operands: high and low halves
+        float o[kManyWaves][BM][kOStride];   // the waves' outputs
+    };
+    float qf[BM];                            // 2^(e - 13) log2(e) / sqrt(HD) of each row (NaN: a row without result)
+    float m[kManyWaves][BM], l[kManyWaves][BM];
+    int e[kManyWaves];
+    float f[kManyWaves][BM];                 // the waves' weights in the sum
+    float lse[BM], inv[BM];
+    uint64_t sees[kTreeMax];
+    int last;
+};
+
+template <int HD, int NB, bool Q8>
+__global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) void many_attention_kernel(ManyArgs a)
+{
+    constexpr int BM = 16 * NB, KS = HD / 32, VB = HD / 16;
+    __shared__ ManyShared<HD, NB> sh;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int m = lane & 15, g = lane >> 4;
+
+    // the workgroup's tile, KV head and chunk: a (tile, KV head) group's
+    // chunks on one XCD where there are eight groups or more
+    const int n_groups = a.slots * a.n_kv_heads;
+    int gi, split;
+    if (n_groups >= kXcds) {
+        const int local = blockIdx.x / kXcds;
+        const int gl = (int)fast_div((uint32_t)local, a.by_splits);
+        split = local - gl * a.splits;
+        gi = gl * kXcds + (blockIdx.x & (kXcds - 1));
+        if (gi >= n_groups) return;
+    } else {
+        split = blockIdx.x / n_groups;
+        gi = blockIdx.x - split * n_groups;
+    }
+    const int slot = (int)fast_div((uint32_t)gi, a.by_kv_heads);
+    const int kvh = gi - slot * a.n_kv_heads;
+    const Place p = find_place<BM>(a, slot, lane);
+    if (p.seq < 0) return;
+    const int rows = p.n * a.group, r0 = p.tile * BM;
+    const int j0 = (int)fast_div((uint32_t)r0, a.by_group);
+    const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(r0 + BM - 1), a.by_group));
+    const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
+    const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
+    if (c0 >= kv_end) return;
+
+    if (a.parent && wave == 0) {
+        const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
+        sh.sees[lane] = t.bad ? 0 : t.sees;
+    }
+    if (a.parent) __syncthreads();
+
+    // ---- Q: rotated, split, into LDS as the products' B operand ----
+    // element (s, g, j) of a row: the order of the contraction over dims,
+    // such that a K load instruction takes whole 64-byte pieces of its rows
+    auto dim_of = [&](int s, int h) {
+        return Q8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h : 32 * s + 16 * h + 4 * g;
+    };
+    for (int nb = wave; nb < NB; nb += kManyWaves) {
+        const int r = r0 + 16 * nb + m;
+        const int j = (int)fast_div((uint32_t)min(r, rows - 1), a.by_group);
+        const int head = kvh * a.group + min(r, rows - 1) - j * a.group;
+        bool good = true;
+        int at = p.p0 + j;
+        if (a.parent) {
+            const uint64_t s = sh.sees[j];
+            good = s != 0;
+            at = p.p0 + max((int)__popcll(s) - 1, 0);  // (a bad node sees none)
+        }
+        const float *src = a.q + ((size_t)(p.first + j) * a.n_heads + head) * HD;
+        float4 x[KS][2];
+        unsigned mx = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int d = dim_of(s, h);
+                x[s][h] = rope4(*reinterpret_cast<const float4 *>(src + d), a.rope[((size_t)at * HD + d) / 4]);
+                mx = max4_bits(mx, x[s][h]);
+            }
+        mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
+        mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
+        good = good && finite_bits(mx);
+        const int e = tile_exp(good ? mx : 0u);
+        if (g == 0) sh.qf[16 * nb + m] = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
+        const float sc = good ? exp2_int(13 - e) : 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            half8v hi, lo;
+            split8(x[s][0], x[s][1], sc, hi, lo);
+            sh.q[nb][s][0][lane] = hi;
+            sh.q[nb][s][1][lane] = lo;
+        }
+    }
+    __syncthreads();
+    // each lane's rows: their tokens
+    int tok[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) tok[nb] = (int)fast_div((uint32_t)min(r0 + 16 * nb + m, rows - 1), a.by_group);
+    half8v qh[NB][KS], ql[NB][KS];  // (NB == 1: in registers; else read from LDS as they are used)
+    if constexpr (NB == 1) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                qh[nb][s] = sh.q[nb][s][0][lane];
+                ql[nb][s] = sh.q[nb][s][1][lane];
+            }
+    }
+
+    // ---- the cache's rows ----
+    const int kv_dim = a.n_kv_heads * HD;
+    const uint32_t row_bytes = (uint32_t)kv_dim * (Q8 ? 1 : 4), head_off = (uint32_t)kvh * HD * (Q8 ? 1 : 4);
+    const size_t base = (size_t)p.seq * a.seq_stride;
+    const uint32_t bytes = (uint32_t)c1 * row_bytes;  // (rows from c1 on read as zero)
+    const auto kr = Q8 ? make_rsrc(a.k8 + base, bytes) : make_rsrc(a.k_cache + base, bytes);
+    const auto vr = Q8 ? make_rsrc(a.v8 + base, bytes) : make_rsrc(a.v_cache + base, bytes);
+    const size_t sbase = (size_t)p.seq * a.scale_stride + (size_t)kvh * a.scale_rows;
+    const auto ksr = make_rsrc(Q8 ? a.ks + sbase : nullptr, Q8 ? (uint32_t)c1 * 4u : 0u);
+    const auto vsr = make_rsrc(Q8 ? a.vs + sbase : nullptr, Q8 ? (uint32_t)c1 * 4u : 0u);
+
+    constexpr int KR = Q8 ? HD / 64 : HD / 16, VR = Q8 ? 1 : HD / 64;
+    float4 kraw[2][KR], vraw[8][VR];
+    float2 vraw8[8];
+    float4 ksc[2], vsc[2];
+    auto load_k = [&](int key0) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const uint32_t off = (uint32_t)(key0 + 16 * b + m) * row_bytes + head_off;
+#pragma unroll
+            for (int i = 0; i < KR; i++)
+                kraw[b][i] = buf_load4(kr, off + (Q8 ? 64 * i + 16 * g : 64 * i + 16 * g));
+            if constexpr (Q8) ksc[b] = buf_load4(ksr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
+        }
+    };
+    auto load_v = [&](int key0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t off = (uint32_t)(key0 + 16 * (j >> 2) + 4 * g + (j & 3)) * row_bytes + head_off;
+            if constexpr (Q8) {
+                if constexpr (HD == 128)
+                    vraw8[j] = buf_load2(vr, off + 8 * m);
+                else
+                    vraw8[j].x = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(vr, (int)(off + 4 * m), 0, 0));
+            } else {
+#pragma unroll
+                for (int i = 0; i < VR; i++) vraw[j][i] = buf_load4(vr, off + 256 * i + 16 * m);
+            }
+        }
+        if constexpr (Q8)
+#pragma unroll
+            for (int b = 0; b < 2; b++) vsc[b] = buf_load4(vsr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
+    };
+
+    f32x4 o[VB][NB];
+    float mrun[NB], lrun[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        mrun[nb] = -__builtin_inff();
+        lrun[nb] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VB; v++) o[v][nb] = f32x4{0, 0, 0, 0};
+    }
+    int erun = -100;  // O's unit is 2^(erun - 13)
+
+    int key0 = c0 + wave * kTileKeys;
+    if (key0 < c1) {
+        load_k(key0);
+        load_v(key0);
+    }
+    for (; key0 < c1; key0 += kPassKeys) {
+        // ---- scores ----
+        if constexpr (NB > 1) asm volatile("" ::: "memory");  // (Q's operands are read from LDS in every pass)
+        unsigned badkeys = 0;  // positions of the tile whose key or value is not finite (bit: position - key0)
+        f32x4 sc[2][NB];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) sc[b][nb] = f32x4{0, 0, 0, 0};
+        float kscale = 1.0f, kinv = 1.0f, vscale = 1.0f;
+        int vexp = erun;
+        if constexpr (!Q8) {
+            unsigned mk = 0;
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < KR; i++) mk = max4_bits(mk, kraw[b][i]);
+            unsigned wk = wave_max_bits(mk);
+            if (!finite_bits(wk)) {
+                mk = 0;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    bool bad = false;
+#pragma unroll
+                    for (int i = 0; i < KR; i++) {
+                        bad |= zero_bad(kraw[b][i]);
+                        mk = max4_bits(mk, kraw[b][i]);
+                    }
+                    uint64_t w = __builtin_amdgcn_ballot_w64(bad);
+                    w |= w >> 32;
+                    w |= w >> 16;
+                    badkeys |= (unsigned)(w & 0xffffu) << (16 * b);
+                }
+                wk = wave_max_bits(mk);
+            }
+            const int ek = tile_exp(wk);
+            kscale = exp2_int(13 - ek);
+            kinv = exp2_int(ek - 13);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                half8v kh, kl;
+                if constexpr (Q8) {
+                    const float4 w = kraw[b][s >> 1];
+                    kh = (s & 1) ? bytes_half8(__float_as_uint(w.z), __float_as_uint(w.w))
+                                 : bytes_half8(__float_as_uint(w.x), __float_as_uint(w.y));
+                } else {
+                    split8(kraw[b][2 * s], kraw[b][2 * s + 1], kscale, kh, kl);
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    half8v h, l;
+                    if constexpr (NB == 1) {
+                        h = qh[nb][s];
+                        l = ql[nb][s];
+                    } else {
+                        h = sh.q[nb][s][0][lane];
+                        l = sh.q[nb][s][1][lane];
+                    }
+                    sc[b][nb] = mfma16(kh, l, sc[b][nb]);
+                    if constexpr (!Q8) sc[b][nb] = mfma16(kl, h, sc[b][nb]);
+                    sc[b][nb] = mfma16(kh, h, sc[b][nb]);
+                }
+            }
+        float4 kscv[2], vscv[2];
+        if constexpr (Q8) {
+            // a row's two scales: NaN in either marks it
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                vscv[b] = vsc[b];
+                kscv[b] = make_float4(ksc[b].x + 0.0f * vsc[b].x, ksc[b].y + 0.0f * vsc[b].y,
+                                      ksc[b].z + 0.0f * vsc[b].z, ksc[b].w + 0.0f * vsc[b].w);
+            }
+            unsigned mv = 0;
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float *e = &vscv[b].x;
+#pragma unroll
+                for (int i = 0; i < 4; i++) mv = max(mv, finite_bits(abs_bits(e[i])) ? abs_bits(e[i]) : 0u);
+            }
+            mv = max(mv, (unsigned)__shfl_xor((int)mv, 16));
+            mv = max(mv, (unsigned)__shfl_xor((int)mv, 32));
+            // (scales to at most 1: a probability of 2^14 times them stays in fp16)
+            vexp = max(erun, min(tile_exp(__builtin_amdgcn_readfirstlane(mv)) + 1, 126));
+            vscale = exp2_int(-vexp);
+        }
+        if constexpr (NB >= 2) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NB <= 2) load_k(key0 + kPassKeys);
+        if constexpr (!Q8) {
+            unsigned mv = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int i = 0; i < VR; i++) mv = max4_bits(mv, vraw[j][i]);
+            unsigned wv = wave_max_bits(mv);
+            if (!finite_bits(wv)) {
+                mv = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    bool bad = false;
+#pragma unroll
+                    for (int i = 0; i < VR; i++) {
+                        bad |= zero_bad(vraw[j][i]);
+                        mv = max4_bits(mv, vraw[j][i]);
+                    }
+                    const uint64_t w = __builtin_amdgcn_ballot_w64(bad);
+                    for (int gg = 0; gg < 4; gg++)
+                        if ((w >> (16 * gg)) & 0xffffu) badkeys |= 1u << (16 * (j >> 2) + 4 * gg + (j & 3));
+                }
+                wv = wave_max_bits(mv);
+            }
+            vexp = max(erun, tile_exp(wv));
+            vscale = exp2_int(13 - vexp);
+        }
+
+        // ---- softmax ----
+        const bool masked = key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > (a.parent ? p.p0 - 1 : p.p0 + j0);
+        const float oscale = exp2_int(max(erun - vexp, -126));
+        erun = vexp;
+        half8v ph[NB], pl[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const float qf = sh.qf[16 * nb + m];
+            float s[8];
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                const int b = t >> 2, i = t & 3;
+                const float f = Q8 ? (&kscv[b].x)[i] * qf : kinv * qf;
+                s[t] = sc[b][nb][i] * f;
+            }
+            if (badkeys)
+#pragma unroll
+                for (int t = 0; t < 8; t++)
+                    if ((badkeys >> (16 * (t >> 2) + 4 * g + (t & 3))) & 1) s[t] = __uint_as_float(0x7fc00000u);
+            if (masked) {
+                // visible: up to `limit`, and of a tree's nodes those of `sees`
+                // (a bad node sees itself alone, as NaN)
+                int limit = p.p0 + tok[nb];
+                uint64_t sees = 0;
+                if (a.parent) {
+                    limit = p.p0 - 1;
+                    sees = sh.sees[tok[nb]];
+                    if (!sees) sees = 1ull << tok[nb];
+                }
+#pragma unroll
+                for (int t = 0; t < 8; t++) {
+                    const int key = key0 + 16 * (t >> 2) + 4 * g + (t & 3);
+                    const bool see = key <= limit || ((sees >> ((key - p.p0) & 63)) & 1);
+                    if (!see || key >= c1) s[t] = -__builtin_inff();
+                }
+            }
+            float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+            mt = fmaxf(mt, __shfl_xor(mt, 16));
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float mn = fmaxf(mrun[nb], mt);
+            const float ref = mn == -__builtin_inff() ? 0.0f : mn;  // (a row that has seen nothing yet)
+            const float alpha = fast_exp2(mrun[nb] - ref);
+            mrun[nb] = mn;
+            float sum = 0.0f;
+            Half8 h, l;
+#pragma unroll
+            for (int t = 0; t < 8; t += 2) {
+                float x = fast_exp2(s[t] - ref + 14.0f), y = fast_exp2(s[t + 1] - ref + 14.0f);
+                sum += x + y;
+                if constexpr (Q8) {
+                    const int b = t >> 2, i = t & 3;
+                    x = x == 0.0f ? 0.0f : x * ((&vscv[b].x)[i] * vscale);
+                    y = y == 0.0f ? 0.0f : y * ((&vscv[b].x)[i + 1] * vscale);
+                }
+                split2(x, y, h.h[t / 2], l.h[t / 2]);
+            }
+            ph[nb] = h.v;
+            pl[nb] = l.v;
+            lrun[nb] = lrun[nb] * alpha + sum;
+            const float os = alpha * oscale;
+#pragma unroll
+            for (int v = 0; v < VB; v++) o[v][nb] *= os;
+        }
+
+        if constexpr (NB >= 2) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NB > 2) load_k(key0 + kPassKeys);  // (here for the registers' sake)
+
+        // ---- weighted values ----
+#pragma unroll
+        for (int v = 0; v < VB; v++) {
+            half8v vh, vl;
+            if constexpr (Q8) {
+                Half8 r;
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const unsigned x = __float_as_uint(v < 4 ? vraw8[j].x : vraw8[j].y) ^ 0x80808080u;
+                    const unsigned y = __float_as_uint(v < 4 ? vraw8[j + 1].x : vraw8[j + 1].y) ^ 0x80808080u;
+                    const unsigned sel = 0x0c000c00u | (unsigned)(4 + (v & 3)) << 16 | (unsigned)(v & 3);
+                    r.h[j / 2] = bytes_half(__builtin_amdgcn_perm(y, x, sel) | 0x64006400u);
+                }
+                vh = r.v;
+            } else {
+                const int i = v >> 2, c = v & 3;
+                auto at = [&](int j) { return (&vraw[j][i].x)[c]; };
+                split8(make_float4(at(0), at(1), at(2), at(3)), make_float4(at(4), at(5), at(6), at(7)), vscale, vh, vl);
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                o[v][nb] = mfma16(vh, pl[nb], o[v][nb]);
+                if constexpr (!Q8) o[v][nb] = mfma16(vl, ph[nb], o[v][nb]);
+                o[v][nb] = mfma16(vh, ph[nb], o[v][nb]);
+            }
+        }
+        load_v(key0 + kPassKeys);
+    }
+
+    // ---- the four waves' results together ----
+    __syncthreads();  // (Q's operands are read; their memory takes the outputs)
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        float l = lrun[nb];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (g == 0) {
+            sh.m[wave][16 * nb + m] = mrun[nb];
+            sh.l[wave][16 * nb + m] = l;
+        }
+        // register i of block v: dim (8 bits) VB (4 g + i) + v, or 64 (v / 4) + 4 (4 g + i) + v % 4
+        float *dst = sh.o[wave][16 * nb + m];
+#pragma unroll
+        for (int v = 0; v < VB; v += 4)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = Q8 ? VB * (4 * g + i) + v : 16 * v + 4 * (4 * g + i);
+                *reinterpret_cast<float4 *>(dst + d) =
+                    make_float4(o[v][nb][i], o[v + 1][nb][i], o[v + 2][nb][i], o[v + 3][nb][i]);
+            }
+    }
+    if (lane == 0) sh.e[wave] = erun;
+    __syncthreads();
+    // (8 bits: V's unit is 2^erun, fp32: 2^(erun - 13); a probability's is 2^-14 in both sums)
+    if (tid < BM) {
+        float mm = sh.m[0][tid];
+        int ee = sh.e[0];
+#pragma unroll
+        for (int w = 1; w < kManyWaves; w++) {
+            mm = fmaxf(mm, sh.m[w][tid]);
+            ee = max(ee, sh.e[w]);
+        }
+        const float ref = mm == -__builtin_inff() ? 0.0f : mm;
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kManyWaves; w++) {
+            const float f = fast_exp2(sh.m[w][tid] - ref);
+            total += f * sh.l[w][tid];
+            sh.f[w][tid] = f * exp2_int(max(sh.e[w] - ee, -126));
+        }
+        // a chunk none of whose positions the row sees: nothing, weight 0
+        const bool none = total == 0.0f;
+        sh.inv[tid] = none ? 0.0f : exp2_int(max(min(Q8 ? ee : ee - 13, 127), -126)) / total;
+        sh.lse[tid] = none ? -__builtin_inff() : ref + log2f(total) - 14.0f;
+    }
+    __syncthreads();
+    const int n_split = a.splits > 1 ? (kv_end + a.chunk - 1) / a.chunk : 1;
+    const size_t rec = ((size_t)gi * a.splits + split) * BM;
+    for (int i = tid; i < BM * (HD / 4); i += kManyThreads) {
+        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+        const int r = r0 + row;
+        if (r >= rows) break;
+        float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < kManyWaves; w++) fma4(acc, sh.f[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
+        scale4(acc, sh.inv[row]);
+        if (n_split == 1) {
+            const int j = (int)fast_div((uint32_t)r, a.by_group);
+            const int head = kvh * a.group + r - j * a.group;
+            *reinterpret_cast<float4 *>(a.out + ((size_t)(p.first + j) * a.n_heads + head) * HD + d) = acc;
+        } else {
+            // records cross XCDs: written through, and read past the L2s (device scope)
+            const auto wr = make_rsrc(a.ws_o + rec * HD, (uint32_t)(BM * HD * 4));
+            buf_store4<kSc1>(wr, (uint32_t)(row * HD + d) * 4u, acc);
+            if (d == 0)
+                __hip_atomic_store(a.ws_lse + rec + row, sh.lse[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (n_split == 1) return;
+
+    // ---- the last chunk to arrive adds up the records ----
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        const int before = __hip_atomic_fetch_add(a.counters + gi, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.last = before == n_split - 1;
+        if (before == n_split - 1)
+            __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    const size_t rec0 = (size_t)gi * a.splits * BM;
+    for (int i = tid; i < BM * (HD / 4); i += kManyThreads) {
+        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+        const int r = r0 + row;
+        if (r >= rows) break;
+        float4 acc = make_float4(0, 0, 0, 0);
+        float top = -__builtin_inff(), total = 0.0f;
+        for (int s = 0; s < n_split; s++) {
+            const float lse = __hip_atomic_load(a.ws_lse + rec0 + (size_t)s * BM + row, __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT);
+            const auto wr = make_rsrc(a.ws_o + (rec0 + (size_t)s * BM) * HD, (uint32_t)(BM * HD * 4));
+            const float4 x = buf_load4<kSc1>(wr, (uint32_t)(row * HD + d) * 4u);
+            const float now = fmaxf(top, lse);
+            const float ref = now == -__builtin_inff() ? 0.0f : now;
+            const float keep = fast_exp2(top - ref), w = fast_exp2(lse - ref);
+            scale4(acc, keep);
+            fma4(acc, w, x);
+            total = total * keep + w;
+            top = now;
+        }
+        scale4(acc, 1.0f / total);
+        const int j = (int)fast_div((uint32_t)r, a.by_group);
+        const int head = kvh * a.group + r - j * a.group;
+        *reinterpret_cast<float4 *>(a.out + ((size_t)(p.first + j) * a.n_heads + head) * HD + d) = acc;
+    }
+}
+
+// ---- rows of a cache, moved ---------------------------------------------------
+
+// The accepted paths' rows, moved together (tree_keep): path[i] of sequence
+// seq goes from row pos + path[i] to pos + i, in every held layer.  A thread
+// has one 16-byte column of one layer's K or V (or, for 8 bits, one head's
+// scales) and moves its rows in order: path ascends, so a row is read
+// before anything is written over it.
+struct KeepArgs {
+    char *k, *v;                       // sequence 0's first layer
+    float *ks, *vs;                    // 8 bits: its scales
+    const int *pos, *path;
+    long long seq_bytes, layer_bytes;  // between sequences, and layers
+    long long scale_seq, scale_layer;  // floats
+    int row_bytes, scale_rows, n_kv_heads;
+    int n_layers, max_path, seq_len;
+    int columns;                       // 16-byte columns of a row
+};
+constexpr int kKeepThreads = 256;
+template <typename T>
+__device__ __forceinline__ void keep_column(T *col, size_t stride, const int *path, int n)
+{
+    for (int i = 0; i < n; i += 8) {
+        T x[8];
+#pragma unroll
+        for (int t = 0; t < 8; t++)
+            x[t] = col[(size_t)path[min(i + t, n - 1)] * stride];
+#pragma unroll
+        for (int t = 0; t < 8; t++)
+            if (i + t < n) col[(size_t)(i + t) * stride] = x[t];
+    }
+}
+template <bool Q8>
+__global__ __launch_bounds__(kKeepThreads) void tree_keep_kernel(KeepArgs a)
+{
+    __shared__ int path[kTreeMax];
+    const int seq = blockIdx.y, tid = threadIdx.x;
+    const int p0 = a.pos[seq];
+    // (a path ends at its first entry that is not above the one before it, or leaves the cache)
+    int n = 0;
+    if (tid < kWave) {
+        const int x = tid < a.max_path ? a.path[(size_t)seq * a.max_path + tid] : -1;
+        const int prev = __shfl_up(x, 1);
+        const bool ok = x < kTreeMax && x > (tid ? prev : -1) && p0 >= 0 && p0 < a.seq_len - x;
+        const uint64_t bad = __builtin_amdgcn_ballot_w64(!ok);
+        n = bad ? __builtin_ctzll(bad) : kWave;
+        path[tid] = tid < n ? x : -1;
+    }
+    __syncthreads();
+    if (tid >= kWave) {
+        while (n < kTreeMax && path[n] >= 0) n++;
+    }
+    const int per_layer = 2 * a.columns + (Q8 ? 2 * a.n_kv_heads : 0);
+    const int at = blockIdx.x * kKeepThreads + tid;
+    if (at >= per_layer * a.n_layers) return;
+    const int layer = at / per_layer;
+    int c = at - layer * per_layer;
+    if (c < 2 * a.columns) {
+        char *base = (c < a.columns ? a.k : a.v) + seq * a.seq_bytes + layer * a.layer_bytes + (size_t)p0 * a.row_bytes;
+        if (c >= a.columns) c -= a.columns;
+        keep_column(reinterpret_cast<f32x4 *>(base + 16 * (size_t)c), (size_t)a.row_bytes / 16, path, n);
+    } else {
+        c -= 2 * a.columns;
+        float *base = (c < a.n_kv_heads ? a.ks : a.vs) + seq * a.scale_seq + layer * a.scale_layer + p0;
+        if (c >= a.n_kv_heads) c -= a.n_kv_heads;
+        keep_column(base + (size_t)c * a.scale_rows, (size_t)1, path, n);
+    }
+}
+
+// Rows [row0, row0 + n) of one sequence and layer between fp32 memory and the
+// cache: quantised on the way in, what they stand for on the way out.
+struct RowsArgs {
+    const float *k_in, *v_in;  // (write: either may be NULL)
+    float *k_out, *v_out;      // (read)
+    int8_t *k8, *v8;           // at row0
+    float *ks, *vs;            // at row0 of KV head 0
+    int scale_rows, n_kv_heads, n;
+};
+template <int HD>
+__global__ __launch_bounds__(256) void q8_write_kernel(RowsArgs a)
+{
+    constexpr int LR = HD / 4;
+    const int per_row = a.n_kv_heads * LR;
+    const long long total = (long long)a.n * per_row;
+    const float *in = blockIdx.y ? a.v_in : a.k_in;
+    int8_t *to = blockIdx.y ? a.v8 : a.k8;
+    float *scales = blockIdx.y ? a.vs : a.ks;
+    if (!in) return;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        float s;
+        const int q = quantize_row<HD>(reinterpret_cast<const float4 *>(in)[i], &s);
+        reinterpret_cast<int *>(to)[i] = q;
+        if (((int)i & (LR - 1)) == 0) {
+            const int row = (int)(i / per_row), h = (int)(i - (long long)row * per_row) / LR;
+            scales[(size_t)h * a.scale_rows + row] = s;
+        }
+    }
+}
+template <int HD>
+__global__ __launch_bounds__(256) void q8_read_kernel(RowsArgs a)
+{
+    constexpr int LR = HD / 4;
+    const int per_row = a.n_kv_heads * LR;
+    const long long total = (long long)a.n * per_row;
+    float *out = blockIdx.y ? a.v_out : a.k_out;
+    const int8_t *from = blockIdx.y ? a.v8 : a.k8;
+    const float *scales = blockIdx.y ? a.vs : a.ks;
+    if (!out) return;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int q = reinterpret_cast<const int *>(from)[i];
+        const int row = (int)(i / per_row), h = (int)(i - (long long)row * per_row) / LR;
+        const float s = scales[(size_t)h * a.scale_rows + row];
+        reinterpret_cast<float4 *>(out)[i] = make_float4((float)(int8_t)q * s, (float)(int8_t)(q >> 8) * s,
+                                                         (float)(int8_t)(q >> 16) * s, (float)(q >> 24) * s);
+    }
+}
+
+}  // namespace leap
