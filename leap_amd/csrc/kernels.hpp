@@ -113,7 +113,8 @@ bool pick_q8(int dim, int gs, int kind, int rows, int n_cu, Q8Launch *out);
 // attention over tiles of 16 nb rows, on an fp32 or 8-bit cache.
 using ManyFn = void (*)(leap::ManyArgs);
 struct ManyKernels {
-    ManyFn append, attention;
+    ManyFn append, attention, merge;
+    int waves;  // of the attention kernel's workgroups
 };
 // The quantising write of an 8-bit cache's rows, and their reading back.
 using RowsFn = void (*)(leap::RowsArgs);
@@ -130,7 +131,7 @@ extern template RowsKernels pick_rows_hd<64>();
 extern template RowsKernels pick_rows_hd<128>();
 inline ManyKernels pick_many(int hd, int nb, bool q8)
 {
-    return hd == 64 ? pick_many_hd<64>(nb, q8) : hd == 128 ? pick_many_hd<128>(nb, q8) : ManyKernels{nullptr, nullptr};
+    return hd == 64 ? pick_many_hd<64>(nb, q8) : hd == 128 ? pick_many_hd<128>(nb, q8) : ManyKernels{};
 }
 inline RowsKernels pick_rows(int hd) { return hd == 64 ? pick_rows_hd<64>() : pick_rows_hd<128>(); }
 // The accepted paths' rows moved together, in an fp32 or 8-bit cache.

@@ -10,11 +10,16 @@ template <int HD>
 ManyKernels pick_many_hd(int nb, bool q8)
 {
     const ManyFn append = q8 ? leap::many_append_kernel<HD, true> : leap::many_append_kernel<HD, false>;
-#define LEAP_CASE(NB) \
-    if (nb == NB) return {append, q8 ? leap::many_attention_kernel<HD, NB, true> : leap::many_attention_kernel<HD, NB, false>};
-    LEAP_CASE(1) LEAP_CASE(2) LEAP_CASE(4)
-#undef LEAP_CASE
-    return {nullptr, nullptr};
+    if (q8) {
+        if (nb == 1) return {append, leap::many_attention_kernel<HD, 1, 8, true>, leap::many_merge_kernel<HD, 1>, 8};
+        if (nb == 2) return {append, leap::many_attention_kernel<HD, 2, 4, true>, leap::many_merge_kernel<HD, 2>, 4};
+        if (nb == 4) return {append, leap::many_attention_kernel<HD, 4, 4, true>, leap::many_merge_kernel<HD, 4>, 4};
+    } else {
+        if (nb == 1) return {append, leap::many_attention_kernel<HD, 1, 4, false>, leap::many_merge_kernel<HD, 1>, 4};
+        if (nb == 2) return {append, leap::many_attention_kernel<HD, 2, 4, false>, leap::many_merge_kernel<HD, 2>, 4};
+        if (nb == 4) return {append, leap::many_attention_kernel<HD, 4, 4, false>, leap::many_merge_kernel<HD, 4>, 4};
+    }
+    return {};
 }
 
 template <int HD>

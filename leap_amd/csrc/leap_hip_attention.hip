@@ -785,32 +785,42 @@ constexpr size_t kManyCounters = 4096;
 
 // What one launch of many_attention_kernel is cut into.
 struct ManyPlan {
+    ManyKernels fn;
     int nb;        // rows of a tile / 16
     int slots;     // tiles of the batch, at most
     int chunk, splits;
-    long long wgs;
+    bool fused;    // the kernel stores the new rows itself
+    bool spread;   // chunks on all XCDs, records added up by a launch of their own
+    long long groups, wgs;
 };
 ManyPlan many_plan(const leap_hip_attention *h, int n_seq, int n_tokens, int max_tokens, int max_pos,
                    long long total_rows)
 {
-    const int group = h->group, n_kv = h->cfg.n_kv_heads;
+    const int group = h->group, n_kv = h->cfg.n_kv_heads, hd = h->cfg.head_dim;
     const long long rows_max = (long long)max_tokens * group;
     ManyPlan p{};
     p.nb = rows_max <= 16 ? 1 : rows_max <= 32 ? 2 : 4;
-    const int bm = 16 * p.nb;
+    p.fn = pick_many(hd, p.nb, h->q8kv);
+    p.fused = max_tokens <= leap::kTreeMax;
+    const int bm = 16 * p.nb, pass = p.fn.waves * leap::kTileKeys;
     p.slots = (int)std::min((long long)n_tokens * group / bm + n_seq, n_seq * ((rows_max + bm - 1) / bm));
-    const long long groups = (long long)p.slots * n_kv;
+    p.groups = (long long)p.slots * n_kv;
     const int total = max_pos + 1;
-    const long long want = (long long)h->n_cu * (p.nb == 4 ? 1 : 2);
-    const int s = (int)std::max<long long>(1, std::min<long long>(64, want / groups));
+    const long long group_bytes = (long long)total * hd * (h->q8kv ? 2 : 8);
+    const int per_cu = p.nb == 4 || p.fn.waves == 8 || (hd == 128 && !h->q8kv) ? 1 : 2;
+    const bool few = p.groups < leap::kXcds && group_bytes < kSpreadBytes;  // on as many XCDs as groups
+    const long long cus = few ? h->n_cu * p.groups / leap::kXcds : h->n_cu;
+    const long long want = std::max<long long>(1, cus * per_cu);
+    const int s = (int)std::max<long long>(1, std::min<long long>(leap::kManySplits, want / p.groups));
     (void)total_rows;
-    p.chunk = std::max(leap::kPassKeys, round_up((total + s - 1) / s, leap::kPassKeys));
+    p.chunk = std::max(pass, round_up((total + s - 1) / s, pass));
     p.splits = (total + p.chunk - 1) / p.chunk;
-    while (p.splits > 1 && ((size_t)groups * p.splits * bm > kManyRecords || (size_t)groups > kManyCounters)) {
+    while (p.splits > 1 && ((size_t)p.groups * p.splits * bm > kManyRecords || (size_t)p.groups > kManyCounters)) {
         p.chunk *= 2;
         p.splits = (total + p.chunk - 1) / p.chunk;
     }
-    p.wgs = groups >= leap::kXcds ? (groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * p.splits : groups * p.splits;
+    p.spread = p.splits > 1 && (p.nb == 4 || (p.groups < leap::kXcds && !few));
+    p.wgs = p.spread ? p.groups * p.splits : (p.groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * p.splits;
     return p;
 }
 
@@ -877,16 +887,19 @@ int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, c
     a.slots = p.slots;
     a.chunk = p.chunk;
     a.splits = p.splits;
+    a.fused = p.fused;
+    a.spread = p.spread;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)h->cfg.head_dim));
     a.by_group = leap::make_fastdiv((uint32_t)h->group);
     a.by_kv_heads = leap::make_fastdiv((uint32_t)h->cfg.n_kv_heads);
     a.by_splits = leap::make_fastdiv((uint32_t)p.splits);
     if (p.wgs > 0x7fffffffLL) return set_err(h, -EINVAL, "%lld workgroups in one launch", p.wgs);
-    const ManyKernels fn = pick_many(h->cfg.head_dim, p.nb, h->q8kv);
-    if (!fn.attention) return set_err(h, -EINVAL, "unsupported head_dim %d", h->cfg.head_dim);
-    HIP_TRY(h, launch_k(fn.append, dim3((unsigned)((n_tokens + leap::kManyWaves - 1) / leap::kManyWaves)),
-                        dim3(leap::kManyThreads), stream, a));
-    HIP_TRY(h, launch_k(fn.attention, dim3((unsigned)p.wgs), dim3(leap::kManyThreads), stream, a));
+    if (!p.fn.attention) return set_err(h, -EINVAL, "unsupported head_dim %d", h->cfg.head_dim);
+    if (!p.fused)
+        HIP_TRY(h, launch_k(p.fn.append, dim3((unsigned)((n_tokens + leap::kAppendWaves - 1) / leap::kAppendWaves)),
+                            dim3(leap::kAppendWaves * leap::kWave), stream, a));
+    HIP_TRY(h, launch_k(p.fn.attention, dim3((unsigned)p.wgs), dim3((unsigned)(p.fn.waves * leap::kWave)), stream, a));
+    if (p.spread) HIP_TRY(h, launch_k(p.fn.merge, dim3((unsigned)(p.groups * p.nb)), dim3(256), stream, a));
     return 0;
 }
 

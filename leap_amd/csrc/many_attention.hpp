@@ -38,10 +38,9 @@ namespace leap {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 
-constexpr int kManyWaves = 4;
-constexpr int kManyThreads = kManyWaves * kWave;
+constexpr int kAppendWaves = 4;                        // waves of a workgroup of the append kernel
 constexpr int kTileKeys = 32;                          // positions a wave takes at a time
-constexpr int kPassKeys = kManyWaves * kTileKeys;      // positions a workgroup takes at a time
+constexpr int kManySplits = 64;                        // chunks of a tile, at most
 constexpr int kTreeMax = 64;                           // nodes of a sequence's tree
 constexpr float kAmaxFloor = 7.888609052210118e-31f;   // 2^-100: the least largest magnitude of an 8-bit head row
 
@@ -64,6 +63,8 @@ struct ManyArgs {
     int n_heads, n_kv_heads, group;
     int slots;                       // tiles of all sequences, at most
     int chunk, splits;               // positions of a chunk, chunks of the longest sequence
+    int fused;                       // the attention kernel stores the new rows itself (else many_append_kernel ran)
+    int spread;                      // a tile's chunks lie on all XCDs, and many_merge_kernel adds up their records
     float scale_log2;
     FastDiv by_group, by_kv_heads, by_splits;
 };
@@ -107,7 +108,8 @@ __device__ __forceinline__ SeqLane seq_lane(const ManyArgs &a, int base, int lan
 }
 
 // The tile `slot` of the batch (tiles of BM rows, a sequence's last first:
-// with causal masks they see the most positions): seq < 0 where there is none.
+// with causal masks they see the most positions): seq < 0 where there is
+// none, n < 0 for a skipped sequence's (with begin, those have no tiles).
 struct Place {
     int seq, tile, first, n, p0;
 };
@@ -120,8 +122,7 @@ __device__ __forceinline__ Place find_place(const ManyArgs &a, int slot, int lan
         const int seq = slot / per;
         if (seq >= a.n_seq) return p;
         const int p0 = a.pos ? a.pos[seq] : a.pos_scalar;
-        if (p0 < 0 || p0 > a.max_pos) return p;
-        return Place{seq, slot - seq * per, seq, 1, p0};
+        return Place{seq, slot - seq * per, seq, p0 < 0 || p0 > a.max_pos ? -1 : 1, p0};
     }
     int before = 0;
     bool stop = false;
@@ -273,190 +274,250 @@ __device__ __forceinline__ int quantize_row(float4 x, float *scale)
     return fin ? q : 0;
 }
 
+// Where token row r of a packed batch goes: its sequence (-1: none has it),
+// cache row, rotary position, and whether its sequence is skipped.
+struct TokenPlace {
+    int seq, row, at;
+    bool skip;
+};
+__device__ __forceinline__ TokenPlace find_token(const ManyArgs &a, int r, int lane)
+{
+    TokenPlace t{-1, 0, 0, false};
+    if (!a.begin) {
+        t.seq = r;
+        t.row = t.at = a.pos ? a.pos[r] : a.pos_scalar;
+        t.skip = t.row < 0 || t.row > a.max_pos;
+        return t;
+    }
+    bool stop = false;
+    for (int base = 0; base < a.n_seq && !stop && t.seq < 0; base += kWave) {
+        const SeqLane s = seq_lane(a, base, lane, &stop);
+        const int i = base + lane;
+        // (a skipped sequence's rows by its own two bounds)
+        const bool has = i < a.n_seq && s.first <= r && r < a.begin[i + 1];
+        const uint64_t who = __builtin_amdgcn_ballot_w64(has);
+        if (!who) continue;
+        const int l = __builtin_ctzll(who);
+        t.seq = base + l;
+        t.skip = __builtin_amdgcn_readlane(s.n, l) < 0;
+        const int j = r - __builtin_amdgcn_readlane(s.first, l);
+        t.row = t.at = __builtin_amdgcn_readlane(s.p0, l) + j;
+        if (a.parent && !t.skip) {
+            const TreeLane w = tree_lane(a.parent + (r - j), __builtin_amdgcn_readlane(s.n, l), lane);
+            const int depth = (int)__popcll(w.sees);
+            t.at = t.row - j + __builtin_amdgcn_readlane(depth, j) - 1;
+        }
+    }
+    if (t.seq < 0 && stop) t = TokenPlace{0, 0, 0, true};  // behind a begin that goes back
+    return t;
+}
+template <int HD>
+__device__ __forceinline__ void fill_nan(float *out, size_t first4, int n4, int i0, int step)
+{
+    const float nan = __uint_as_float(0x7fc00000u);
+    for (int i = i0; i < n4; i += step) reinterpret_cast<float4 *>(out)[first4 + i] = make_float4(nan, nan, nan, nan);
+}
+
+// A head row of the cache, LR = HD / 4 lanes of a float4 each: element i of
+// the [kv_dim / 4] words of (seq, row).
+template <int HD, bool Q8>
+__device__ __forceinline__ void store_row(const ManyArgs &a, int seq, int row, int i, float4 x, bool value)
+{
+    constexpr int LR = HD / 4;
+    const size_t to = (size_t)seq * a.seq_stride + (size_t)row * (a.n_kv_heads * HD);
+    if constexpr (Q8) {
+        float sc;
+        const int q = quantize_row<HD>(x, &sc);
+        reinterpret_cast<int *>((value ? a.v8 : a.k8) + to)[i] = q;
+        if ((i & (LR - 1)) == 0)
+            (value ? a.vs : a.ks)[(size_t)seq * a.scale_stride + (size_t)(i / LR) * a.scale_rows + row] = sc;
+    } else {
+        reinterpret_cast<float4 *>((value ? a.v_cache : a.k_cache) + to)[i] = x;
+    }
+}
+
 // A wave per token: its K rows rotated and its V rows as they are, into
 // cache row p0 + j of its sequence; NaN into the output rows of skipped
-// sequences.  Rows behind the last sequence are left alone.
+// sequences.  Rows behind the last sequence are left alone.  For calls of
+// many tokens a sequence, whose tiles read each other's rows; for few, the
+// attention kernel does it (fused), one launch less.
 template <int HD, bool Q8>
-__global__ __launch_bounds__(kManyThreads) void many_append_kernel(ManyArgs a)
+__global__ __launch_bounds__(kAppendWaves * kWave) void many_append_kernel(ManyArgs a)
 {
     const int lane = threadIdx.x & (kWave - 1);
-    const int r = blockIdx.x * kManyWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r = blockIdx.x * kAppendWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (r >= a.n_tokens) return;
-    int seq = -1, row = 0, at = 0;
-    bool skip = false;
-    if (!a.begin) {
-        seq = r;
-        row = at = a.pos ? a.pos[r] : a.pos_scalar;
-        skip = row < 0 || row > a.max_pos;
-    } else {
-        bool stop = false;
-        for (int base = 0; base < a.n_seq && !stop && seq < 0; base += kWave) {
-            const SeqLane s = seq_lane(a, base, lane, &stop);
-            const int i = base + lane;
-            // (a skipped sequence's rows by its own two bounds)
-            const bool has = i < a.n_seq && s.first <= r && r < a.begin[i + 1];
-            const uint64_t who = __builtin_amdgcn_ballot_w64(has);
-            if (!who) continue;
-            const int l = __builtin_ctzll(who);
-            seq = base + l;
-            skip = __builtin_amdgcn_readlane(s.n, l) < 0;
-            const int j = r - __builtin_amdgcn_readlane(s.first, l);
-            row = at = __builtin_amdgcn_readlane(s.p0, l) + j;
-            if (a.parent && !skip) {
-                const TreeLane t = tree_lane(a.parent + (r - j), __builtin_amdgcn_readlane(s.n, l), lane);
-                const int depth = (int)__popcll(t.sees);
-                at = row - j + __builtin_amdgcn_readlane(depth, j) - 1;
-            }
-        }
-        if (seq < 0 && !stop) return;
-        if (seq < 0) skip = true;
-    }
-    if (skip) {
-        const float nan = __uint_as_float(0x7fc00000u);
-        float4 *o = reinterpret_cast<float4 *>(a.out + (size_t)r * a.n_heads * HD);
-        for (int i = lane; i < a.n_heads * (HD / 4); i += kWave) o[i] = make_float4(nan, nan, nan, nan);
+    const TokenPlace t = find_token(a, r, lane);
+    if (t.seq < 0) return;
+    if (t.skip) {
+        fill_nan<HD>(a.out, (size_t)r * a.n_heads * (HD / 4), a.n_heads * (HD / 4), lane, kWave);
         return;
     }
     constexpr int LR = HD / 4;  // lanes of a head row
-    const int kv_dim = a.n_kv_heads * HD;
-    const float4 turn = a.rope[(size_t)at * LR + (lane & (LR - 1))];
-    const float4 *kn = reinterpret_cast<const float4 *>(a.k_new + (size_t)r * kv_dim);
-    const float4 *vn = reinterpret_cast<const float4 *>(a.v_new + (size_t)r * kv_dim);
-    const size_t to = (size_t)seq * a.seq_stride + (size_t)row * kv_dim;
-    for (int i = lane; i < kv_dim / 4; i += kWave) {
-        const float4 k = rope4(kn[i], turn), v = vn[i];
-        if constexpr (Q8) {
-            float sk, sv;
-            const int qk = quantize_row<HD>(k, &sk), qv = quantize_row<HD>(v, &sv);
-            reinterpret_cast<int *>(a.k8 + to)[i] = qk;
-            reinterpret_cast<int *>(a.v8 + to)[i] = qv;
-            if ((lane & (LR - 1)) == 0) {
-                const size_t s = (size_t)seq * a.scale_stride + (size_t)(i / LR) * a.scale_rows + row;
-                a.ks[s] = sk;
-                a.vs[s] = sv;
-            }
-        } else {
-            reinterpret_cast<float4 *>(a.k_cache + to)[i] = k;
-            reinterpret_cast<float4 *>(a.v_cache + to)[i] = v;
-        }
+    const int words = a.n_kv_heads * LR;
+    const float4 turn = a.rope[(size_t)t.at * LR + (lane & (LR - 1))];
+    const float4 *kn = reinterpret_cast<const float4 *>(a.k_new) + (size_t)r * words;
+    const float4 *vn = reinterpret_cast<const float4 *>(a.v_new) + (size_t)r * words;
+    for (int i = lane; i < words; i += kWave) {
+        const float4 k = kn[i], v = vn[i];
+        store_row<HD, Q8>(a, t.seq, t.row, i, rope4(k, turn), false);
+        store_row<HD, Q8>(a, t.seq, t.row, i, v, true);
     }
 }
 
 // ---- the attention kernel -----------------------------------------------------
 
-template <int HD, int NB>
+template <int HD, int NB, int W>
 struct ManyShared {
     static constexpr int BM = 16 * NB;
     static constexpr int kOStride = HD + 4;  // floats between rows of a wave's output (16 rows on 16 banks' groups)
     union {
         half8v q[NB][HD / 32][2][kWave];     // Q's operands: high and low halves
-        float o[kManyWaves][BM][kOStride];   // the waves' outputs
+        float o[W][BM][kOStride];            // the waves' outputs
+        struct {
+            float w[16][kManySplits + 1];    // the merge: weights of a row's records
+            float4 part[W * kWave];          // and partial sums of them
+        } merge;
     };
     float qf[BM];                            // 2^(e - 13) log2(e) / sqrt(HD) of each row (NaN: a row without result)
-    float m[kManyWaves][BM], l[kManyWaves][BM];
-    int e[kManyWaves];
-    float f[kManyWaves][BM];                 // the waves' weights in the sum
+    float m[W][BM], l[W][BM];
+    int e[W];
+    float f[W][BM];                 // the waves' weights in the sum
     float lse[BM], inv[BM];
     uint64_t sees[kTreeMax];
     int last;
 };
 
-template <int HD, int NB, bool Q8>
-__global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) void many_attention_kernel(ManyArgs a)
+// The sum of a tile's records, for its 16 rows from row block rb on, by T >=
+// 256 threads: record s of row i counts 2^(lse_s - max lse) / their sum.
+template <int HD, int BM, int T, typename Merge>
+__device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi, int n_split, const Place &p, int kvh, int rb,
+                                           int tid)
 {
-    constexpr int BM = 16 * NB, KS = HD / 32, VB = HD / 16;
-    __shared__ ManyShared<HD, NB> sh;
+    constexpr int LR = HD / 4;
+    const int rows = p.n * a.group, r0 = p.tile * BM + 16 * rb;
+    if (r0 >= rows) return;
+    const size_t rec0 = (size_t)gi * a.splits * BM + 16 * rb;
+    const float ninf = -__builtin_inff();
+    if (T == 256 || tid < 256) {
+        const int row = tid >> 4, l = tid & 15;
+        const auto lr = make_rsrc(a.ws_lse + rec0, (uint32_t)n_split * BM * 4u);
+        float x[kManySplits / 16], top = ninf;
+#pragma unroll
+        for (int k = 0; k < kManySplits / 16; k++) {
+            const int s = l + 16 * k;
+            x[k] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (s * BM + row) * 4, 0, kSc1));
+            if (s >= n_split) x[k] = ninf;
+        }
+#pragma unroll
+        for (int k = 0; k < kManySplits / 16; k++) top = fmaxf(top, x[k]);
+        top = fmaxf(top, dpp<0x121>(top));
+        top = fmaxf(top, dpp<0x122>(top));
+        top = fmaxf(top, dpp<0x124>(top));
+        top = fmaxf(top, dpp<0x128>(top));
+        if (top == ninf) top = 0.0f;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kManySplits / 16; k++) {
+            x[k] = fast_exp2(x[k] - top);
+            sum += x[k];
+        }
+        sum += dpp<0x121>(sum);
+        sum += dpp<0x122>(sum);
+        sum += dpp<0x124>(sum);
+        sum += dpp<0x128>(sum);
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int k = 0; k < kManySplits / 16; k++)
+            if (l + 16 * k < n_split) sh.w[row][l + 16 * k] = x[k] * inv;
+    }
+    __syncthreads();
+    // the rows' float4 words, `items` of them; with fewer than threads the
+    // records are dealt to `parts` threads a word
+    const int items = min(16, rows - r0) * LR;
+    int parts = 1;
+    while (2 * parts * items <= T) parts *= 2;
+    const auto wr = make_rsrc(a.ws_o + rec0 * HD, (uint32_t)n_split * BM * HD * 4u);
+    for (int i0 = 0; i0 < items; i0 += T) {
+        const int part = parts > 1 ? tid / items : 0, i = i0 + tid - part * items;
+        float4 acc = make_float4(0, 0, 0, 0);
+        const int row = i / LR;
+        if (i < items && part < parts) {
+            for (int s = part; s < n_split; s += 8 * parts) {
+                float4 x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    x[k] = buf_load4<kSc1>(wr, (uint32_t)((s + k * parts) * BM * HD + 4 * i) * 4u);  // (past the last: 0)
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (s + k * parts < n_split) fma4(acc, sh.w[row][s + k * parts], x[k]);
+            }
+        }
+        if (parts > 1) {
+            sh.part[tid] = acc;
+            __syncthreads();
+            if (part == 0 && i < items)
+                for (int t = 1; t < parts; t++) fma4(acc, 1.0f, sh.part[t * items + i]);
+        }
+        if (part == 0 && i < items) {
+            const int r = r0 + row;
+            const int j = (int)fast_div((uint32_t)r, a.by_group);
+            const int head = kvh * a.group + r - j * a.group;
+            reinterpret_cast<float4 *>(a.out)[((size_t)(p.first + j) * a.n_heads + head) * LR + (i - row * LR)] = acc;
+        }
+    }
+}
+
+template <int HD, int NB, int W, bool Q8>
+__global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) void many_attention_kernel(ManyArgs a)
+{
+    constexpr int BM = 16 * NB, KS = HD / 32, VB = HD / 16, LR = HD / 4;
+    constexpr int kThreads = W * kWave, kPassKeys = W * kTileKeys;
+    __shared__ ManyShared<HD, NB, W> sh;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, g = lane >> 4;
 
     // the workgroup's tile, KV head and chunk: a (tile, KV head) group's
-    // chunks on one XCD where there are eight groups or more
+    // chunks on one XCD, or (spread) on all
     const int n_groups = a.slots * a.n_kv_heads;
     int gi, split;
-    if (n_groups >= kXcds) {
+    if (a.spread) {
+        split = blockIdx.x / n_groups;
+        gi = blockIdx.x - split * n_groups;
+    } else {
         const int local = blockIdx.x / kXcds;
         const int gl = (int)fast_div((uint32_t)local, a.by_splits);
         split = local - gl * a.splits;
         gi = gl * kXcds + (blockIdx.x & (kXcds - 1));
-        if (gi >= n_groups) return;
-    } else {
-        split = blockIdx.x / n_groups;
-        gi = blockIdx.x - split * n_groups;
     }
+    if (a.fused && a.begin && blockIdx.x == 0) {
+        // skipped sequences' output rows, if there are any
+        bool stop = false, any = false;
+        for (int base = 0; base < a.n_seq && !stop && !any; base += kWave)
+            any = __builtin_amdgcn_ballot_w64(seq_lane(a, base, lane, &stop).n < 0) != 0;
+        if (any)
+            for (int r = wave; r < a.n_tokens; r += W) {
+                const TokenPlace t = find_token(a, r, lane);
+                if (t.seq >= 0 && t.skip)
+                    fill_nan<HD>(a.out, (size_t)r * a.n_heads * LR, a.n_heads * LR, lane, kWave);
+            }
+    }
+    if (gi >= n_groups) return;
     const int slot = (int)fast_div((uint32_t)gi, a.by_kv_heads);
     const int kvh = gi - slot * a.n_kv_heads;
     const Place p = find_place<BM>(a, slot, lane);
     if (p.seq < 0) return;
+    if (p.n < 0) {
+        if (split == 0)
+            fill_nan<HD>(a.out, ((size_t)p.first * a.n_heads + kvh * a.group) * LR, a.group * LR, tid, kThreads);
+        return;
+    }
     const int rows = p.n * a.group, r0 = p.tile * BM;
     const int j0 = (int)fast_div((uint32_t)r0, a.by_group);
     const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(r0 + BM - 1), a.by_group));
     const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
     const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
     if (c0 >= kv_end) return;
-
-    if (a.parent && wave == 0) {
-        const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
-        sh.sees[lane] = t.bad ? 0 : t.sees;
-    }
-    if (a.parent) __syncthreads();
-
-    // ---- Q: rotated, split, into LDS as the products' B operand ----
-    // element (s, g, j) of a row: the order of the contraction over dims,
-    // such that a K load instruction takes whole 64-byte pieces of its rows
-    auto dim_of = [&](int s, int h) {
-        return Q8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h : 32 * s + 16 * h + 4 * g;
-    };
-    for (int nb = wave; nb < NB; nb += kManyWaves) {
-        const int r = r0 + 16 * nb + m;
-        const int j = (int)fast_div((uint32_t)min(r, rows - 1), a.by_group);
-        const int head = kvh * a.group + min(r, rows - 1) - j * a.group;
-        bool good = true;
-        int at = p.p0 + j;
-        if (a.parent) {
-            const uint64_t s = sh.sees[j];
-            good = s != 0;
-            at = p.p0 + max((int)__popcll(s) - 1, 0);  // (a bad node sees none)
-        }
-        const float *src = a.q + ((size_t)(p.first + j) * a.n_heads + head) * HD;
-        float4 x[KS][2];
-        unsigned mx = 0;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int d = dim_of(s, h);
-                x[s][h] = rope4(*reinterpret_cast<const float4 *>(src + d), a.rope[((size_t)at * HD + d) / 4]);
-                mx = max4_bits(mx, x[s][h]);
-            }
-        mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
-        mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
-        good = good && finite_bits(mx);
-        const int e = tile_exp(good ? mx : 0u);
-        if (g == 0) sh.qf[16 * nb + m] = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
-        const float sc = good ? exp2_int(13 - e) : 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            half8v hi, lo;
-            split8(x[s][0], x[s][1], sc, hi, lo);
-            sh.q[nb][s][0][lane] = hi;
-            sh.q[nb][s][1][lane] = lo;
-        }
-    }
-    __syncthreads();
-    // each lane's rows: their tokens
-    int tok[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) tok[nb] = (int)fast_div((uint32_t)min(r0 + 16 * nb + m, rows - 1), a.by_group);
-    half8v qh[NB][KS], ql[NB][KS];  // (NB == 1: in registers; else read from LDS as they are used)
-    if constexpr (NB == 1) {
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                qh[nb][s] = sh.q[nb][s][0][lane];
-                ql[nb][s] = sh.q[nb][s][1][lane];
-            }
-    }
 
     // ---- the cache's rows ----
     const int kv_dim = a.n_kv_heads * HD;
@@ -478,8 +539,7 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
         for (int b = 0; b < 2; b++) {
             const uint32_t off = (uint32_t)(key0 + 16 * b + m) * row_bytes + head_off;
 #pragma unroll
-            for (int i = 0; i < KR; i++)
-                kraw[b][i] = buf_load4(kr, off + (Q8 ? 64 * i + 16 * g : 64 * i + 16 * g));
+            for (int i = 0; i < KR; i++) kraw[b][i] = buf_load4(kr, off + 64 * i + 16 * g);
             if constexpr (Q8) ksc[b] = buf_load4(ksr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
         }
     };
@@ -502,6 +562,101 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
             for (int b = 0; b < 2; b++) vsc[b] = buf_load4(vsr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
     };
 
+    // ---- Q: rotated, split, into LDS as the products' B operand ----
+    // element (s, g, j) of a row: the order of the contraction over dims,
+    // such that a K load instruction takes whole 64-byte pieces of its rows
+    auto dim_of = [&](int s, int h) {
+        return Q8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h : 32 * s + 16 * h + 4 * g;
+    };
+    // The loads go out in the order they are needed: Q's, then the first
+    // tile's rows (where this call does not store any of them).
+    float4 x[KS][2];
+    auto q_row = [&](int nb, int *j) {
+        const int r = min(r0 + 16 * nb + m, rows - 1);
+        *j = (int)fast_div((uint32_t)r, a.by_group);
+        return a.q + ((size_t)(p.first + *j) * a.n_heads + kvh * a.group + r - *j * a.group) * HD;
+    };
+    auto load_q = [&](int nb) {
+        int j;
+        const float *src = q_row(nb, &j);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) x[s][h] = *reinterpret_cast<const float4 *>(src + dim_of(s, h));
+    };
+    int key0 = c0 + wave * kTileKeys;
+    const bool early = key0 < c1 && (!a.fused || key0 + kTileKeys <= p.p0);
+    if (wave < NB) load_q(wave);
+    if (early) {
+        load_k(key0);
+        load_v(key0);
+    }
+    if (a.parent) {
+        if (wave == W - 1) {
+            const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
+            sh.sees[lane] = t.bad ? 0 : t.sees;
+        }
+        __syncthreads();
+    }
+    // position of token j (and of a bad node: as if it hung on the cached rows)
+    auto place_of = [&](int j) { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
+
+    // ---- the new rows of this chunk into the cache ----
+    const int t0 = a.fused ? max(c0 - p.p0, 0) : 0, t1 = a.fused ? min(c1 - p.p0, p.n) : 0;
+    if (t0 < t1) {
+        // (every tile and chunk that reads a row stores it first, the same
+        // bytes each; K rows, then V rows, LR threads each)
+        for (int i = tid / LR; i < 2 * (t1 - t0); i += kThreads / LR) {
+            const bool value = i >= t1 - t0;
+            const int j = t0 + (value ? i - (t1 - t0) : i), w = kvh * LR + (tid & (LR - 1));
+            const float4 *src = reinterpret_cast<const float4 *>(value ? a.v_new : a.k_new);
+            float4 y = src[(size_t)(p.first + j) * (a.n_kv_heads * LR) + w];
+            if (!value) y = rope4(y, a.rope[(size_t)place_of(j) * LR + (tid & (LR - 1))]);
+            store_row<HD, Q8>(a, p.seq, p.p0 + j, w, y, value);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    for (int nb = wave; nb < NB; nb += W) {
+        if (nb != wave) load_q(nb);
+        int j;
+        q_row(nb, &j);
+        const int at = place_of(j);
+        bool good = !a.parent || sh.sees[j] != 0;
+        unsigned mx = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                x[s][h] = rope4(x[s][h], a.rope[((size_t)at * HD + dim_of(s, h)) / 4]);
+                mx = max4_bits(mx, x[s][h]);
+            }
+        mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
+        mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
+        good = good && finite_bits(mx);
+        const int e = tile_exp(good ? mx : 0u);
+        if (g == 0) sh.qf[16 * nb + m] = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
+        const float sc = good ? exp2_int(13 - e) : 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            half8v hi, lo;
+            split8(x[s][0], x[s][1], sc, hi, lo);
+            sh.q[nb][s][0][lane] = hi;
+            sh.q[nb][s][1][lane] = lo;
+        }
+    }
+    __syncthreads();
+    if (t0 < t1) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (L1 may hold parts of the new rows' lines)
+    half8v qh[NB][KS], ql[NB][KS];  // (NB == 1: in registers; else read from LDS as they are used)
+    if constexpr (NB == 1) {
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                qh[nb][s] = sh.q[nb][s][0][lane];
+                ql[nb][s] = sh.q[nb][s][1][lane];
+            }
+    }
+
     f32x4 o[VB][NB];
     float mrun[NB], lrun[NB];
 #pragma unroll
@@ -513,8 +668,7 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
     }
     int erun = -100;  // O's unit is 2^(erun - 13)
 
-    int key0 = c0 + wave * kTileKeys;
-    if (key0 < c1) {
+    if (!early && key0 < c1) {
         load_k(key0);
         load_v(key0);
     }
@@ -562,6 +716,7 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 half8v kh, kl;
+                if constexpr (NB == 4) __builtin_amdgcn_sched_barrier(0);
                 if constexpr (Q8) {
                     const float4 w = kraw[b][s >> 1];
                     kh = (s & 1) ? bytes_half8(__float_as_uint(w.z), __float_as_uint(w.w))
@@ -657,12 +812,13 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
             if (masked) {
                 // visible: up to `limit`, and of a tree's nodes those of `sees`
                 // (a bad node sees itself alone, as NaN)
-                int limit = p.p0 + tok[nb];
+                const int tok = (int)fast_div((uint32_t)min(r0 + 16 * nb + m, rows - 1), a.by_group);
+                int limit = p.p0 + tok;
                 uint64_t sees = 0;
                 if (a.parent) {
                     limit = p.p0 - 1;
-                    sees = sh.sees[tok[nb]];
-                    if (!sees) sees = 1ull << tok[nb];
+                    sees = sh.sees[tok];
+                    if (!sees) sees = 1ull << tok;
                 }
 #pragma unroll
                 for (int t = 0; t < 8; t++) {
@@ -731,7 +887,7 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
         load_v(key0 + kPassKeys);
     }
 
-    // ---- the four waves' results together ----
+    // ---- the waves' results together ----
     __syncthreads();  // (Q's operands are read; their memory takes the outputs)
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
@@ -760,14 +916,14 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
         float mm = sh.m[0][tid];
         int ee = sh.e[0];
 #pragma unroll
-        for (int w = 1; w < kManyWaves; w++) {
+        for (int w = 1; w < W; w++) {
             mm = fmaxf(mm, sh.m[w][tid]);
             ee = max(ee, sh.e[w]);
         }
         const float ref = mm == -__builtin_inff() ? 0.0f : mm;
         float total = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kManyWaves; w++) {
+        for (int w = 0; w < W; w++) {
             const float f = fast_exp2(sh.m[w][tid] - ref);
             total += f * sh.l[w][tid];
             sh.f[w][tid] = f * exp2_int(max(sh.e[w] - ee, -126));
@@ -780,64 +936,59 @@ __global__ __launch_bounds__(kManyThreads, NB == 4 || (HD == 128 && !Q8) ? 1 : 2
     __syncthreads();
     const int n_split = a.splits > 1 ? (kv_end + a.chunk - 1) / a.chunk : 1;
     const size_t rec = ((size_t)gi * a.splits + split) * BM;
-    for (int i = tid; i < BM * (HD / 4); i += kManyThreads) {
+    for (int i = tid; i < BM * (HD / 4); i += kThreads) {
         const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
         const int r = r0 + row;
         if (r >= rows) break;
         float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
-        for (int w = 0; w < kManyWaves; w++) fma4(acc, sh.f[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
+        for (int w = 0; w < W; w++) fma4(acc, sh.f[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
         scale4(acc, sh.inv[row]);
         if (n_split == 1) {
             const int j = (int)fast_div((uint32_t)r, a.by_group);
             const int head = kvh * a.group + r - j * a.group;
             *reinterpret_cast<float4 *>(a.out + ((size_t)(p.first + j) * a.n_heads + head) * HD + d) = acc;
         } else {
-            // records cross XCDs: written through, and read past the L2s (device scope)
-            const auto wr = make_rsrc(a.ws_o + rec * HD, (uint32_t)(BM * HD * 4));
-            buf_store4<kSc1>(wr, (uint32_t)(row * HD + d) * 4u, acc);
-            if (d == 0)
-                __hip_atomic_store(a.ws_lse + rec + row, sh.lse[row], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *reinterpret_cast<float4 *>(a.ws_o + (rec + row) * HD + d) = acc;
+            if (d == 0) a.ws_lse[rec + row] = sh.lse[row];
         }
     }
-    if (n_split == 1) return;
+    if (n_split == 1 || a.spread) return;
 
     // ---- the last chunk to arrive adds up the records ----
+    // (all in one XCD's L2: the stores have drained to it, the counter is an
+    // L2 atomic, and the loads miss in L1)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
         const int before = __hip_atomic_fetch_add(a.counters + gi, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         sh.last = before == n_split - 1;
-        if (before == n_split - 1)
-            __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == n_split - 1) __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!sh.last) return;
-    const size_t rec0 = (size_t)gi * a.splits * BM;
-    for (int i = tid; i < BM * (HD / 4); i += kManyThreads) {
-        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
-        const int r = r0 + row;
-        if (r >= rows) break;
-        float4 acc = make_float4(0, 0, 0, 0);
-        float top = -__builtin_inff(), total = 0.0f;
-        for (int s = 0; s < n_split; s++) {
-            const float lse = __hip_atomic_load(a.ws_lse + rec0 + (size_t)s * BM + row, __ATOMIC_RELAXED,
-                                                __HIP_MEMORY_SCOPE_AGENT);
-            const auto wr = make_rsrc(a.ws_o + (rec0 + (size_t)s * BM) * HD, (uint32_t)(BM * HD * 4));
-            const float4 x = buf_load4<kSc1>(wr, (uint32_t)(row * HD + d) * 4u);
-            const float now = fmaxf(top, lse);
-            const float ref = now == -__builtin_inff() ? 0.0f : now;
-            const float keep = fast_exp2(top - ref), w = fast_exp2(lse - ref);
-            scale4(acc, keep);
-            fma4(acc, w, x);
-            total = total * keep + w;
-            top = now;
-        }
-        scale4(acc, 1.0f / total);
-        const int j = (int)fast_div((uint32_t)r, a.by_group);
-        const int head = kvh * a.group + r - j * a.group;
-        *reinterpret_cast<float4 *>(a.out + ((size_t)(p.first + j) * a.n_heads + head) * HD + d) = acc;
+    for (int rb = 0; rb < NB; rb++) {
+        merge_rows<HD, BM, kThreads>(a, sh.merge, gi, n_split, p, kvh, rb, tid);
+        if (NB > 1) __syncthreads();
     }
+}
+
+// The records of a spread launch's tiles added up: a workgroup per 16 rows.
+template <int HD, int NB>
+__global__ __launch_bounds__(256) void many_merge_kernel(ManyArgs a)
+{
+    constexpr int BM = 16 * NB;
+    __shared__ decltype(ManyShared<HD, NB, 4>::merge) sh;
+    const int tid = threadIdx.x;
+    const int gi = blockIdx.x / NB, rb = blockIdx.x - gi * NB;
+    const int slot = (int)fast_div((uint32_t)gi, a.by_kv_heads);
+    const int kvh = gi - slot * a.n_kv_heads;
+    const Place p = find_place<BM>(a, slot, tid & (kWave - 1));
+    if (p.seq < 0 || p.n < 0) return;
+    const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(p.tile * BM + BM - 1), a.by_group));
+    const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
+    const int n_split = (kv_end + a.chunk - 1) / a.chunk;
+    if (n_split > 1) merge_rows<HD, BM, 256>(a, sh, gi, n_split, p, kvh, rb, tid);
 }
 
 // ---- rows of a cache, moved ---------------------------------------------------
