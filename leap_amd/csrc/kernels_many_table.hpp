@@ -3,6 +3,7 @@
 #pragma once
 
 #include "kernels.hpp"
+#include "wide_attention.hpp"
 
 namespace leap_kernels {
 
@@ -10,16 +11,11 @@ template <int HD>
 ManyKernels pick_many_hd(int nb, bool q8)
 {
     const ManyFn append = q8 ? leap::many_append_kernel<HD, true> : leap::many_append_kernel<HD, false>;
-    if (q8) {
-        if (nb == 1) return {append, leap::many_attention_kernel<HD, 1, 8, true>, leap::many_merge_kernel<HD, 1>, 8};
-        if (nb == 2) return {append, leap::many_attention_kernel<HD, 2, 4, true>, leap::many_merge_kernel<HD, 2>, 4};
-        if (nb == 4) return {append, leap::many_attention_kernel<HD, 4, 4, true>, leap::many_merge_kernel<HD, 4>, 4};
-    } else {
-        if (nb == 1) return {append, leap::many_attention_kernel<HD, 1, 4, false>, leap::many_merge_kernel<HD, 1>, 4};
-        if (nb == 2) return {append, leap::many_attention_kernel<HD, 2, 4, false>, leap::many_merge_kernel<HD, 2>, 4};
-        if (nb == 4) return {append, leap::many_attention_kernel<HD, 4, 4, false>, leap::many_merge_kernel<HD, 4>, 4};
-    }
-    return {};
+    if (nb == 1)
+        return q8 ? ManyKernels{append, leap::many_attention_kernel<HD, 1, 8, true>, leap::many_merge_kernel<HD, 16>, 8, 16}
+                  : ManyKernels{append, leap::many_attention_kernel<HD, 1, 4, false>, leap::many_merge_kernel<HD, 16>, 4, 16};
+    return {append, q8 ? leap::wide_attention_kernel<HD, true> : leap::wide_attention_kernel<HD, false>,
+            leap::many_merge_kernel<HD, leap::kWideRows>, leap::kWideWaves, leap::kWideRows};
 }
 
 template <int HD>

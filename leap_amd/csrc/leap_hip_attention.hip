@@ -799,28 +799,29 @@ ManyPlan many_plan(const leap_hip_attention *h, int n_seq, int n_tokens, int max
     const int group = h->group, n_kv = h->cfg.n_kv_heads, hd = h->cfg.head_dim;
     const long long rows_max = (long long)max_tokens * group;
     ManyPlan p{};
-    p.nb = rows_max <= 16 ? 1 : rows_max <= 32 ? 2 : 4;
+    p.nb = rows_max <= 16 ? 1 : 2;
     p.fn = pick_many(hd, p.nb, h->q8kv);
     p.fused = max_tokens <= leap::kTreeMax;
-    const int bm = 16 * p.nb, pass = p.fn.waves * leap::kTileKeys;
+    const bool wide = p.nb > 1;
+    const int bm = p.fn.rows, pass = wide ? leap::kTileKeys : p.fn.waves * leap::kTileKeys;
     p.slots = (int)std::min((long long)n_tokens * group / bm + n_seq, n_seq * ((rows_max + bm - 1) / bm));
     p.groups = (long long)p.slots * n_kv;
     const int total = max_pos + 1;
     const long long group_bytes = (long long)total * hd * (h->q8kv ? 2 : 8);
-    const int per_cu = p.nb == 4 || p.fn.waves == 8 || (hd == 128 && !h->q8kv) ? 1 : 2;
-    const bool few = p.groups < leap::kXcds && group_bytes < kSpreadBytes;  // on as many XCDs as groups
+    const int per_cu = wide || p.fn.waves == 8 || (hd == 128 && !h->q8kv) ? 1 : 2;
+    const bool few = !wide && p.groups < leap::kXcds && group_bytes < kSpreadBytes;  // on as many XCDs as groups
     const long long cus = few ? h->n_cu * p.groups / leap::kXcds : h->n_cu;
     const long long want = std::max<long long>(1, cus * per_cu);
     const int s = (int)std::max<long long>(1, std::min<long long>(leap::kManySplits, want / p.groups));
     (void)total_rows;
-    p.chunk = std::max(pass, round_up((total + s - 1) / s, pass));
+    p.chunk = std::max(wide ? 128 : pass, round_up((total + s - 1) / s, pass));
     p.splits = (total + p.chunk - 1) / p.chunk;
     while (p.splits > 1 && ((size_t)p.groups * p.splits * bm > kManyRecords || (size_t)p.groups > kManyCounters)) {
         p.chunk *= 2;
         p.splits = (total + p.chunk - 1) / p.chunk;
     }
-    p.spread = p.splits > 1 && (p.nb == 4 || (p.groups < leap::kXcds && !few));
-    p.wgs = p.spread ? p.groups * p.splits : (p.groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * p.splits;
+    p.spread = p.splits > 1 && (wide || (p.groups < leap::kXcds && !few));
+    p.wgs = wide || p.spread ? p.groups * p.splits : (p.groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * p.splits;
     return p;
 }
 
@@ -899,7 +900,7 @@ int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, c
         HIP_TRY(h, launch_k(p.fn.append, dim3((unsigned)((n_tokens + leap::kAppendWaves - 1) / leap::kAppendWaves)),
                             dim3(leap::kAppendWaves * leap::kWave), stream, a));
     HIP_TRY(h, launch_k(p.fn.attention, dim3((unsigned)p.wgs), dim3((unsigned)(p.fn.waves * leap::kWave)), stream, a));
-    if (p.spread) HIP_TRY(h, launch_k(p.fn.merge, dim3((unsigned)(p.groups * p.nb)), dim3(256), stream, a));
+    if (p.spread) HIP_TRY(h, launch_k(p.fn.merge, dim3((unsigned)(p.groups * (p.fn.rows / leap::kMergeRows))), dim3(256), stream, a));
     return 0;
 }
 

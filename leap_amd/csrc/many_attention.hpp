@@ -118,11 +118,10 @@ __device__ __forceinline__ Place find_place(const ManyArgs &a, int slot, int lan
 {
     Place p{-1, 0, 0, 0, 0};
     if (!a.begin) {
-        const int per = (a.group + BM - 1) / BM;
-        const int seq = slot / per;
-        if (seq >= a.n_seq) return p;
-        const int p0 = a.pos ? a.pos[seq] : a.pos_scalar;
-        return Place{seq, slot - seq * per, seq, p0 < 0 || p0 > a.max_pos ? -1 : 1, p0};
+        // (one tile a sequence: group <= 16)
+        if (slot >= a.n_seq) return p;
+        const int p0 = a.pos ? a.pos[slot] : a.pos_scalar;
+        return Place{slot, 0, slot, p0 < 0 || p0 > a.max_pos ? -1 : 1, p0};
     }
     int before = 0;
     bool stop = false;
@@ -260,18 +259,25 @@ __device__ __forceinline__ f32x4 mfma16(half8v a, half8v b, f32x4 c)
 // a = max(largest magnitude, 2^-100), scale a / 127, value rint(x (127 / a)),
 // in fp32.  With an infinity or a NaN the scale is NaN, which is what the
 // row then stands for.  Every lane returns its four values and the scale.
+__device__ __forceinline__ void quantize_scale(unsigned max_bits, float *r, float *scale)
+{
+    const float a = fmaxf(__uint_as_float(max_bits), kAmaxFloor);
+    *r = 127.0f / a;
+    *scale = finite_bits(max_bits) ? a / 127.0f : __uint_as_float(0x7fc00000u);
+}
+__device__ __forceinline__ int quantize4(float4 x, float r)
+{
+    return ((int)rintf(x.x * r) & 255) | (((int)rintf(x.y * r) & 255) << 8) | (((int)rintf(x.z * r) & 255) << 16) |
+           ((int)rintf(x.w * r) << 24);
+}
 template <int HD>
 __device__ __forceinline__ int quantize_row(float4 x, float *scale)
 {
     unsigned m = dpp_max16(max4_bits(0u, x));
     if (HD == 128) m = max(m, (unsigned)__shfl_xor((int)m, 16));
-    const bool fin = finite_bits(m);
-    const float a = fmaxf(__uint_as_float(m), kAmaxFloor);
-    const float r = 127.0f / a;
-    *scale = fin ? a / 127.0f : __uint_as_float(0x7fc00000u);
-    const int q = ((int)rintf(x.x * r) & 255) | (((int)rintf(x.y * r) & 255) << 8) |
-                  (((int)rintf(x.z * r) & 255) << 16) | ((int)rintf(x.w * r) << 24);
-    return fin ? q : 0;
+    float r;
+    quantize_scale(m, &r, scale);
+    return finite_bits(m) ? quantize4(x, r) : 0;
 }
 
 // Where token row r of a packed batch goes: its sequence (-1: none has it),
@@ -319,15 +325,14 @@ __device__ __forceinline__ void fill_nan(float *out, size_t first4, int n4, int 
 }
 
 // A head row of the cache, LR = HD / 4 lanes of a float4 each: element i of
-// the [kv_dim / 4] words of (seq, row).
+// the [kv_dim / 4] words of (seq, row).  8 bits: q and sc are what
+// quantize_row gives.
 template <int HD, bool Q8>
-__device__ __forceinline__ void store_row(const ManyArgs &a, int seq, int row, int i, float4 x, bool value)
+__device__ __forceinline__ void store_row(const ManyArgs &a, int seq, int row, int i, float4 x, int q, float sc, bool value)
 {
     constexpr int LR = HD / 4;
     const size_t to = (size_t)seq * a.seq_stride + (size_t)row * (a.n_kv_heads * HD);
     if constexpr (Q8) {
-        float sc;
-        const int q = quantize_row<HD>(x, &sc);
         reinterpret_cast<int *>((value ? a.v8 : a.k8) + to)[i] = q;
         if ((i & (LR - 1)) == 0)
             (value ? a.vs : a.ks)[(size_t)seq * a.scale_stride + (size_t)(i / LR) * a.scale_rows + row] = sc;
@@ -359,20 +364,37 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void many_append_kernel(ManyA
     const float4 *kn = reinterpret_cast<const float4 *>(a.k_new) + (size_t)r * words;
     const float4 *vn = reinterpret_cast<const float4 *>(a.v_new) + (size_t)r * words;
     for (int i = lane; i < words; i += kWave) {
-        const float4 k = kn[i], v = vn[i];
-        store_row<HD, Q8>(a, t.seq, t.row, i, rope4(k, turn), false);
-        store_row<HD, Q8>(a, t.seq, t.row, i, v, true);
+        const float4 k = rope4(kn[i], turn), v = vn[i];
+        float sk = 0.0f, sv = 0.0f;
+        const int qk = Q8 ? quantize_row<HD>(k, &sk) : 0, qv = Q8 ? quantize_row<HD>(v, &sv) : 0;
+        store_row<HD, Q8>(a, t.seq, t.row, i, k, qk, sk, false);
+        store_row<HD, Q8>(a, t.seq, t.row, i, v, qv, sv, true);
     }
 }
 
 // ---- the attention kernel -----------------------------------------------------
 
-template <int HD, int NB, int W>
+// The new rows of a chunk in a fused call, K and V by token, as the cache
+// holds them (rows 16 bytes apart in their banks).
+template <int HD, int BM, bool Q8>
+struct NewRows {
+    float x[2][BM][HD + 4];
+};
+template <int HD, int BM>
+struct NewRows<HD, BM, true> {
+    int x[2][BM][HD / 4 + 4];
+    float scale[2][BM];
+};
+
+template <int HD, int NB, int W, bool Q8>
 struct ManyShared {
     static constexpr int BM = 16 * NB;
     static constexpr int kOStride = HD + 4;  // floats between rows of a wave's output (16 rows on 16 banks' groups)
     union {
-        half8v q[NB][HD / 32][2][kWave];     // Q's operands: high and low halves
+        struct {
+            half8v q[NB][HD / 32][2][kWave]; // Q's operands: high and low halves
+            NewRows<HD, BM, Q8> fresh;
+        };
         float o[W][BM][kOStride];            // the waves' outputs
         struct {
             float w[16][kManySplits + 1];    // the merge: weights of a row's records
@@ -388,18 +410,18 @@ struct ManyShared {
     int last;
 };
 
-// The sum of a tile's records, for its 16 rows from row block rb on, by T >=
-// 256 threads: record s of row i counts 2^(lse_s - max lse) / their sum.
-template <int HD, int BM, int T, typename Merge>
+// The sum of a tile's records, for R rows from R rb on, by T >= 256 threads:
+// record s of row i counts 2^(lse_s - max lse) / their sum.
+template <int HD, int BM, int R, int T, typename Merge>
 __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi, int n_split, const Place &p, int kvh, int rb,
                                            int tid)
 {
     constexpr int LR = HD / 4;
-    const int rows = p.n * a.group, r0 = p.tile * BM + 16 * rb;
+    const int rows = p.n * a.group, r0 = p.tile * BM + R * rb;
     if (r0 >= rows) return;
-    const size_t rec0 = (size_t)gi * a.splits * BM + 16 * rb;
+    const size_t rec0 = (size_t)gi * a.splits * BM + R * rb;
     const float ninf = -__builtin_inff();
-    if (T == 256 || tid < 256) {
+    if (T == 16 * R || tid < 16 * R) {
         const int row = tid >> 4, l = tid & 15;
         const auto lr = make_rsrc(a.ws_lse + rec0, (uint32_t)n_split * BM * 4u);
         float x[kManySplits / 16], top = ninf;
@@ -434,7 +456,7 @@ __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi,
     __syncthreads();
     // the rows' float4 words, `items` of them; with fewer than threads the
     // records are dealt to `parts` threads a word
-    const int items = min(16, rows - r0) * LR;
+    const int items = min(R, rows - r0) * LR;
     int parts = 1;
     while (2 * parts * items <= T) parts *= 2;
     const auto wr = make_rsrc(a.ws_o + rec0 * HD, (uint32_t)n_split * BM * HD * 4u);
@@ -473,7 +495,7 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
 {
     constexpr int BM = 16 * NB, KS = HD / 32, VB = HD / 16, LR = HD / 4;
     constexpr int kThreads = W * kWave, kPassKeys = W * kTileKeys;
-    __shared__ ManyShared<HD, NB, W> sh;
+    __shared__ ManyShared<HD, NB, W, Q8> sh;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, g = lane >> 4;
 
@@ -523,12 +545,13 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     const int kv_dim = a.n_kv_heads * HD;
     const uint32_t row_bytes = (uint32_t)kv_dim * (Q8 ? 1 : 4), head_off = (uint32_t)kvh * HD * (Q8 ? 1 : 4);
     const size_t base = (size_t)p.seq * a.seq_stride;
-    const uint32_t bytes = (uint32_t)c1 * row_bytes;  // (rows from c1 on read as zero)
+    const int old1 = a.fused ? min(c1, p.p0) : c1;         // cached rows of the chunk: up to here
+    const uint32_t bytes = (uint32_t)old1 * row_bytes;     // (rows from there on read as zero)
     const auto kr = Q8 ? make_rsrc(a.k8 + base, bytes) : make_rsrc(a.k_cache + base, bytes);
     const auto vr = Q8 ? make_rsrc(a.v8 + base, bytes) : make_rsrc(a.v_cache + base, bytes);
     const size_t sbase = (size_t)p.seq * a.scale_stride + (size_t)kvh * a.scale_rows;
-    const auto ksr = make_rsrc(Q8 ? a.ks + sbase : nullptr, Q8 ? (uint32_t)c1 * 4u : 0u);
-    const auto vsr = make_rsrc(Q8 ? a.vs + sbase : nullptr, Q8 ? (uint32_t)c1 * 4u : 0u);
+    const auto ksr = make_rsrc(Q8 ? a.ks + sbase : nullptr, Q8 ? (uint32_t)old1 * 4u : 0u);
+    const auto vsr = make_rsrc(Q8 ? a.vs + sbase : nullptr, Q8 ? (uint32_t)old1 * 4u : 0u);
 
     constexpr int KR = Q8 ? HD / 64 : HD / 16, VR = Q8 ? 1 : HD / 64;
     float4 kraw[2][KR], vraw[8][VR];
@@ -562,14 +585,57 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
             for (int b = 0; b < 2; b++) vsc[b] = buf_load4(vsr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
     };
 
+    // The chunk's new rows: tokens [t0, t0 + n_new).
+    const int t0 = a.fused ? max(c0 - p.p0, 0) : 0, n_new = a.fused ? max(min(c1 - p.p0, p.n) - t0, 0) : 0;
+    auto is_new = [&](int j) { return (unsigned)(j - t0) < (unsigned)n_new; };
+    // The rows of a tile that this call brings, in place of what was read.
+    auto fresh_k = [&](int key0) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int j = key0 + 16 * b + m - p.p0;
+            if (is_new(j)) {
+#pragma unroll
+                for (int i = 0; i < KR; i++)
+                    kraw[b][i] = *reinterpret_cast<const float4 *>(&sh.fresh.x[0][j][16 * i + 4 * g]);
+            }
+            if constexpr (Q8)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = key0 + 16 * b + 4 * g + i - p.p0;
+                    if (is_new(t)) {
+                        (&ksc[b].x)[i] = sh.fresh.scale[0][t];
+                        (&vsc[b].x)[i] = sh.fresh.scale[1][t];
+                    }
+                }
+        }
+    };
+    auto fresh_v = [&](int key0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int t = key0 + 16 * (j >> 2) + 4 * g + (j & 3) - p.p0;
+            if (is_new(t)) {
+                if constexpr (Q8) {
+                    if constexpr (HD == 128)
+                        vraw8[j] = *reinterpret_cast<const float2 *>(&sh.fresh.x[1][t][2 * m]);
+                    else
+                        vraw8[j].x = __int_as_float(sh.fresh.x[1][t][m]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VR; i++)
+                        vraw[j][i] = *reinterpret_cast<const float4 *>(&sh.fresh.x[1][t][64 * i + 4 * m]);
+                }
+            }
+        }
+    };
+
     // ---- Q: rotated, split, into LDS as the products' B operand ----
     // element (s, g, j) of a row: the order of the contraction over dims,
     // such that a K load instruction takes whole 64-byte pieces of its rows
     auto dim_of = [&](int s, int h) {
         return Q8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h : 32 * s + 16 * h + 4 * g;
     };
-    // The loads go out in the order they are needed: Q's, then the first
-    // tile's rows (where this call does not store any of them).
+    // The loads go out in the order they are needed: Q's, the new rows', then
+    // the first tile's.
     float4 x[KS][2];
     auto q_row = [&](int nb, int *j) {
         const int r = min(r0 + 16 * nb + m, rows - 1);
@@ -584,10 +650,18 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
 #pragma unroll
             for (int h = 0; h < 2; h++) x[s][h] = *reinterpret_cast<const float4 *>(src + dim_of(s, h));
     };
+    // New row i of K, then of V, LR threads each.
+    const int lr = tid & (LR - 1);
+    auto new_row = [&](int i) {
+        const bool value = i >= n_new;
+        const int j = t0 + (value ? i - n_new : i);
+        return reinterpret_cast<const float4 *>(value ? a.v_new : a.k_new)[((size_t)(p.first + j) * a.n_kv_heads + kvh) * LR + lr];
+    };
     int key0 = c0 + wave * kTileKeys;
-    const bool early = key0 < c1 && (!a.fused || key0 + kTileKeys <= p.p0);
     if (wave < NB) load_q(wave);
-    if (early) {
+    float4 y = make_float4(0, 0, 0, 0);
+    if (tid / LR < 2 * n_new) y = new_row(tid / LR);
+    if (key0 < c1) {
         load_k(key0);
         load_v(key0);
     }
@@ -601,20 +675,24 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     // position of token j (and of a bad node: as if it hung on the cached rows)
     auto place_of = [&](int j) { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
 
-    // ---- the new rows of this chunk into the cache ----
-    const int t0 = a.fused ? max(c0 - p.p0, 0) : 0, t1 = a.fused ? min(c1 - p.p0, p.n) : 0;
-    if (t0 < t1) {
-        // (every tile and chunk that reads a row stores it first, the same
-        // bytes each; K rows, then V rows, LR threads each)
-        for (int i = tid / LR; i < 2 * (t1 - t0); i += kThreads / LR) {
-            const bool value = i >= t1 - t0;
-            const int j = t0 + (value ? i - (t1 - t0) : i), w = kvh * LR + (tid & (LR - 1));
-            const float4 *src = reinterpret_cast<const float4 *>(value ? a.v_new : a.k_new);
-            float4 y = src[(size_t)(p.first + j) * (a.n_kv_heads * LR) + w];
-            if (!value) y = rope4(y, a.rope[(size_t)place_of(j) * LR + (tid & (LR - 1))]);
-            store_row<HD, Q8>(a, p.seq, p.p0 + j, w, y, value);
+    // ---- the new rows of this chunk into LDS, and (by the last tile, which
+    // sees them all) into the cache ----
+    const bool stores = r0 + BM >= rows;
+    for (int i = tid / LR; i < 2 * n_new; i += kThreads / LR) {
+        if (i != tid / LR) y = new_row(i);
+        const bool value = i >= n_new;
+        const int j = t0 + (value ? i - n_new : i);
+        if (!value) y = rope4(y, a.rope[(size_t)place_of(j) * LR + lr]);
+        int q = 0;
+        float sc = 0.0f;
+        if constexpr (Q8) {
+            q = quantize_row<HD>(y, &sc);
+            sh.fresh.x[value][j][lr] = q;
+            if (lr == 0) sh.fresh.scale[value][j] = sc;
+        } else {
+            *reinterpret_cast<float4 *>(&sh.fresh.x[value][j][4 * lr]) = y;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (stores) store_row<HD, Q8>(a, p.seq, p.p0 + j, kvh * LR + lr, y, q, sc, value);
     }
     for (int nb = wave; nb < NB; nb += W) {
         if (nb != wave) load_q(nb);
@@ -645,7 +723,6 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
         }
     }
     __syncthreads();
-    if (t0 < t1) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (L1 may hold parts of the new rows' lines)
     half8v qh[NB][KS], ql[NB][KS];  // (NB == 1: in registers; else read from LDS as they are used)
     if constexpr (NB == 1) {
 #pragma unroll
@@ -668,13 +745,11 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     }
     int erun = -100;  // O's unit is 2^(erun - 13)
 
-    if (!early && key0 < c1) {
-        load_k(key0);
-        load_v(key0);
-    }
     for (; key0 < c1; key0 += kPassKeys) {
         // ---- scores ----
         if constexpr (NB > 1) asm volatile("" ::: "memory");  // (Q's operands are read from LDS in every pass)
+        const bool fresh = n_new > 0 && key0 + kTileKeys > p.p0;
+        if (fresh) fresh_k(key0);
         unsigned badkeys = 0;  // positions of the tile whose key or value is not finite (bit: position - key0)
         f32x4 sc[2][NB];
 #pragma unroll
@@ -740,14 +815,15 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
                 }
             }
         float4 kscv[2], vscv[2];
-        if constexpr (Q8) {
-            // a row's two scales: NaN in either marks it
+        if constexpr (Q8)
 #pragma unroll
             for (int b = 0; b < 2; b++) {
+                // a row's two scales: NaN in either marks it
                 vscv[b] = vsc[b];
                 kscv[b] = make_float4(ksc[b].x + 0.0f * vsc[b].x, ksc[b].y + 0.0f * vsc[b].y,
                                       ksc[b].z + 0.0f * vsc[b].z, ksc[b].w + 0.0f * vsc[b].w);
             }
+        if constexpr (Q8) {
             unsigned mv = 0;
 #pragma unroll
             for (int b = 0; b < 2; b++) {
@@ -763,6 +839,7 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
         }
         if constexpr (NB >= 2) __builtin_amdgcn_sched_barrier(0);
         if constexpr (NB <= 2) load_k(key0 + kPassKeys);
+        if (fresh) fresh_v(key0);
         if constexpr (!Q8) {
             unsigned mv = 0;
 #pragma unroll
@@ -968,19 +1045,23 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     __syncthreads();
     if (!sh.last) return;
     for (int rb = 0; rb < NB; rb++) {
-        merge_rows<HD, BM, kThreads>(a, sh.merge, gi, n_split, p, kvh, rb, tid);
+        merge_rows<HD, BM, 16, kThreads>(a, sh.merge, gi, n_split, p, kvh, rb, tid);
         if (NB > 1) __syncthreads();
     }
 }
 
-// The records of a spread launch's tiles added up: a workgroup per 16 rows.
-template <int HD, int NB>
+// The records of a spread launch's tiles of BM rows added up, kMergeRows rows
+// a workgroup.
+constexpr int kMergeRows = 4;
+template <int HD, int BM>
 __global__ __launch_bounds__(256) void many_merge_kernel(ManyArgs a)
 {
-    constexpr int BM = 16 * NB;
-    __shared__ decltype(ManyShared<HD, NB, 4>::merge) sh;
+    __shared__ struct {
+        float w[kMergeRows][kManySplits + 1];
+        float4 part[256];
+    } sh;
     const int tid = threadIdx.x;
-    const int gi = blockIdx.x / NB, rb = blockIdx.x - gi * NB;
+    const int gi = blockIdx.x / (BM / kMergeRows), rb = blockIdx.x % (BM / kMergeRows);
     const int slot = (int)fast_div((uint32_t)gi, a.by_kv_heads);
     const int kvh = gi - slot * a.n_kv_heads;
     const Place p = find_place<BM>(a, slot, tid & (kWave - 1));
@@ -988,7 +1069,7 @@ __global__ __launch_bounds__(256) void many_merge_kernel(ManyArgs a)
     const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(p.tile * BM + BM - 1), a.by_group));
     const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
     const int n_split = (kv_end + a.chunk - 1) / a.chunk;
-    if (n_split > 1) merge_rows<HD, BM, 256>(a, sh, gi, n_split, p, kvh, rb, tid);
+    if (n_split > 1) merge_rows<HD, BM, kMergeRows, 256>(a, sh, gi, n_split, p, kvh, rb, tid);
 }
 
 // ---- rows of a cache, moved ---------------------------------------------------

@@ -1,0 +1,576 @@
+// Attention of many rows over a cache: prompts, and trees of more than 16
+// (token, q head) rows a KV head.  The rows, products, splits into fp16 halves
+// and records are those of many_attention.hpp; here a workgroup of eight
+// waves takes a tile of 256 rows, 32 a wave, and the positions of its chunk
+// in tiles of 32, split into fp16 halves once, in LDS, for all of them.
+//
+// Per wave and tile of 32 positions at head_dim 128: 48 32x32x16 MFMAs (three
+// products of S^T = K Q^T and of O^T = V^T P^T), 1536 cycles of the matrix
+// core, and about 300 vector instructions (scaling, maximum, 16 exponentials,
+// the split of P, a share of the next tile's split), 1200 cycles.  The two
+// waves of a SIMD do these in turn: waves 0-3 are in the matrix phase (the
+// scores of tile i + 1, the weighted values of tile i) while waves 4-7 are in
+// the vector phase, a barrier between the half-steps.
+//
+// Half-step h of waves 0-3: scores of tile 0 at h = 0, vector phase i at
+// 2 i + 1, matrix phase i at 2 i + 2; waves 4-7 one half-step later.  Waves
+// 4-7 bring K: tile i + 2 in vector phase i (h = 2 i + 2), read from h = 2 (i
+// + 2) on, when the buffer's last tile i was read last at h = 2 i + 1: two
+// buffers.  Waves 0-3 bring V: tile i + 1 in vector phase i (h = 2 i + 1),
+// whose quads' exponents the vector phase i + 1 needs, read last at h = 2 i +
+// 5: three buffers.
+//
+// Scales: a tile's positions in quads of four, K's and V's exponents by quad.
+// K's multiply the scores, V's go into the probabilities, relative to the
+// largest exponent so far (vrun), O's unit.  8-bit caches: K's scales by
+// position likewise, V's too.
+//
+// The running maximum is a reference that moves only when a score exceeds it
+// by more than 2^8 (then O and the sum are rescaled): probabilities are
+// 2^(s - ref + 7) <= 2^15.
+//
+// A call of few tokens (fused) has its new rows rotated, quantised and stored
+// here, ahead of the first tile.
+#pragma once
+
+#include "many_attention.hpp"
+
+namespace leap {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kWideWaves = 8;
+constexpr int kWideThreads = kWideWaves * kWave;
+constexpr int kWideRows = 32 * kWideWaves;
+constexpr float kWideBias = 7.0f;
+
+template <int HD, bool Q8>
+struct WideShared {
+    static constexpr int P = Q8 ? 1 : 2;  // halves: high (and low)
+    half8v k[2][P][32 * HD / 8];          // [position][dims], 16-byte pieces swizzled by position
+    half8v v[3][P][HD * 32 / 8];          // [dim][positions], pieces swizzled by dim
+    // fp32: by quad, [lane half][4]; 8 bits: by position, [lane half][16]
+    float kfac[4][2][Q8 ? 16 : 4], vfac[4][2][Q8 ? 16 : 4];
+    int bad[4][kWideWaves];               // positions that are not finite, by the wave that brought them
+    uint64_t sees[kTreeMax];
+    // the low halves of Q of each wave's last kQLow steps, for which there are no registers
+    static constexpr int kQLow = HD == 128 ? (Q8 ? 4 : 6) : 0;
+    half8v ql[kWideWaves][kQLow ? kQLow : 1][kWave];
+};
+
+__device__ __forceinline__ f32x16 mfma32(half8v a, half8v b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// max / sum of a lane's value and the one of the lane 32 away
+__device__ __forceinline__ float half_max(float x)
+{
+    float y = x;
+    asm("" : "+v"(y));  // (two registers: the swap of one with itself would be folded)
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int HD, bool Q8>
+__global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArgs a)
+{
+    constexpr int BM = kWideRows, KS = HD / 16, VB = HD / 32, LR = HD / 4;
+    constexpr int C = HD / 8;  // 16-byte pieces of a K row
+    __shared__ WideShared<HD, Q8> sh;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int n = lane & 31, g = lane >> 5;
+    const bool brings_v = wave < 4;
+    const int w = wave & 3;
+
+    // the workgroup's tile, KV head and chunk: neighbouring ids go to other XCDs
+    const int n_groups = a.slots * a.n_kv_heads;
+    int group_i, split;
+    if (a.spread) {
+        split = blockIdx.x / n_groups;
+        group_i = blockIdx.x - split * n_groups;
+    } else {
+        split = 0;
+        group_i = blockIdx.x;
+    }
+    if (a.fused && a.begin && blockIdx.x == 0) {
+        bool stop = false, any = false;
+        for (int base = 0; base < a.n_seq && !stop && !any; base += kWave)
+            any = __builtin_amdgcn_ballot_w64(seq_lane(a, base, lane, &stop).n < 0) != 0;
+        if (any)
+            for (int r = wave; r < a.n_tokens; r += kWideWaves) {
+                const TokenPlace t = find_token(a, r, lane);
+                if (t.seq >= 0 && t.skip)
+                    fill_nan<HD>(a.out, (size_t)r * a.n_heads * LR, a.n_heads * LR, lane, kWave);
+            }
+    }
+    const int slot = (int)fast_div((uint32_t)group_i, a.by_kv_heads);
+    const int kvh = group_i - slot * a.n_kv_heads;
+    const Place p = find_place<BM>(a, slot, lane);
+    if (p.seq < 0) return;
+    const int rows = p.n * a.group, r0 = p.tile * BM;
+    const int j0 = (int)fast_div((uint32_t)r0, a.by_group);
+    const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(r0 + BM - 1), a.by_group));
+    const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
+    const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
+    if (c0 >= kv_end) return;
+    const int n_tiles = (c1 - c0 + kTileKeys - 1) / kTileKeys;
+    auto tile_key = [&](int i) { return c0 + kTileKeys * i; };
+
+    if (a.parent) {
+        if (wave == kWideWaves - 1) {
+            const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
+            sh.sees[lane] = t.bad ? 0 : t.sees;
+        }
+        __syncthreads();
+    }
+    auto place_of = [&](int j) { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
+
+    // ---- the cache's rows ----
+    const int kv_dim = a.n_kv_heads * HD;
+    const uint32_t row_bytes = (uint32_t)kv_dim * (Q8 ? 1 : 4), head_off = (uint32_t)kvh * HD * (Q8 ? 1 : 4);
+    const size_t base = (size_t)p.seq * a.seq_stride;
+    const uint32_t bytes = (uint32_t)c1 * row_bytes;  // (rows from there on read as zero)
+    const auto rows_r = Q8 ? make_rsrc((brings_v ? a.v8 : a.k8) + base, bytes)
+                           : make_rsrc((brings_v ? a.v_cache : a.k_cache) + base, bytes);
+    const size_t sbase = (size_t)p.seq * a.scale_stride + (size_t)kvh * a.scale_rows;
+    const auto ksr = make_rsrc(Q8 ? a.ks + sbase : nullptr, Q8 ? (uint32_t)c1 * 4u : 0u);
+    const auto vsr = make_rsrc(Q8 ? a.vs + sbase : nullptr, Q8 ? (uint32_t)c1 * 4u : 0u);
+    // A wave's share of a tile, as it comes from memory.
+    //   K, fp32: quads w and w + 4; lane: position lane / 16 of each, C / 2 dims
+    //   V, fp32: the same quads; lane: dims lane (and lane + 64), 4 positions
+    //   K, 8 bits: positions 8 w + lane / 8, HD / 8 dims (bytes)
+    //   V, 8 bits: quad w + 4 (lane / 32) (head_dim 64: 4 w + lane / 16, w < 2), dims 4 (lane % (HD / 4)), 4 positions
+    constexpr int RAW = Q8 ? 4 : HD / 8;
+    float raw[RAW], sck = 0.0f, scv = 0.0f;
+    float sv4[4];
+    const int v8_quad = HD == 128 ? w + 4 * (lane >> 5) : 4 * w + (lane >> 4), v8_dim = 4 * (lane & (LR - 1));
+    // (the lane's part of an offset into a tile; a tile's rows add a uniform one)
+    const uint32_t lane_off = head_off + (Q8 ? (brings_v ? 4u * v8_quad * row_bytes + v8_dim : (8u * w + (lane >> 3)) * row_bytes + (HD / 8) * (lane & 7))
+                                             : (brings_v ? 4u * lane : (lane >> 4) * row_bytes + (HD / 4) * (lane & 15)));
+    auto load_tile = [&](int i) {
+        if (i >= n_tiles) return;
+        const uint32_t at = (uint32_t)tile_key(i) * row_bytes + lane_off;
+        if constexpr (!Q8) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const uint32_t quad = 4u * (w + 4 * t) * row_bytes;
+                if (!brings_v) {
+#pragma unroll
+                    for (int u = 0; u < HD / 64; u++) {
+                        const float4 x = buf_load4(rows_r, at + quad + 16 * u);
+                        raw[(HD / 16) * t + 4 * u] = x.x;
+                        raw[(HD / 16) * t + 4 * u + 1] = x.y;
+                        raw[(HD / 16) * t + 4 * u + 2] = x.z;
+                        raw[(HD / 16) * t + 4 * u + 3] = x.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int u = 0; u < HD / 64; u++)
+                            raw[(HD / 16) * t + 4 * u + j] = __int_as_float(
+                                __builtin_amdgcn_raw_buffer_load_b32(rows_r, (int)(at + (quad + j * row_bytes) + 256 * u), 0, 0));
+                }
+            }
+        } else if (!brings_v) {
+            if constexpr (HD == 128) {
+                const float4 x = buf_load4(rows_r, at);
+                raw[0] = x.x;
+                raw[1] = x.y;
+                raw[2] = x.z;
+                raw[3] = x.w;
+            } else {
+                const float2 x = buf_load2(rows_r, at);
+                raw[0] = x.x;
+                raw[1] = x.y;
+            }
+            const int row4 = 4 * (tile_key(i) + 8 * w + (lane >> 3));
+            sck = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksr, row4, 0, 0));
+            scv = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsr, row4, 0, 0));
+        } else if (HD == 128 || w < 2) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                raw[j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_r, (int)(at + j * row_bytes), 0, 0));
+            const float4 x = buf_load4(vsr, 4u * (tile_key(i) + 4 * v8_quad));
+            sv4[0] = x.x;
+            sv4[1] = x.y;
+            sv4[2] = x.z;
+            sv4[3] = x.w;
+        }
+    };
+    // That share into LDS, split, with its factors.
+    auto v_piece = [&](int d, int piece) { return d * 4 + (piece ^ (((d >> 1) ^ (d >> 3)) & 3)); };
+    auto stage_tile = [&](int i) {
+        if (i >= n_tiles) return;
+        int badbits = 0;
+        if constexpr (!Q8) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                constexpr int N = HD / 16;
+                float *x = raw + N * t;
+                unsigned mx = 0;
+#pragma unroll
+                for (int e = 0; e < N; e++) mx = max(mx, abs_bits(x[e]));
+                unsigned wx = wave_max_bits(mx);
+                const int quad = w + 4 * t;
+                if (!finite_bits(wx)) {
+                    // zeros in their place, and their positions noted
+                    mx = 0;
+                    int bits = 0;
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (!finite_bits(abs_bits(x[e]))) {
+                            x[e] = 0.0f;
+                            bits |= brings_v ? 1 << (e & 3) : 1 << (lane >> 4);
+                        } else {
+                            mx = max(mx, abs_bits(x[e]));
+                        }
+#pragma unroll
+                    for (int b = 0; b < 4; b++)
+                        if (__builtin_amdgcn_ballot_w64((bits >> b) & 1)) badbits |= 1 << (4 * t + b);
+                    wx = wave_max_bits(mx);
+                }
+                const int e = tile_exp(wx);
+                const float sc = exp2_int(13 - e);
+                if (lane == 0) (brings_v ? sh.vfac : sh.kfac)[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
+                half2v h[N / 2], l[N / 2];
+#pragma unroll
+                for (int e2 = 0; e2 < N / 2; e2++) split2(x[2 * e2] * sc, x[2 * e2 + 1] * sc, h[e2], l[e2]);
+                if (!brings_v) {
+                    const int pos = 4 * quad + (lane >> 4);
+                    if constexpr (HD == 128) {
+                        const int at = pos * C + ((lane & 15) ^ (pos & (C - 1)));
+                        Half8 x8;
+#pragma unroll
+                        for (int u = 0; u < 4; u++) x8.h[u] = h[u];
+                        sh.k[i & 1][0][at] = x8.v;
+#pragma unroll
+                        for (int u = 0; u < 4; u++) x8.h[u] = l[u];
+                        sh.k[i & 1][1][at] = x8.v;
+                    } else {
+                        const int at = pos * C + (((lane & 15) >> 1) ^ (pos & (C - 1)));
+                        half2v *hp = reinterpret_cast<half2v *>(&sh.k[i & 1][0][at]) + 2 * (lane & 1);
+                        half2v *lp = reinterpret_cast<half2v *>(&sh.k[i & 1][1][at]) + 2 * (lane & 1);
+                        *reinterpret_cast<u32x2 *>(hp) = u32x2{__builtin_bit_cast(unsigned, h[0]), __builtin_bit_cast(unsigned, h[1])};
+                        *reinterpret_cast<u32x2 *>(lp) = u32x2{__builtin_bit_cast(unsigned, l[0]), __builtin_bit_cast(unsigned, l[1])};
+                    }
+                } else {
+                    const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
+#pragma unroll
+                    for (int u = 0; u < HD / 64; u++) {
+                        const int d = lane + 64 * u, at = v_piece(d, piece);
+                        u32x2 *hp = reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][at]) + half;
+                        u32x2 *lp = reinterpret_cast<u32x2 *>(&sh.v[i % 3][1][at]) + half;
+                        *hp = u32x2{__builtin_bit_cast(unsigned, h[2 * u]), __builtin_bit_cast(unsigned, h[2 * u + 1])};
+                        *lp = u32x2{__builtin_bit_cast(unsigned, l[2 * u]), __builtin_bit_cast(unsigned, l[2 * u + 1])};
+                    }
+                }
+            }
+        } else if (!brings_v) {
+            int pos = 8 * w + (lane >> 3);
+            asm volatile("" : "+v"(pos));
+            if constexpr (HD == 128) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+                    sh.k[i & 1][0][pos * C + ((2 * (lane & 7) + u) ^ (pos & (C - 1)))] =
+                        bytes_half8(__float_as_uint(raw[2 * u]), __float_as_uint(raw[2 * u + 1]));
+            } else {
+                sh.k[i & 1][0][pos * C + ((lane & 7) ^ (pos & (C - 1)))] =
+                    bytes_half8(__float_as_uint(raw[0]), __float_as_uint(raw[1]));
+            }
+            if ((lane & 7) == 0) sh.kfac[i & 3][(pos >> 2) & 1][4 * (pos >> 3) + (pos & 3)] = sck + 0.0f * scv;
+        } else if (HD == 128 || w < 2) {
+            int quad = v8_quad, d0 = v8_dim;
+            asm volatile("" : "+v"(quad), "+v"(d0));  // (addresses formed anew, as below)
+            const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
+            unsigned x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = __float_as_uint(raw[j]) ^ 0x80808080u;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const unsigned sel = 0x0c000c00u | (unsigned)(4 + c) << 16 | (unsigned)c;
+                const half2v p0 = bytes_half(__builtin_amdgcn_perm(x[1], x[0], sel) | 0x64006400u);
+                const half2v p1 = bytes_half(__builtin_amdgcn_perm(x[3], x[2], sel) | 0x64006400u);
+                const int d = d0 + c;
+                *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][v_piece(d, piece)]) + half) =
+                    u32x2{__builtin_bit_cast(unsigned, p0), __builtin_bit_cast(unsigned, p1)};
+            }
+            if ((lane & (LR - 1)) == 0)
+#pragma unroll
+                for (int j = 0; j < 4; j++) sh.vfac[i & 3][quad & 1][4 * (quad >> 1) + j] = sv4[j];
+        }
+        if (!Q8 && lane == 0) sh.bad[i & 3][wave] = badbits;
+    };
+
+    // ---- Q: 32 rows a wave, in registers as the products' B operand ----
+    // K's first two tiles and V's first are on their way meanwhile, if this
+    // call does not bring rows of them; the chunk's new rows go to the cache
+    // first (by every workgroup that reads them, the same bytes).
+    const int t0 = a.fused ? max(c0 - p.p0, 0) : 0, n_new = a.fused ? max(min(c1 - p.p0, p.n) - t0, 0) : 0;
+    const bool early = n_new == 0 || c0 + 2 * kTileKeys <= p.p0;
+    if (early) load_tile(0);
+    for (int i = tid / LR; i < 2 * n_new; i += kWideThreads / LR) {
+        const bool value = i >= n_new;
+        const int j = t0 + (value ? i - n_new : i), lr = tid & (LR - 1);
+        float4 y = reinterpret_cast<const float4 *>(value ? a.v_new : a.k_new)[((size_t)(p.first + j) * a.n_kv_heads + kvh) * LR + lr];
+        if (!value) y = rope4(y, a.rope[(size_t)place_of(j) * LR + lr]);
+        float f = 0.0f;
+        const int q = Q8 ? quantize_row<HD>(y, &f) : 0;
+        store_row<HD, Q8>(a, p.seq, p.p0 + j, kvh * LR + lr, y, q, f, value);
+    }
+    constexpr int QL = WideShared<HD, Q8>::kQLow, QR = KS - QL;  // low halves of Q in LDS, in registers
+    half8v qh[KS], ql[QR];
+    float qf;
+    // a lane's row, its token and its offset in q and out (formed anew where they are used, for the registers' sake)
+    auto my_row = [&](int *r, int *j) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        *r = min(r0 + 32 * wave + (l & 31), rows - 1);
+        *j = (int)fast_div((uint32_t)*r, a.by_group);
+        return ((size_t)(p.first + *j) * a.n_heads + kvh * a.group + *r - *j * a.group) * HD;
+    };
+    {
+        int my_r, my_j;
+        const float *src = a.q + my_row(&my_r, &my_j);
+        const int at = place_of(my_j);
+        bool good = !a.parent || sh.sees[my_j] != 0;
+        float4 x[KS][2];
+        unsigned mx = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int d = 16 * s + 8 * g + 4 * h;
+                x[s][h] = rope4(*reinterpret_cast<const float4 *>(src + d), a.rope[((size_t)at * HD + d) / 4]);
+                mx = max4_bits(mx, x[s][h]);
+            }
+        mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
+        good = good && finite_bits(mx);
+        const int e = tile_exp(good ? mx : 0u);
+        qf = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
+        const float sc = good ? exp2_int(13 - e) : 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            half8v low;
+            split8(x[s][0], x[s][1], sc, qh[s], low);
+            if (s < QR)
+                ql[s] = low;
+            else
+                sh.ql[wave][s - QR][lane] = low;
+        }
+    }
+    if (n_new) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (L1 may hold parts of the new rows' lines)
+    }
+    if (!early) load_tile(0);
+    stage_tile(0);
+    load_tile(1);
+    if (!brings_v) {
+        stage_tile(1);
+        load_tile(2);
+    }
+    const bool idle = r0 + 32 * wave >= rows;  // no rows: this wave only brings its share
+
+    f32x16 o[VB], s;
+#pragma unroll
+    for (int v = 0; v < VB; v++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[v][r] = 0.0f;
+    half8v ph[2], pl[2];
+    float ref = -__builtin_inff(), sum = 0.0f, vrun = exp2_int(-113);
+
+    // (a lane's pieces: K piece 2 t + g of position n, V piece 2 u + g of dim
+    // 32 v + n; the swizzles leave t and u as an exclusive or on the first's
+    // index.  Formed anew in each phase: kept, they would take 16 registers.)
+    const int k_first = n * C + (g ^ (n & (C - 1))), v_first = v_piece(n, g);
+    auto clear_scores = [&] {
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+    };
+    auto scores = [&](int i) {
+        clear_scores();
+        const half8v *k = sh.k[i & 1][0];
+#pragma unroll
+        for (int t = 0; t < KS; t++) {
+            const int at = k_first ^ (2 * t);
+            const half8v kh = k[at];
+            s = mfma32(kh, t < QR ? ql[t < QR ? t : 0] : sh.ql[wave][t < QR ? 0 : t - QR][lane], s);
+            if constexpr (!Q8) s = mfma32(k[at + 32 * C], qh[t], s);
+            s = mfma32(kh, qh[t], s);
+        }
+    };
+    auto values = [&](int i) {
+        const half8v *x = sh.v[i % 3][0];
+#pragma unroll
+        for (int t = 0; t < KS; t++) {
+            const int u = t / VB, v = t % VB, at = (v_first ^ (2 * u)) + 128 * v;
+            const half8v vh = x[at];
+            o[v] = mfma32(vh, pl[u], o[v]);
+            if constexpr (!Q8) o[v] = mfma32(x[at + 4 * HD], ph[u], o[v]);
+            o[v] = mfma32(vh, ph[u], o[v]);
+        }
+    };
+    // Both, in turns: a product that adds to the one before it would wait for
+    // it (two accumulators of 32x32x16 keep the matrix core fed, one does not).
+    auto matrix = [&](int i) {
+        clear_scores();
+        int kf = k_first, vf = v_first;
+        asm volatile("" : "+v"(kf), "+v"(vf));
+        const half8v *k = sh.k[(i + 1) & 1][0], *x = sh.v[i % 3][0];
+        half8v kh[2], kl[2], vh[2], vl[2], low[2];  // a step's operands, read one step ahead
+        auto read = [&](int t) {
+            const int ka = kf ^ (2 * t), va = (vf ^ (2 * (t / VB))) + 128 * (t % VB);
+            kh[t & 1] = k[ka];
+            vh[t & 1] = x[va];
+            low[t & 1] = t < QR ? ql[t < QR ? t : 0] : sh.ql[wave][t < QR ? 0 : t - QR][lane];
+            if constexpr (!Q8) {
+                kl[t & 1] = k[ka + 32 * C];
+                vl[t & 1] = x[va + 4 * HD];
+            }
+        };
+        read(0);
+#pragma unroll
+        for (int t = 0; t < KS; t++) {
+            const int u = t / VB, v = t % VB, e = t & 1;
+            if (t + 1 < KS) read(t + 1);
+            s = mfma32(kh[e], low[e], s);
+            o[v] = mfma32(vh[e], pl[u], o[v]);
+            if constexpr (!Q8) {
+                s = mfma32(kl[e], qh[t], s);
+                o[v] = mfma32(vl[e], ph[u], o[v]);
+            }
+            s = mfma32(kh[e], qh[t], s);
+            o[v] = mfma32(vh[e], ph[u], o[v]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto softmax = [&](int i) {
+        const int key0 = tile_key(i);
+        constexpr int F = Q8 ? 16 : 4, Q = 16 / F;  // factors of a lane, scores of each
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] *= sh.kfac[i & 3][g][r / Q] * qf;
+        float vtop = 0.0f;
+#pragma unroll
+        for (int t = 0; t < F; t++) vtop = fmaxf(vtop, sh.vfac[i & 3][g][t]);  // (a NaN counts as nothing)
+        vtop = half_max(vtop);
+        if constexpr (!Q8) {
+            int bad = 0;
+#pragma unroll
+            for (int t = 0; t < kWideWaves; t++) bad |= sh.bad[i & 3][t];
+            if (bad)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int quad = 2 * (r >> 2) + g;  // waves quad & 3 brought it, V and K
+                    const int both = sh.bad[i & 3][quad & 3] | sh.bad[i & 3][4 + (quad & 3)];
+                    if ((both >> (4 * (quad >> 2) + (r & 3))) & 1) s[r] = __uint_as_float(0x7fc00000u);
+                }
+        }
+        if (key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > (a.parent ? p.p0 - 1 : p.p0 + j0)) {
+            // visible: positions up to `limit`, and of a tree's nodes those of `sees`
+            int my_r, my_j;
+            my_row(&my_r, &my_j);
+            int limit = p.p0 + my_j;
+            uint64_t sees = 0;
+            if (a.parent) {
+                limit = p.p0 - 1;
+                sees = sh.sees[my_j];
+                if (!sees) sees = 1ull << my_j;  // (a bad node sees itself alone, as NaN)
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int key = key0 + 8 * (r >> 2) + 4 * g + (r & 3);
+                const bool see = key <= limit || ((sees >> ((key - p.p0) & 63)) & 1);
+                if (!see || key >= c1) s[r] = -__builtin_inff();
+            }
+        }
+        float mt = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
+        mt = half_max(mt);
+        // V's unit: a power of two not below the tile's largest factor
+        const float vpow = Q8 ? exp2_int(min(tile_exp(__float_as_uint(vtop)) + 1, 120)) : vtop;
+        const bool grows = mt > ref + 8.0f, vgrows = vpow > vrun;
+        if (__builtin_amdgcn_ballot_w64(grows || vgrows)) {
+            const float now = grows ? mt : ref;
+            float alpha = now == -__builtin_inff() ? 1.0f : fast_exp2(ref - now);
+            sum *= alpha;
+            ref = now;
+            if (vgrows) {
+                alpha *= vrun / vpow;
+                vrun = vpow;
+            }
+#pragma unroll
+            for (int v = 0; v < VB; v++) o[v] *= alpha;
+        }
+        const float off = (ref == -__builtin_inff() ? 0.0f : ref) - kWideBias;
+        const float vinv = 1.0f / vrun;
+        if constexpr (Q8) asm volatile("" ::: "memory");  // (sixteen factors are read again rather than kept)
+        float vf[F];
+#pragma unroll
+        for (int t = 0; t < F; t++) vf[t] = sh.vfac[i & 3][g][t] * vinv;
+        Half8 h[2], l[2];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            float x = fast_exp2(s[r] - off), y = fast_exp2(s[r + 1] - off);
+            sum += x + y;
+            if constexpr (Q8) {  // (a scale of NaN marks a row that a masked score must not meet)
+                x = x == 0.0f ? 0.0f : x * vf[r];
+                y = y == 0.0f ? 0.0f : y * vf[r + 1];
+            } else {
+                x *= vf[r / Q];
+                y *= vf[r / Q];
+            }
+            split2(x, y, h[r >> 3].h[(r & 7) / 2], l[r >> 3].h[(r & 7) / 2]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            ph[u] = h[u].v;
+            pl[u] = l[u].v;
+        }
+    };
+
+    // ---- the half-steps ----
+    __syncthreads();
+    if (!brings_v) __syncthreads();
+    if (!idle) scores(0);
+    __syncthreads();
+    for (int i = 0; i < n_tiles; i++) {
+        const int next = brings_v ? i + 1 : i + 2;
+        if (!idle) softmax(i);
+        stage_tile(next);
+        load_tile(next + 1);
+        __syncthreads();
+        if (!idle) {
+            if (i + 1 < n_tiles)
+                matrix(i);
+            else
+                values(i);
+        }
+        __syncthreads();
+    }
+    if (brings_v) __syncthreads();
+    if (idle) return;
+
+    // ---- results: register r of block v is dim 32 v + 8 (r / 4) + 4 g + r % 4 ----
+    sum += __shfl_xor(sum, 32);
+    const bool none = sum == 0.0f;  // (a chunk none of whose positions the row sees)
+    const float inv = none ? 0.0f : vrun / sum;
+    if (r0 + 32 * wave + n >= rows) return;
+    int my_r, my_j;
+    const size_t at = my_row(&my_r, &my_j);
+    const int n_split = a.spread ? (kv_end + a.chunk - 1) / a.chunk : 1;
+    const size_t rec = ((size_t)group_i * a.splits + split) * BM + 32 * wave + n;
+    float *dst = n_split == 1 ? a.out + at : a.ws_o + rec * HD;
+#pragma unroll
+    for (int v = 0; v < VB; v++)
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            *reinterpret_cast<float4 *>(dst + 32 * v + 8 * t + 4 * g) =
+                make_float4(o[v][4 * t] * inv, o[v][4 * t + 1] * inv, o[v][4 * t + 2] * inv, o[v][4 * t + 3] * inv);
+    if (n_split > 1 && g == 0) a.ws_lse[rec] = none ? -__builtin_inff() : ref + log2f(sum) - kWideBias;
+}
+
+}  // namespace leap
