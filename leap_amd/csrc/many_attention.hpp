@@ -221,6 +221,19 @@ __device__ __forceinline__ void split8(float4 a, float4 b, float sc, half8v &hi,
     lo = l.v;
 }
 
+// The same of x * sc and y * sc, two fused mixed-precision operations each.
+// (What comes out goes to LDS: the compiler knows no hazards of instructions
+// it does not see, so these never feed a matrix instruction.)
+__device__ __forceinline__ void split2_scaled(float x, float y, float sc, unsigned &h, unsigned &l)
+{
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x), "s"(sc));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(y), "s"(sc));
+    asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x), "s"(sc), "v"(h));
+    asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y), "s"(sc), "v"(h));
+}
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_abs(float m, float x) { return __builtin_elementwise_maximum(m, __builtin_fabsf(x)); }
+
 // Infinities and NaN replaced by zero; whether there were any.
 __device__ __forceinline__ bool zero_bad(float4 &x)
 {

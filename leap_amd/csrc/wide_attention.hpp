@@ -52,6 +52,7 @@ struct WideShared {
     // fp32: by quad, [lane half][4]; 8 bits: by position, [lane half][16]
     float kfac[4][2][Q8 ? 16 : 4], vfac[4][2][Q8 ? 16 : 4];
     int bad[4][kWideWaves];               // positions that are not finite, by the wave that brought them
+    int any_bad;                          // whether any tile so far had one
     uint64_t sees[kTreeMax];
     // the low halves of Q of each wave's last kQLow steps, for which there are no registers
     static constexpr int kQLow = HD == 128 ? (Q8 ? 4 : 6) : 0;
@@ -115,6 +116,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
     if (c0 >= kv_end) return;
     const int n_tiles = (c1 - c0 + kTileKeys - 1) / kTileKeys;
+    if (tid == 0) sh.any_bad = 0;
+    __syncthreads();
     auto tile_key = [&](int i) { return c0 + kTileKeys * i; };
 
     if (a.parent) {
@@ -209,14 +212,14 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             for (int t = 0; t < 2; t++) {
                 constexpr int N = HD / 16;
                 float *x = raw + N * t;
-                unsigned mx = 0;
+                float top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < N; e++) mx = max(mx, abs_bits(x[e]));
-                unsigned wx = wave_max_bits(mx);
+                for (int e = 0; e < N; e++) top = max_abs(top, x[e]);
+                unsigned wx = wave_max_bits(__float_as_uint(top));
                 const int quad = w + 4 * t;
                 if (!finite_bits(wx)) {
                     // zeros in their place, and their positions noted
-                    mx = 0;
+                    unsigned mx = 0;
                     int bits = 0;
 #pragma unroll
                     for (int e = 0; e < N; e++)
@@ -233,37 +236,33 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 }
                 const int e = tile_exp(wx);
                 const float sc = exp2_int(13 - e);
-                if (lane == 0) (brings_v ? sh.vfac : sh.kfac)[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
-                half2v h[N / 2], l[N / 2];
+                if (lane == 0) {
+                    if (brings_v)
+                        sh.vfac[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
+                    else
+                        sh.kfac[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
+                }
+                unsigned h[N / 2], l[N / 2];
 #pragma unroll
-                for (int e2 = 0; e2 < N / 2; e2++) split2(x[2 * e2] * sc, x[2 * e2 + 1] * sc, h[e2], l[e2]);
+                for (int e2 = 0; e2 < N / 2; e2++) split2_scaled(x[2 * e2], x[2 * e2 + 1], sc, h[e2], l[e2]);
                 if (!brings_v) {
                     const int pos = 4 * quad + (lane >> 4);
                     if constexpr (HD == 128) {
                         const int at = pos * C + ((lane & 15) ^ (pos & (C - 1)));
-                        Half8 x8;
-#pragma unroll
-                        for (int u = 0; u < 4; u++) x8.h[u] = h[u];
-                        sh.k[i & 1][0][at] = x8.v;
-#pragma unroll
-                        for (int u = 0; u < 4; u++) x8.h[u] = l[u];
-                        sh.k[i & 1][1][at] = x8.v;
+                        *reinterpret_cast<u32x4 *>(&sh.k[i & 1][0][at]) = u32x4{h[0], h[1], h[2], h[3]};
+                        *reinterpret_cast<u32x4 *>(&sh.k[i & 1][1][at]) = u32x4{l[0], l[1], l[2], l[3]};
                     } else {
                         const int at = pos * C + (((lane & 15) >> 1) ^ (pos & (C - 1)));
-                        half2v *hp = reinterpret_cast<half2v *>(&sh.k[i & 1][0][at]) + 2 * (lane & 1);
-                        half2v *lp = reinterpret_cast<half2v *>(&sh.k[i & 1][1][at]) + 2 * (lane & 1);
-                        *reinterpret_cast<u32x2 *>(hp) = u32x2{__builtin_bit_cast(unsigned, h[0]), __builtin_bit_cast(unsigned, h[1])};
-                        *reinterpret_cast<u32x2 *>(lp) = u32x2{__builtin_bit_cast(unsigned, l[0]), __builtin_bit_cast(unsigned, l[1])};
+                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][0][at]) + (lane & 1)) = u32x2{h[0], h[1]};
+                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][1][at]) + (lane & 1)) = u32x2{l[0], l[1]};
                     }
                 } else {
                     const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
 #pragma unroll
                     for (int u = 0; u < HD / 64; u++) {
                         const int d = lane + 64 * u, at = v_piece(d, piece);
-                        u32x2 *hp = reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][at]) + half;
-                        u32x2 *lp = reinterpret_cast<u32x2 *>(&sh.v[i % 3][1][at]) + half;
-                        *hp = u32x2{__builtin_bit_cast(unsigned, h[2 * u]), __builtin_bit_cast(unsigned, h[2 * u + 1])};
-                        *lp = u32x2{__builtin_bit_cast(unsigned, l[2 * u]), __builtin_bit_cast(unsigned, l[2 * u + 1])};
+                        *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][at]) + half) = u32x2{h[2 * u], h[2 * u + 1]};
+                        *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][1][at]) + half) = u32x2{l[2 * u], l[2 * u + 1]};
                     }
                 }
             }
@@ -300,7 +299,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
                 for (int j = 0; j < 4; j++) sh.vfac[i & 3][quad & 1][4 * (quad >> 1) + j] = sv4[j];
         }
-        if (!Q8 && lane == 0) sh.bad[i & 3][wave] = badbits;
+        if (!Q8 && lane == 0) {
+            sh.bad[i & 3][wave] = badbits;
+            if (badbits) sh.any_bad = 1;
+        }
     };
 
     // ---- Q: 32 rows a wave, in registers as the products' B operand ----
@@ -450,23 +452,25 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     auto softmax = [&](int i) {
         const int key0 = tile_key(i);
         constexpr int F = Q8 ? 16 : 4, Q = 16 / F;  // factors of a lane, scores of each
+        // scores are s[r] kf[r / Q]; the factors are positive (or NaN in a row without result)
+        float kf[F];
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] *= sh.kfac[i & 3][g][r / Q] * qf;
+        for (int t = 0; t < F; t++) kf[t] = sh.kfac[i & 3][g][t] * qf;
+        if constexpr (Q8) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] *= kf[r];
+        }
         float vtop = 0.0f;
 #pragma unroll
         for (int t = 0; t < F; t++) vtop = fmaxf(vtop, sh.vfac[i & 3][g][t]);  // (a NaN counts as nothing)
         vtop = half_max(vtop);
-        if constexpr (!Q8) {
-            int bad = 0;
+        if (!Q8 && __builtin_amdgcn_readfirstlane(sh.any_bad)) {
 #pragma unroll
-            for (int t = 0; t < kWideWaves; t++) bad |= sh.bad[i & 3][t];
-            if (bad)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int quad = 2 * (r >> 2) + g;  // waves quad & 3 brought it, V and K
-                    const int both = sh.bad[i & 3][quad & 3] | sh.bad[i & 3][4 + (quad & 3)];
-                    if ((both >> (4 * (quad >> 2) + (r & 3))) & 1) s[r] = __uint_as_float(0x7fc00000u);
-                }
+            for (int r = 0; r < 16; r++) {
+                const int quad = 2 * (r >> 2) + g;  // waves quad & 3 brought it, V and K
+                const int both = sh.bad[i & 3][quad & 3] | sh.bad[i & 3][4 + (quad & 3)];
+                if ((both >> (4 * (quad >> 2) + (r & 3))) & 1) s[r] = __uint_as_float(0x7fc00000u);
+            }
         }
         if (key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > (a.parent ? p.p0 - 1 : p.p0 + j0)) {
             // visible: positions up to `limit`, and of a tree's nodes those of `sees`
@@ -485,10 +489,19 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 const bool see = key <= limit || ((sees >> ((key - p.p0) & 63)) & 1);
                 if (!see || key >= c1) s[r] = -__builtin_inff();
             }
-        }
-        float mt = s[0];
+            if constexpr (!Q8)
 #pragma unroll
-        for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
+                for (int t = 0; t < F; t++) kf[t] = kf[t] == 0.0f ? 1e-38f : kf[t];  // (an underflown factor times -inf)
+        }
+        float mt = -__builtin_inff();
+        if constexpr (Q8) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[r]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < F; t++)
+                mt = fmaxf(mt, kf[t] * fmaxf(fmaxf(s[4 * t], s[4 * t + 1]), fmaxf(s[4 * t + 2], s[4 * t + 3])));
+        }
         mt = half_max(mt);
         // V's unit: a power of two not below the tile's largest factor
         const float vpow = Q8 ? exp2_int(min(tile_exp(__float_as_uint(vtop)) + 1, 120)) : vtop;
@@ -506,7 +519,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             for (int v = 0; v < VB; v++) o[v] *= alpha;
         }
         const float off = (ref == -__builtin_inff() ? 0.0f : ref) - kWideBias;
-        const float vinv = 1.0f / vrun;
+        const float vinv = __uint_as_float(0x7f000000u - __float_as_uint(vrun));  // 1 / vrun, a power of two
         if constexpr (Q8) asm volatile("" ::: "memory");  // (sixteen factors are read again rather than kept)
         float vf[F];
 #pragma unroll
@@ -514,7 +527,14 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         Half8 h[2], l[2];
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            float x = fast_exp2(s[r] - off), y = fast_exp2(s[r + 1] - off);
+            float x, y;
+            if constexpr (Q8) {
+                x = fast_exp2(s[r] - off);
+                y = fast_exp2(s[r + 1] - off);
+            } else {
+                x = fast_exp2(__builtin_fmaf(s[r], kf[r / Q], -off));
+                y = fast_exp2(__builtin_fmaf(s[r + 1], kf[r / Q], -off));
+            }
             sum += x + y;
             if constexpr (Q8) {  // (a scale of NaN marks a row that a masked score must not meet)
                 x = x == 0.0f ? 0.0f : x * vf[r];
@@ -544,10 +564,12 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         load_tile(next + 1);
         __syncthreads();
         if (!idle) {
+            __builtin_amdgcn_s_setprio(1);  // (the matrix phase's few instructions before the vector phase's many)
             if (i + 1 < n_tiles)
                 matrix(i);
             else
                 values(i);
+            __builtin_amdgcn_s_setprio(0);
         }
         __syncthreads();
     }
