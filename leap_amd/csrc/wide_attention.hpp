@@ -37,6 +37,10 @@
 
 namespace leap {
 
+// (the lambdas below are used once or twice each, in a kernel that has no
+// registers for calls)
+#define LEAP_INLINE __attribute__((always_inline))
+
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideWaves = 8;
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     const int n_tiles = (c1 - c0 + kTileKeys - 1) / kTileKeys;
     if (tid == 0) sh.any_bad = 0;
     __syncthreads();
-    auto tile_key = [&](int i) { return c0 + kTileKeys * i; };
+    auto tile_key = [&](int i) LEAP_INLINE { return c0 + kTileKeys * i; };
 
     if (a.parent) {
         if (wave == kWideWaves - 1) {
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         }
         __syncthreads();
     }
-    auto place_of = [&](int j) { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
+    auto place_of = [&](int j) LEAP_INLINE { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
 
     // ---- the cache's rows ----
     const int kv_dim = a.n_kv_heads * HD;
@@ -151,14 +155,15 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     // (the lane's part of an offset into a tile; a tile's rows add a uniform one)
     const uint32_t lane_off = head_off + (Q8 ? (brings_v ? 4u * v8_quad * row_bytes + v8_dim : (8u * w + (lane >> 3)) * row_bytes + (HD / 8) * (lane & 7))
                                              : (brings_v ? 4u * lane : (lane >> 4) * row_bytes + (HD / 4) * (lane & 15)));
-    auto load_tile = [&](int i) {
+    auto load_tile = [&](auto role, int i) LEAP_INLINE {
+        constexpr bool V = decltype(role)::value;
         if (i >= n_tiles) return;
         const uint32_t at = (uint32_t)tile_key(i) * row_bytes + lane_off;
         if constexpr (!Q8) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const uint32_t quad = 4u * (w + 4 * t) * row_bytes;
-                if (!brings_v) {
+                if constexpr (!V) {
 #pragma unroll
                     for (int u = 0; u < HD / 64; u++) {
                         const float4 x = buf_load4(rows_r, at + quad + 16 * u);
@@ -176,7 +181,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                                 __builtin_amdgcn_raw_buffer_load_b32(rows_r, (int)(at + (quad + j * row_bytes) + 256 * u), 0, 0));
                 }
             }
-        } else if (!brings_v) {
+        } else if constexpr (!V) {
             if constexpr (HD == 128) {
                 const float4 x = buf_load4(rows_r, at);
                 raw[0] = x.x;
@@ -203,10 +208,12 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         }
     };
     // That share into LDS, split, with its factors.
-    auto v_piece = [&](int d, int piece) { return d * 4 + (piece ^ (((d >> 1) ^ (d >> 3)) & 3)); };
-    auto stage_tile = [&](int i) {
+    auto v_piece = [&](int d, int piece) LEAP_INLINE { return d * 4 + (piece ^ (((d >> 1) ^ (d >> 3)) & 3)); };
+    auto stage_tile = [&](auto role, int i) LEAP_INLINE {
+        constexpr bool V = decltype(role)::value;
         if (i >= n_tiles) return;
-        int badbits = 0;
+        int badbits = 0, ln = lane;
+        asm volatile("" : "+v"(ln));  // (addresses formed anew, as in my_row)
         if constexpr (!Q8) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -217,7 +224,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 for (int e = 0; e < N; e++) top = max_abs(top, x[e]);
                 unsigned wx = wave_max_bits(__float_as_uint(top));
                 const int quad = w + 4 * t;
-                if (!finite_bits(wx)) {
+                if (__builtin_expect(!finite_bits(wx), 0)) {
                     // zeros in their place, and their positions noted
                     unsigned mx = 0;
                     int bits = 0;
@@ -225,7 +232,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                     for (int e = 0; e < N; e++)
                         if (!finite_bits(abs_bits(x[e]))) {
                             x[e] = 0.0f;
-                            bits |= brings_v ? 1 << (e & 3) : 1 << (lane >> 4);
+                            bits |= V ? 1 << (e & 3) : 1 << (ln >> 4);
                         } else {
                             mx = max(mx, abs_bits(x[e]));
                         }
@@ -236,49 +243,47 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 }
                 const int e = tile_exp(wx);
                 const float sc = exp2_int(13 - e);
-                if (lane == 0) {
-                    if (brings_v)
-                        sh.vfac[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
-                    else
-                        sh.kfac[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
-                }
+                // (every lane writes the same: no branch)
+                if constexpr (V)
+                    sh.vfac[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
+                else
+                    sh.kfac[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
                 unsigned h[N / 2], l[N / 2];
 #pragma unroll
                 for (int e2 = 0; e2 < N / 2; e2++) split2_scaled(x[2 * e2], x[2 * e2 + 1], sc, h[e2], l[e2]);
-                if (!brings_v) {
-                    const int pos = 4 * quad + (lane >> 4);
+                if constexpr (!V) {
+                    const int pos = 4 * quad + (ln >> 4);
                     if constexpr (HD == 128) {
-                        const int at = pos * C + ((lane & 15) ^ (pos & (C - 1)));
+                        const int at = pos * C + ((ln & 15) ^ (pos & (C - 1)));
                         *reinterpret_cast<u32x4 *>(&sh.k[i & 1][0][at]) = u32x4{h[0], h[1], h[2], h[3]};
                         *reinterpret_cast<u32x4 *>(&sh.k[i & 1][1][at]) = u32x4{l[0], l[1], l[2], l[3]};
                     } else {
-                        const int at = pos * C + (((lane & 15) >> 1) ^ (pos & (C - 1)));
-                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][0][at]) + (lane & 1)) = u32x2{h[0], h[1]};
-                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][1][at]) + (lane & 1)) = u32x2{l[0], l[1]};
+                        const int at = pos * C + (((ln & 15) >> 1) ^ (pos & (C - 1)));
+                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][0][at]) + (ln & 1)) = u32x2{h[0], h[1]};
+                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][1][at]) + (ln & 1)) = u32x2{l[0], l[1]};
                     }
                 } else {
                     const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
 #pragma unroll
                     for (int u = 0; u < HD / 64; u++) {
-                        const int d = lane + 64 * u, at = v_piece(d, piece);
+                        const int d = ln + 64 * u, at = v_piece(d, piece);
                         *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][at]) + half) = u32x2{h[2 * u], h[2 * u + 1]};
                         *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][1][at]) + half) = u32x2{l[2 * u], l[2 * u + 1]};
                     }
                 }
             }
-        } else if (!brings_v) {
-            int pos = 8 * w + (lane >> 3);
-            asm volatile("" : "+v"(pos));
+        } else if constexpr (!V) {
+            const int pos = 8 * w + (ln >> 3);
             if constexpr (HD == 128) {
 #pragma unroll
                 for (int u = 0; u < 2; u++)
-                    sh.k[i & 1][0][pos * C + ((2 * (lane & 7) + u) ^ (pos & (C - 1)))] =
+                    sh.k[i & 1][0][pos * C + ((2 * (ln & 7) + u) ^ (pos & (C - 1)))] =
                         bytes_half8(__float_as_uint(raw[2 * u]), __float_as_uint(raw[2 * u + 1]));
             } else {
-                sh.k[i & 1][0][pos * C + ((lane & 7) ^ (pos & (C - 1)))] =
+                sh.k[i & 1][0][pos * C + ((ln & 7) ^ (pos & (C - 1)))] =
                     bytes_half8(__float_as_uint(raw[0]), __float_as_uint(raw[1]));
             }
-            if ((lane & 7) == 0) sh.kfac[i & 3][(pos >> 2) & 1][4 * (pos >> 3) + (pos & 3)] = sck + 0.0f * scv;
+            if ((ln & 7) == 0) sh.kfac[i & 3][(pos >> 2) & 1][4 * (pos >> 3) + (pos & 3)] = sck + 0.0f * scv;
         } else if (HD == 128 || w < 2) {
             int quad = v8_quad, d0 = v8_dim;
             asm volatile("" : "+v"(quad), "+v"(d0));  // (addresses formed anew, as below)
@@ -295,13 +300,13 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][v_piece(d, piece)]) + half) =
                     u32x2{__builtin_bit_cast(unsigned, p0), __builtin_bit_cast(unsigned, p1)};
             }
-            if ((lane & (LR - 1)) == 0)
+            if ((ln & (LR - 1)) == 0)
 #pragma unroll
                 for (int j = 0; j < 4; j++) sh.vfac[i & 3][quad & 1][4 * (quad >> 1) + j] = sv4[j];
         }
-        if (!Q8 && lane == 0) {
+        if constexpr (!Q8) {
             sh.bad[i & 3][wave] = badbits;
-            if (badbits) sh.any_bad = 1;
+            if (__builtin_expect(badbits != 0, 0)) sh.any_bad = 1;
         }
     };
 
@@ -311,7 +316,13 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     // first (by every workgroup that reads them, the same bytes).
     const int t0 = a.fused ? max(c0 - p.p0, 0) : 0, n_new = a.fused ? max(min(c1 - p.p0, p.n) - t0, 0) : 0;
     const bool early = n_new == 0 || c0 + 2 * kTileKeys <= p.p0;
-    if (early) load_tile(0);
+    auto by_role = [&](auto f) LEAP_INLINE {
+        if (brings_v)
+            f(std::true_type{});
+        else
+            f(std::false_type{});
+    };
+    if (early) by_role([&](auto role) LEAP_INLINE { load_tile(role, 0); });
     for (int i = tid / LR; i < 2 * n_new; i += kWideThreads / LR) {
         const bool value = i >= n_new;
         const int j = t0 + (value ? i - n_new : i), lr = tid & (LR - 1);
@@ -325,7 +336,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     half8v qh[KS], ql[QR];
     float qf;
     // a lane's row, its token and its offset in q and out (formed anew where they are used, for the registers' sake)
-    auto my_row = [&](int *r, int *j) {
+    auto my_row = [&](int *r, int *j) LEAP_INLINE {
         int l = lane;
         asm volatile("" : "+v"(l));
         *r = min(r0 + 32 * wave + (l & 31), rows - 1);
@@ -367,15 +378,9 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         __syncthreads();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (L1 may hold parts of the new rows' lines)
     }
-    if (!early) load_tile(0);
-    stage_tile(0);
-    load_tile(1);
-    if (!brings_v) {
-        stage_tile(1);
-        load_tile(2);
-    }
     const bool idle = r0 + 32 * wave >= rows;  // no rows: this wave only brings its share
 
+    const int all_see = a.parent ? p.p0 - 1 : p.p0 + j0;  // the last position that every row of the tile sees
     f32x16 o[VB], s;
 #pragma unroll
     for (int v = 0; v < VB; v++)
@@ -388,68 +393,63 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     // 32 v + n; the swizzles leave t and u as an exclusive or on the first's
     // index.  Formed anew in each phase: kept, they would take 16 registers.)
     const int k_first = n * C + (g ^ (n & (C - 1))), v_first = v_piece(n, g);
-    auto clear_scores = [&] {
+    auto clear_scores = [&]() LEAP_INLINE {
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
     };
-    auto scores = [&](int i) {
+    auto scores = [&](int i) LEAP_INLINE {
         clear_scores();
         const half8v *k = sh.k[i & 1][0];
+        int kf = k_first;
+        asm volatile("" : "+v"(kf));
 #pragma unroll
         for (int t = 0; t < KS; t++) {
-            const int at = k_first ^ (2 * t);
+            const int at = kf ^ (2 * t);
             const half8v kh = k[at];
             s = mfma32(kh, t < QR ? ql[t < QR ? t : 0] : sh.ql[wave][t < QR ? 0 : t - QR][lane], s);
             if constexpr (!Q8) s = mfma32(k[at + 32 * C], qh[t], s);
             s = mfma32(kh, qh[t], s);
         }
     };
-    auto values = [&](int i) {
-        const half8v *x = sh.v[i % 3][0];
-#pragma unroll
-        for (int t = 0; t < KS; t++) {
-            const int u = t / VB, v = t % VB, at = (v_first ^ (2 * u)) + 128 * v;
-            const half8v vh = x[at];
-            o[v] = mfma32(vh, pl[u], o[v]);
-            if constexpr (!Q8) o[v] = mfma32(x[at + 4 * HD], ph[u], o[v]);
-            o[v] = mfma32(vh, ph[u], o[v]);
-        }
-    };
-    // Both, in turns: a product that adds to the one before it would wait for
-    // it (two accumulators of 32x32x16 keep the matrix core fed, one does not).
-    auto matrix = [&](int i) {
+    // The scores of tile i + 1 and the weighted values of tile i, in turns: a
+    // product that adds to the one before it would wait for it.  (After the
+    // last tile the scores are of what an earlier one left, and not used.)
+    auto matrix = [&](int i) LEAP_INLINE {
         clear_scores();
         int kf = k_first, vf = v_first;
         asm volatile("" : "+v"(kf), "+v"(vf));
         const half8v *k = sh.k[(i + 1) & 1][0], *x = sh.v[i % 3][0];
-        half8v kh[2], kl[2], vh[2], vl[2], low[2];  // a step's operands, read one step ahead
-        auto read = [&](int t) {
-            const int ka = kf ^ (2 * t), va = (vf ^ (2 * (t / VB))) + 128 * (t % VB);
-            kh[t & 1] = k[ka];
-            vh[t & 1] = x[va];
-            low[t & 1] = t < QR ? ql[t < QR ? t : 0] : sh.ql[wave][t < QR ? 0 : t - QR][lane];
-            if constexpr (!Q8) {
-                kl[t & 1] = k[ka + 32 * C];
-                vl[t & 1] = x[va + 4 * HD];
-            }
+        constexpr int D = 2;  // steps that the operands are read ahead
+        half8v kh[D + 1], kl[D + 1], vh[D + 1], vl[D + 1], low[D + 1];
+        auto read = [&](int t) LEAP_INLINE {
+            const int ka = kf ^ (2 * t), va = (vf ^ (2 * (t / VB))) + 128 * (t % VB), e = t % (D + 1);
+            kh[e] = k[ka];
+            if constexpr (!Q8) kl[e] = k[ka + 32 * C];
+            low[e] = t < QR ? ql[t < QR ? t : 0] : sh.ql[wave][t < QR ? 0 : t - QR][lane];
+            vh[e] = x[va];
+            if constexpr (!Q8) vl[e] = x[va + 4 * HD];
         };
-        read(0);
+#pragma unroll
+        for (int t = 0; t < D; t++) read(t);
 #pragma unroll
         for (int t = 0; t < KS; t++) {
-            const int u = t / VB, v = t % VB, e = t & 1;
-            if (t + 1 < KS) read(t + 1);
-            s = mfma32(kh[e], low[e], s);
+            const int u = t / VB, v = t % VB, e = t % (D + 1);
+            if (t + D < KS) read(t + D);
+            __builtin_amdgcn_sched_barrier(0);
+            s = mfma32(kh[e], qh[t], s);
             o[v] = mfma32(vh[e], pl[u], o[v]);
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (!Q8) {
                 s = mfma32(kl[e], qh[t], s);
                 o[v] = mfma32(vl[e], ph[u], o[v]);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            s = mfma32(kh[e], qh[t], s);
+            s = mfma32(kh[e], low[e], s);
             o[v] = mfma32(vh[e], ph[u], o[v]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto softmax = [&](int i) {
+    auto softmax = [&](int i) LEAP_INLINE {
         const int key0 = tile_key(i);
         constexpr int F = Q8 ? 16 : 4, Q = 16 / F;  // factors of a lane, scores of each
         // scores are s[r] kf[r / Q]; the factors are positive (or NaN in a row without result)
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
         for (int t = 0; t < F; t++) vtop = fmaxf(vtop, sh.vfac[i & 3][g][t]);  // (a NaN counts as nothing)
         vtop = half_max(vtop);
-        if (!Q8 && __builtin_amdgcn_readfirstlane(sh.any_bad)) {
+        if (!Q8 && __builtin_expect(__builtin_amdgcn_readfirstlane(sh.any_bad), 0)) {
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int quad = 2 * (r >> 2) + g;  // waves quad & 3 brought it, V and K
@@ -472,10 +472,12 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 if ((both >> (4 * (quad >> 2) + (r & 3))) & 1) s[r] = __uint_as_float(0x7fc00000u);
             }
         }
-        if (key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > (a.parent ? p.p0 - 1 : p.p0 + j0)) {
+        if (__builtin_expect(key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > all_see, 0)) {
             // visible: positions up to `limit`, and of a tree's nodes those of `sees`
-            int my_r, my_j;
+            int my_r, my_j, first = lane;
             my_row(&my_r, &my_j);
+            asm volatile("" : "+v"(first));
+            first = key0 + 4 * (first >> 5);
             int limit = p.p0 + my_j;
             uint64_t sees = 0;
             if (a.parent) {
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const int key = key0 + 8 * (r >> 2) + 4 * g + (r & 3);
+                const int key = first + 8 * (r >> 2) + (r & 3);
                 const bool see = key <= limit || ((sees >> ((key - p.p0) & 63)) & 1);
                 if (!see || key >= c1) s[r] = -__builtin_inff();
             }
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         // V's unit: a power of two not below the tile's largest factor
         const float vpow = Q8 ? exp2_int(min(tile_exp(__float_as_uint(vtop)) + 1, 120)) : vtop;
         const bool grows = mt > ref + 8.0f, vgrows = vpow > vrun;
-        if (__builtin_amdgcn_ballot_w64(grows || vgrows)) {
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(grows || vgrows) != 0, 0)) {
             const float now = grows ? mt : ref;
             float alpha = now == -__builtin_inff() ? 1.0f : fast_exp2(ref - now);
             sum *= alpha;
@@ -553,27 +555,35 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     };
 
     // ---- the half-steps ----
-    __syncthreads();
-    if (!brings_v) __syncthreads();
-    if (!idle) scores(0);
-    __syncthreads();
-    for (int i = 0; i < n_tiles; i++) {
-        const int next = brings_v ? i + 1 : i + 2;
-        if (!idle) softmax(i);
-        stage_tile(next);
-        load_tile(next + 1);
-        __syncthreads();
-        if (!idle) {
-            __builtin_amdgcn_s_setprio(1);  // (the matrix phase's few instructions before the vector phase's many)
-            if (i + 1 < n_tiles)
-                matrix(i);
-            else
-                values(i);
-            __builtin_amdgcn_s_setprio(0);
+    by_role([&](auto role) LEAP_INLINE {
+        constexpr bool V = decltype(role)::value;
+        if (!early) load_tile(role, 0);
+        stage_tile(role, 0);
+        load_tile(role, 1);
+        if constexpr (!V) {
+            stage_tile(role, 1);
+            load_tile(role, 2);
         }
         __syncthreads();
-    }
-    if (brings_v) __syncthreads();
+        if constexpr (!V) __syncthreads();
+        if (!idle) scores(0);
+        __syncthreads();
+        for (int i = 0; i < n_tiles; i++) {
+            const int next = V ? i + 1 : i + 2;
+            if (!idle) softmax(i);
+            __builtin_amdgcn_sched_barrier(0);
+            stage_tile(role, next);
+            load_tile(role, next + 1);
+            __syncthreads();
+            if (!idle) {
+                __builtin_amdgcn_s_setprio(1);  // (the matrix phase's few instructions before the vector phase's many)
+                matrix(i);
+                __builtin_amdgcn_s_setprio(0);
+            }
+            __syncthreads();
+        }
+        if constexpr (V) __syncthreads();
+    });
     if (idle) return;
 
     // ---- results: register r of block v is dim 32 v + 8 (r / 4) + 4 g + r % 4 ----
@@ -596,3 +606,5 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 }
 
 }  // namespace leap
+
+#undef LEAP_INLINE
