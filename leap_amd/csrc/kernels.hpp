@@ -109,8 +109,11 @@ bool q8_supported(int dim, int gs);
 // rows each, by the smallest such size; false for a shape without kernels.
 bool pick_q8(int dim, int gs, int kind, int rows, int n_cu, Q8Launch *out);
 
-// Prompts, trees and the 8-bit cache: the append of the new rows and the
-// attention over tiles of 16 nb rows, on an fp32 or 8-bit cache.
+// Prompts, trees and the 8-bit cache: the append of the new rows, the
+// attention over tiles of (token, q head) rows on an fp32 or 8-bit cache, and
+// the sum of a spread launch's records.  kManyStep: one token a sequence, on
+// an 8-bit cache; kManySmall: tiles of 16 rows; kManyWide: of 256.
+enum ManyKind { kManyStep, kManySmall, kManyWide };
 using ManyFn = void (*)(leap::ManyArgs);
 struct ManyKernels {
     ManyFn append, attention, merge;
@@ -122,16 +125,16 @@ struct RowsKernels {
     RowsFn write, read;
 };
 template <int HD>
-ManyKernels pick_many_hd(int nb, bool q8);
+ManyKernels pick_many_hd(ManyKind kind, bool q8);
 template <int HD>
 RowsKernels pick_rows_hd();
-extern template ManyKernels pick_many_hd<64>(int, bool);
-extern template ManyKernels pick_many_hd<128>(int, bool);
+extern template ManyKernels pick_many_hd<64>(ManyKind, bool);
+extern template ManyKernels pick_many_hd<128>(ManyKind, bool);
 extern template RowsKernels pick_rows_hd<64>();
 extern template RowsKernels pick_rows_hd<128>();
-inline ManyKernels pick_many(int hd, int nb, bool q8)
+inline ManyKernels pick_many(int hd, ManyKind kind, bool q8)
 {
-    return hd == 64 ? pick_many_hd<64>(nb, q8) : hd == 128 ? pick_many_hd<128>(nb, q8) : ManyKernels{};
+    return hd == 64 ? pick_many_hd<64>(kind, q8) : hd == 128 ? pick_many_hd<128>(kind, q8) : ManyKernels{};
 }
 inline RowsKernels pick_rows(int hd) { return hd == 64 ? pick_rows_hd<64>() : pick_rows_hd<128>(); }
 // The accepted paths' rows moved together, in an fp32 or 8-bit cache.

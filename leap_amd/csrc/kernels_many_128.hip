@@ -3,7 +3,7 @@
 #include "kernels_many_table.hpp"
 
 namespace leap_kernels {
-template ManyKernels pick_many_hd<128>(int, bool);
+template ManyKernels pick_many_hd<128>(ManyKind, bool);
 template RowsKernels pick_rows_hd<128>();
 KeepFn pick_keep(bool q8) { return q8 ? leap::tree_keep_kernel<true> : leap::tree_keep_kernel<false>; }
 }  // namespace leap_kernels

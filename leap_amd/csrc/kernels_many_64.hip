@@ -2,6 +2,6 @@
 #include "kernels_many_table.hpp"
 
 namespace leap_kernels {
-template ManyKernels pick_many_hd<64>(int, bool);
+template ManyKernels pick_many_hd<64>(ManyKind, bool);
 template RowsKernels pick_rows_hd<64>();
 }  // namespace leap_kernels

@@ -8,14 +8,16 @@
 namespace leap_kernels {
 
 template <int HD>
-ManyKernels pick_many_hd(int nb, bool q8)
+ManyKernels pick_many_hd(ManyKind kind, bool q8)
 {
+    constexpr int R = leap::kManyRows;
     const ManyFn append = q8 ? leap::many_append_kernel<HD, true> : leap::many_append_kernel<HD, false>;
-    if (nb == 1)
-        return q8 ? ManyKernels{append, leap::many_attention_kernel<HD, 1, 8, true>, leap::many_merge_kernel<HD, 16>, 8, 16}
-                  : ManyKernels{append, leap::many_attention_kernel<HD, 1, 4, false>, leap::many_merge_kernel<HD, 16>, 4, 16};
-    return {append, q8 ? leap::wide_attention_kernel<HD, true> : leap::wide_attention_kernel<HD, false>,
-            leap::many_merge_kernel<HD, leap::kWideRows>, leap::kWideWaves, leap::kWideRows};
+    if (kind == kManyWide)
+        return {append, q8 ? leap::wide_attention_kernel<HD, true> : leap::wide_attention_kernel<HD, false>,
+                leap::many_merge_kernel<HD, leap::kWideRows>, leap::kWideWaves, leap::kWideRows};
+    if (!q8) return {append, leap::many_attention_kernel<HD, 4, false, false>, leap::many_merge_kernel<HD, R>, 4, R};
+    return {append, kind == kManyStep ? leap::many_attention_kernel<HD, 8, true, true> : leap::many_attention_kernel<HD, 8, true, false>,
+            leap::many_merge_kernel<HD, R>, 8, R};
 }
 
 template <int HD>

@@ -772,7 +772,7 @@ int alloc_all(leap_hip_attention *h, std::initializer_list<std::pair<void **, si
 hipError_t load_many_table(int head_dim)
 {
     hipFuncAttributes attr;
-    return hipFuncGetAttributes(&attr, reinterpret_cast<const void *>(pick_many(head_dim, 1, false).attention));
+    return hipFuncGetAttributes(&attr, reinterpret_cast<const void *>(pick_many(head_dim, kManySmall, false).attention));
 }
 
 // ---- prompts, trees and the 8-bit cache ----------------------------------
@@ -783,38 +783,67 @@ hipError_t load_many_table(int head_dim)
 constexpr size_t kManyRecords = 65536;
 constexpr size_t kManyCounters = 4096;
 
-// What one launch of many_attention_kernel is cut into.
+// What a call is cut into.
 struct ManyPlan {
     ManyKernels fn;
-    int nb;        // rows of a tile / 16
     int slots;     // tiles of the batch, at most
     int chunk, splits;
     bool fused;    // the kernel stores the new rows itself
     bool spread;   // chunks on all XCDs, records added up by a launch of their own
     long long groups, wgs;
 };
-ManyPlan many_plan(const leap_hip_attention *h, int n_seq, int n_tokens, int max_tokens, int max_pos,
-                   long long total_rows)
+ManyPlan many_plan(const leap_hip_attention *h, bool step, int n_seq, int n_tokens, int max_tokens, int max_pos)
 {
-    const int group = h->group, n_kv = h->cfg.n_kv_heads, hd = h->cfg.head_dim;
+    const int group = h->group, n_kv = h->cfg.n_kv_heads, hd = h->cfg.head_dim, total = max_pos + 1;
     const long long rows_max = (long long)max_tokens * group;
+    const auto slots = [&](int bm) {
+        return (int)std::min((long long)n_tokens * group / bm + n_seq, n_seq * ((rows_max + bm - 1) / bm));
+    };
+    // Tiles of 16 or of 256 rows: those of 256 split each K and V row into
+    // halves once for 16 times the rows, but start about 10 us later and fill
+    // fewer CUs.  The time of either is near a + b * (tiles * (passes + 1)),
+    // and the line lies where the two cross (us, 16 : 256 rows; heads/KV
+    // heads/head_dim, sequences x tokens at context):
+    //   fp32, 32/8/128: 1x64 at 64 11.7 : 25.2, 1x64 at 4096 62.6 : 45.0,
+    //     8x16 at 1024 33.3 : 40.7, 8x32 at 1024 66.2 : 46.2
+    //   fp32, 32/4/64: 1x64 at 4096 30.0 : 30.9, 1x100 at 4096 48.3 : 40.5,
+    //     32x16 at 512 33.2 : 42.6, 32x32 at 512 59.0 : 57.2
+    //   8 bits, 32/8/128: 1x100 at 4096 40.8 : 54.0, 8x64 at 1024 60.2 : 60.1,
+    //     32x32 at 512 83.7 : 44.5
+    //   8 bits, 32/4/64: 1x100 at 4096 28.8 : 40.2, 8x64 at 1024 39.5 : 48.5,
+    //     32x32 at 512 56.3 : 56.9, 32x64 at 512 107 : 54
+    bool wide = false;
+    if (rows_max > leap::kManyRows) {
+        const int keys = h->q8kv ? 256 : 128;
+        const long long units = (long long)((max_pos + keys) / keys + 1) * (keys / leap::kTileKeys) * n_kv;
+        const long long base = h->q8kv ? (hd == 64 ? 36000 : 24000) : hd == 64 ? 12000 : 5000;
+        wide = slots(leap::kManyRows) * units > base + (hd == 64 ? 6 : 3) * slots(leap::kWideRows) * units;
+    }
     ManyPlan p{};
-    p.nb = rows_max <= 16 ? 1 : 2;
-    p.fn = pick_many(hd, p.nb, h->q8kv);
-    p.fused = max_tokens <= leap::kTreeMax;
-    const bool wide = p.nb > 1;
-    const int bm = p.fn.rows, pass = wide ? leap::kTileKeys : p.fn.waves * leap::kTileKeys;
-    p.slots = (int)std::min((long long)n_tokens * group / bm + n_seq, n_seq * ((rows_max + bm - 1) / bm));
+    p.fn = pick_many(hd, step ? kManyStep : wide ? kManyWide : kManySmall, h->q8kv);
+    p.slots = slots(p.fn.rows);
     p.groups = (long long)p.slots * n_kv;
-    const int total = max_pos + 1;
+    // New rows are stored by the attention kernel where that costs less than
+    // a launch for them (2 us): every workgroup forms those of its chunk, so
+    // with few tokens and few rounds of workgroups (us, one launch : two;
+    // 32/8/128 in fp32: 1x8 at 8 8.9 : 10.7, 1x32 at 32 12.0 : 10.9, 8x16 at
+    // 1024 33.5 : 37.0, 8x32 at 1024 66.0 : 65.3; 256 rows: 1x64 at 1024 37.8
+    // : 38.7, 8x64 at 1024 65.2 : 64.0, 32x16 at 512 56.5 : 47.3).
+    p.fused = step || (wide ? max_tokens <= leap::kTreeMax && p.groups <= h->n_cu / 4
+                            : max_tokens <= leap::kSmallNew && p.groups <= 2 * h->n_cu);
+    const int bm = p.fn.rows, pass = wide ? leap::kTileKeys : p.fn.waves * leap::kTileKeys;
     const long long group_bytes = (long long)total * hd * (h->q8kv ? 2 : 8);
-    const int per_cu = wide || p.fn.waves == 8 || (hd == 128 && !h->q8kv) ? 1 : 2;
+    const int per_cu = wide || p.fn.waves == 8 || hd == 128 ? 1 : 2;
     const bool few = !wide && p.groups < leap::kXcds && group_bytes < kSpreadBytes;  // on as many XCDs as groups
     const long long cus = few ? h->n_cu * p.groups / leap::kXcds : h->n_cu;
     const long long want = std::max<long long>(1, cus * per_cu);
     const int s = (int)std::max<long long>(1, std::min<long long>(leap::kManySplits, want / p.groups));
-    (void)total_rows;
     p.chunk = std::max(wide ? 128 : pass, round_up((total + s - 1) / s, pass));
+    // Two passes in one chunk take less than records and their sum, but for
+    // fp32 at head_dim 128 (us, one : two chunks; 8-bit steps at 500
+    // positions 32/4/64 6.7 : 7.6, 32/8/128 8.9 : 9.4; fp32 trees of 4x31 at
+    // 250 32/4/64 11.2 : 14.2, of 8 at 250 32/32/128 13.7 : 13.1).
+    if (!wide && (h->q8kv || hd == 64) && total <= 2 * pass) p.chunk = 2 * pass;
     p.splits = (total + p.chunk - 1) / p.chunk;
     while (p.splits > 1 && ((size_t)p.groups * p.splits * bm > kManyRecords || (size_t)p.groups > kManyCounters)) {
         p.chunk *= 2;
@@ -846,13 +875,13 @@ int many_reserve(leap_hip_attention *h, hipStream_t stream)
 // Enqueue the append of the new tokens' rows and their attention.  begin
 // NULL: one token of each of n_seq sequences (pos_dev, or pos_scalar).
 int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, const int *pos_dev, int pos_scalar,
-                const int *parent, int n_tokens, int max_tokens, int max_pos, long long total_rows, const float *q,
-                const float *k, const float *v, float *out, hipStream_t stream)
+                const int *parent, int n_tokens, int max_tokens, int max_pos, const float *q, const float *k, const float *v,
+                float *out, hipStream_t stream)
 {
     if (int rc = many_reserve(h, stream)) return rc;
     const size_t li = (size_t)(layer - h->cfg.layer_begin);
     const size_t loff = li * h->layer_floats;
-    const ManyPlan p = many_plan(h, n_seq, n_tokens, max_tokens, max_pos, total_rows);
+    const ManyPlan p = many_plan(h, !begin, n_seq, n_tokens, max_tokens, max_pos);
     leap::ManyArgs a{};
     a.q = q;
     a.k_new = k;
@@ -939,8 +968,8 @@ int launch(leap_hip_attention *h, int layer, int n_seq, const int *pos_dev, int 
 {
     if (h->q8kv) {
         if (kind != kDecode) return set_err(h, -EINVAL, "the floor launches read fp32 caches; this handle's holds 8 bits");
-        return launch_many(h, layer, n_seq, nullptr, pos_dev, pos_scalar, nullptr, n_seq, 1, max_pos, total_rows, q, k, v,
-                           out, stream);
+        return launch_many(h, layer, n_seq, nullptr, pos_dev, pos_scalar, nullptr, n_seq, 1, max_pos, q, k, v, out,
+                           stream);
     }
     if (!shape_supported(h->cfg.head_dim, h->group))
         return set_err(h, -EINVAL, "unsupported head_dim %d / group %d", h->cfg.head_dim, h->group);
@@ -2084,8 +2113,8 @@ static int many_async(leap_hip_attention *h, int layer, int n_seq, const int *be
         !aligned4(parent))
         return set_err(h, -EINVAL, "q, k_new, v_new and out must be 16-byte aligned, the int arrays 4-byte aligned");
     HIP_TRY(h, hipSetDevice(h->cfg.device));
-    return launch_many(h, layer, n_seq, begin, pos, 0, tree ? parent : nullptr, n_tokens, max_tokens, max_pos, 0, q, k_new,
-                       v_new, out, (hipStream_t)stream);
+    return launch_many(h, layer, n_seq, begin, pos, 0, tree ? parent : nullptr, n_tokens, max_tokens, max_pos, q, k_new, v_new,
+                       out, (hipStream_t)stream);
 }
 
 // The same with host pointers: everything is checked, staged in, run and
@@ -2135,8 +2164,8 @@ static int many_host(leap_hip_attention *h, int layer, int n_seq, const int *beg
     HIP_TRY(h, hipMemcpyAsync(bd, begin, (n_seq + 1) * sizeof(int), hipMemcpyHostToDevice, s));
     HIP_TRY(h, hipMemcpyAsync(pd, pos, n_seq * sizeof(int), hipMemcpyHostToDevice, s));
     if (tree) HIP_TRY(h, hipMemcpyAsync(td, parent, n_tokens * sizeof(int), hipMemcpyHostToDevice, s));
-    if (int rc = launch_many(h, layer, n_seq, bd, pd, 0, tree ? td : nullptr, (int)n_tokens, max_tokens, max_pos, 0, qd,
-                             kd, vd, od, s))
+    if (int rc = launch_many(h, layer, n_seq, bd, pd, 0, tree ? td : nullptr, (int)n_tokens, max_tokens, max_pos, qd, kd,
+                             vd, od, s))
         return rc;
     HIP_TRY(h, hipMemcpyAsync(out + first * h->q_dim, od + first * h->q_dim, (n_tokens - first) * h->q_dim * sizeof(float),
                               hipMemcpyDeviceToHost, s));

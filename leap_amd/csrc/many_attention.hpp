@@ -3,11 +3,12 @@
 //
 // For the q heads that share a KV head, the (token, head) pairs of a
 // sequence are the rows r = token * group + head of one product: tiles of
-// 16 NB rows of Q against the cache's rows, so that a K or V row is read
-// once for all of a tile's rows.  A workgroup takes one tile and one chunk of
-// positions; its four waves take 32 positions each in turn and keep an online
-// softmax of their own, combined at the end.  Chunks of one tile leave records
-// (output, log2 of the sum) that the last one to arrive adds up.
+// 16 rows of Q (wide_attention.hpp: of 256) against the cache's rows, so that
+// a K or V row is read once for all of a tile's rows.  A workgroup takes one
+// tile and one chunk of positions; its waves, four or (8 bits, whose rows are
+// a quarter of the bytes) eight, take 32 positions each in turn and keep an
+// online softmax of their own, combined at the end.  Chunks of one tile leave
+// records (output, log2 of the sum) that the last one to arrive adds up.
 //
 // Products.  S^T = K Q^T and O^T = V^T P^T as 16x16x32 MFMAs in fp16, with a
 // lane holding one row of Q throughout: S^T's column is the lane's row, its
@@ -234,6 +235,11 @@ __device__ __forceinline__ void split2_scaled(float x, float y, float sc, unsign
 // The larger magnitude; NaN if either is.
 __device__ __forceinline__ float max_abs(float m, float x) { return __builtin_elementwise_maximum(m, __builtin_fabsf(x)); }
 
+__device__ __forceinline__ float max4_abs(float m, float4 x)
+{
+    return max_abs(max_abs(max_abs(max_abs(m, x.x), x.y), x.z), x.w);
+}
+
 // Infinities and NaN replaced by zero; whether there were any.
 __device__ __forceinline__ bool zero_bad(float4 &x)
 {
@@ -389,41 +395,57 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void many_append_kernel(ManyA
 
 // The new rows of a chunk in a fused call, K and V by token, as the cache
 // holds them (rows 16 bytes apart in their banks).
-template <int HD, int BM, bool Q8>
+template <int HD, bool Q8, int N>
 struct NewRows {
-    float x[2][BM][HD + 4];
+    float x[2][N][HD + 4];
 };
-template <int HD, int BM>
-struct NewRows<HD, BM, true> {
-    int x[2][BM][HD / 4 + 4];
-    float scale[2][BM];
+template <int HD, int N>
+struct NewRows<HD, true, N> {
+    int x[2][N][HD / 4 + 4];
+    float scale[2][N];
 };
 
-template <int HD, int NB, int W, bool Q8>
+constexpr int kManyRows = 16;   // rows of a tile of many_attention_kernel
+constexpr int kWideRows = 256;  // and of wide_attention_kernel
+constexpr int kSmallNew = 32;   // new tokens of a sequence that fused calls of the former hold
+
+template <int HD, int W, bool Q8, bool STEP>
 struct ManyShared {
-    static constexpr int BM = 16 * NB;
-    static constexpr int kOStride = HD + 4;  // floats between rows of a wave's output (16 rows on 16 banks' groups)
     union {
         struct {
-            half8v q[NB][HD / 32][2][kWave]; // Q's operands: high and low halves
-            NewRows<HD, BM, Q8> fresh;
+            half8v q[HD / 32][2][kWave];     // Q's operand: high and low halves
+            NewRows<HD, Q8, STEP ? 1 : kSmallNew> fresh;
         };
-        float o[W][BM][kOStride];            // the waves' outputs
+        float o[W][kManyRows][HD + 4];       // the waves' outputs
         struct {
-            float w[16][kManySplits + 1];    // the merge: weights of a row's records
-            float4 part[W * kWave];          // and partial sums of them
+            float w[kManyRows][kManySplits + 1];  // the merge: weights of a row's records
+            float4 part[W * kWave];               // and partial sums of them
         } merge;
     };
-    float qf[BM];                            // 2^(e - 13) log2(e) / sqrt(HD) of each row (NaN: a row without result)
-    float m[W][BM], l[W][BM];
-    int e[W];
-    float f[W][BM];                 // the waves' weights in the sum
-    float lse[BM], inv[BM];
-    uint64_t sees[kTreeMax];
+    float qf[kManyRows];                     // 2^(e - 13) log2(e) / sqrt(HD) of each row (NaN: a row without result)
+    float m[W][kManyRows], l[W][kManyRows];
+    float unit[W];                           // O's unit of each wave
+    uint64_t sees[STEP ? 1 : kTreeMax];
     int last;
 };
 
-// The sum of a tile's records, for R rows from R rb on, by T >= 256 threads:
+// max / sum of a lane's value and those of the lanes 16, 32 and 48 away (the
+// swaps of one register with itself would be folded: each takes a copy)
+template <bool MAX>
+__device__ __forceinline__ float rows4(float x)
+{
+    auto op = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+    float y = x;
+    asm("" : "+v"(y));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    y = x;
+    asm("" : "+v"(y));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return op(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+// The sum of a tile's records, for R rows from R rb on, by T >= 16 R threads:
 // record s of row i counts 2^(lse_s - max lse) / their sum.
 template <int HD, int BM, int R, int T, typename Merge>
 __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi, int n_split, const Place &p, int kvh, int rb,
@@ -434,18 +456,31 @@ __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi,
     if (r0 >= rows) return;
     const size_t rec0 = (size_t)gi * a.splits * BM + R * rb;
     const float ninf = -__builtin_inff();
+    // the rows' float4 words, `items` of them; with fewer than threads the
+    // records are dealt to `parts` threads a word
+    const int items = min(R, rows - r0) * LR;
+    int parts = 1;
+    while (2 * parts * items <= T) parts *= 2;
+    const auto wr = make_rsrc(a.ws_o + rec0 * HD, (uint32_t)n_split * BM * HD * 4u);
+    const int part = parts > 1 ? tid / items : 0;
+    float4 x[8];
+    auto load = [&](int i, int s) {  // (past the last record: 0)
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = buf_load4<kSc1>(wr, (uint32_t)((s + k * parts) * BM * HD + 4 * i) * 4u);
+    };
+    load(tid - part * items, part);  // on their way while the weights are formed
     if (T == 16 * R || tid < 16 * R) {
         const int row = tid >> 4, l = tid & 15;
         const auto lr = make_rsrc(a.ws_lse + rec0, (uint32_t)n_split * BM * 4u);
-        float x[kManySplits / 16], top = ninf;
+        float y[kManySplits / 16], top = ninf;
 #pragma unroll
         for (int k = 0; k < kManySplits / 16; k++) {
             const int s = l + 16 * k;
-            x[k] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (s * BM + row) * 4, 0, kSc1));
-            if (s >= n_split) x[k] = ninf;
+            y[k] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (s * BM + row) * 4, 0, kSc1));
+            if (s >= n_split) y[k] = ninf;
         }
 #pragma unroll
-        for (int k = 0; k < kManySplits / 16; k++) top = fmaxf(top, x[k]);
+        for (int k = 0; k < kManySplits / 16; k++) top = fmaxf(top, y[k]);
         top = fmaxf(top, dpp<0x121>(top));
         top = fmaxf(top, dpp<0x122>(top));
         top = fmaxf(top, dpp<0x124>(top));
@@ -454,8 +489,8 @@ __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi,
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < kManySplits / 16; k++) {
-            x[k] = fast_exp2(x[k] - top);
-            sum += x[k];
+            y[k] = fast_exp2(y[k] - top);
+            sum += y[k];
         }
         sum += dpp<0x121>(sum);
         sum += dpp<0x122>(sum);
@@ -464,37 +499,27 @@ __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi,
         const float inv = 1.0f / sum;
 #pragma unroll
         for (int k = 0; k < kManySplits / 16; k++)
-            if (l + 16 * k < n_split) sh.w[row][l + 16 * k] = x[k] * inv;
+            if (l + 16 * k < n_split) sh.w[row][l + 16 * k] = y[k] * inv;
     }
     __syncthreads();
-    // the rows' float4 words, `items` of them; with fewer than threads the
-    // records are dealt to `parts` threads a word
-    const int items = min(R, rows - r0) * LR;
-    int parts = 1;
-    while (2 * parts * items <= T) parts *= 2;
-    const auto wr = make_rsrc(a.ws_o + rec0 * HD, (uint32_t)n_split * BM * HD * 4u);
     for (int i0 = 0; i0 < items; i0 += T) {
-        const int part = parts > 1 ? tid / items : 0, i = i0 + tid - part * items;
+        const int i = i0 + tid - part * items, row = i / LR;
+        const bool mine = i < items && part < parts;
         float4 acc = make_float4(0, 0, 0, 0);
-        const int row = i / LR;
-        if (i < items && part < parts) {
-            for (int s = part; s < n_split; s += 8 * parts) {
-                float4 x[8];
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    x[k] = buf_load4<kSc1>(wr, (uint32_t)((s + k * parts) * BM * HD + 4 * i) * 4u);  // (past the last: 0)
+        for (int s = part; s < n_split; s += 8 * parts) {
+            if (i0 > 0 || s != part) load(i, s);
+            if (mine)
 #pragma unroll
                 for (int k = 0; k < 8; k++)
                     if (s + k * parts < n_split) fma4(acc, sh.w[row][s + k * parts], x[k]);
-            }
         }
         if (parts > 1) {
             sh.part[tid] = acc;
             __syncthreads();
-            if (part == 0 && i < items)
+            if (part == 0 && mine)
                 for (int t = 1; t < parts; t++) fma4(acc, 1.0f, sh.part[t * items + i]);
         }
-        if (part == 0 && i < items) {
+        if (part == 0 && mine) {
             const int r = r0 + row;
             const int j = (int)fast_div((uint32_t)r, a.by_group);
             const int head = kvh * a.group + r - j * a.group;
@@ -503,12 +528,14 @@ __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi,
     }
 }
 
-template <int HD, int NB, int W, bool Q8>
-__global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) void many_attention_kernel(ManyArgs a)
+// Tiles of 16 rows, W waves.  STEP: calls of one token a sequence (begin
+// NULL), whose rows all see the whole chunk.
+template <int HD, int W, bool Q8, bool STEP>
+__global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_attention_kernel(ManyArgs a)
 {
-    constexpr int BM = 16 * NB, KS = HD / 32, VB = HD / 16, LR = HD / 4;
+    constexpr int BM = kManyRows, KS = HD / 32, VB = HD / 16, LR = HD / 4;
     constexpr int kThreads = W * kWave, kPassKeys = W * kTileKeys;
-    __shared__ ManyShared<HD, NB, W, Q8> sh;
+    __shared__ ManyShared<HD, W, Q8, STEP> sh;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, g = lane >> 4;
 
@@ -525,7 +552,7 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
         split = local - gl * a.splits;
         gi = gl * kXcds + (blockIdx.x & (kXcds - 1));
     }
-    if (a.fused && a.begin && blockIdx.x == 0) {
+    if (!STEP && a.fused && blockIdx.x == 0) {
         // skipped sequences' output rows, if there are any
         bool stop = false, any = false;
         for (int base = 0; base < a.n_seq && !stop && !any; base += kWave)
@@ -540,17 +567,24 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     if (gi >= n_groups) return;
     const int slot = (int)fast_div((uint32_t)gi, a.by_kv_heads);
     const int kvh = gi - slot * a.n_kv_heads;
-    const Place p = find_place<BM>(a, slot, lane);
-    if (p.seq < 0) return;
-    if (p.n < 0) {
-        if (split == 0)
-            fill_nan<HD>(a.out, ((size_t)p.first * a.n_heads + kvh * a.group) * LR, a.group * LR, tid, kThreads);
-        return;
+    Place p;
+    if constexpr (STEP) {
+        const int p0 = a.pos ? a.pos[slot] : a.pos_scalar;
+        if (p0 < 0 || p0 > a.max_pos) {
+            if (split == 0)
+                fill_nan<HD>(a.out, ((size_t)slot * a.n_heads + kvh * a.group) * LR, a.group * LR, tid, kThreads);
+            return;
+        }
+        p = Place{slot, 0, slot, 1, p0};
+    } else {
+        p = find_place<BM>(a, slot, lane);
+        if (p.seq < 0) return;
     }
-    const int rows = p.n * a.group, r0 = p.tile * BM;
-    const int j0 = (int)fast_div((uint32_t)r0, a.by_group);
-    const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(r0 + BM - 1), a.by_group));
-    const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
+    const int rows = p.n * a.group, r0 = p.tile * BM, n_rows = min(BM, rows - r0);
+    const int j0 = STEP ? 0 : (int)fast_div((uint32_t)r0, a.by_group);
+    const int j1 = STEP ? 0 : min(p.n - 1, (int)fast_div((uint32_t)(r0 + BM - 1), a.by_group));
+    const bool tree = !STEP && a.parent, fused = STEP || a.fused;
+    const int kv_end = tree ? p.p0 + p.n : p.p0 + j1 + 1;
     const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
     if (c0 >= kv_end) return;
 
@@ -558,7 +592,7 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     const int kv_dim = a.n_kv_heads * HD;
     const uint32_t row_bytes = (uint32_t)kv_dim * (Q8 ? 1 : 4), head_off = (uint32_t)kvh * HD * (Q8 ? 1 : 4);
     const size_t base = (size_t)p.seq * a.seq_stride;
-    const int old1 = a.fused ? min(c1, p.p0) : c1;         // cached rows of the chunk: up to here
+    const int old1 = fused ? min(c1, p.p0) : c1;           // cached rows of the chunk: up to here
     const uint32_t bytes = (uint32_t)old1 * row_bytes;     // (rows from there on read as zero)
     const auto kr = Q8 ? make_rsrc(a.k8 + base, bytes) : make_rsrc(a.k_cache + base, bytes);
     const auto vr = Q8 ? make_rsrc(a.v8 + base, bytes) : make_rsrc(a.v_cache + base, bytes);
@@ -570,36 +604,37 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
     float4 kraw[2][KR], vraw[8][VR];
     float2 vraw8[8];
     float4 ksc[2], vsc[2];
+    const uint32_t k_lane = m * row_bytes + head_off + 16 * g;
+    const uint32_t v_lane = 4 * g * row_bytes + head_off + (Q8 ? HD / 16 : 16) * m;
     auto load_k = [&](int key0) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const uint32_t off = (uint32_t)(key0 + 16 * b + m) * row_bytes + head_off;
+            const uint32_t off = k_lane + (uint32_t)(key0 + 16 * b) * row_bytes;
 #pragma unroll
-            for (int i = 0; i < KR; i++) kraw[b][i] = buf_load4(kr, off + 64 * i + 16 * g);
+            for (int i = 0; i < KR; i++) kraw[b][i] = buf_load4(kr, off + 64 * i);
             if constexpr (Q8) ksc[b] = buf_load4(ksr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
         }
     };
     auto load_v = [&](int key0) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const uint32_t off = (uint32_t)(key0 + 16 * (j >> 2) + 4 * g + (j & 3)) * row_bytes + head_off;
+            const uint32_t off = v_lane + (uint32_t)(key0 + 16 * (j >> 2) + (j & 3)) * row_bytes;
             if constexpr (Q8) {
                 if constexpr (HD == 128)
-                    vraw8[j] = buf_load2(vr, off + 8 * m);
+                    vraw8[j] = buf_load2(vr, off);
                 else
-                    vraw8[j].x = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(vr, (int)(off + 4 * m), 0, 0));
+                    vraw8[j].x = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(vr, (int)off, 0, 0));
             } else {
 #pragma unroll
-                for (int i = 0; i < VR; i++) vraw[j][i] = buf_load4(vr, off + 256 * i + 16 * m);
+                for (int i = 0; i < VR; i++) vraw[j][i] = buf_load4(vr, off + 256 * i);
             }
         }
         if constexpr (Q8)
 #pragma unroll
             for (int b = 0; b < 2; b++) vsc[b] = buf_load4(vsr, (uint32_t)(key0 + 16 * b + 4 * g) * 4u);
     };
-
     // The chunk's new rows: tokens [t0, t0 + n_new).
-    const int t0 = a.fused ? max(c0 - p.p0, 0) : 0, n_new = a.fused ? max(min(c1 - p.p0, p.n) - t0, 0) : 0;
+    const int t0 = fused ? max(c0 - p.p0, 0) : 0, n_new = fused ? max(min(c1 - p.p0, p.n) - t0, 0) : 0;
     auto is_new = [&](int j) { return (unsigned)(j - t0) < (unsigned)n_new; };
     // The rows of a tile that this call brings, in place of what was read.
     auto fresh_k = [&](int key0) {
@@ -609,15 +644,15 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
             if (is_new(j)) {
 #pragma unroll
                 for (int i = 0; i < KR; i++)
-                    kraw[b][i] = *reinterpret_cast<const float4 *>(&sh.fresh.x[0][j][16 * i + 4 * g]);
+                    kraw[b][i] = *reinterpret_cast<const float4 *>(&sh.fresh.x[0][STEP ? 0 : j][16 * i + 4 * g]);
             }
             if constexpr (Q8)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int t = key0 + 16 * b + 4 * g + i - p.p0;
                     if (is_new(t)) {
-                        (&ksc[b].x)[i] = sh.fresh.scale[0][t];
-                        (&vsc[b].x)[i] = sh.fresh.scale[1][t];
+                        (&ksc[b].x)[i] = sh.fresh.scale[0][STEP ? 0 : t];
+                        (&vsc[b].x)[i] = sh.fresh.scale[1][STEP ? 0 : t];
                     }
                 }
         }
@@ -627,159 +662,140 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
         for (int j = 0; j < 8; j++) {
             const int t = key0 + 16 * (j >> 2) + 4 * g + (j & 3) - p.p0;
             if (is_new(t)) {
+                const int at = STEP ? 0 : t;
                 if constexpr (Q8) {
                     if constexpr (HD == 128)
-                        vraw8[j] = *reinterpret_cast<const float2 *>(&sh.fresh.x[1][t][2 * m]);
+                        vraw8[j] = *reinterpret_cast<const float2 *>(&sh.fresh.x[1][at][2 * m]);
                     else
-                        vraw8[j].x = __int_as_float(sh.fresh.x[1][t][m]);
+                        vraw8[j].x = __int_as_float(sh.fresh.x[1][at][m]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < VR; i++)
-                        vraw[j][i] = *reinterpret_cast<const float4 *>(&sh.fresh.x[1][t][64 * i + 4 * m]);
+                        vraw[j][i] = *reinterpret_cast<const float4 *>(&sh.fresh.x[1][at][64 * i + 4 * m]);
                 }
             }
         }
     };
 
-    // ---- Q: rotated, split, into LDS as the products' B operand ----
-    // element (s, g, j) of a row: the order of the contraction over dims,
-    // such that a K load instruction takes whole 64-byte pieces of its rows
-    auto dim_of = [&](int s, int h) {
-        return Q8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h : 32 * s + 16 * h + 4 * g;
+    // ---- the tile's rows of Q and the chunk's new rows ----
+    // LR threads a row: rows of Q first, then new K rows, then new V rows.
+    // The loads go out in the order they are needed: these rows', then the
+    // first tile's.
+    const int lr = tid & (LR - 1), n_jobs = n_rows + 2 * n_new;
+    auto token_of = [&](int job) {
+        return job < n_rows ? (STEP ? 0 : (int)fast_div((uint32_t)(r0 + job), a.by_group))
+                            : t0 + (job - n_rows < n_new ? job - n_rows : job - n_rows - n_new);
     };
-    // The loads go out in the order they are needed: Q's, the new rows', then
-    // the first tile's.
-    float4 x[KS][2];
-    auto q_row = [&](int nb, int *j) {
-        const int r = min(r0 + 16 * nb + m, rows - 1);
-        *j = (int)fast_div((uint32_t)r, a.by_group);
-        return a.q + ((size_t)(p.first + *j) * a.n_heads + kvh * a.group + r - *j * a.group) * HD;
+    auto load_row = [&](int job) {
+        const int j = token_of(job);
+        const float *src = job < n_rows ? a.q + ((size_t)(p.first + j) * a.n_heads + kvh * a.group + r0 + job - j * a.group) * HD
+                                        : (job < n_rows + n_new ? a.k_new : a.v_new) + ((size_t)(p.first + j) * a.n_kv_heads + kvh) * HD;
+        return reinterpret_cast<const float4 *>(src)[lr];
     };
-    auto load_q = [&](int nb) {
-        int j;
-        const float *src = q_row(nb, &j);
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) x[s][h] = *reinterpret_cast<const float4 *>(src + dim_of(s, h));
-    };
-    // New row i of K, then of V, LR threads each.
-    const int lr = tid & (LR - 1);
-    auto new_row = [&](int i) {
-        const bool value = i >= n_new;
-        const int j = t0 + (value ? i - n_new : i);
-        return reinterpret_cast<const float4 *>(value ? a.v_new : a.k_new)[((size_t)(p.first + j) * a.n_kv_heads + kvh) * LR + lr];
+    auto load_turn = [&](int job, int at) {
+        return job < n_rows + n_new ? a.rope[(size_t)at * LR + lr] : make_float4(1, 0, 1, 0);
     };
     int key0 = c0 + wave * kTileKeys;
-    if (wave < NB) load_q(wave);
-    float4 y = make_float4(0, 0, 0, 0);
-    if (tid / LR < 2 * n_new) y = new_row(tid / LR);
+    constexpr int kJobs = kThreads / LR;
+    // (a bad node stands as if it hung on the cached rows)
+    auto pos_of = [&](int job) {
+        const int j = token_of(job);
+        return p.p0 + (tree ? max((int)__popcll(sh.sees[j]) - 1, 0) : j);
+    };
+    float4 y = make_float4(0, 0, 0, 0), turn = y;
+    int job = tid / LR;
+    if (job < n_jobs) {
+        y = load_row(job);
+        if (!tree) turn = load_turn(job, pos_of(job));
+    }
     if (key0 < c1) {
         load_k(key0);
         load_v(key0);
     }
-    if (a.parent) {
+    if (tree) {
         if (wave == W - 1) {
             const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
             sh.sees[lane] = t.bad ? 0 : t.sees;
         }
         __syncthreads();
     }
-    // position of token j (and of a bad node: as if it hung on the cached rows)
-    auto place_of = [&](int j) { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
-
-    // ---- the new rows of this chunk into LDS, and (by the last tile, which
-    // sees them all) into the cache ----
-    const bool stores = r0 + BM >= rows;
-    for (int i = tid / LR; i < 2 * n_new; i += kThreads / LR) {
-        if (i != tid / LR) y = new_row(i);
-        const bool value = i >= n_new;
-        const int j = t0 + (value ? i - n_new : i);
-        if (!value) y = rope4(y, a.rope[(size_t)place_of(j) * LR + lr]);
-        int q = 0;
-        float sc = 0.0f;
-        if constexpr (Q8) {
-            q = quantize_row<HD>(y, &sc);
-            sh.fresh.x[value][j][lr] = q;
-            if (lr == 0) sh.fresh.scale[value][j] = sc;
+    const bool stores = r0 + BM >= rows;  // the last tile sees all new rows: it puts them into the cache
+    if (tree && job < n_jobs) turn = load_turn(job, pos_of(job));
+    for (; job < n_jobs; job += kJobs) {
+        float4 y1 = make_float4(0, 0, 0, 0), turn1 = y1;  // the next one's, on their way
+        if (job + kJobs < n_jobs) {
+            y1 = load_row(job + kJobs);
+            turn1 = load_turn(job + kJobs, pos_of(job + kJobs));
+        }
+        if (job < n_rows) {
+            // rotated, split, and where the products' B operand has it: the
+            // contraction takes the dims in an order such that a K load
+            // instruction reads whole 64-byte pieces of its rows
+            const float4 x = rope4(y, turn);
+            unsigned mx = dpp_max16(max4_bits(0u, x));
+            if constexpr (HD == 128) mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
+            const bool good = finite_bits(mx) && !(tree && sh.sees[token_of(job)] == 0);
+            const int e = tile_exp(good ? mx : 0u);
+            const float sc = good ? exp2_int(13 - e) : 0.0f;
+            half2v h[2], l[2];
+            split2(x.x * sc, x.y * sc, h[0], l[0]);
+            split2(x.z * sc, x.w * sc, h[1], l[1]);
+            const int d = 4 * lr;
+            const int s = Q8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5, gg = Q8 ? (d >> 4) & 3 : (d >> 2) & 3;
+            const int half = Q8 ? (d >> 2) & 1 : (d >> 4) & 1;
+            u32x2 *to = reinterpret_cast<u32x2 *>(&sh.q[s][0][16 * gg + job]) + half;
+            to[0] = u32x2{__builtin_bit_cast(unsigned, h[0]), __builtin_bit_cast(unsigned, h[1])};
+            to[2 * kWave] = u32x2{__builtin_bit_cast(unsigned, l[0]), __builtin_bit_cast(unsigned, l[1])};
+            if (lr == 0) sh.qf[job] = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
         } else {
-            *reinterpret_cast<float4 *>(&sh.fresh.x[value][j][4 * lr]) = y;
-        }
-        if (stores) store_row<HD, Q8>(a, p.seq, p.p0 + j, kvh * LR + lr, y, q, sc, value);
-    }
-    for (int nb = wave; nb < NB; nb += W) {
-        if (nb != wave) load_q(nb);
-        int j;
-        q_row(nb, &j);
-        const int at = place_of(j);
-        bool good = !a.parent || sh.sees[j] != 0;
-        unsigned mx = 0;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                x[s][h] = rope4(x[s][h], a.rope[((size_t)at * HD + dim_of(s, h)) / 4]);
-                mx = max4_bits(mx, x[s][h]);
+            const int j = token_of(job);
+            const bool value = job >= n_rows + n_new;
+            if (!value) y = rope4(y, turn);
+            int q = 0;
+            float sc = 0.0f;
+            if constexpr (Q8) {
+                q = quantize_row<HD>(y, &sc);
+                sh.fresh.x[value][STEP ? 0 : j][lr] = q;
+                if (lr == 0) sh.fresh.scale[value][STEP ? 0 : j] = sc;
+            } else {
+                *reinterpret_cast<float4 *>(&sh.fresh.x[value][j][4 * lr]) = y;
             }
-        mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
-        mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
-        good = good && finite_bits(mx);
-        const int e = tile_exp(good ? mx : 0u);
-        if (g == 0) sh.qf[16 * nb + m] = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
-        const float sc = good ? exp2_int(13 - e) : 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            half8v hi, lo;
-            split8(x[s][0], x[s][1], sc, hi, lo);
-            sh.q[nb][s][0][lane] = hi;
-            sh.q[nb][s][1][lane] = lo;
+            if (stores) store_row<HD, Q8>(a, p.seq, p.p0 + j, kvh * LR + lr, y, q, sc, value);
         }
+        y = y1;
+        turn = turn1;
     }
     __syncthreads();
-    half8v qh[NB][KS], ql[NB][KS];  // (NB == 1: in registers; else read from LDS as they are used)
-    if constexpr (NB == 1) {
+    half8v qh[KS], ql[KS];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                qh[nb][s] = sh.q[nb][s][0][lane];
-                ql[nb][s] = sh.q[nb][s][1][lane];
-            }
+    for (int s = 0; s < KS; s++) {
+        qh[s] = sh.q[s][0][lane];
+        ql[s] = sh.q[s][1][lane];
     }
+    const float qf = sh.qf[m];
 
-    f32x4 o[VB][NB];
-    float mrun[NB], lrun[NB];
+    f32x4 o[VB];
+    float mrun = -__builtin_inff(), lrun = 0.0f;
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        mrun[nb] = -__builtin_inff();
-        lrun[nb] = 0.0f;
-#pragma unroll
-        for (int v = 0; v < VB; v++) o[v][nb] = f32x4{0, 0, 0, 0};
-    }
-    int erun = -100;  // O's unit is 2^(erun - 13)
+    for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
+    int erun = -100;  // O's unit is 2^(erun - 13) (8 bits: 2^erun)
 
     for (; key0 < c1; key0 += kPassKeys) {
         // ---- scores ----
-        if constexpr (NB > 1) asm volatile("" ::: "memory");  // (Q's operands are read from LDS in every pass)
         const bool fresh = n_new > 0 && key0 + kTileKeys > p.p0;
         if (fresh) fresh_k(key0);
         unsigned badkeys = 0;  // positions of the tile whose key or value is not finite (bit: position - key0)
-        f32x4 sc[2][NB];
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) sc[b][nb] = f32x4{0, 0, 0, 0};
         float kscale = 1.0f, kinv = 1.0f, vscale = 1.0f;
         int vexp = erun;
         if constexpr (!Q8) {
-            unsigned mk = 0;
+            float top = 0.0f;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int i = 0; i < KR; i++) mk = max4_bits(mk, kraw[b][i]);
-            unsigned wk = wave_max_bits(mk);
-            if (!finite_bits(wk)) {
-                mk = 0;
+                for (int i = 0; i < KR; i++) top = max4_abs(top, kraw[b][i]);
+            unsigned wk = wave_max_bits(__float_as_uint(top));
+            if (__builtin_expect(!finite_bits(wk), 0)) {
+                unsigned mk = 0;
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
                     bool bad = false;
@@ -799,12 +815,14 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
             kscale = exp2_int(13 - ek);
             kinv = exp2_int(ek - 13);
         }
+        f32x4 sc[2], sl[2];  // (two accumulators each: products that add to the one before them wait for it)
 #pragma unroll
-        for (int b = 0; b < 2; b++)
+        for (int b = 0; b < 2; b++) sc[b] = sl[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
                 half8v kh, kl;
-                if constexpr (NB == 4) __builtin_amdgcn_sched_barrier(0);
                 if constexpr (Q8) {
                     const float4 w = kraw[b][s >> 1];
                     kh = (s & 1) ? bytes_half8(__float_as_uint(w.z), __float_as_uint(w.w))
@@ -812,23 +830,12 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
                 } else {
                     split8(kraw[b][2 * s], kraw[b][2 * s + 1], kscale, kh, kl);
                 }
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-                    half8v h, l;
-                    if constexpr (NB == 1) {
-                        h = qh[nb][s];
-                        l = ql[nb][s];
-                    } else {
-                        h = sh.q[nb][s][0][lane];
-                        l = sh.q[nb][s][1][lane];
-                    }
-                    sc[b][nb] = mfma16(kh, l, sc[b][nb]);
-                    if constexpr (!Q8) sc[b][nb] = mfma16(kl, h, sc[b][nb]);
-                    sc[b][nb] = mfma16(kh, h, sc[b][nb]);
-                }
+                sl[b] = mfma16(kh, ql[s], sl[b]);
+                sc[b] = mfma16(kh, qh[s], sc[b]);
+                if constexpr (!Q8) sl[b] = mfma16(kl, qh[s], sl[b]);
             }
         float4 kscv[2], vscv[2];
-        if constexpr (Q8)
+        if constexpr (Q8) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 // a row's two scales: NaN in either marks it
@@ -836,32 +843,25 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
                 kscv[b] = make_float4(ksc[b].x + 0.0f * vsc[b].x, ksc[b].y + 0.0f * vsc[b].y,
                                       ksc[b].z + 0.0f * vsc[b].z, ksc[b].w + 0.0f * vsc[b].w);
             }
-        if constexpr (Q8) {
-            unsigned mv = 0;
+            float mv = 0.0f;
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const float *e = &vscv[b].x;
-#pragma unroll
-                for (int i = 0; i < 4; i++) mv = max(mv, finite_bits(abs_bits(e[i])) ? abs_bits(e[i]) : 0u);
-            }
-            mv = max(mv, (unsigned)__shfl_xor((int)mv, 16));
-            mv = max(mv, (unsigned)__shfl_xor((int)mv, 32));
+            for (int b = 0; b < 2; b++)
+                mv = fmaxf(mv, fmaxf(fmaxf(vscv[b].x, vscv[b].y), fmaxf(vscv[b].z, vscv[b].w)));  // (NaN counts as nothing)
             // (scales to at most 1: a probability of 2^14 times them stays in fp16)
-            vexp = max(erun, min(tile_exp(__builtin_amdgcn_readfirstlane(mv)) + 1, 126));
+            vexp = max(erun, min(tile_exp(__float_as_uint(rows4<true>(mv))) + 1, 126));
             vscale = exp2_int(-vexp);
         }
-        if constexpr (NB >= 2) __builtin_amdgcn_sched_barrier(0);
-        if constexpr (NB <= 2) load_k(key0 + kPassKeys);
+        load_k(key0 + kPassKeys);
         if (fresh) fresh_v(key0);
         if constexpr (!Q8) {
-            unsigned mv = 0;
+            float top = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
-                for (int i = 0; i < VR; i++) mv = max4_bits(mv, vraw[j][i]);
-            unsigned wv = wave_max_bits(mv);
-            if (!finite_bits(wv)) {
-                mv = 0;
+                for (int i = 0; i < VR; i++) top = max4_abs(top, vraw[j][i]);
+            unsigned wv = wave_max_bits(__float_as_uint(top));
+            if (__builtin_expect(!finite_bits(wv), 0)) {
+                unsigned mv = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     bool bad = false;
@@ -881,85 +881,76 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
         }
 
         // ---- softmax ----
-        const bool masked = key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > (a.parent ? p.p0 - 1 : p.p0 + j0);
         const float oscale = exp2_int(max(erun - vexp, -126));
         erun = vexp;
-        half8v ph[NB], pl[NB];
+        float s[8];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-            const float qf = sh.qf[16 * nb + m];
-            float s[8];
+        for (int t = 0; t < 8; t++) {
+            const int b = t >> 2, i = t & 3;
+            const float f = Q8 ? (&kscv[b].x)[i] * qf : kinv * qf;
+            s[t] = (sc[b][i] + sl[b][i]) * f;
+        }
+        if (__builtin_expect(badkeys != 0, 0))
 #pragma unroll
-            for (int t = 0; t < 8; t++) {
-                const int b = t >> 2, i = t & 3;
-                const float f = Q8 ? (&kscv[b].x)[i] * qf : kinv * qf;
-                s[t] = sc[b][nb][i] * f;
-            }
-            if (badkeys)
-#pragma unroll
-                for (int t = 0; t < 8; t++)
-                    if ((badkeys >> (16 * (t >> 2) + 4 * g + (t & 3))) & 1) s[t] = __uint_as_float(0x7fc00000u);
-            if (masked) {
-                // visible: up to `limit`, and of a tree's nodes those of `sees`
-                // (a bad node sees itself alone, as NaN)
-                const int tok = (int)fast_div((uint32_t)min(r0 + 16 * nb + m, rows - 1), a.by_group);
-                int limit = p.p0 + tok;
-                uint64_t sees = 0;
-                if (a.parent) {
+            for (int t = 0; t < 8; t++)
+                if ((badkeys >> (16 * (t >> 2) + 4 * g + (t & 3))) & 1) s[t] = __uint_as_float(0x7fc00000u);
+        if (key0 + kTileKeys > c1 || (!STEP && key0 + kTileKeys - 1 > (tree ? p.p0 - 1 : p.p0 + j0))) {
+            // visible: up to `limit`, and of a tree's nodes those of `sees`
+            // (a bad node sees itself alone, as NaN)
+            int limit = c1 - 1;
+            uint64_t sees = 0;
+            if constexpr (!STEP) {
+                const int tok = (int)fast_div((uint32_t)min(r0 + m, rows - 1), a.by_group);
+                limit = p.p0 + tok;
+                if (tree) {
                     limit = p.p0 - 1;
                     sees = sh.sees[tok];
                     if (!sees) sees = 1ull << tok;
                 }
-#pragma unroll
-                for (int t = 0; t < 8; t++) {
-                    const int key = key0 + 16 * (t >> 2) + 4 * g + (t & 3);
-                    const bool see = key <= limit || ((sees >> ((key - p.p0) & 63)) & 1);
-                    if (!see || key >= c1) s[t] = -__builtin_inff();
-                }
             }
-            float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-            mt = fmaxf(mt, __shfl_xor(mt, 16));
-            mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const float mn = fmaxf(mrun[nb], mt);
-            const float ref = mn == -__builtin_inff() ? 0.0f : mn;  // (a row that has seen nothing yet)
-            const float alpha = fast_exp2(mrun[nb] - ref);
-            mrun[nb] = mn;
-            float sum = 0.0f;
-            Half8 h, l;
 #pragma unroll
-            for (int t = 0; t < 8; t += 2) {
-                float x = fast_exp2(s[t] - ref + 14.0f), y = fast_exp2(s[t + 1] - ref + 14.0f);
-                sum += x + y;
-                if constexpr (Q8) {
-                    const int b = t >> 2, i = t & 3;
-                    x = x == 0.0f ? 0.0f : x * ((&vscv[b].x)[i] * vscale);
-                    y = y == 0.0f ? 0.0f : y * ((&vscv[b].x)[i + 1] * vscale);
-                }
-                split2(x, y, h.h[t / 2], l.h[t / 2]);
+            for (int t = 0; t < 8; t++) {
+                const int key = key0 + 16 * (t >> 2) + 4 * g + (t & 3);
+                const bool see = key <= limit || (!STEP && ((sees >> ((key - p.p0) & 63)) & 1));
+                if (!see || key >= c1) s[t] = -__builtin_inff();
             }
-            ph[nb] = h.v;
-            pl[nb] = l.v;
-            lrun[nb] = lrun[nb] * alpha + sum;
-            const float os = alpha * oscale;
-#pragma unroll
-            for (int v = 0; v < VB; v++) o[v][nb] *= os;
         }
-
-        if constexpr (NB >= 2) __builtin_amdgcn_sched_barrier(0);
-        if constexpr (NB > 2) load_k(key0 + kPassKeys);  // (here for the registers' sake)
+        const float mt = rows4<true>(
+            fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
+        const float mn = fmaxf(mrun, mt);
+        const float ref = mn == -__builtin_inff() ? 0.0f : mn;  // (a row that has seen nothing yet)
+        const float alpha = fast_exp2(mrun - ref);
+        mrun = mn;
+        float sum = 0.0f;
+        Half8 h, l;
+#pragma unroll
+        for (int t = 0; t < 8; t += 2) {
+            float x = fast_exp2(s[t] - ref + 14.0f), z = fast_exp2(s[t + 1] - ref + 14.0f);
+            sum += x + z;
+            if constexpr (Q8) {
+                const int b = t >> 2, i = t & 3;
+                x = x == 0.0f ? 0.0f : x * ((&vscv[b].x)[i] * vscale);
+                z = z == 0.0f ? 0.0f : z * ((&vscv[b].x)[i + 1] * vscale);
+            }
+            split2(x, z, h.h[t / 2], l.h[t / 2]);
+        }
+        const half8v ph = h.v, pl = l.v;
+        lrun = lrun * alpha + sum;
+        const float os = alpha * oscale;
 
         // ---- weighted values ----
 #pragma unroll
         for (int v = 0; v < VB; v++) {
+            o[v] *= os;
             half8v vh, vl;
             if constexpr (Q8) {
                 Half8 r;
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const unsigned x = __float_as_uint(v < 4 ? vraw8[j].x : vraw8[j].y) ^ 0x80808080u;
-                    const unsigned y = __float_as_uint(v < 4 ? vraw8[j + 1].x : vraw8[j + 1].y) ^ 0x80808080u;
+                    const unsigned z = __float_as_uint(v < 4 ? vraw8[j + 1].x : vraw8[j + 1].y) ^ 0x80808080u;
                     const unsigned sel = 0x0c000c00u | (unsigned)(4 + (v & 3)) << 16 | (unsigned)(v & 3);
-                    r.h[j / 2] = bytes_half(__builtin_amdgcn_perm(y, x, sel) | 0x64006400u);
+                    r.h[j / 2] = bytes_half(__builtin_amdgcn_perm(z, x, sel) | 0x64006400u);
                 }
                 vh = r.v;
             } else {
@@ -967,80 +958,56 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
                 auto at = [&](int j) { return (&vraw[j][i].x)[c]; };
                 split8(make_float4(at(0), at(1), at(2), at(3)), make_float4(at(4), at(5), at(6), at(7)), vscale, vh, vl);
             }
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                o[v][nb] = mfma16(vh, pl[nb], o[v][nb]);
-                if constexpr (!Q8) o[v][nb] = mfma16(vl, ph[nb], o[v][nb]);
-                o[v][nb] = mfma16(vh, ph[nb], o[v][nb]);
-            }
+            o[v] = mfma16(vh, pl, o[v]);
+            if constexpr (!Q8) o[v] = mfma16(vl, ph, o[v]);
+            o[v] = mfma16(vh, ph, o[v]);
         }
         load_v(key0 + kPassKeys);
     }
 
     // ---- the waves' results together ----
-    __syncthreads();  // (Q's operands are read; their memory takes the outputs)
-#pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        float l = lrun[nb];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        if (g == 0) {
-            sh.m[wave][16 * nb + m] = mrun[nb];
-            sh.l[wave][16 * nb + m] = l;
-        }
-        // register i of block v: dim (8 bits) VB (4 g + i) + v, or 64 (v / 4) + 4 (4 g + i) + v % 4
-        float *dst = sh.o[wave][16 * nb + m];
-#pragma unroll
-        for (int v = 0; v < VB; v += 4)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int d = Q8 ? VB * (4 * g + i) + v : 16 * v + 4 * (4 * g + i);
-                *reinterpret_cast<float4 *>(dst + d) =
-                    make_float4(o[v][nb][i], o[v + 1][nb][i], o[v + 2][nb][i], o[v + 3][nb][i]);
-            }
+    lrun = rows4<false>(lrun);
+    __syncthreads();  // (Q's operand is read; its memory takes the outputs)
+    if (g == 0) {
+        sh.m[wave][m] = mrun;
+        sh.l[wave][m] = lrun;
     }
-    if (lane == 0) sh.e[wave] = erun;
-    __syncthreads();
-    // (8 bits: V's unit is 2^erun, fp32: 2^(erun - 13); a probability's is 2^-14 in both sums)
-    if (tid < BM) {
-        float mm = sh.m[0][tid];
-        int ee = sh.e[0];
+    // register i of block v: dim (8 bits) VB (4 g + i) + v, or 64 (v / 4) + 4 (4 g + i) + v % 4
 #pragma unroll
-        for (int w = 1; w < W; w++) {
-            mm = fmaxf(mm, sh.m[w][tid]);
-            ee = max(ee, sh.e[w]);
+    for (int v = 0; v < VB; v += 4)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = Q8 ? VB * (4 * g + i) + v : 16 * v + 4 * (4 * g + i);
+            *reinterpret_cast<float4 *>(&sh.o[wave][m][d]) = make_float4(o[v][i], o[v + 1][i], o[v + 2][i], o[v + 3][i]);
         }
-        const float ref = mm == -__builtin_inff() ? 0.0f : mm;
+    if (lane == 0) sh.unit[wave] = exp2_int(max(min(Q8 ? erun : erun - 13, 127), -126));
+    __syncthreads();
+    // (a probability's unit, 2^-14, is in both sums)
+    const int n_split = a.splits > 1 ? (kv_end + a.chunk - 1) / a.chunk : 1;
+    const size_t rec = ((size_t)gi * a.splits + split) * BM;
+    for (int i = tid; i < n_rows * LR; i += kThreads) {
+        const int row = i / LR, d = (i - row * LR) * 4, r = r0 + row;
+        float top = sh.m[0][row];
+#pragma unroll
+        for (int w = 1; w < W; w++) top = fmaxf(top, sh.m[w][row]);
+        if (top == -__builtin_inff()) top = 0.0f;
+        float4 acc = make_float4(0, 0, 0, 0);
         float total = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            const float f = fast_exp2(sh.m[w][tid] - ref);
-            total += f * sh.l[w][tid];
-            sh.f[w][tid] = f * exp2_int(max(sh.e[w] - ee, -126));
+            const float f = fast_exp2(sh.m[w][row] - top);
+            total += f * sh.l[w][row];
+            fma4(acc, f * sh.unit[w], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
         }
-        // a chunk none of whose positions the row sees: nothing, weight 0
-        const bool none = total == 0.0f;
-        sh.inv[tid] = none ? 0.0f : exp2_int(max(min(Q8 ? ee : ee - 13, 127), -126)) / total;
-        sh.lse[tid] = none ? -__builtin_inff() : ref + log2f(total) - 14.0f;
-    }
-    __syncthreads();
-    const int n_split = a.splits > 1 ? (kv_end + a.chunk - 1) / a.chunk : 1;
-    const size_t rec = ((size_t)gi * a.splits + split) * BM;
-    for (int i = tid; i < BM * (HD / 4); i += kThreads) {
-        const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
-        const int r = r0 + row;
-        if (r >= rows) break;
-        float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int w = 0; w < W; w++) fma4(acc, sh.f[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
-        scale4(acc, sh.inv[row]);
+        const bool none = total == 0.0f;  // a chunk none of whose positions the row sees: nothing, weight 0
+        scale4(acc, none ? 0.0f : 1.0f / total);
         if (n_split == 1) {
-            const int j = (int)fast_div((uint32_t)r, a.by_group);
+            const int j = STEP ? 0 : (int)fast_div((uint32_t)r, a.by_group);
             const int head = kvh * a.group + r - j * a.group;
             *reinterpret_cast<float4 *>(a.out + ((size_t)(p.first + j) * a.n_heads + head) * HD + d) = acc;
         } else {
             *reinterpret_cast<float4 *>(a.ws_o + (rec + row) * HD + d) = acc;
-            if (d == 0) a.ws_lse[rec + row] = sh.lse[row];
+            if (d == 0) a.ws_lse[rec + row] = none ? -__builtin_inff() : top + log2f(total) - 14.0f;
         }
     }
     if (n_split == 1 || a.spread) return;
@@ -1056,11 +1023,7 @@ __global__ __launch_bounds__(W * kWave, NB == 4 || (HD == 128 && !Q8) ? 1 : 2) v
         if (before == n_split - 1) __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (!sh.last) return;
-    for (int rb = 0; rb < NB; rb++) {
-        merge_rows<HD, BM, 16, kThreads>(a, sh.merge, gi, n_split, p, kvh, rb, tid);
-        if (NB > 1) __syncthreads();
-    }
+    if (sh.last) merge_rows<HD, BM, BM, kThreads>(a, sh.merge, gi, n_split, p, kvh, 0, tid);
 }
 
 // The records of a spread launch's tiles of BM rows added up, kMergeRows rows

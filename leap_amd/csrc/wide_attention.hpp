@@ -45,7 +45,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = kWideWaves * kWave;
-constexpr int kWideRows = 32 * kWideWaves;
 constexpr float kWideBias = 7.0f;
 
 template <int HD, bool Q8>
