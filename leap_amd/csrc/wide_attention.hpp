@@ -50,16 +50,23 @@ constexpr float kWideBias = 7.0f;
 template <int HD, bool Q8>
 struct WideShared {
     static constexpr int P = Q8 ? 1 : 2;  // halves: high (and low)
-    half8v k[2][P][32 * HD / 8];          // [position][dims], 16-byte pieces swizzled by position
-    half8v v[3][P][HD * 32 / 8];          // [dim][positions], pieces swizzled by dim
+    // the low halves of Q of each wave's last kQLow steps, for which there are no registers
+    static constexpr int kQLow = HD == 128 ? (Q8 ? 4 : 6) : 0;
+    union {
+        struct {
+            half8v k[2][P][32 * HD / 8];  // [position][dims], 16-byte pieces swizzled by position
+            half8v v[3][P][HD * 32 / 8];  // [dim][positions], pieces swizzled by dim
+            half8v ql[kWideWaves][kQLow ? kQLow : 1][kWave];
+        };
+        half8v q[kWideWaves][2][32 * HD / 8];  // first: rows of Q on their way into registers
+        float4 o[kWideWaves][32 * HD / 4];     // last: rows of the result on theirs out
+    };
+    float qf[kWideWaves][32];             // factors of Q's rows
     // fp32: by quad, [lane half][4]; 8 bits: by position, [lane half][16]
     float kfac[4][2][Q8 ? 16 : 4], vfac[4][2][Q8 ? 16 : 4];
     int bad[4][kWideWaves];               // positions that are not finite, by the wave that brought them
     int any_bad;                          // whether any tile so far had one
     uint64_t sees[kTreeMax];
-    // the low halves of Q of each wave's last kQLow steps, for which there are no registers
-    static constexpr int kQLow = HD == 128 ? (Q8 ? 4 : 6) : 0;
-    half8v ql[kWideWaves][kQLow ? kQLow : 1][kWave];
 };
 
 __device__ __forceinline__ f32x16 mfma32(half8v a, half8v b, f32x16 c)
@@ -212,7 +219,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         constexpr bool V = decltype(role)::value;
         if (i >= n_tiles) return;
         int badbits = 0, ln = lane;
-        asm volatile("" : "+v"(ln));  // (addresses formed anew, as in my_row)
+        asm volatile("" : "+v"(ln));  // (addresses formed anew, for the registers' sake)
         if constexpr (!Q8) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -332,52 +339,62 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         store_row<HD, Q8>(a, p.seq, p.p0 + j, kvh * LR + lr, y, q, f, value);
     }
     constexpr int QL = WideShared<HD, Q8>::kQLow, QR = KS - QL;  // low halves of Q in LDS, in registers
-    half8v qh[KS], ql[QR];
-    float qf;
-    // a lane's row, its token and its offset in q and out (formed anew where they are used, for the registers' sake)
-    auto my_row = [&](int *r, int *j) LEAP_INLINE {
-        int l = lane;
-        asm volatile("" : "+v"(l));
-        *r = min(r0 + 32 * wave + (l & 31), rows - 1);
-        *j = (int)fast_div((uint32_t)*r, a.by_group);
-        return ((size_t)(p.first + *j) * a.n_heads + kvh * a.group + *r - *j * a.group) * HD;
+    const bool idle = r0 + 32 * wave >= rows;  // no rows: this wave only brings its share
+    // Rows of q and out are read and written whole, LR lanes a row, and turned
+    // through LDS; all waves take turns with the tile's rows of q.
+    constexpr int RW = kWave / LR, kAhead = 8;
+    const int lr = lane & (LR - 1), sub = lane / LR;
+    auto row_at = [&](int r, int *j) LEAP_INLINE {
+        *j = (int)fast_div((uint32_t)r, a.by_group);
+        return ((size_t)(p.first + *j) * a.n_heads + kvh * a.group + r - *j * a.group) * LR + lr;
     };
     {
-        int my_r, my_j;
-        const float *src = a.q + my_row(&my_r, &my_j);
-        const int at = place_of(my_j);
-        bool good = !a.parent || sh.sees[my_j] != 0;
-        float4 x[KS][2];
-        unsigned mx = 0;
+        const int n_rows = (min(BM, rows - r0) + 31) & ~31;
+        for (int b = RW * wave + sub; b < n_rows; b += RW * kWideWaves * kAhead) {
+            float4 x[kAhead], turn[kAhead];
+            int j[kAhead];
 #pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int d = 16 * s + 8 * g + 4 * h;
-                x[s][h] = rope4(*reinterpret_cast<const float4 *>(src + d), a.rope[((size_t)at * HD + d) / 4]);
-                mx = max4_bits(mx, x[s][h]);
+            for (int i = 0; i < kAhead; i++) {
+                const int r = min(r0 + b + RW * kWideWaves * i, rows - 1);
+                x[i] = reinterpret_cast<const float4 *>(a.q)[row_at(r, &j[i])];
+                turn[i] = a.rope[(size_t)place_of(j[i]) * LR + lr];
             }
-        mx = max(mx, (unsigned)__shfl_xor((int)mx, 32));
-        good = good && finite_bits(mx);
-        const int e = tile_exp(good ? mx : 0u);
-        qf = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
-        const float sc = good ? exp2_int(13 - e) : 0.0f;
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            half8v low;
-            split8(x[s][0], x[s][1], sc, qh[s], low);
-            if (s < QR)
-                ql[s] = low;
-            else
-                sh.ql[wave][s - QR][lane] = low;
+            for (int i = 0; i < kAhead; i++) {
+                const int row = b + RW * kWideWaves * i;
+                if (row >= n_rows) break;
+                const float4 y = rope4(x[i], turn[i]);
+                unsigned mx = dpp_max16(max4_bits(0u, y));
+                if constexpr (HD == 128) mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
+                const bool good = finite_bits(mx) && !(a.parent && sh.sees[j[i]] == 0);
+                const int e = tile_exp(good ? mx : 0u);
+                const float sc = good ? exp2_int(13 - e) : 0.0f;
+                half2v h[2], l[2];
+                split2(y.x * sc, y.y * sc, h[0], l[0]);
+                split2(y.z * sc, y.w * sc, h[1], l[1]);
+                const int at = (row & 31) * C + ((lr >> 1) ^ (row & (C - 1)));
+                *(reinterpret_cast<u32x2 *>(&sh.q[row >> 5][0][at]) + (lr & 1)) =
+                    u32x2{__builtin_bit_cast(unsigned, h[0]), __builtin_bit_cast(unsigned, h[1])};
+                *(reinterpret_cast<u32x2 *>(&sh.q[row >> 5][1][at]) + (lr & 1)) =
+                    u32x2{__builtin_bit_cast(unsigned, l[0]), __builtin_bit_cast(unsigned, l[1])};
+                if (lr == 0) sh.qf[row >> 5][row & 31] = good ? exp2_int(e - 13) * a.scale_log2 : __uint_as_float(0x7fc00000u);
+            }
         }
     }
-    if (n_new) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (L1 may hold parts of the new rows' lines)
+    if (n_new) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (n_new) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (L1 may hold parts of the new rows' lines)
+    half8v qh[KS], ql[KS];
+#pragma unroll
+    for (int t = 0; t < KS; t++) {
+        const int at = n * C + ((2 * t + g) ^ (n & (C - 1)));
+        qh[t] = sh.q[wave][0][at];
+        ql[t] = sh.q[wave][1][at];
     }
-    const bool idle = r0 + 32 * wave >= rows;  // no rows: this wave only brings its share
+    const float qf = sh.qf[wave][n];
+    __syncthreads();
+#pragma unroll
+    for (int t = QR; t < KS; t++) sh.ql[wave][t - QR][lane] = ql[t];
 
     const int all_see = a.parent ? p.p0 - 1 : p.p0 + j0;  // the last position that every row of the tile sees
     f32x16 o[VB], s;
@@ -473,10 +490,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         }
         if (__builtin_expect(key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > all_see, 0)) {
             // visible: positions up to `limit`, and of a tree's nodes those of `sees`
-            int my_r, my_j, first = lane;
-            my_row(&my_r, &my_j);
-            asm volatile("" : "+v"(first));
-            first = key0 + 4 * (first >> 5);
+            int ln = lane;
+            asm volatile("" : "+v"(ln));  // (formed anew, for the registers' sake)
+            const int my_j = (int)fast_div((uint32_t)min(r0 + 32 * wave + (ln & 31), rows - 1), a.by_group);
+            const int first = key0 + 4 * (ln >> 5);
             int limit = p.p0 + my_j;
             uint64_t sees = 0;
             if (a.parent) {
@@ -589,19 +606,29 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     sum += __shfl_xor(sum, 32);
     const bool none = sum == 0.0f;  // (a chunk none of whose positions the row sees)
     const float inv = none ? 0.0f : vrun / sum;
-    if (r0 + 32 * wave + n >= rows) return;
-    int my_r, my_j;
-    const size_t at = my_row(&my_r, &my_j);
-    const int n_split = a.spread ? (kv_end + a.chunk - 1) / a.chunk : 1;
-    const size_t rec = ((size_t)group_i * a.splits + split) * BM + 32 * wave + n;
-    float *dst = n_split == 1 ? a.out + at : a.ws_o + rec * HD;
+    float4 *rows_o = sh.o[wave];
 #pragma unroll
     for (int v = 0; v < VB; v++)
 #pragma unroll
         for (int t = 0; t < 4; t++)
-            *reinterpret_cast<float4 *>(dst + 32 * v + 8 * t + 4 * g) =
+            rows_o[n * LR + ((8 * v + 2 * t + g) ^ (n & (LR - 1)))] =
                 make_float4(o[v][4 * t] * inv, o[v][4 * t + 1] * inv, o[v][4 * t + 2] * inv, o[v][4 * t + 3] * inv);
-    if (n_split > 1 && g == 0) a.ws_lse[rec] = none ? -__builtin_inff() : ref + log2f(sum) - kWideBias;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (this wave's own rows)
+    __builtin_amdgcn_wave_barrier();
+    const int n_split = a.spread ? (kv_end + a.chunk - 1) / a.chunk : 1;
+    const size_t rec = ((size_t)group_i * a.splits + split) * BM + 32 * wave;
+    for (int b = 0; b < 32; b += RW) {
+        const int row = b + sub, r = r0 + 32 * wave + row;
+        if (r >= rows) break;
+        const float4 x = rows_o[row * LR + (lr ^ (row & (LR - 1)))];
+        int j;
+        if (n_split == 1)
+            reinterpret_cast<float4 *>(a.out)[row_at(r, &j)] = x;
+        else
+            reinterpret_cast<float4 *>(a.ws_o)[(rec + row) * LR + lr] = x;
+    }
+    if (n_split > 1 && g == 0 && r0 + 32 * wave + n < rows)
+        a.ws_lse[rec + n] = none ? -__builtin_inff() : ref + log2f(sum) - kWideBias;
 }
 
 }  // namespace leap
