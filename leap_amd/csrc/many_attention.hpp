@@ -24,7 +24,7 @@
 // fp16's subnormals), and h h' + h l' + l h' leaves out l l' < 2^-22 |x x'|,
 // of either sign: on sums of 128 terms and more that is fp32's own error.
 // Three fp16 MFMAs take 3/16 of the time of the fp32 MFMAs of the product.
-// The probabilities are split the same way, with 2^14 folded into their
+// The probabilities are split the same way, with 2^7 folded into their
 // exponent.  8-bit values are exact in fp16 and take two products.
 //
 // Rows with infinities or NaN: such a key or value makes NaN of the output
@@ -43,6 +43,7 @@ constexpr int kAppendWaves = 4;                        // waves of a workgroup o
 constexpr int kTileKeys = 32;                          // positions a wave takes at a time
 constexpr int kManySplits = 64;                        // chunks of a tile, at most
 constexpr int kTreeMax = 64;                           // nodes of a sequence's tree
+constexpr float kProbBias = 7.0f, kProbRoom = 8.0f;    // probabilities are 2^(score - reference + 7) <= 2^15
 constexpr float kAmaxFloor = 7.888609052210118e-31f;   // 2^-100: the least largest magnitude of an 8-bit head row
 
 // One launch over one layer.  begin NULL: one token a sequence, row i of
@@ -254,6 +255,12 @@ __device__ __forceinline__ bool zero_bad(float4 &x)
 __device__ __forceinline__ half2v bytes_half(unsigned two)
 {
     return __builtin_bit_cast(half2v, two) - half2v{(_Float16)1152.0f, (_Float16)1152.0f};
+}
+// The same of bytes alone (the halves 0x0000 | byte): values times 2^-24,
+// fp16's subnormals, as exact.
+__device__ __forceinline__ half2v bytes_small(unsigned two)
+{
+    return __builtin_bit_cast(half2v, two) - __builtin_bit_cast(half2v, 0x00800080u);
 }
 __device__ __forceinline__ half8v bytes_half8(unsigned a, unsigned b)
 {
@@ -778,7 +785,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     float mrun = -__builtin_inff(), lrun = 0.0f;
 #pragma unroll
     for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
-    int erun = -100;  // O's unit is 2^(erun - 13) (8 bits: 2^erun)
+    int erun = -100;  // O's unit is 2^(erun - 13) (8 bits: 2^erun, and values are 2^-24 times theirs)
 
     for (; key0 < c1; key0 += kPassKeys) {
         // ---- scores ----
@@ -847,7 +854,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
 #pragma unroll
             for (int b = 0; b < 2; b++)
                 mv = fmaxf(mv, fmaxf(fmaxf(vscv[b].x, vscv[b].y), fmaxf(vscv[b].z, vscv[b].w)));  // (NaN counts as nothing)
-            // (scales to at most 1: a probability of 2^14 times them stays in fp16)
+            // (scales to at most 1: a probability of 2^15 times them stays in fp16)
             vexp = max(erun, min(tile_exp(__float_as_uint(rows4<true>(mv))) + 1, 126));
             vscale = exp2_int(-vexp);
         }
@@ -881,8 +888,6 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         }
 
         // ---- softmax ----
-        const float oscale = exp2_int(max(erun - vexp, -126));
-        erun = vexp;
         float s[8];
 #pragma unroll
         for (int t = 0; t < 8; t++) {
@@ -917,31 +922,37 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         }
         const float mt = rows4<true>(
             fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
-        const float mn = fmaxf(mrun, mt);
-        const float ref = mn == -__builtin_inff() ? 0.0f : mn;  // (a row that has seen nothing yet)
-        const float alpha = fast_exp2(mrun - ref);
-        mrun = mn;
-        float sum = 0.0f;
+        // (the reference moves only when a score exceeds it by more than 2^8:
+        // most tiles leave O and the sum as they are)
+        const bool grows = mt > mrun + kProbRoom;
+        if (__builtin_amdgcn_ballot_w64(grows || vexp != erun)) {
+            const float now = grows ? mt : mrun;
+            const float alpha = now == -__builtin_inff() ? 1.0f : fast_exp2(mrun - now);
+            const float os = alpha * exp2_int(max(erun - vexp, -126));
+            lrun *= alpha;
+            mrun = now;
+            erun = vexp;
+#pragma unroll
+            for (int v = 0; v < VB; v++) o[v] *= os;
+        }
+        const float off = (mrun == -__builtin_inff() ? 0.0f : mrun) - kProbBias;  // (a row that has seen nothing yet)
         Half8 h, l;
 #pragma unroll
         for (int t = 0; t < 8; t += 2) {
-            float x = fast_exp2(s[t] - ref + 14.0f), z = fast_exp2(s[t + 1] - ref + 14.0f);
-            sum += x + z;
-            if constexpr (Q8) {
+            float x = fast_exp2(s[t] - off), z = fast_exp2(s[t + 1] - off);
+            lrun += x + z;
+            if constexpr (Q8) {  // (a scale of NaN marks a row that a masked score must not meet)
                 const int b = t >> 2, i = t & 3;
-                x = x == 0.0f ? 0.0f : x * ((&vscv[b].x)[i] * vscale);
-                z = z == 0.0f ? 0.0f : z * ((&vscv[b].x)[i + 1] * vscale);
+                x *= fmaxf((&vscv[b].x)[i] * vscale, 0.0f);
+                z *= fmaxf((&vscv[b].x)[i + 1] * vscale, 0.0f);
             }
             split2(x, z, h.h[t / 2], l.h[t / 2]);
         }
         const half8v ph = h.v, pl = l.v;
-        lrun = lrun * alpha + sum;
-        const float os = alpha * oscale;
 
         // ---- weighted values ----
 #pragma unroll
         for (int v = 0; v < VB; v++) {
-            o[v] *= os;
             half8v vh, vl;
             if constexpr (Q8) {
                 Half8 r;
@@ -950,7 +961,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
                     const unsigned x = __float_as_uint(v < 4 ? vraw8[j].x : vraw8[j].y) ^ 0x80808080u;
                     const unsigned z = __float_as_uint(v < 4 ? vraw8[j + 1].x : vraw8[j + 1].y) ^ 0x80808080u;
                     const unsigned sel = 0x0c000c00u | (unsigned)(4 + (v & 3)) << 16 | (unsigned)(v & 3);
-                    r.h[j / 2] = bytes_half(__builtin_amdgcn_perm(z, x, sel) | 0x64006400u);
+                    r.h[j / 2] = bytes_small(__builtin_amdgcn_perm(z, x, sel));
                 }
                 vh = r.v;
             } else {
@@ -982,7 +993,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         }
     if (lane == 0) sh.unit[wave] = exp2_int(max(min(Q8 ? erun : erun - 13, 127), -126));
     __syncthreads();
-    // (a probability's unit, 2^-14, is in both sums)
+    // (a probability's unit is in both sums)
     const int n_split = a.splits > 1 ? (kv_end + a.chunk - 1) / a.chunk : 1;
     const size_t rec = ((size_t)gi * a.splits + split) * BM;
     for (int i = tid; i < n_rows * LR; i += kThreads) {
@@ -1000,14 +1011,14 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             fma4(acc, f * sh.unit[w], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
         }
         const bool none = total == 0.0f;  // a chunk none of whose positions the row sees: nothing, weight 0
-        scale4(acc, none ? 0.0f : 1.0f / total);
+        scale4(acc, none ? 0.0f : (Q8 ? 0x1p24f : 1.0f) / total);
         if (n_split == 1) {
             const int j = STEP ? 0 : (int)fast_div((uint32_t)r, a.by_group);
             const int head = kvh * a.group + r - j * a.group;
             *reinterpret_cast<float4 *>(a.out + ((size_t)(p.first + j) * a.n_heads + head) * HD + d) = acc;
         } else {
             *reinterpret_cast<float4 *>(a.ws_o + (rec + row) * HD + d) = acc;
-            if (d == 0) a.ws_lse[rec + row] = none ? -__builtin_inff() : top + log2f(total) - 14.0f;
+            if (d == 0) a.ws_lse[rec + row] = none ? -__builtin_inff() : top + log2f(total) - kProbBias;
         }
     }
     if (n_split == 1 || a.spread) return;

@@ -45,7 +45,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = kWideWaves * kWave;
-constexpr float kWideBias = 7.0f;
 
 template <int HD, bool Q8>
 struct WideShared {
@@ -523,7 +522,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         mt = half_max(mt);
         // V's unit: a power of two not below the tile's largest factor
         const float vpow = Q8 ? exp2_int(min(tile_exp(__float_as_uint(vtop)) + 1, 120)) : vtop;
-        const bool grows = mt > ref + 8.0f, vgrows = vpow > vrun;
+        const bool grows = mt > ref + kProbRoom, vgrows = vpow > vrun;
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(grows || vgrows) != 0, 0)) {
             const float now = grows ? mt : ref;
             float alpha = now == -__builtin_inff() ? 1.0f : fast_exp2(ref - now);
@@ -536,7 +535,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
             for (int v = 0; v < VB; v++) o[v] *= alpha;
         }
-        const float off = (ref == -__builtin_inff() ? 0.0f : ref) - kWideBias;
+        const float off = (ref == -__builtin_inff() ? 0.0f : ref) - kProbBias;
         const float vinv = __uint_as_float(0x7f000000u - __float_as_uint(vrun));  // 1 / vrun, a power of two
         if constexpr (Q8) asm volatile("" ::: "memory");  // (sixteen factors are read again rather than kept)
         float vf[F];
@@ -628,7 +627,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             reinterpret_cast<float4 *>(a.ws_o)[(rec + row) * LR + lr] = x;
     }
     if (n_split > 1 && g == 0 && r0 + 32 * wave + n < rows)
-        a.ws_lse[rec + n] = none ? -__builtin_inff() : ref + log2f(sum) - kWideBias;
+        a.ws_lse[rec + n] = none ? -__builtin_inff() : ref + log2f(sum) - kProbBias;
 }
 
 }  // namespace leap
