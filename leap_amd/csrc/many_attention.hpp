@@ -19,13 +19,15 @@
 //
 // fp32 operands in fp16 products: x = 2^e (h + l), h = fp16(x 2^-e) and
 // l = fp16(x 2^-e - h), both rounded to nearest, with e such that the
-// largest of x's tile is in [2^13, 2^14).  h and l together hold x to 2^-22
-// relative (elements below 2^-28 of the tile's largest to 2^-39 of that,
-// fp16's subnormals), and h h' + h l' + l h' leaves out l l' < 2^-22 |x x'|,
-// of either sign: on sums of 128 terms and more that is fp32's own error.
-// Three fp16 MFMAs take 3/16 of the time of the fp32 MFMAs of the product.
-// The probabilities are split the same way, with 2^7 folded into their
-// exponent.  8-bit values are exact in fp16 and take two products.
+// largest of x's row (wide_attention.hpp: of a quad of rows, where these are
+// alike) is in [2^13, 2^14).  h and l together hold x to 2^-22 relative
+// (elements below 2^-28 of the row's largest to 2^-39 of that, fp16's
+// subnormals), and h h' + h l' + l h' leaves out l l' < 2^-22 |x x'|, of either
+// sign: on sums of 128 terms and more that is fp32's own error.  Three fp16
+// MFMAs take 3/16 of the time of the fp32 MFMAs of the product.  The
+// probabilities are split the same way, with 2^7 folded into their exponent
+// and each value row's 2^e, over the largest that the row of Q has seen, into
+// them.  8-bit values are exact in fp16 and take two products.
 //
 // Rows with infinities or NaN: such a key or value makes NaN of the output
 // rows that see it, and of those only: its elements are replaced by zero in
@@ -212,13 +214,14 @@ union Half8 {
     half8v v;
     half2v h[4];
 };
-__device__ __forceinline__ void split8(float4 a, float4 b, float sc, half8v &hi, half8v &lo)
+__device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
+__device__ __forceinline__ void split8(float4 a, float4 b, half8v &hi, half8v &lo)
 {
     Half8 h, l;
-    split2(a.x * sc, a.y * sc, h.h[0], l.h[0]);
-    split2(a.z * sc, a.w * sc, h.h[1], l.h[1]);
-    split2(b.x * sc, b.y * sc, h.h[2], l.h[2]);
-    split2(b.z * sc, b.w * sc, h.h[3], l.h[3]);
+    split2(a.x, a.y, h.h[0], l.h[0]);
+    split2(a.z, a.w, h.h[1], l.h[1]);
+    split2(b.x, b.y, h.h[2], l.h[2]);
+    split2(b.z, b.w, h.h[3], l.h[3]);
     hi = h.v;
     lo = l.v;
 }
@@ -431,7 +434,8 @@ struct ManyShared {
     };
     float qf[kManyRows];                     // 2^(e - 13) log2(e) / sqrt(HD) of each row (NaN: a row without result)
     float m[W][kManyRows], l[W][kManyRows];
-    float unit[W];                           // O's unit of each wave
+    float unit[W][kManyRows];                // O's unit of each wave and row
+    float kf[W][kTileKeys];                  // fp32: K's factors of each wave's tile
     uint64_t sees[STEP ? 1 : kTreeMax];
     int last;
 };
@@ -450,6 +454,18 @@ __device__ __forceinline__ float rows4(float x)
     asm("" : "+v"(y));
     const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return op(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+__device__ __forceinline__ unsigned rows4_bits(unsigned x)
+{
+    unsigned y = x;
+    asm("" : "+v"(y));
+    const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    x = max((unsigned)r[0], (unsigned)r[1]);
+    y = x;
+    asm("" : "+v"(y));
+    const auto t = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    return max((unsigned)t[0], (unsigned)t[1]);
 }
 
 // The sum of a tile's records, for R rows from R rb on, by T >= 16 R threads:
@@ -785,26 +801,28 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     float mrun = -__builtin_inff(), lrun = 0.0f;
 #pragma unroll
     for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
-    int erun = -100;  // O's unit is 2^(erun - 13) (8 bits: 2^erun, and values are 2^-24 times theirs)
+    int erun = -100;  // O's unit in the lane's row is 2^(erun - 12) (8 bits: 2^erun, and values are 2^-24 times theirs)
 
     for (; key0 < c1; key0 += kPassKeys) {
         // ---- scores ----
         const bool fresh = n_new > 0 && key0 + kTileKeys > p.p0;
         if (fresh) fresh_k(key0);
         unsigned badkeys = 0;  // positions of the tile whose key or value is not finite (bit: position - key0)
-        float kscale = 1.0f, kinv = 1.0f, vscale = 1.0f;
-        int vexp = erun;
+        float kscale[2];
         if constexpr (!Q8) {
-            float top = 0.0f;
+            // each position by its own largest element (block b: position 16 b + m)
+            unsigned top[2];
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+            for (int b = 0; b < 2; b++) {
+                float x = 0.0f;
 #pragma unroll
-                for (int i = 0; i < KR; i++) top = max4_abs(top, kraw[b][i]);
-            unsigned wk = wave_max_bits(__float_as_uint(top));
-            if (__builtin_expect(!finite_bits(wk), 0)) {
-                unsigned mk = 0;
+                for (int i = 0; i < KR; i++) x = max4_abs(x, kraw[b][i]);
+                top[b] = rows4_bits(__float_as_uint(x));
+            }
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(!finite_bits(max(top[0], top[1]))) != 0, 0)) {
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
+                    unsigned mk = 0;
                     bool bad = false;
 #pragma unroll
                     for (int i = 0; i < KR; i++) {
@@ -815,12 +833,16 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
                     w |= w >> 32;
                     w |= w >> 16;
                     badkeys |= (unsigned)(w & 0xffffu) << (16 * b);
+                    top[b] = rows4_bits(mk);
                 }
-                wk = wave_max_bits(mk);
             }
-            const int ek = tile_exp(wk);
-            kscale = exp2_int(13 - ek);
-            kinv = exp2_int(ek - 13);
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const int e = tile_exp(top[b]);
+                kscale[b] = exp2_int(13 - e);
+                sh.kf[wave][16 * b + m] = exp2_int(e - 13);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         }
         f32x4 sc[2], sl[2];  // (two accumulators each: products that add to the one before them wait for it)
 #pragma unroll
@@ -835,12 +857,14 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
                     kh = (s & 1) ? bytes_half8(__float_as_uint(w.z), __float_as_uint(w.w))
                                  : bytes_half8(__float_as_uint(w.x), __float_as_uint(w.y));
                 } else {
-                    split8(kraw[b][2 * s], kraw[b][2 * s + 1], kscale, kh, kl);
+                    const float4 f = make_float4(kscale[b], kscale[b], kscale[b], kscale[b]);
+                    split8(mul4(kraw[b][2 * s], f), mul4(kraw[b][2 * s + 1], f), kh, kl);
                 }
                 sl[b] = mfma16(kh, ql[s], sl[b]);
                 sc[b] = mfma16(kh, qh[s], sc[b]);
                 if constexpr (!Q8) sl[b] = mfma16(kl, qh[s], sl[b]);
             }
+        // K's and V's factors of the lane's positions 16 b + 4 g + i
         float4 kscv[2], vscv[2];
         if constexpr (Q8) {
 #pragma unroll
@@ -850,41 +874,46 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
                 kscv[b] = make_float4(ksc[b].x + 0.0f * vsc[b].x, ksc[b].y + 0.0f * vsc[b].y,
                                       ksc[b].z + 0.0f * vsc[b].z, ksc[b].w + 0.0f * vsc[b].w);
             }
-            float mv = 0.0f;
+        } else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-            for (int b = 0; b < 2; b++)
-                mv = fmaxf(mv, fmaxf(fmaxf(vscv[b].x, vscv[b].y), fmaxf(vscv[b].z, vscv[b].w)));  // (NaN counts as nothing)
-            // (scales to at most 1: a probability of 2^15 times them stays in fp16)
-            vexp = max(erun, min(tile_exp(__float_as_uint(rows4<true>(mv))) + 1, 126));
-            vscale = exp2_int(-vexp);
+            for (int b = 0; b < 2; b++) kscv[b] = *reinterpret_cast<const float4 *>(&sh.kf[wave][16 * b + 4 * g]);
         }
         load_k(key0 + kPassKeys);
         if (fresh) fresh_v(key0);
+        float4 vin[2];  // fp32: what V's rows are multiplied by
         if constexpr (!Q8) {
-            float top = 0.0f;
+            unsigned top[8], all = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+            for (int j = 0; j < 8; j++) {
+                float x = 0.0f;
 #pragma unroll
-                for (int i = 0; i < VR; i++) top = max4_abs(top, vraw[j][i]);
-            unsigned wv = wave_max_bits(__float_as_uint(top));
-            if (__builtin_expect(!finite_bits(wv), 0)) {
-                unsigned mv = 0;
+                for (int i = 0; i < VR; i++) x = max4_abs(x, vraw[j][i]);
+                top[j] = dpp_max16(__float_as_uint(x));
+                all = max(all, top[j]);
+            }
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(!finite_bits(all)) != 0, 0)) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
+                    unsigned mv = 0;
                     bool bad = false;
 #pragma unroll
                     for (int i = 0; i < VR; i++) {
                         bad |= zero_bad(vraw[j][i]);
                         mv = max4_bits(mv, vraw[j][i]);
                     }
+                    top[j] = dpp_max16(mv);
                     const uint64_t w = __builtin_amdgcn_ballot_w64(bad);
                     for (int gg = 0; gg < 4; gg++)
                         if ((w >> (16 * gg)) & 0xffffu) badkeys |= 1u << (16 * (j >> 2) + 4 * gg + (j & 3));
                 }
-                wv = wave_max_bits(mv);
             }
-            vexp = max(erun, tile_exp(wv));
-            vscale = exp2_int(13 - vexp);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int e = tile_exp(top[j]);
+                (&vscv[j >> 2].x)[j & 3] = exp2_int(e - 1);
+                (&vin[j >> 2].x)[j & 3] = exp2_int(13 - e);
+            }
         }
 
         // ---- softmax ----
@@ -892,8 +921,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
 #pragma unroll
         for (int t = 0; t < 8; t++) {
             const int b = t >> 2, i = t & 3;
-            const float f = Q8 ? (&kscv[b].x)[i] * qf : kinv * qf;
-            s[t] = (sc[b][i] + sl[b][i]) * f;
+            s[t] = (sc[b][i] + sl[b][i]) * ((&kscv[b].x)[i] * qf);
         }
         if (__builtin_expect(badkeys != 0, 0))
 #pragma unroll
@@ -917,9 +945,18 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             for (int t = 0; t < 8; t++) {
                 const int key = key0 + 16 * (t >> 2) + 4 * g + (t & 3);
                 const bool see = key <= limit || (!STEP && ((sees >> ((key - p.p0) & 63)) & 1));
-                if (!see || key >= c1) s[t] = -__builtin_inff();
+                if (!see || key >= c1) {
+                    s[t] = -__builtin_inff();
+                    (&vscv[t >> 2].x)[t & 3] = 0.0f;
+                }
             }
         }
+        // O's unit in this row: a power of two not below the factors of the
+        // values it has seen, so that P times them stays in fp16
+        float vtop = fmaxf(fmaxf(fmaxf(vscv[0].x, vscv[0].y), fmaxf(vscv[0].z, vscv[0].w)),
+                           fmaxf(fmaxf(vscv[1].x, vscv[1].y), fmaxf(vscv[1].z, vscv[1].w)));  // (NaN counts as nothing)
+        vtop = rows4<true>(vtop);
+        const int vexp = max(erun, min(tile_exp(__float_as_uint(vtop)) + (Q8 ? 1 : 0), 126));
         const float mt = rows4<true>(
             fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
         // (the reference moves only when a score exceeds it by more than 2^8:
@@ -936,16 +973,15 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             for (int v = 0; v < VB; v++) o[v] *= os;
         }
         const float off = (mrun == -__builtin_inff() ? 0.0f : mrun) - kProbBias;  // (a row that has seen nothing yet)
+        const float vscale = exp2_int(-vexp);
         Half8 h, l;
 #pragma unroll
         for (int t = 0; t < 8; t += 2) {
             float x = fast_exp2(s[t] - off), z = fast_exp2(s[t + 1] - off);
             lrun += x + z;
-            if constexpr (Q8) {  // (a scale of NaN marks a row that a masked score must not meet)
-                const int b = t >> 2, i = t & 3;
-                x *= fmaxf((&vscv[b].x)[i] * vscale, 0.0f);
-                z *= fmaxf((&vscv[b].x)[i + 1] * vscale, 0.0f);
-            }
+            // (a scale of NaN marks a row that a masked score must not meet)
+            x *= fmaxf((&vscv[t >> 2].x)[t & 3] * vscale, 0.0f);
+            z *= fmaxf((&vscv[t >> 2].x)[(t & 3) + 1] * vscale, 0.0f);
             split2(x, z, h.h[t / 2], l.h[t / 2]);
         }
         const half8v ph = h.v, pl = l.v;
@@ -967,7 +1003,8 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             } else {
                 const int i = v >> 2, c = v & 3;
                 auto at = [&](int j) { return (&vraw[j][i].x)[c]; };
-                split8(make_float4(at(0), at(1), at(2), at(3)), make_float4(at(4), at(5), at(6), at(7)), vscale, vh, vl);
+                split8(mul4(make_float4(at(0), at(1), at(2), at(3)), vin[0]),
+                       mul4(make_float4(at(4), at(5), at(6), at(7)), vin[1]), vh, vl);
             }
             o[v] = mfma16(vh, pl, o[v]);
             if constexpr (!Q8) o[v] = mfma16(vl, ph, o[v]);
@@ -982,6 +1019,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     if (g == 0) {
         sh.m[wave][m] = mrun;
         sh.l[wave][m] = lrun;
+        sh.unit[wave][m] = exp2_int(max(Q8 ? erun : erun - 12, -126));
     }
     // register i of block v: dim (8 bits) VB (4 g + i) + v, or 64 (v / 4) + 4 (4 g + i) + v % 4
 #pragma unroll
@@ -991,7 +1029,6 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             const int d = Q8 ? VB * (4 * g + i) + v : 16 * v + 4 * (4 * g + i);
             *reinterpret_cast<float4 *>(&sh.o[wave][m][d]) = make_float4(o[v][i], o[v + 1][i], o[v + 2][i], o[v + 3][i]);
         }
-    if (lane == 0) sh.unit[wave] = exp2_int(max(min(Q8 ? erun : erun - 13, 127), -126));
     __syncthreads();
     // (a probability's unit is in both sums)
     const int n_split = a.splits > 1 ? (kv_end + a.chunk - 1) / a.chunk : 1;
@@ -1008,7 +1045,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         for (int w = 0; w < W; w++) {
             const float f = fast_exp2(sh.m[w][row] - top);
             total += f * sh.l[w][row];
-            fma4(acc, f * sh.unit[w], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
+            fma4(acc, f * sh.unit[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
         }
         const bool none = total == 0.0f;  // a chunk none of whose positions the row sees: nothing, weight 0
         scale4(acc, none ? 0.0f : (Q8 ? 0x1p24f : 1.0f) / total);

@@ -602,3 +602,166 @@ def test_block_on_an_8_bit_cache():
         # the new row has at most all of a head's weight: one half step in v, and
         # the keys' half steps move weights by |q| sqrt(hd) / 254 relative at most
         assert np.abs(a - b).max() <= 0.05 * np.abs(b - x).max()
+
+
+# (heads, KV heads, head_dim, cache, tokens): enough (token, head) rows for
+# the tiles of 256, after which the tokens are few enough for those of 16
+BOTH = [(32, 8, 128, "f32", 600), (32, 8, 128, "q8", 600), (32, 8, 64, "f32", 600), (16, 4, 64, "q8", 1700),
+        (8, 2, 128, "f32", 90), (8, 2, 64, "q8", 90)]
+
+
+@pytest.mark.parametrize("where,bad", [("k", 1e30), ("v", 1e30), ("v", np.finfo(np.float32).max), ("k", -1e25), ("v", np.nan)])
+@pytest.mark.parametrize("nh,nkv,hd,cache,n", BOTH)
+def test_huge_rows_that_are_masked_move_nothing(nh, nkv, hd, cache, n, where, bad):
+    """Keys and values of later tokens, ten powers of ten and more above the
+    rest: rows ahead of them, in the same tiles, keep their accuracy."""
+    m = Model(nh, nkv, hd, 2048, 1, cache, key=n)
+    with m.h:
+        m.fill(0, 150)
+        q, k, v = m.tokens(n)
+        for t in (5, 37, 38, 70, n - 3):
+            {"k": k, "v": v}[where][t, t % 7::13] = bad
+        got = m.h.prompt(0, [0, n], [150], q, k, v)
+        # (each stretch of tokens by itself: what is behind it cannot matter)
+        clean = k.copy(), v.copy()
+        for x in clean:
+            x[np.isnan(x) | (np.abs(x) > 1e20)] = 0
+        want = m.want([0, n], [150], q, *clean)
+        _close(got[:5], want[:5])
+        if where == "v" and np.isnan(bad):
+            assert np.isnan(got[n - 3:]).any()
+    m = Model(nh, nkv, hd, 2048, 8, cache, key=n + 1)
+    with m.h:
+        cached = [1900, 3, 700, 0, 33, 1500, 1800, 64]
+        for i, c in enumerate(cached):
+            m.fill(i, c)
+        begin = _begin([64] * 8)
+        parent = np.concatenate([[-1] + [int(m.rng.integers(max(-1, j - 9), j)) for j in range(1, 64)] for _ in range(8)])
+        for i in range(8):  # node 20 of each tree is a leaf
+            p = parent[64 * i:64 * i + 64]
+            p[p == 20] = 19
+        q, k, v = m.tokens(begin[-1])
+        want = m.want(begin, cached, q, k, v, parent)
+        {"k": k, "v": v}[where][20::64] = bad
+        got = m.h.tree(0, begin, cached, parent, q, k, v)
+        ok = np.ones(512, bool)
+        ok[20::64] = False
+        _close(got[ok], want[ok])
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (32, 8, 64)])
+@pytest.mark.parametrize("spread", [1e4, 1e9, 1e14])
+@pytest.mark.parametrize("n", [25, 700])
+def test_keys_and_values_of_unlike_rows(nh, nkv, hd, spread, n):
+    """Neighbouring rows that differ by `spread`, each by its own scale: rows
+    that only see the small ones are as exact as those that see the large."""
+    m = Model(nh, nkv, hd, 1024, 1, "f32", key=int(np.log10(spread)) + n)
+    with m.h:
+        q, k, v = m.tokens(n)
+        k[1::2] *= np.float32(1e-3)
+        v[n // 2::3] *= np.float32(spread)
+        got = m.h.prompt(0, [0, n], [0], q, k, v)
+        want = m.want([0, n], [0], q, k, v)
+        _close(got[:n // 2], want[:n // 2])
+        _close(got[n // 2:], want[n // 2:])
+
+
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+def test_more_than_a_wave_of_sequences(cache):
+    """130 sequences of 0 to 5 tokens, and one step of all of them, some skipped."""
+    import torch
+    n_seq = 130
+    m = Model(8, 2, 64, 128, n_seq, cache)
+    with m.h:
+        lens = m.rng.integers(0, 6, n_seq)
+        cached = m.rng.integers(0, 100, n_seq)
+        for i, c in enumerate(cached):
+            m.fill(i, int(c))
+        begin = _begin(lens)
+        q, k, v = m.tokens(begin[-1])
+        got = m.h.prompt(0, begin, cached, q, k, v)
+        _close(got, m.want(begin, cached, q, k, v))
+        pos = (cached + lens).astype(np.int32)
+        q, k, v = m.tokens(n_seq)
+        want = m.want(np.arange(n_seq + 1), pos, q, k, v)
+        pos[[0, 64, 129]] = [-1, 125, 128]
+        d = [torch.from_numpy(x).cuda() for x in (q, k, v)]
+        out = torch.zeros(n_seq, 512, device="cuda")
+        dp = torch.from_numpy(pos).cuda()
+        m.h.step_batched_async(0, n_seq, _ptr(dp), 110, *map(_ptr, d), _ptr(out), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        assert np.isnan(got[[0, 64, 129]]).all()
+        ok = np.ones(n_seq, bool)
+        ok[[0, 64, 129]] = False
+        _close(got[ok], want[ok])
+
+
+@pytest.mark.parametrize("nh,nkv,hd,cache", [(32, 8, 128, "f32"), (64, 8, 128, "q8"), (64, 8, 64, "f32"), (64, 4, 64, "q8")])
+def test_large_trees_over_a_long_cache(nh, nkv, hd, cache):
+    """64 nodes after 4000 rows: one launch that stores the nodes, chunks on
+    all XCDs; on a stream of its own, behind other work, captured and replayed."""
+    import torch
+    m = Model(nh, nkv, hd, 4096, 1, cache)
+    with m.h:
+        m.fill(0, 4000)
+        parent = np.array([max(-1, j - 1 - j % 5) for j in range(64)], np.int32)
+        q, k, v = m.tokens(64)
+        want = m.want([0, 64], [4000], q, k, v, parent)
+        i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+        begin, pos, par = i32([0, 64]), i32([4000]), i32(parent)
+        src = [torch.from_numpy(x).cuda() for x in (q, k, v)]
+        d = [torch.zeros_like(x) for x in src]
+        out = torch.full((64, nh * hd), 7.0, device="cuda")
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+
+        def call():
+            m.h.tree_async(0, 1, _ptr(begin), _ptr(pos), _ptr(par), 64, 64, 4095, *map(_ptr, d), _ptr(out), s.cuda_stream)
+        with torch.cuda.stream(s):
+            big = torch.randn(2048, 2048, device="cuda")
+            for _ in range(4):
+                big = big @ big * 1e-3
+            for a, b in zip(d, src):
+                a.copy_(b)
+            call()
+        s.synchronize()
+        first = out.cpu().numpy()
+        _close(first, want)
+        m.check_cache([4064])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            call()
+        for _ in range(3):
+            out.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(out.cpu().numpy(), first)
+
+
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+def test_keeping_paths_on_the_device(cache):
+    """Paths that end early, do not ascend, are no nodes or leave the cache."""
+    import torch
+    m = Model(6, 3, 64, 100, 6, cache, layers=2)
+    with m.h:
+        for i in range(6):
+            for l in range(2):
+                k = m.rng.standard_normal((100, 192)).astype(np.float32)
+                m.h.kv_upload(i, l, 0, k, -k)
+        before = [[m.h.kv_download(i, l, 0, 100) for l in range(2)] for i in range(6)]
+        pos = [10, 10, 10, 97, -1, 99]
+        path = [[0, 2, 5, 9], [3, 3, 4, 5], [1, 64, 65, 66], [1, 2, 3, 4], [0, 1, 2, 3], [0, -1, 5, 6]]
+        kept = [4, 1, 1, 2, 0, 1]
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+        dp, dx = i32(pos), i32(path)
+        m.h.tree_keep_async(6, _ptr(dp), _ptr(dx), 4, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        for i in range(6):
+            for l in range(2):
+                for was, now in zip(before[i][l], m.h.kv_download(i, l, 0, 100)):
+                    want = was.copy()
+                    for t in range(kept[i]):
+                        want[pos[i] + t] = was[pos[i] + path[i][t]]
+                    assert np.array_equal(now, want)
