@@ -259,11 +259,13 @@ __device__ __forceinline__ half2v bytes_half(unsigned two)
 {
     return __builtin_bit_cast(half2v, two) - half2v{(_Float16)1152.0f, (_Float16)1152.0f};
 }
-// The same of bytes alone (the halves 0x0000 | byte): values times 2^-24,
-// fp16's subnormals, as exact.
+// The same of bytes alone (the halves 0x0000 | byte, subnormals of fp16):
+// values times 2^-9, as exact.  (Left subnormal, values cost the products
+// bits: errors of 1.7e-6 for 5e-7.)
 __device__ __forceinline__ half2v bytes_small(unsigned two)
 {
-    return __builtin_bit_cast(half2v, two) - __builtin_bit_cast(half2v, 0x00800080u);
+    const _Float16 up = (_Float16)32768.0f, off = (_Float16)-0.25f;
+    return __builtin_elementwise_fma(__builtin_bit_cast(half2v, two), half2v{up, up}, half2v{off, off});
 }
 __device__ __forceinline__ half8v bytes_half8(unsigned a, unsigned b)
 {
@@ -801,7 +803,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     float mrun = -__builtin_inff(), lrun = 0.0f;
 #pragma unroll
     for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
-    int erun = -100;  // O's unit in the lane's row is 2^(erun - 12) (8 bits: 2^erun, and values are 2^-24 times theirs)
+    int erun = -100;  // O's unit in the lane's row is 2^(erun - 12) (8 bits: 2^erun, and values are 2^-9 times theirs)
 
     for (; key0 < c1; key0 += kPassKeys) {
         // ---- scores ----
@@ -1048,7 +1050,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             fma4(acc, f * sh.unit[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
         }
         const bool none = total == 0.0f;  // a chunk none of whose positions the row sees: nothing, weight 0
-        scale4(acc, none ? 0.0f : (Q8 ? 0x1p24f : 1.0f) / total);
+        scale4(acc, none ? 0.0f : (Q8 ? 0x1p9f : 1.0f) / total);
         if (n_split == 1) {
             const int j = STEP ? 0 : (int)fast_div((uint32_t)r, a.by_group);
             const int head = kvh * a.group + r - j * a.group;
