@@ -6,28 +6,32 @@
 //
 // Per wave and tile of 32 positions at head_dim 128: 48 32x32x16 MFMAs (three
 // products of S^T = K Q^T and of O^T = V^T P^T), 1536 cycles of the matrix
-// core, and about 300 vector instructions (scaling, maximum, 16 exponentials,
-// the split of P, a share of the next tile's split), 1200 cycles.  The two
-// waves of a SIMD do these in turn: waves 0-3 are in the matrix phase (the
-// scores of tile i + 1, the weighted values of tile i) while waves 4-7 are in
-// the vector phase, a barrier between the half-steps.
+// core, and about 300 vector instructions: 250 of the vector phase (the
+// scores' scaling, maximum and 16 exponentials, the split of P, the largest
+// magnitudes of a share of the next tile) and that share's split, which fills
+// the waits between the products of the matrix phase (in the vector phase it
+// took 4 to 10% longer).  The two waves of a SIMD do these in turn: waves 0-3
+// are in the matrix phase (the scores of tile i + 1, the weighted values of
+// tile i) while waves 4-7 are in the vector phase, a barrier between the
+// half-steps.
 //
 // Half-step h of waves 0-3: scores of tile 0 at h = 0, vector phase i at
 // 2 i + 1, matrix phase i at 2 i + 2; waves 4-7 one half-step later.  Waves
-// 4-7 bring K: tile i + 2 in vector phase i (h = 2 i + 2), read from h = 2 (i
+// 4-7 bring K: tile i + 2 in matrix phase i (h = 2 i + 3), read from h = 2 (i
 // + 2) on, when the buffer's last tile i was read last at h = 2 i + 1: two
-// buffers.  Waves 0-3 bring V: tile i + 1 in vector phase i (h = 2 i + 1),
-// whose quads' exponents the vector phase i + 1 needs, read last at h = 2 i +
-// 5: three buffers.
+// buffers.  Waves 0-3 bring V: tile i + 1 in matrix phase i (h = 2 i + 2),
+// read from h = 2 i + 4 to 2 i + 5: three buffers.  The factors are written a
+// half-step earlier, K's of tile i + 2 at h = 2 i + 2, V's of tile i + 1 at
+// 2 i + 1, and read in vector phases until h = 2 i + 6 and 2 i + 4: four.
 //
 // Scales: K's and V's exponents by quads of four positions (8-bit caches:
 // scales by position).  K's multiply the scores, V's go into the
 // probabilities, relative to the largest that the row has seen so far (vrun),
 // O's unit in that row.  A quad of positions whose magnitudes are unlike gets
-// an exponent for each, counted in its tile's scores and probabilities: so what a row does not see, or weighs at nothing,
-// takes none of its accuracy.  (On one card in turns, 32 q heads, 8 KV heads,
-// head_dim 128, 8192 tokens: 1817 us, for 1721 with exponents by quad and
-// one unit alone, and 10 to 20% more than that by position throughout.)
+// an exponent for each, counted in its tile's scores and probabilities: so what
+// a row does not see takes none of its accuracy.  (On one card in turns, 32 q
+// heads, 8 KV heads, head_dim 128, 8192 tokens: 6% more time than exponents by
+// quad and one unit for all rows; by position throughout 10 to 20% more.)
 //
 // The running maximum is a reference that moves only when a score exceeds it
 // by more than 2^8 (then O and the sum are rescaled): probabilities are
@@ -222,15 +226,19 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     };
     // That share into LDS, split, with its factors.
     auto v_piece = [&](int d, int piece) LEAP_INLINE { return d * 4 + (piece ^ (((d >> 1) ^ (d >> 3)) & 3)); };
-    auto stage_tile = [&](auto role, int i) LEAP_INLINE {
+    // First looked over, in the vector phase, then split, between the products
+    // of the matrix phase (whose waits that fills).
+    constexpr int N = HD / 16;  // fp32: a lane's elements of a quad
+    constexpr int kPieces = Q8 ? 1 : N;
+    float stage_sc[2];
+    auto stage_look = [&](auto role, int i) LEAP_INLINE {
         constexpr bool V = decltype(role)::value;
-        if (i >= n_tiles) return;
+        if (Q8 || i >= n_tiles) return;
         int oddbits = 0, ln = lane;
         asm volatile("" : "+v"(ln));  // (addresses formed anew, for the registers' sake)
         if constexpr (!Q8) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                constexpr int N = HD / 16;
                 float *x = raw + N * t;
                 const int quad = w + 4 * t;
                 // the lane's largest by position (K: of its one), the quad's;
@@ -278,7 +286,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                     look();
                 }
                 const int e = tile_exp(most);
-                const float sc = exp2_int(13 - e);
+                stage_sc[t] = exp2_int(13 - e);
                 if (__builtin_expect(unlike, 0)) {
                     // positions far below their neighbours: each by its own exponent
 #pragma unroll
@@ -300,66 +308,76 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                     sh.vquad[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
                 else
                     sh.kquad[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
-                unsigned h[N / 2], l[N / 2];
-#pragma unroll
-                for (int e2 = 0; e2 < N / 2; e2++) split2_scaled(x[2 * e2], x[2 * e2 + 1], sc, h[e2], l[e2]);
-                if constexpr (!V) {
-                    const int pos = 4 * quad + (ln >> 4);
-                    if constexpr (HD == 128) {
-                        const int at = pos * C + ((ln & 15) ^ (pos & (C - 1)));
-                        *reinterpret_cast<u32x4 *>(&sh.k[i & 1][0][at]) = u32x4{h[0], h[1], h[2], h[3]};
-                        *reinterpret_cast<u32x4 *>(&sh.k[i & 1][1][at]) = u32x4{l[0], l[1], l[2], l[3]};
-                    } else {
-                        const int at = pos * C + (((ln & 15) >> 1) ^ (pos & (C - 1)));
-                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][0][at]) + (ln & 1)) = u32x2{h[0], h[1]};
-                        *(reinterpret_cast<u32x2 *>(&sh.k[i & 1][1][at]) + (ln & 1)) = u32x2{l[0], l[1]};
-                    }
-                } else {
-                    const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
-#pragma unroll
-                    for (int u = 0; u < HD / 64; u++) {
-                        const int d = ln + 64 * u, at = v_piece(d, piece);
-                        *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][at]) + half) = u32x2{h[2 * u], h[2 * u + 1]};
-                        *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][1][at]) + half) = u32x2{l[2 * u], l[2 * u + 1]};
-                    }
-                }
             }
-        } else if constexpr (!V) {
-            const int pos = 8 * w + (ln >> 3);
-            if constexpr (HD == 128) {
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-                    sh.k[i & 1][0][pos * C + ((2 * (ln & 7) + u) ^ (pos & (C - 1)))] =
-                        bytes_half8(__float_as_uint(raw[2 * u]), __float_as_uint(raw[2 * u + 1]));
-            } else {
-                sh.k[i & 1][0][pos * C + ((ln & 7) ^ (pos & (C - 1)))] =
-                    bytes_half8(__float_as_uint(raw[0]), __float_as_uint(raw[1]));
-            }
-            if ((ln & 7) == 0) sh.kfac[i & 3][(pos >> 2) & 1][4 * (pos >> 3) + (pos & 3)] = sck + 0.0f * scv;
-        } else if (HD == 128 || w < 2) {
-            int quad = v8_quad, d0 = v8_dim;
-            asm volatile("" : "+v"(quad), "+v"(d0));  // (addresses formed anew, as below)
-            const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
-            unsigned x[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = __float_as_uint(raw[j]) ^ 0x80808080u;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const unsigned sel = 0x0c000c00u | (unsigned)(4 + c) << 16 | (unsigned)c;
-                const half2v p0 = bytes_half(__builtin_amdgcn_perm(x[1], x[0], sel) | 0x64006400u);
-                const half2v p1 = bytes_half(__builtin_amdgcn_perm(x[3], x[2], sel) | 0x64006400u);
-                const int d = d0 + c;
-                *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][v_piece(d, piece)]) + half) =
-                    u32x2{__builtin_bit_cast(unsigned, p0), __builtin_bit_cast(unsigned, p1)};
-            }
-            if ((ln & (LR - 1)) == 0)
-#pragma unroll
-                for (int j = 0; j < 4; j++) sh.vfac[i & 3][quad & 1][4 * (quad >> 1) + j] = sv4[j];
         }
+        sh.odd[i & 3][wave] = oddbits;
+        if (__builtin_expect(oddbits != 0, 0)) sh.any_odd = 1;
+    };
+    unsigned hi[2], lo[2];
+    constexpr int P = WideShared<HD, Q8>::P;
+    // (fp32: the lane's first place; the others are 16 positions of K on, 64
+    // dims of V on, or in the piece 2 away, where the swizzles repeat)
+    auto stage_place = [&](auto role) LEAP_INLINE {
+        constexpr bool V = decltype(role)::value;
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int pos = 4 * w + (ln >> 4);
+        return V ? 2 * v_piece(ln, w & 1) + (w >> 1)
+                 : 2 * (pos * C + ((HD == 128 ? ln & 15 : (ln & 15) >> 1) ^ (pos & (C - 1)))) + (HD == 128 ? 0 : ln & 1);
+    };
+    // (a tile past the chunk's last goes where none is read any more)
+    auto stage_piece = [&](auto role, int i, int piece, int place) LEAP_INLINE {
+        constexpr bool V = decltype(role)::value;
         if constexpr (!Q8) {
-            sh.odd[i & 3][wave] = oddbits;
-            if (__builtin_expect(oddbits != 0, 0)) sh.any_odd = 1;
+            const int t = piece / (N / 2), e2 = piece % (N / 2), h = e2 & 1;
+            split2_scaled(raw[N * t + 2 * e2], raw[N * t + 2 * e2 + 1], stage_sc[t], hi[h], lo[h]);
+            if (h == 0) return;
+            const int at = V ? (t ? place ^ 4 : place) + 2 * 4 * 64 * (e2 >> 1) : place + 2 * 16 * C * t + (e2 >> 1);
+            u32x2 *to_h = reinterpret_cast<u32x2 *>(V ? sh.v[i % 3][0] : sh.k[i & 1][0]);
+            u32x2 *to_l = reinterpret_cast<u32x2 *>(V ? sh.v[i % 3][P - 1] : sh.k[i & 1][P - 1]);
+            to_h[at] = u32x2{hi[0], hi[1]};
+            to_l[at] = u32x2{lo[0], lo[1]};
+        } else {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            if constexpr (!V) {
+                const int pos = 8 * w + (ln >> 3);
+                if constexpr (HD == 128) {
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        sh.k[i & 1][0][pos * C + ((2 * (ln & 7) + u) ^ (pos & (C - 1)))] =
+                            bytes_half8(__float_as_uint(raw[2 * u]), __float_as_uint(raw[2 * u + 1]));
+                } else {
+                    sh.k[i & 1][0][pos * C + ((ln & 7) ^ (pos & (C - 1)))] =
+                        bytes_half8(__float_as_uint(raw[0]), __float_as_uint(raw[1]));
+                }
+                if ((ln & 7) == 0) sh.kfac[i & 3][(pos >> 2) & 1][4 * (pos >> 3) + (pos & 3)] = sck + 0.0f * scv;
+            } else if (HD == 128 || w < 2) {
+                int quad = v8_quad, d0 = v8_dim;
+                asm volatile("" : "+v"(quad), "+v"(d0));  // (addresses formed anew, as below)
+                const int piece = 2 * (quad >> 2) + (quad & 1), half = (quad >> 1) & 1;
+                unsigned x[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] = __float_as_uint(raw[j]) ^ 0x80808080u;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const unsigned sel = 0x0c000c00u | (unsigned)(4 + c) << 16 | (unsigned)c;
+                    const half2v p0 = bytes_half(__builtin_amdgcn_perm(x[1], x[0], sel) | 0x64006400u);
+                    const half2v p1 = bytes_half(__builtin_amdgcn_perm(x[3], x[2], sel) | 0x64006400u);
+                    const int d = d0 + c;
+                    *(reinterpret_cast<u32x2 *>(&sh.v[i % 3][0][v_piece(d, piece)]) + half) =
+                        u32x2{__builtin_bit_cast(unsigned, p0), __builtin_bit_cast(unsigned, p1)};
+                }
+                if ((ln & (LR - 1)) == 0)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sh.vfac[i & 3][quad & 1][4 * (quad >> 1) + j] = sv4[j];
+            }
         }
+    };
+    auto stage_tile = [&](auto role, int i) LEAP_INLINE {
+        stage_look(role, i);
+#pragma unroll
+        for (int x = 0; x < kPieces; x++) stage_piece(role, i, x, stage_place(role));
     };
 
     // ---- Q: 32 rows a wave, in registers as the products' B operand ----
@@ -476,10 +494,11 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     // The scores of tile i + 1 and the weighted values of tile i, in turns: a
     // product that adds to the one before it would wait for it.  (After the
     // last tile the scores are of what an earlier one left, and not used.)
-    auto matrix = [&](int i) LEAP_INLINE {
+    auto matrix = [&](auto role, int i, int next) LEAP_INLINE {
         clear_scores();
         int kf = k_first, vf = v_first;
         asm volatile("" : "+v"(kf), "+v"(vf));
+        const int place = Q8 ? 0 : stage_place(role);
         const half8v *k = sh.k[(i + 1) & 1][0], *x = sh.v[i % 3][0];
         constexpr int D = 2;  // steps that the operands are read ahead
         half8v kh[D + 1], kl[D + 1], vh[D + 1], vl[D + 1], low[D + 1];
@@ -501,6 +520,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             s = mfma32(kh[e], qh[t], s);
             o[v] = mfma32(vh[e], pl[u], o[v]);
             __builtin_amdgcn_sched_barrier(0);
+            if (Q8 ? t == 1 : t < kPieces) stage_piece(role, next, Q8 ? 0 : t, place);
             if constexpr (!Q8) {
                 s = mfma32(kl[e], qh[t], s);
                 o[v] = mfma32(vl[e], ph[u], o[v]);
@@ -671,14 +691,17 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             const int next = V ? i + 1 : i + 2;
             if (!idle) softmax(i);
             __builtin_amdgcn_sched_barrier(0);
-            stage_tile(role, next);
-            load_tile(role, next + 1);
+            stage_look(role, next);
             __syncthreads();
             if (!idle) {
                 __builtin_amdgcn_s_setprio(1);  // (the matrix phase's few instructions before the vector phase's many)
-                matrix(i);
+                matrix(role, i, next);
                 __builtin_amdgcn_s_setprio(0);
+            } else {
+#pragma unroll
+                for (int x = 0; x < kPieces; x++) stage_piece(role, next, x, stage_place(role));
             }
+            load_tile(role, next + 1);
             __syncthreads();
         }
         if constexpr (V) __syncthreads();
