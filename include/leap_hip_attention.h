@@ -181,9 +181,13 @@ int leap_hip_attention_step_noalloc(const leap_hip_attention_config *cfg, int po
  * every token is rotated for its position, its k and v are stored, and it
  * attends causally, to the rows [0, pos[i] + j] (cached ones and those of
  * this call).  A sequence may have no tokens; rows behind begin[n_seq] and
- * before begin[0] are left alone.  Sizes, tile and chunk lengths move results
- * by fp32 rounding only.  An output row that attends to a key or value row
- * with an infinity or a NaN is NaN; rows that do not are not affected.
+ * before begin[0] are left alone.  Tile and chunk lengths, which sizes choose,
+ * move results by fp32 rounding only: keys, values and weights are held to
+ * 2^-22 of themselves (below 2^-28 of their row's largest element, to 2^-39 of
+ * that; values whose rows are below 2^-12 of the largest row attended to, to
+ * 2^-32 of that one), sums are fp32.  An output row that attends to a key or
+ * value row with an infinity or a NaN is NaN; what a row does not attend to
+ * does not affect it, whatever its size.
  * Host pointers: begin [n_seq+1] ascending from >= 0, pos [n_seq]; returns
  * when `out` is written.  -EINVAL, with nothing changed, if a sequence's
  * positions leave [0, seq_len). */

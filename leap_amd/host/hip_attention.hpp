@@ -27,6 +27,7 @@ public:
         float rope_theta = 500000.0f;  // FloatTransformer.cpp:65
         int max_batch = 1;
         int device = 0;
+        bool cache_q8 = false;  // an 8-bit cache (leap_hip_attention_create_q8kv)
     };
 
     explicit HipAttention(const Dims &d)
@@ -34,7 +35,7 @@ public:
         const leap_hip_attention_config c{d.n_layers, d.layer_begin, d.layer_end, d.n_heads,
                                           d.n_kv_heads, d.head_dim,    d.seq_len,   d.rope_theta,
                                           d.max_batch,  d.device};
-        check(leap_hip_attention_create(&c, &h_), nullptr);
+        check(d.cache_q8 ? leap_hip_attention_create_q8kv(&c, &h_) : leap_hip_attention_create(&c, &h_), nullptr);
         q_dim_ = d.n_heads * d.head_dim;
         kv_dim_ = d.n_kv_heads * d.head_dim;
     }
@@ -52,6 +53,38 @@ public:
             (int)v_new.size() != kv_dim_)
             throw std::invalid_argument("HipAttention::step: buffer sizes do not match the model");
         check(leap_hip_attention_step(h_, layer, pos, q.data(), k_new.data(), v_new.data(), out.data()), h_);
+    }
+
+    // step() over whole prompts: tokens begin[i] .. begin[i+1] - 1 of the packed
+    // rows are sequence i's, from position pos[i] on.
+    void prompt(int layer, std::span<const int> begin, std::span<const int> pos, std::span<const float> q,
+                std::span<const float> k_new, std::span<const float> v_new, std::span<float> out)
+    {
+        check_rows("prompt", begin, pos, q, k_new, v_new, out);
+        check(leap_hip_attention_prompt(h_, layer, (int)pos.size(), begin.data(), pos.data(), q.data(), k_new.data(),
+                                        v_new.data(), out.data()),
+              h_);
+    }
+
+    // The same of drafted trees: parent of each node within its tree, or -1.
+    void tree(int layer, std::span<const int> begin, std::span<const int> pos, std::span<const int> parent,
+              std::span<const float> q, std::span<const float> k_new, std::span<const float> v_new, std::span<float> out)
+    {
+        check_rows("tree", begin, pos, q, k_new, v_new, out);
+        if (parent.size() * (size_t)q_dim_ != q.size())
+            throw std::invalid_argument("HipAttention::tree: one parent a row");
+        check(leap_hip_attention_tree(h_, layer, (int)pos.size(), begin.data(), pos.data(), parent.data(), q.data(),
+                                      k_new.data(), v_new.data(), out.data()),
+              h_);
+    }
+
+    // The accepted paths' rows ([pos.size()][max_path] nodes, ended by -1) to
+    // pos[i], pos[i] + 1, ..., in every held layer.
+    void tree_keep(std::span<const int> pos, std::span<const int> path, int max_path)
+    {
+        if (max_path < 0 || path.size() != pos.size() * (size_t)max_path)
+            throw std::invalid_argument("HipAttention::tree_keep: path must hold max_path nodes a sequence");
+        check(leap_hip_attention_tree_keep(h_, (int)pos.size(), pos.data(), path.data(), max_path), h_);
     }
 
     // Weights of one held layer for block(): the layer's slices of
@@ -168,6 +201,16 @@ private:
         if (rc != 0)
             throw std::runtime_error(std::string("leap_hip_attention: ") + leap_hip_attention_last_error(h) +
                                      " (status " + std::to_string(rc) + ")");
+    }
+
+    void check_rows(const char *what, std::span<const int> begin, std::span<const int> pos, std::span<const float> q,
+                    std::span<const float> k_new, std::span<const float> v_new, std::span<float> out) const
+    {
+        const size_t n = q.size() / (size_t)q_dim_;
+        if (pos.empty() || begin.size() != pos.size() + 1 || begin.back() < 0 || (size_t)begin.back() > n ||
+            q.size() != n * (size_t)q_dim_ || out.size() != q.size() || k_new.size() != n * (size_t)kv_dim_ ||
+            v_new.size() != k_new.size())
+            throw std::invalid_argument(std::string("HipAttention::") + what + ": buffer sizes do not match");
     }
 
     leap_hip_attention *h_ = nullptr;
