@@ -863,12 +863,15 @@ int many_reserve(leap_hip_attention *h, hipStream_t stream)
     if (cap != hipStreamCaptureStatusNone)
         return set_err(h, -EINVAL, "a handle's first prompt or tree call allocates its workspace: make one before capturing");
     HIP_TRY(h, load_many_table(h->cfg.head_dim));
-    if (int rc = alloc_all(h, {{(void **)&h->many_o, kManyRecords * h->cfg.head_dim * sizeof(float)},
-                               {(void **)&h->many_lse, kManyRecords * sizeof(float)},
-                               {(void **)&h->many_counters, kManyCounters * sizeof(int)}}))
-        return rc;
+    float *o = nullptr;  // (in the handle once the others are ready)
+    if (!h->many_counters)
+        if (int rc = alloc_all(h, {{(void **)&h->many_lse, kManyRecords * sizeof(float)},
+                                   {(void **)&h->many_counters, kManyCounters * sizeof(int)}}))
+            return rc;
     HIP_TRY(h, hipMemsetAsync(h->many_counters, 0, kManyCounters * sizeof(int), h->stream));
     HIP_TRY(h, hipStreamSynchronize(h->stream));
+    if (int rc = alloc_all(h, {{(void **)&o, kManyRecords * h->cfg.head_dim * sizeof(float)}})) return rc;
+    h->many_o = o;
     return 0;
 }
 
