@@ -116,8 +116,8 @@ bool pick_q8(int dim, int gs, int kind, int rows, int n_cu, Q8Launch *out);
 enum ManyKind { kManyStep, kManySmall, kManyWide };
 using ManyFn = void (*)(leap::ManyArgs);
 struct ManyKernels {
-    ManyFn append, attention, merge;
-    int waves, rows;  // of the attention kernel's workgroups
+    ManyFn append, attention, merge[2];  // (merge: kMergeRows rows a workgroup)
+    int waves, rows;                     // of the attention kernel's workgroups
 };
 // The quantising write of an 8-bit cache's rows, and their reading back.
 using RowsFn = void (*)(leap::RowsArgs);

@@ -10,14 +10,16 @@ namespace leap_kernels {
 template <int HD>
 ManyKernels pick_many_hd(ManyKind kind, bool q8)
 {
-    constexpr int R = leap::kManyRows;
+    constexpr int R = leap::kManyRows, B = leap::kWideRows;
     const ManyFn append = q8 ? leap::many_append_kernel<HD, true> : leap::many_append_kernel<HD, false>;
     if (kind == kManyWide)
         return {append, q8 ? leap::wide_attention_kernel<HD, true> : leap::wide_attention_kernel<HD, false>,
-                leap::many_merge_kernel<HD, leap::kWideRows>, leap::kWideWaves, leap::kWideRows};
-    if (!q8) return {append, leap::many_attention_kernel<HD, 4, false, false>, leap::many_merge_kernel<HD, R>, 4, R};
+                {leap::many_merge_kernel<HD, B, 4>, leap::many_merge_kernel<HD, B, 16>}, leap::kWideWaves, B};
+    // (tiles of 16 rows are spread in groups of fewer than 8: never the merge of many)
+    const ManyFn merge = leap::many_merge_kernel<HD, R, 4>;
+    if (!q8) return {append, leap::many_attention_kernel<HD, 4, false, false>, {merge, nullptr}, 4, R};
     return {append, kind == kManyStep ? leap::many_attention_kernel<HD, 8, true, true> : leap::many_attention_kernel<HD, 8, true, false>,
-            leap::many_merge_kernel<HD, R>, 8, R};
+            {merge, nullptr}, 8, R};
 }
 
 template <int HD>

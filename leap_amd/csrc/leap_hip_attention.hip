@@ -932,7 +932,10 @@ int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, c
         HIP_TRY(h, launch_k(p.fn.append, dim3((unsigned)((n_tokens + leap::kAppendWaves - 1) / leap::kAppendWaves)),
                             dim3(leap::kAppendWaves * leap::kWave), stream, a));
     HIP_TRY(h, launch_k(p.fn.attention, dim3((unsigned)p.wgs), dim3((unsigned)(p.fn.waves * leap::kWave)), stream, a));
-    if (p.spread) HIP_TRY(h, launch_k(p.fn.merge, dim3((unsigned)(p.groups * (p.fn.rows / leap::kMergeRows))), dim3(256), stream, a));
+    if (p.spread) {
+        const int many = p.fn.merge[1] && p.groups * p.fn.rows / leap::kMergeRows[1] >= 4 * h->n_cu;
+        HIP_TRY(h, launch_k(p.fn.merge[many], dim3((unsigned)(p.groups * (p.fn.rows / leap::kMergeRows[many]))), dim3(256), stream, a));
+    }
     return 0;
 }
 

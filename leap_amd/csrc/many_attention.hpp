@@ -383,23 +383,39 @@ __global__ __launch_bounds__(kAppendWaves * kWave) void many_append_kernel(ManyA
     const int lane = threadIdx.x & (kWave - 1);
     const int r = blockIdx.x * kAppendWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (r >= a.n_tokens) return;
+    constexpr int LR = HD / 4, kAhead = 4;  // lanes of a head row, words a lane has on their way
+    const int words = a.n_kv_heads * LR;
+    const float4 *kn = reinterpret_cast<const float4 *>(a.k_new) + (size_t)r * words;
+    const float4 *vn = reinterpret_cast<const float4 *>(a.v_new) + (size_t)r * words;
+    float4 k[kAhead], v[kAhead];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int i = first + kWave * u + lane;
+            k[u] = i < words ? kn[i] : make_float4(0, 0, 0, 0);
+            v[u] = i < words ? vn[i] : make_float4(0, 0, 0, 0);
+        }
+    };
+    load(0);  // (ahead of the token's place)
     const TokenPlace t = find_token(a, r, lane);
     if (t.seq < 0) return;
     if (t.skip) {
-        fill_nan<HD>(a.out, (size_t)r * a.n_heads * (HD / 4), a.n_heads * (HD / 4), lane, kWave);
+        fill_nan<HD>(a.out, (size_t)r * a.n_heads * LR, a.n_heads * LR, lane, kWave);
         return;
     }
-    constexpr int LR = HD / 4;  // lanes of a head row
-    const int words = a.n_kv_heads * LR;
     const float4 turn = a.rope[(size_t)t.at * LR + (lane & (LR - 1))];
-    const float4 *kn = reinterpret_cast<const float4 *>(a.k_new) + (size_t)r * words;
-    const float4 *vn = reinterpret_cast<const float4 *>(a.v_new) + (size_t)r * words;
-    for (int i = lane; i < words; i += kWave) {
-        const float4 k = rope4(kn[i], turn), v = vn[i];
-        float sk = 0.0f, sv = 0.0f;
-        const int qk = Q8 ? quantize_row<HD>(k, &sk) : 0, qv = Q8 ? quantize_row<HD>(v, &sv) : 0;
-        store_row<HD, Q8>(a, t.seq, t.row, i, k, qk, sk, false);
-        store_row<HD, Q8>(a, t.seq, t.row, i, v, qv, sv, true);
+    for (int first = 0; first < words; first += kWave * kAhead) {
+        if (first) load(first);
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const int i = first + kWave * u + lane;
+            if (i >= words) break;
+            const float4 y = rope4(k[u], turn);
+            float sk = 0.0f, sv = 0.0f;
+            const int qk = Q8 ? quantize_row<HD>(y, &sk) : 0, qv = Q8 ? quantize_row<HD>(v[u], &sv) : 0;
+            store_row<HD, Q8>(a, t.seq, t.row, i, y, qk, sk, false);
+            store_row<HD, Q8>(a, t.seq, t.row, i, v[u], qv, sv, true);
+        }
     }
 }
 
@@ -1076,18 +1092,21 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     if (sh.last) merge_rows<HD, BM, BM, kThreads>(a, sh.merge, gi, n_split, p, kvh, 0, tid);
 }
 
-// The records of a spread launch's tiles of BM rows added up, kMergeRows rows
-// a workgroup.
-constexpr int kMergeRows = 4;
-template <int HD, int BM>
+// The records of a spread launch's tiles of BM rows added up, R rows a
+// workgroup: 4, or 16 where those are four workgroups a CU and more (256-row
+// tiles at head_dim 128, us with 4 : 16: 8 trees of 64 nodes of 64/8 heads in
+// two chunks 21.2 : 11.8, a tree of 31 nodes of 32/8 heads in 32 chunks
+// 7.0 : 9.5).
+constexpr int kMergeRows[2] = {4, 16};
+template <int HD, int BM, int R>
 __global__ __launch_bounds__(256) void many_merge_kernel(ManyArgs a)
 {
     __shared__ struct {
-        float w[kMergeRows][kManySplits + 1];
+        float w[R][kManySplits + 1];
         float4 part[256];
     } sh;
     const int tid = threadIdx.x;
-    const int gi = blockIdx.x / (BM / kMergeRows), rb = blockIdx.x % (BM / kMergeRows);
+    const int gi = blockIdx.x / (BM / R), rb = blockIdx.x % (BM / R);
     const int slot = (int)fast_div((uint32_t)gi, a.by_kv_heads);
     const int kvh = gi - slot * a.n_kv_heads;
     const Place p = find_place<BM>(a, slot, tid & (kWave - 1));
@@ -1095,7 +1114,7 @@ __global__ __launch_bounds__(256) void many_merge_kernel(ManyArgs a)
     const int j1 = min(p.n - 1, (int)fast_div((uint32_t)(p.tile * BM + BM - 1), a.by_group));
     const int kv_end = a.parent ? p.p0 + p.n : p.p0 + j1 + 1;
     const int n_split = (kv_end + a.chunk - 1) / a.chunk;
-    if (n_split > 1) merge_rows<HD, BM, kMergeRows, 256>(a, sh, gi, n_split, p, kvh, rb, tid);
+    if (n_split > 1) merge_rows<HD, BM, R, 256>(a, sh, gi, n_split, p, kvh, rb, tid);
 }
 
 // ---- rows of a cache, moved ---------------------------------------------------
