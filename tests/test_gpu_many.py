@@ -765,3 +765,36 @@ def test_keeping_paths_on_the_device(cache):
                     for t in range(kept[i]):
                         want[pos[i] + t] = was[pos[i] + path[i][t]]
                     assert np.array_equal(now, want)
+
+
+def test_rows_past_two_gibibytes():
+    """A layer slab of 2.9 GB, on a handle that holds the second of three
+    layers: rows of zeros but for the last ones, whose byte offsets pass 2^31."""
+    nh, hd, seq_len, real = 32, 128, 180000, 40
+    rng = rng_for(0x32676962)
+    with HipAttention(nh, nh, hd, seq_len, n_layers=3, layer_begin=1, layer_end=2) as h:
+        cos, sin = h.rope_download()
+        for n, pos, tree in ((3, seq_len - 3, False), (64, seq_len - 64, True)):
+            h.clear()
+            k0, v0 = (rng.standard_normal((real, nh * hd)).astype(np.float32) for _ in range(2))
+            h.kv_upload(0, 1, pos - real, k0, v0)
+            q, k, v = (s * rng.standard_normal((n, nh * hd)).astype(np.float32) for s in (4.0, 1.0, 1.0))
+            q, k, v = (x.astype(np.float32) for x in (q, k, v))
+            parent = np.full(n, -1, np.int32)
+            got = h.tree(1, [0, n], [pos], parent, q, k, v) if tree else h.prompt(1, [0, n], [pos], q, k, v)
+            want = np.zeros((n, nh, hd))
+            for j in range(n):
+                at = pos if tree else pos + j
+                qr = rope_f32(q[j], cos[at], sin[at]).astype(np.float64).reshape(nh, hd)
+                own = [j] if tree else list(range(j + 1))
+                ks = np.concatenate([k0] + [rope_f32(k[t], cos[pos if tree else pos + t], sin[pos if tree else pos + t])[None]
+                                            for t in own]).astype(np.float64).reshape(-1, nh, hd)
+                vs = np.concatenate([v0] + [v[t][None] for t in own]).astype(np.float64).reshape(-1, nh, hd)
+                s = np.einsum("hd,thd->ht", qr, ks) / np.sqrt(hd)
+                w = np.exp(s - np.maximum(s.max(axis=1, keepdims=True), 0))
+                zeros = (pos - real) * np.exp(-np.maximum(s.max(axis=1), 0))
+                want[j] = np.einsum("ht,thd->hd", w, vs) / (w.sum(axis=1) + zeros)[:, None]
+            _close(got, want.reshape(n, -1))
+            kk, vv = h.kv_download(0, 1, pos, pos + n)
+            assert np.array_equal(vv, v)
+            assert not np.any(h.kv_download(0, 1, 0, 1000)[0]) and not np.any(h.kv_download(0, 1, pos - real - 1000, pos - real)[1])
