@@ -798,3 +798,24 @@ def test_rows_past_two_gibibytes():
             kk, vv = h.kv_download(0, 1, pos, pos + n)
             assert np.array_equal(vv, v)
             assert not np.any(h.kv_download(0, 1, 0, 1000)[0]) and not np.any(h.kv_download(0, 1, pos - real - 1000, pos - real)[1])
+
+
+@pytest.mark.parametrize("nh,nkv,hd,cache,n", [(32, 8, 128, "f32", 600), (32, 8, 64, "f32", 600), (32, 8, 128, "q8", 600)])
+@pytest.mark.parametrize("where,bad", [("k", np.inf), ("k", np.nan), ("v", -np.inf)])
+def test_infinities_in_tiles_of_many_rows(nh, nkv, hd, cache, n, where, bad):
+    """One key or value of KV head 3 that is not finite at token 333, and a
+    quad of unlike neighbours beside it."""
+    m = Model(nh, nkv, hd, 1024, 1, cache, key=n + 7)
+    with m.h:
+        m.fill(0, 61)
+        q, k, v = m.tokens(n)
+        v[329:331] *= np.float32(1e-7)
+        k[331] *= np.float32(1e-6)
+        want = m.want([0, n], [61], q, k, v).reshape(n, nh, hd)
+        {"k": k, "v": v}[where][333, 3 * hd + 11] = bad
+        got = m.h.prompt(0, [0, n], [61], q, k, v).reshape(n, nh, hd)
+        seen = np.zeros((n, nh), bool)
+        group = nh // nkv
+        seen[333:, 3 * group:4 * group] = True
+        assert np.isnan(got[seen]).all()
+        _close(got[~seen], want[~seen])
