@@ -2134,10 +2134,12 @@ static int many_host(leap_hip_attention *h, int layer, int n_seq, const int *beg
         return set_err(h, -EINVAL, "n_seq %d outside [1, %d]", n_seq, h->cfg.max_batch);
     if (!begin || !pos || (tree && !parent)) return set_err(h, -EINVAL, "NULL buffer");
     if (begin[0] < 0) return set_err(h, -EINVAL, "begin[0] = %d is negative", begin[0]);
-    int max_tokens = 0, max_pos = 0;
-    for (int i = 0; i < n_seq; i++) {
+    // (all of them, ahead of the parents: those end at begin[n_seq])
+    for (int i = 0; i < n_seq; i++)
         if (begin[i + 1] < begin[i])
             return set_err(h, -EINVAL, "begin[%d] = %d is below begin[%d] = %d", i + 1, begin[i + 1], i, begin[i]);
+    int max_tokens = 0, max_pos = 0;
+    for (int i = 0; i < n_seq; i++) {
         const int n = begin[i + 1] - begin[i];
         if (n == 0) continue;
         if (tree && n > leap::kTreeMax)

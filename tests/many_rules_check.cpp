@@ -92,10 +92,25 @@ int plans()
     return 0;
 }
 
+// begins that go backwards: the rows of the arrays are begin's last, and a
+// tree's parents behind them are none of its.
+int refusals()
+{
+    leap_hip_attention h = handle(8, 2, 128, 64, 2, false);
+    const int begin[] = {0, 5, 4}, pos[] = {0, 0};
+    const int parent[] = {-1, 0, 1, 2, /* not the caller's: */ 77};
+    float x[4];
+    REQUIRE(leap_hip_attention_tree(&h, 0, 2, begin, pos, parent, x, x, x, x) == -EINVAL, "tree");
+    REQUIRE(h.err.find("below") != std::string::npos, "%s", h.err.c_str());
+    REQUIRE(leap_hip_attention_prompt(&h, 0, 2, begin, pos, x, x, x, x) == -EINVAL, "prompt");
+    REQUIRE(h.err.find("below") != std::string::npos, "%s", h.err.c_str());
+    return 0;
+}
+
 }  // namespace
 
 int main(int argc, char **argv)
 {
     const std::string what = argc > 1 ? argv[1] : "";
-    return what == "plan" ? plans() : sweep();
+    return what == "plan" ? plans() : what == "refuse" ? refusals() : sweep();
 }

@@ -1,5 +1,6 @@
 """What prompts, trees and 8-bit steps are cut into, on the CPU from the
-library's own source: kernels and workspace for every call."""
+library's own source: kernels and workspace for every call, and the host-pointer
+calls' checks."""
 import atexit
 import functools
 import os
@@ -69,3 +70,8 @@ def test_every_call_has_kernels_and_workspace():
 def test_calls_take_the_side_that_measured_faster(nh, nkv, hd, cache, lens, pos, rows, fused):
     p = plan(nh, nkv, hd, cache, lens, pos)
     assert (p.rows, p.fused) == (rows, fused), p
+
+
+def test_begins_that_go_backwards_are_refused_before_any_parent_is_read():
+    r = subprocess.run([_program(), "refuse"], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
