@@ -150,7 +150,7 @@ __device__ __forceinline__ Place find_place(const ManyArgs &a, int slot, int lan
 
 // Lane j's node j of a tree of n <= 64 nodes: the bits of its ancestors and
 // itself, by six doublings of the steps upwards.  A parent outside [-1, j)
-// marks the node and its descendants bad.
+// counts as -1 there, and marks the node and its descendants bad: no results.
 struct TreeLane {
     uint64_t sees;
     bool bad;
@@ -455,7 +455,7 @@ struct ManyShared {
     float m[W][kManyRows], l[W][kManyRows];
     float unit[W][kManyRows];                // O's unit of each wave and row
     float kf[W][kTileKeys];                  // fp32: K's factors of each wave's tile
-    uint64_t sees[STEP ? 1 : kTreeMax];
+    uint64_t sees[STEP ? 1 : kTreeMax], bad;  // tree_lane of each node, and the bad ones
     int last;
 };
 
@@ -750,10 +750,9 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     };
     int key0 = c0 + wave * kTileKeys;
     constexpr int kJobs = kThreads / LR;
-    // (a bad node stands as if it hung on the cached rows)
     auto pos_of = [&](int job) {
         const int j = token_of(job);
-        return p.p0 + (tree ? max((int)__popcll(sh.sees[j]) - 1, 0) : j);
+        return p.p0 + (tree ? (int)__popcll(sh.sees[j]) - 1 : j);
     };
     float4 y = make_float4(0, 0, 0, 0), turn = y;
     int job = tid / LR;
@@ -768,7 +767,9 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     if (tree) {
         if (wave == W - 1) {
             const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
-            sh.sees[lane] = t.bad ? 0 : t.sees;
+            sh.sees[lane] = t.sees;
+            const uint64_t bad = __builtin_amdgcn_ballot_w64(t.bad);
+            if (lane == 0) sh.bad = bad;
         }
         __syncthreads();
     }
@@ -787,7 +788,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             const float4 x = rope4(y, turn);
             unsigned mx = dpp_max16(max4_bits(0u, x));
             if constexpr (HD == 128) mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
-            const bool good = finite_bits(mx) && !(tree && sh.sees[token_of(job)] == 0);
+            const bool good = finite_bits(mx) && !(tree && (sh.bad >> token_of(job) & 1));
             const int e = tile_exp(good ? mx : 0u);
             const float sc = good ? exp2_int(13 - e) : 0.0f;
             half2v h[2], l[2];
@@ -959,7 +960,6 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
                 if ((badkeys >> (16 * (t >> 2) + 4 * g + (t & 3))) & 1) s[t] = __uint_as_float(0x7fc00000u);
         if (key0 + kTileKeys > c1 || (!STEP && key0 + kTileKeys - 1 > (tree ? p.p0 - 1 : p.p0 + j0))) {
             // visible: up to `limit`, and of a tree's nodes those of `sees`
-            // (a bad node sees itself alone, as NaN)
             int limit = c1 - 1;
             uint64_t sees = 0;
             if constexpr (!STEP) {
@@ -968,7 +968,6 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
                 if (tree) {
                     limit = p.p0 - 1;
                     sees = sh.sees[tok];
-                    if (!sees) sees = 1ull << tok;
                 }
             }
 #pragma unroll

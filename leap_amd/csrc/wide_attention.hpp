@@ -83,7 +83,7 @@ struct WideShared {
     // by the wave that brought them: positions that are not finite (bits
     // 0-7), quads of unlike positions (bits 8-9); any: of a tile so far
     int odd[4][kWideWaves], any_odd;
-    uint64_t sees[kTreeMax];
+    uint64_t sees[kTreeMax], bad;  // tree_lane of each node, and the bad ones
 };
 
 __device__ __forceinline__ f32x16 mfma32(half8v a, half8v b, f32x16 c)
@@ -150,11 +150,13 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     if (a.parent) {
         if (wave == kWideWaves - 1) {
             const TreeLane t = tree_lane(a.parent + p.first, p.n, lane);
-            sh.sees[lane] = t.bad ? 0 : t.sees;
+            sh.sees[lane] = t.sees;
+            const uint64_t bad = __builtin_amdgcn_ballot_w64(t.bad);
+            if (lane == 0) sh.bad = bad;
         }
         __syncthreads();
     }
-    auto place_of = [&](int j) LEAP_INLINE { return a.parent ? p.p0 + max((int)__popcll(sh.sees[j]) - 1, 0) : p.p0 + j; };
+    auto place_of = [&](int j) LEAP_INLINE { return p.p0 + (a.parent ? (int)__popcll(sh.sees[j]) - 1 : j); };
 
     // ---- the cache's rows ----
     const int kv_dim = a.n_kv_heads * HD;
@@ -436,7 +438,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 const float4 y = rope4(x[i], turn[i]);
                 unsigned mx = dpp_max16(max4_bits(0u, y));
                 if constexpr (HD == 128) mx = max(mx, (unsigned)__shfl_xor((int)mx, 16));
-                const bool good = finite_bits(mx) && !(a.parent && sh.sees[j[i]] == 0);
+                const bool good = finite_bits(mx) && !(a.parent && (sh.bad >> j[i] & 1));
                 const int e = tile_exp(good ? mx : 0u);
                 const float sc = good ? exp2_int(13 - e) : 0.0f;
                 half2v h[2], l[2];
@@ -588,7 +590,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             if (a.parent) {
                 limit = p.p0 - 1;
                 sees = sh.sees[my_j];
-                if (!sees) sees = 1ull << my_j;  // (a bad node sees itself alone, as NaN)
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {

@@ -1,0 +1,181 @@
+"""Prompts, trees and the 8-bit cache on inputs of very unlike magnitudes,
+element by element against 64 bits, within bounds derived from what the header
+states; each case asserts the kernel that it takes."""
+import numpy as np
+import pytest
+
+from tests.helpers import rng_for, rope_f32
+from tests.test_gpu_many import Model, _begin, _ptr
+from tests.test_many_rules import plan
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _needs_gpu(hip_device):
+    return hip_device
+
+
+# The bound of one output element.  Writing y for the rotated row of q, N_t for
+# sum_i |y_i| |k_ti| / sqrt(hd) with every factor that is not 0 raised by 2^-14 of its row's
+# largest (elements of q, k and v are held to 2^-22 of themselves, or 2^-36 of
+# that largest, which is 2^-22 * 2^-14 of it):
+#   a score is off by at most E = 2^-18 max N_t: 3 * 2^-22 for q, k and the
+#     product of the low halves, under 2^-22 for the rotation, 8 * 2^-22 for
+#     fp32 sums of 3 * 128 products in chains of at most 24 instructions,
+#     3 * 2^-24 for its factors and the exponent: 16 * 2^-22 hold them all;
+#   which moves an output by at most E sum_t p_t |v_t - out| (to first order,
+#     E < 2^-6 here: 5% more), so by 2.1 E sum_t p_t |v_t| in any case;
+#   values, probabilities, products and sums: 2^-20 sum_t p_t |v_t| (2^-22
+#     twice, 2^-22 for the low halves, fp32 sums and the rounding of records);
+#   values far below their row's largest m_t: 2^-36 sum_t p_t m_t;
+#   weighted values p_t m_t far below the row of q's largest: each to 2^-30 of
+#     that (2^-31 in a chunk and wave, and again where these are added up), and
+#     never by more than itself.
+def reference(m, q, at, kr, vr, see, tight=False):
+    """Outputs and bounds of the rows q (rotated at `at`) over the cache rows kr and vr [rows][kv_dim], see[row][cache row]."""
+    nh, nkv, hd = m.nh, m.nkv, m.hd
+    n, group = len(q), nh // nkv
+    y = rotated(m, q.astype(np.float64), at).reshape(n, nh, hd)
+    out, bound = np.empty((n, nh, hd)), np.empty((n, nh, hd))
+    floor = lambda x: np.where(x == 0, 0, np.abs(x) + 2.0 ** -14 * np.abs(x).max(axis=1, keepdims=True))  # noqa: E731
+    for h in range(nh):
+        k, v = (x.reshape(-1, nkv, hd)[:, h // group] for x in (kr, vr))
+        s = np.where(see, y[:, h] @ k.T / np.sqrt(hd), -np.inf)
+        p = np.exp(s - s.max(axis=1, keepdims=True))
+        p /= p.sum(axis=1, keepdims=True)
+        out[:, h] = p @ v
+        e = 2.0 ** -18 * np.where(see, floor(y[:, h]) @ floor(k).T / np.sqrt(hd), 0).max(axis=1, keepdims=True)
+        assert e.max() < 2.0 ** -6
+        mass = p @ np.abs(v)
+        top = np.abs(v).max(axis=1)
+        if tight:
+            moved = 1.05 * np.stack([p[r] @ np.abs(v - out[r, h]) for r in range(n)])
+        else:
+            moved = 2.1 * mass
+        bound[:, h] = (e * moved + 2.0 ** -20 * mass + 2.0 ** -36 * (p @ top)[:, None]
+                       + np.minimum(p * top, see * 2.0 ** -30 * (p * top).max(axis=1, keepdims=True))
+                       @ (np.abs(v) / np.maximum(top, 1e-300)[:, None]))
+    return out.reshape(n, -1), bound.reshape(n, -1)
+
+
+def rotated(m, x, at, back=False):
+    """Rows of heads turned to their positions (back: from them), in 64 bits."""
+    c, s = (np.repeat(t[at].astype(np.float64)[:, None], x.shape[1] // m.hd, axis=1) for t in (m.cos, m.sin))
+    s = -s if back else s
+    x = x.reshape(len(x), -1, m.hd)
+    y = np.empty_like(x)
+    y[..., 0::2], y[..., 1::2] = x[..., 0::2] * c - x[..., 1::2] * s, x[..., 1::2] * c + x[..., 0::2] * s
+    return y.reshape(len(x), -1)
+
+
+def within(got, want, bound):
+    assert np.isfinite(got).all()
+    worst = (np.abs(got - want) / np.maximum(bound, 1e-300)).max()
+    assert worst <= 1, worst
+
+
+class Run:
+    """One sequence: `cached` rows, then n tokens as a prompt (or a step), with the caches' rows and q given."""
+
+    def __init__(self, nh, nkv, hd, cache, cached, n, rows, step=False, key=0):
+        assert plan(nh, nkv, hd, cache, (n,), (cached,), step).rows == rows
+        self.m = Model(nh, nkv, hd, cached + n + 5, 1, cache, key=7919 * n + cached + key)
+        self.cached, self.n, self.step = cached, n, step
+        self.at = np.arange(cached, cached + n)
+        self.see = np.arange(cached + n)[None] <= self.at[:, None]
+
+    def out(self, y, k, v):
+        """The call's outputs and the reference's for rotated queries y [n][q_dim] and the rows k and v of cache
+        and tokens as they are to stand in the cache [cached + n][kv_dim], with the bound."""
+        m, c = self.m, self.cached
+        k, v = k.astype(np.float32), v.astype(np.float32)
+        q = rotated(m, y, self.at, back=True).astype(np.float32)
+        new = rotated(m, k[c:].astype(np.float64), self.at, back=True).astype(np.float32)
+        if c:
+            m.h.kv_upload(0, 0, 0, k[:c], v[:c])
+        if self.step:
+            got = m.h.step(0, c, q[0], new[0], v[c])[None]
+        else:
+            got = m.h.prompt(0, [0, self.n], [c], q, new, v[c:])
+        kn = np.stack([rope_f32(new[j], m.cos[c + j], m.sin[c + j]) for j in range(self.n)])
+        kr, vr = (np.concatenate([m.held(a), m.held(b)]) if c else m.held(b) for a, b in ((k[:c], kn), (v[:c], v[c:])))
+        return got, q, kr, vr
+
+    def check(self, y, k, v, rows=slice(None), tight=False):
+        got, q, kr, vr = self.out(y, k, v)
+        want, bound = reference(self.m, q[rows], self.at[rows], kr, vr, self.see[rows], tight)
+        within(got[rows], want, bound)
+
+
+# (heads, KV heads, head_dim, cache, cached rows, tokens, rows of a tile, a step)
+KINDS = [
+    (32, 8, 128, "f32", 500, 20, 16, False), (32, 4, 64, "f32", 700, 9, 16, False),
+    (32, 8, 128, "f32", 500, 300, 256, False), (32, 8, 64, "f32", 300, 600, 256, False),
+    (32, 8, 128, "q8", 900, 1, 16, True), (32, 4, 64, "q8", 333, 1, 16, True),
+    (32, 8, 128, "q8", 500, 20, 16, False), (32, 8, 128, "q8", 300, 600, 256, False),
+    (16, 4, 64, "q8", 300, 1700, 256, False),
+]
+
+
+def _directed(run, spread):
+    """Queries along one direction of each KV head, and keys whose parts along it spread the scores by `spread`."""
+    m, rng = run.m, run.m.rng
+    T = run.cached + run.n
+    u = rng.standard_normal((m.nkv, m.hd))
+    u /= np.linalg.norm(u, axis=1, keepdims=True)
+    b = 2.0 * np.sqrt(m.hd)
+    y = np.repeat(b * u, m.nh // m.nkv, axis=0)[None] + 0.3 * rng.standard_normal((run.n, m.nh, m.hd))
+    k = 0.3 * rng.standard_normal((T, m.nkv, m.hd))
+    k -= (k * u).sum(axis=2, keepdims=True) * u
+    score = spread * rng.standard_normal((T, m.nkv, 1))
+    return y.reshape(run.n, -1), k, u, score, lambda s: (k + s * (np.sqrt(m.hd) / b) * u).reshape(T, -1)
+
+
+# ---- bad nodes, bad bounds ---------------------------------------------------
+
+# (heads, KV heads, head_dim, tokens, cached rows, rows of a tile, one launch)
+TREES = [
+    (8, 2, 128, (5,), (50,), 16, True), (32, 4, 64, (9, 3, 5), (7, 200, 0), 16, True),
+    (8, 2, 128, (40, 5), (50, 3), 16, False), (32, 8, 128, (64,), (4000,), 256, True),
+    (64, 8, 128, (40,), (4000,), 256, True), (32, 8, 128, (64,) * 9, (700,) * 9, 256, False),
+]
+
+
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+@pytest.mark.parametrize("nh,nkv,hd,lens,cached,rows,fused", TREES)
+def test_what_is_stored_below_a_bad_node(nh, nkv, hd, lens, cached, rows, fused, cache):
+    """A node whose parent is none counts as one on the cached rows for what is
+    stored, and its descendants by their depth below it, in every form of call."""
+    import torch
+    got = plan(nh, nkv, hd, cache, lens, cached)
+    if cache == "f32":
+        assert (got.rows, got.fused) == (rows, fused), got
+    m = Model(nh, nkv, hd, max(cached) + 70, len(lens), cache, key=sum(lens))
+    with m.h:
+        for i, c in enumerate(cached):
+            m.fill(i, c)
+        begin = _begin(lens)
+        parent = np.concatenate([[j - 1 if j % 4 or not j else j - 3 for j in range(n)] for n in lens]).astype(np.int32)
+        stored, bad = parent.copy(), np.zeros(len(parent), bool)
+        for i, n in enumerate(lens):
+            parent[begin[i] + n // 2] = (n // 2, -2, 77)[i % 3]  # itself, or no node at all
+            stored[begin[i] + n // 2] = -1
+            bad[begin[i] + n // 2] = True
+            for j in range(n):
+                if stored[begin[i] + j] >= 0:
+                    bad[begin[i] + j] |= bad[begin[i] + stored[begin[i] + j]]
+        assert bad.sum() > len(lens)
+        q, k, v = m.tokens(begin[-1])
+        want = m.want(begin, cached, q, k, v, stored)
+        i32 = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+        d = [torch.from_numpy(x).cuda() for x in (q, k, v)]
+        b, p, t = i32(begin), i32(cached), i32(parent)
+        out = torch.full((len(q), nh * hd), 7.0, device="cuda")
+        m.h.tree_async(0, len(lens), _ptr(b), _ptr(p), _ptr(t), len(q), max(lens), max(a + n - 1 for a, n in zip(cached, lens)),
+                       *map(_ptr, d), _ptr(out), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        assert np.isnan(got[bad]).all()
+        assert np.abs(got[~bad] - want[~bad]).max() <= 1e-5 * np.abs(want[~bad]).max()
+        m.check_cache([a + n for a, n in zip(cached, lens)])
