@@ -184,8 +184,8 @@ int leap_hip_attention_step_noalloc(const leap_hip_attention_config *cfg, int po
  * before begin[0] are left alone.  Tile and chunk lengths, which sizes choose,
  * move results by fp32 rounding only: keys, values and weights are held to
  * 2^-22 of themselves (below 2^-28 of their row's largest element, to 2^-39 of
- * that; values whose rows are below 2^-12 of the largest row attended to, to
- * 2^-32 of that one), sums are fp32.  An output row that attends to a key or
+ * that), a weight times its value row's largest element also to 2^-30 of the
+ * largest such product of the output row, sums are fp32.  An output row that attends to a key or
  * value row with an infinity or a NaN is NaN; what a row does not attend to
  * does not affect it, whatever its size.
  * Host pointers: begin [n_seq+1] ascending from >= 0, pos [n_seq]; returns

@@ -26,8 +26,10 @@
 // sign: on sums of 128 terms and more that is fp32's own error.  Three fp16
 // MFMAs take 3/16 of the time of the fp32 MFMAs of the product.  The
 // probabilities are split the same way, with 2^7 folded into their exponent
-// and each value row's 2^e, over the largest that the row of Q has seen, into
-// them.  8-bit values are exact in fp16 and take two products.
+// and each value row's 2^e into them, over a power of two that follows the
+// largest such product that the row of Q has met (next_unit): its weighted
+// values are held to 2^-22 of themselves, or 2^-30 of the largest.  8-bit
+// values are exact in fp16 and take two products.
 //
 // Rows with infinities or NaN: such a key or value makes NaN of the output
 // rows that see it, and of those only: its elements are replaced by zero in
@@ -46,6 +48,8 @@ constexpr int kTileKeys = 32;                          // positions a wave takes
 constexpr int kManySplits = 64;                        // chunks of a tile, at most
 constexpr int kTreeMax = 64;                           // nodes of a sequence's tree
 constexpr float kProbBias = 7.0f, kProbRoom = 8.0f;    // probabilities are 2^(score - reference + 7) <= 2^15
+constexpr int kLeastUnit = -110;                       // the least exponent of O's unit
+constexpr int kRoom = 16;                              // 2^16: probabilities times factors over that are finite
 constexpr float kAmaxFloor = 7.888609052210118e-31f;   // 2^-100: the least largest magnitude of an 8-bit head row
 
 // One launch over one layer.  begin NULL: one token a sequence, row i of
@@ -459,6 +463,21 @@ struct ManyShared {
     int last;
 };
 
+// The exponent of O's unit in a row, whose largest probability times factor
+// in a tile is top 2^scale of the units it had.  The unit is a power of two
+// such that these products, whose halves are held to 2^-25 at least, stay in
+// fp16 and are not small where they are all that the row is made of: with
+// products of 2^15 and more it goes up, to where they are near 2^6, and where
+// the softmax reference has moved (up by `up`, which took 2^-up off O) and
+// they are below 2^5, it goes down as far; but not by over 2^60 more than O
+// has lost, which then outweighs them.
+__device__ __forceinline__ int next_unit(int unit, float top, int scale, float up)
+{
+    const int e = (int)(__float_as_uint(top) >> 23) - 127 + scale;
+    if (e < 15 && (up == 0.0f || e >= 5)) return unit;
+    return min(max(unit + e - 6, max(kLeastUnit, unit - (int)fminf(up + 60.0f, 300.0f))), 126);
+}
+
 // max / sum of a lane's value and those of the lanes 16, 32 and 48 away (the
 // swaps of one register with itself would be folded: each takes a copy)
 template <bool MAX>
@@ -832,7 +851,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     float mrun = -__builtin_inff(), lrun = 0.0f;
 #pragma unroll
     for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
-    int erun = -100;  // O's unit in the lane's row is 2^(erun - 12) (8 bits: 2^erun, and values are 2^-9 times theirs)
+    int erun = 0;  // O's unit in the lane's row is 2^(erun - 12) (8 bits: 2^erun, and values are 2^-9 times theirs)
 
     for (; key0 < c1; key0 += kPassKeys) {
         // ---- scores ----
@@ -900,8 +919,10 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         if constexpr (Q8) {
 #pragma unroll
             for (int b = 0; b < 2; b++) {
-                // a row's two scales: NaN in either marks it
-                vscv[b] = vsc[b];
+                // a row's two scales: NaN in either marks it (and V's is then
+                // 0 here, which a masked probability may meet)
+                auto f = [](float x) { return fmaxf(x, 0.0f) * exp2_int(-kRoom); };
+                vscv[b] = make_float4(f(vsc[b].x), f(vsc[b].y), f(vsc[b].z), f(vsc[b].w));
                 kscv[b] = make_float4(ksc[b].x + 0.0f * vsc[b].x, ksc[b].y + 0.0f * vsc[b].y,
                                       ksc[b].z + 0.0f * vsc[b].z, ksc[b].w + 0.0f * vsc[b].w);
             }
@@ -942,7 +963,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int e = tile_exp(top[j]);
-                (&vscv[j >> 2].x)[j & 3] = exp2_int(e - 1);
+                (&vscv[j >> 2].x)[j & 3] = exp2_int(e - 1 - kRoom);
                 (&vin[j >> 2].x)[j & 3] = exp2_int(13 - e);
             }
         }
@@ -974,45 +995,47 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             for (int t = 0; t < 8; t++) {
                 const int key = key0 + 16 * (t >> 2) + 4 * g + (t & 3);
                 const bool see = key <= limit || (!STEP && ((sees >> ((key - p.p0) & 63)) & 1));
-                if (!see || key >= c1) {
-                    s[t] = -__builtin_inff();
-                    (&vscv[t >> 2].x)[t & 3] = 0.0f;
-                }
+                if (!see || key >= c1) s[t] = -__builtin_inff();
             }
         }
-        // O's unit in this row: a power of two not below the factors of the
-        // values it has seen, so that P times them stays in fp16
-        float vtop = fmaxf(fmaxf(fmaxf(vscv[0].x, vscv[0].y), fmaxf(vscv[0].z, vscv[0].w)),
-                           fmaxf(fmaxf(vscv[1].x, vscv[1].y), fmaxf(vscv[1].z, vscv[1].w)));  // (NaN counts as nothing)
-        vtop = rows4<true>(vtop);
-        const int vexp = max(erun, min(tile_exp(__float_as_uint(vtop)) + (Q8 ? 1 : 0), 126));
-        const float mt = rows4<true>(
-            fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
-        // (the reference moves only when a score exceeds it by more than 2^8:
-        // most tiles leave O and the sum as they are)
-        const bool grows = mt > mrun + kProbRoom;
-        if (__builtin_amdgcn_ballot_w64(grows || vexp != erun)) {
-            const float now = grows ? mt : mrun;
-            const float alpha = now == -__builtin_inff() ? 1.0f : fast_exp2(mrun - now);
-            const float os = alpha * exp2_int(max(erun - vexp, -126));
-            lrun *= alpha;
+        // The reference, a whole number, moves only when a score exceeds it by
+        // more than 2^8: most tiles leave O and the sum as they are, and need
+        // no maximum over the row's lanes.
+        auto largest = [&]() {
+            return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        };
+        float mt = largest(), up = 0.0f;
+        const bool moves = __builtin_amdgcn_ballot_w64(mt > mrun + kProbRoom) != 0;
+        if (moves) {
+            mt = rows4<true>(mt);
+            const float now = mt > mrun + kProbRoom ? ceilf(mt) : mrun;
+            if (now != mrun) up = now - mrun;  // (infinite from nothing)
+            lrun *= fast_exp2(-up);
             mrun = now;
-            erun = vexp;
+        }
+        const float off = (mrun == -__builtin_inff() ? 0.0f : mrun) - kProbBias;  // (a row that has seen nothing yet)
+        // Probabilities times their value rows' factors (2^-16 of them: these
+        // products are finite, and as small as fp32 holds).
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            const float x = fast_exp2(s[t] - off);
+            lrun += x;
+            s[t] = x * (&vscv[t >> 2].x)[t & 3];
+        }
+        float top = largest();
+        if (moves || __builtin_amdgcn_ballot_w64(top > exp2_int(erun - kRoom + 15))) {
+            const int now = next_unit(erun, rows4<true>(top), kRoom - erun, up);
+            const float os = fast_exp2((float)(erun - now) - up);
+            erun = now;
 #pragma unroll
             for (int v = 0; v < VB; v++) o[v] *= os;
         }
-        const float off = (mrun == -__builtin_inff() ? 0.0f : mrun) - kProbBias;  // (a row that has seen nothing yet)
-        const float vscale = exp2_int(-vexp);
+        const float vscale = exp2_int(kRoom - erun);
+#pragma unroll
+        for (int t = 0; t < 8; t++) s[t] *= vscale;
         Half8 h, l;
 #pragma unroll
-        for (int t = 0; t < 8; t += 2) {
-            float x = fast_exp2(s[t] - off), z = fast_exp2(s[t + 1] - off);
-            lrun += x + z;
-            // (a scale of NaN marks a row that a masked score must not meet)
-            x *= fmaxf((&vscv[t >> 2].x)[t & 3] * vscale, 0.0f);
-            z *= fmaxf((&vscv[t >> 2].x)[(t & 3) + 1] * vscale, 0.0f);
-            split2(x, z, h.h[t / 2], l.h[t / 2]);
-        }
+        for (int t = 0; t < 8; t += 2) split2(s[t], s[t + 1], h.h[t / 2], l.h[t / 2]);
         const half8v ph = h.v, pl = l.v;
 
         // ---- weighted values ----

@@ -26,8 +26,7 @@
 //
 // Scales: K's and V's exponents by quads of four positions (8-bit caches:
 // scales by position).  K's multiply the scores, V's go into the
-// probabilities, relative to the largest that the row has seen so far (vrun),
-// O's unit in that row.  A quad of positions whose magnitudes are unlike gets
+// probabilities, over O's unit in the row (vrun, next_unit).  A quad of positions whose magnitudes are unlike gets
 // an exponent for each, counted in its tile's scores and probabilities: so what
 // a row does not see takes none of its accuracy.  (On one card in turns, 32 q
 // heads, 8 KV heads, head_dim 128, 8192 tokens: 6% more time than exponents by
@@ -59,6 +58,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = kWideWaves * kWave;
+constexpr int kOrdinary = 50;  // fp32 values of 2^-50 .. 2^50: no probability times factors over O's unit overflows
 constexpr unsigned kUnlike = 12;  // binary orders between positions of a quad from which each has an exponent of its own
 
 template <int HD, bool Q8>
@@ -83,6 +83,7 @@ struct WideShared {
     // by the wave that brought them: positions that are not finite (bits
     // 0-7), quads of unlike positions (bits 8-9); any: of a tile so far
     int odd[4][kWideWaves], any_odd;
+    int any_extreme;  // fp32 values so far outside 2^-50 .. 2^50
     uint64_t sees[kTreeMax], bad;  // tree_lane of each node, and the bad ones
 };
 
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
     if (c0 >= kv_end) return;
     const int n_tiles = (c1 - c0 + kTileKeys - 1) / kTileKeys;
-    if (tid == 0) sh.any_odd = 0;
+    if (tid == 0) sh.any_odd = sh.any_extreme = 0;
     __syncthreads();
     auto tile_key = [&](int i) LEAP_INLINE { return c0 + kTileKeys * i; };
 
@@ -243,6 +244,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         constexpr bool V = decltype(role)::value;
         if (Q8 || i >= n_tiles) return;
         int oddbits = 0, ln = lane;
+        bool extreme = false;
         asm volatile("" : "+v"(ln));  // (addresses formed anew, for the registers' sake)
         if constexpr (!Q8) {
 #pragma unroll
@@ -293,14 +295,16 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                         if (__builtin_amdgcn_ballot_w64((bits >> b) & 1)) oddbits |= 1 << (4 * t + b);
                     look();
                 }
-                const int e = tile_exp(most);
+                const int e = V && most == 0 ? 0 : tile_exp(most);
                 stage_sc[t] = exp2_int(13 - e);
+                if constexpr (V) extreme |= (unsigned)(e + kOrdinary) > 2u * kOrdinary;
                 if (__builtin_expect(unlike, 0)) {
                     // positions far below their neighbours: each by its own exponent
 #pragma unroll
                     for (int j = 0; j < Y; j++) {
                         const unsigned top = V ? wave_max_bits(__float_as_uint(y[j])) : dpp_max16(__float_as_uint(y[j]));
                         const int by = top == 0 ? 0 : min(e - tile_exp(top), 126);
+                        if constexpr (V) extreme |= e - by < -kOrdinary;
                         const float up = exp2_int(by);
 #pragma unroll
                         for (int u = j; u < N; u += Y) x[u] *= up;
@@ -319,7 +323,10 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             }
         }
         sh.odd[i & 3][wave] = oddbits;
-        if (__builtin_expect(oddbits != 0, 0)) sh.any_odd = 1;
+        if (__builtin_expect(oddbits != 0 || extreme, 0)) {
+            if (extreme) sh.any_extreme = 1;
+            sh.any_odd = 1;
+        }
     };
     unsigned hi[2], lo[2];
     constexpr int P = WideShared<HD, Q8>::P;
@@ -475,7 +482,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
         for (int r = 0; r < 16; r++) o[v][r] = 0.0f;
     half8v ph[2], pl[2];
-    float ref = -__builtin_inff(), sum = 0.0f, vrun = exp2_int(-113);
+    float ref = -__builtin_inff(), sum = 0.0f, vrun = 1.0f;  // (vrun: O's unit in the lane's row)
 
     // (a lane's pieces: K piece 2 t + g of position n, V piece 2 u + g of dim
     // 32 v + n; the swizzles leave t and u as an exclusive or on the first's
@@ -550,17 +557,16 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         const int key0 = tile_key(i);
         const float *kfs = Q8 ? sh.kfac[i & 3][g] : sh.kquad[i & 3][g], *vfs = Q8 ? sh.vfac[i & 3][g] : sh.vquad[i & 3][g];
         // scores are s[r] kf[r / P] (8 bits: s[r]); the factors are positive (or NaN in a row without result)
-        float kf[F], vtop = 0.0f;
+        float kf[F];
 #pragma unroll
         for (int t = 0; t < F; t++) kf[t] = kfs[t] * qf;
         if constexpr (Q8) {
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] *= kf[r];
         }
-#pragma unroll
-        for (int t = 0; t < F; t++) vtop = fmaxf(vtop, vfs[t]);  // (a NaN counts as nothing)
-        bool odd = false;
+        bool odd = false, extreme = false;
         if (!Q8 && __builtin_expect(__builtin_amdgcn_readfirstlane(sh.any_odd), 0)) {
+            extreme = __builtin_amdgcn_readfirstlane(sh.any_extreme);
             int bits = 0;
 #pragma unroll
             for (int x = 0; x < kWideWaves; x++) bits |= sh.odd[i & 3][x];
@@ -584,7 +590,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             asm volatile("" : "+v"(ln));  // (formed anew, for the registers' sake)
             const int my_j = (int)fast_div((uint32_t)min(r0 + 32 * wave + (ln & 31), rows - 1), a.by_group);
             const int first = key0 + 4 * (ln >> 5);
-            vtop = 0.0f;
             int limit = p.p0 + my_j;
             uint64_t sees = 0;
             if (a.parent) {
@@ -596,15 +601,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 const int key = first + 8 * (r >> 2) + (r & 3);
                 const bool see = key <= limit || ((sees >> ((key - p.p0) & 63)) & 1);
                 if (!see || key >= c1) s[r] = -__builtin_inff();
-            }
-            auto seen = [&](float x, float f) LEAP_INLINE { vtop = fmaxf(vtop, x == -__builtin_inff() ? 0.0f : f); };
-            if (Q8 || __builtin_expect(odd, 0)) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) seen(s[r], Q8 ? sh.vfac[i & 3][ln >> 5][r] : v_factor(i, ln >> 5, r));
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; r += 4)
-                    seen(fmaxf(fmaxf(s[r], s[r + 1]), fmaxf(s[r + 2], s[r + 3])), vfs[r / P]);
             }
             if constexpr (!Q8)
 #pragma unroll
@@ -619,31 +615,35 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
             for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[r]);
         }
-        mt = half_max(mt);
-        // V's unit in this row: a power of two not below the factors of what it has seen
-        vtop = half_max(vtop);
-        const float vpow = Q8 ? exp2_int(min(tile_exp(__float_as_uint(vtop)) + 1, 120)) : vtop;
-        const bool grows = mt > ref + kProbRoom, vgrows = vpow > vrun;
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(grows || vgrows) != 0, 0)) {
-            const float now = grows ? mt : ref;
-            float alpha = now == -__builtin_inff() ? 1.0f : fast_exp2(ref - now);
-            sum *= alpha;
+        // The reference, a whole number, moves only when a score exceeds it by
+        // more than 2^8: most tiles leave O and the sum as they are, and need
+        // no maximum over both lanes of a row.
+        const bool moves = __builtin_amdgcn_ballot_w64(mt > ref + kProbRoom) != 0;
+        float up = 0.0f;
+        if (__builtin_expect(moves, 0)) {
+            mt = half_max(mt);
+            const float now = mt > ref + kProbRoom ? ceilf(mt) : ref;
+            if (now != ref) up = now - ref;  // (infinite from nothing)
+            sum *= fast_exp2(-up);
             ref = now;
-            if (vgrows) {
-                alpha *= vrun / vpow;
-                vrun = vpow;
+            if constexpr (!Q8) {
+                // (a first guess at O's unit, for values alike)
+                const float f = half_max(fmaxf(fmaxf(vfs[0], vfs[1]), fmaxf(vfs[2], vfs[3])));
+                if (up == __builtin_inff()) vrun = 0.5f * f;
             }
-#pragma unroll
-            for (int v = 0; v < VB; v++) o[v] *= alpha;
         }
         const float off = (ref == -__builtin_inff() ? 0.0f : ref) - kProbBias;
-        const float vinv = __uint_as_float(0x7f000000u - __float_as_uint(vrun));  // 1 / vrun, a power of two
         if constexpr (Q8) asm volatile("" ::: "memory");  // (sixteen factors are read again rather than kept)
-        // (at most 1 where the row sees the position, and no NaN or infinity where it does not)
+        // Probabilities times their value rows' factors: in O's unit, or (8
+        // bits, and once there were fp32 values of extreme sizes) times 2^-16,
+        // which is finite and as small as fp32 holds.  0 for a scale of NaN,
+        // which a masked probability may meet.
+        auto inverse = [](float x) LEAP_INLINE { return __uint_as_float(0x7f000000u - __float_as_uint(x)); };  // (of powers of two)
+        const bool plain = Q8 || extreme;
+        const float vmul = plain ? exp2_int(-kRoom) : inverse(vrun);
         float vf[F];
 #pragma unroll
-        for (int t = 0; t < F; t++) vf[t] = __builtin_amdgcn_fmed3f(vfs[t] * vinv, 0.0f, 1.0f);
-        Half8 h[2], l[2];
+        for (int t = 0; t < F; t++) vf[t] = Q8 ? fmaxf(vfs[t], 0.0f) * vmul : odd ? 1.0f : vfs[t] * vmul;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
             float x, y;
@@ -655,23 +655,45 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 y = fast_exp2(s[r + 1] - off);
             }
             sum += x + y;
-            x *= vf[r / P];
-            y *= vf[(r + 1) / P];
-            split2(x, y, h[r >> 3].h[(r & 7) / 2], l[r >> 3].h[(r & 7) / 2]);
+            s[r] = x * vf[r / P];
+            s[r + 1] = y * vf[(r + 1) / P];
         }
         if (!Q8 && __builtin_expect(odd, 0)) {
-            // (powers of two, which leave the halves as they are, down to fp16's subnormals)
             int gg = lane;
             asm volatile("" : "+v"(gg)::"memory");
             gg >>= 5;
-            auto factor = [&](float f) LEAP_INLINE { return __builtin_amdgcn_fmed3f(f * vinv, 0.0f, 1.0f); };
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float by = fminf(1.0f / factor(sh.vquad[i & 3][gg][r >> 2]), 0x1p100f);
-                const half2v c = {(_Float16)(factor(v_factor(i, gg, r)) * by), (_Float16)(factor(v_factor(i, gg, r + 1)) * by)};
-                h[r >> 3].h[(r & 7) / 2] *= c;
-                l[r >> 3].h[(r & 7) / 2] *= c;
+            for (int r = 0; r < 16; r++) s[r] *= v_factor(i, gg, r) * vmul;
+        }
+        Half8 h[2], l[2];
+        auto split = [&]() LEAP_INLINE {
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) split2(s[r], s[r + 1], h[r >> 3].h[(r & 7) / 2], l[r >> 3].h[(r & 7) / 2]);
+        };
+        if constexpr (!Q8) split();  // (as it nearly always stays; the check below would be waited for)
+        float top3[5];
+#pragma unroll
+        for (int r = 0; r < 5; r++) top3[r] = fmaxf(fmaxf(s[3 * r], s[3 * r + 1]), s[3 * r + 2]);
+        float top = fmaxf(fmaxf(fmaxf(fmaxf(top3[0], top3[1]), top3[2]), fmaxf(top3[3], top3[4])), s[15]);
+        if (__builtin_expect(moves || extreme || __builtin_amdgcn_ballot_w64(top > (plain ? 0.5f * vrun : 0x1p15f)) != 0, 0)) {
+            const int was = (int)(__float_as_uint(vrun) >> 23) - 127;
+            const int now = next_unit(was, half_max(top), plain ? kRoom - was : 0, up);
+            const float os = fast_exp2((float)(was - now) - up);
+            vrun = exp2_int(now);
+#pragma unroll
+            for (int v = 0; v < VB; v++) o[v] *= os;
+            if (!Q8 && __builtin_expect(extreme || __builtin_amdgcn_ballot_w64(now != was) != 0, 0)) {
+                const float by = exp2_int(extreme ? kRoom - now : was - now);
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] *= by;
+                split();
             }
+        }
+        if constexpr (Q8) {
+            const float by = inverse(vrun) * exp2_int(kRoom);
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] *= by;
+            split();
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {

@@ -132,6 +132,36 @@ def _directed(run, spread):
     return y.reshape(run.n, -1), k, u, score, lambda s: (k + s * (np.sqrt(m.hd) / b) * u).reshape(T, -1)
 
 
+@pytest.mark.parametrize("factor", [1e6, 1e10, 1e26])
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_large_value_row_without_weight(kind, factor):
+    """One visible value row larger than the rest by a factor, its score 60
+    below them: next to nothing of it is in the outputs, and all of the rest."""
+    run = Run(*kind, key=int(np.log10(factor)))
+    with run.m.h:
+        for where in (3, run.cached - 1):
+            y, k, u, score, keys = _directed(run, 1.0)
+            score[where] = -60.0
+            v = run.m.rng.standard_normal((run.cached + run.n, run.m.nkv * run.m.hd))
+            v[where] *= factor
+            run.check(y, keys(score), v)
+
+
+@pytest.mark.parametrize("order", ["mixed", "heavy last", "heavy first"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_values_of_all_magnitudes_under_weights_of_all(kind, order):
+    """Value rows from 1e-12 to 1e12 and scores over +-60: what outputs are
+    made of is neither the heaviest nor the largest row."""
+    run = Run(*kind, key=len(order))
+    with run.m.h:
+        y, k, u, score, keys = _directed(run, 20.0)
+        T = run.cached + run.n
+        if order != "mixed":
+            score = np.sort(score, axis=0)[::1 if order == "heavy last" else -1]
+        size = 10.0 ** run.m.rng.uniform(-12, 12, (T, 1))
+        run.check(y, keys(score), size * run.m.rng.standard_normal((T, run.m.nkv * run.m.hd)))
+
+
 # ---- bad nodes, bad bounds ---------------------------------------------------
 
 # (heads, KV heads, head_dim, tokens, cached rows, rows of a tile, one launch)
