@@ -1071,7 +1071,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     if (g == 0) {
         sh.m[wave][m] = mrun;
         sh.l[wave][m] = lrun;
-        sh.unit[wave][m] = exp2_int(max(Q8 ? erun : erun - 12, -126));
+        sh.unit[wave][m] = exp2_int(Q8 ? erun : erun - 12);
     }
     // register i of block v: dim (8 bits) VB (4 g + i) + v, or 64 (v / 4) + 4 (4 g + i) + v % 4
 #pragma unroll
@@ -1091,16 +1091,23 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
 #pragma unroll
         for (int w = 1; w < W; w++) top = fmaxf(top, sh.m[w][row]);
         if (top == -__builtin_inff()) top = 0.0f;
-        float4 acc = make_float4(0, 0, 0, 0);
-        float total = 0.0f;
+        float f[W], total = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            const float f = fast_exp2(sh.m[w][row] - top);
-            total += f * sh.l[w][row];
-            fma4(acc, f * sh.unit[w][row], *reinterpret_cast<const float4 *>(&sh.o[w][row][d]));
+            f[w] = fast_exp2(sh.m[w][row] - top);
+            total += f[w] * sh.l[w][row];
         }
+        // (weights before units: their product with a sum of values is no
+        // larger than the values, which may fill fp32's range)
         const bool none = total == 0.0f;  // a chunk none of whose positions the row sees: nothing, weight 0
-        scale4(acc, none ? 0.0f : (Q8 ? 0x1p9f : 1.0f) / total);
+        const float inv = none ? 0.0f : (Q8 ? 0x1p9f : 1.0f) / total;
+        float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            float4 x = *reinterpret_cast<const float4 *>(&sh.o[w][row][d]);
+            scale4(x, f[w] * inv);
+            fma4(acc, sh.unit[w][row], x);
+        }
         if (n_split == 1) {
             const int j = STEP ? 0 : (int)fast_div((uint32_t)r, a.by_group);
             const int head = kvh * a.group + r - j * a.group;

@@ -162,6 +162,20 @@ def test_values_of_all_magnitudes_under_weights_of_all(kind, order):
         run.check(y, keys(score), size * run.m.rng.standard_normal((T, run.m.nkv * run.m.hd)))
 
 
+@pytest.mark.parametrize("size", [1e38, 1e-28])
+@pytest.mark.parametrize("kind", KINDS)
+def test_values_at_the_ends_of_fp32(kind, size):
+    """Values up to 3e38, whose weighted mean is finite, and near 1e-28."""
+    run = Run(*kind, key=int(np.log10(size)) + 99)
+    with run.m.h:
+        y, k, u, score, keys = _directed(run, 1.0)
+        shape = (run.cached + run.n, run.m.nkv * run.m.hd)
+        run.check(y, keys(score), size * run.m.rng.uniform(1, 3, shape) * run.m.rng.choice([-1, 1], shape))
+
+
+F32 = [k for k in KINDS if k[3] == "f32"]
+
+
 # ---- bad nodes, bad bounds ---------------------------------------------------
 
 # (heads, KV heads, head_dim, tokens, cached rows, rows of a tile, one launch)
