@@ -182,12 +182,13 @@ int leap_hip_attention_step_noalloc(const leap_hip_attention_config *cfg, int po
  * attends causally, to the rows [0, pos[i] + j] (cached ones and those of
  * this call).  A sequence may have no tokens; rows behind begin[n_seq] and
  * before begin[0] are left alone.  Tile and chunk lengths, which sizes choose,
- * move results by fp32 rounding only: keys, values and weights are held to
- * 2^-22 of themselves (below 2^-28 of their row's largest element, to 2^-39 of
- * that), a weight times its value row's largest element also to 2^-30 of the
- * largest such product of the output row, sums are fp32.  An output row that attends to a key or
- * value row with an infinity or a NaN is NaN; what a row does not attend to
- * does not affect it, whatever its size.
+ * move results by fp32 rounding only: queries, keys and values are held to
+ * 2^-22 of themselves or 2^-34 of their head row's largest element, whichever
+ * is more (rows of less than 2^-100: to 2^-138), a weight times its value row's
+ * largest element to 2^-22 of itself or 2^-30 of the largest such product of
+ * the output row, sums are fp32.  An output row that attends to a key or value
+ * row with an infinity or a NaN is NaN; what a row does not attend to does not
+ * affect it further, whatever its size.
  * Host pointers: begin [n_seq+1] ascending from >= 0, pos [n_seq]; returns
  * when `out` is written.  -EINVAL, with nothing changed, if a sequence's
  * positions leave [0, seq_len). */

@@ -19,10 +19,11 @@
 //
 // fp32 operands in fp16 products: x = 2^e (h + l), h = fp16(x 2^-e) and
 // l = fp16(x 2^-e - h), both rounded to nearest, with e such that the
-// largest of x's row (wide_attention.hpp: of a quad of rows, where these are
-// alike) is in [2^13, 2^14).  h and l together hold x to 2^-22 relative
-// (elements below 2^-28 of the row's largest to 2^-39 of that, fp16's
-// subnormals), and h h' + h l' + l h' leaves out l l' < 2^-22 |x x'|, of either
+// largest of x's row is in [2^13, 2^14) (wide_attention.hpp: of a quad of
+// rows, where these are within 2^4 of each other).  h and l together hold x to
+// 2^-22 of itself, or to 2^-38 of the row's largest (quads: 2^-34), half of
+// fp16's least step, whichever is more; rows below 2^-100 to 2^-138.
+// h h' + h l' + l h' leaves out l l' < 2^-22 |x x'|, of either
 // sign: on sums of 128 terms and more that is fp32's own error.  Three fp16
 // MFMAs take 3/16 of the time of the fp32 MFMAs of the product.  The
 // probabilities are split the same way, with 2^7 folded into their exponent

@@ -26,11 +26,12 @@
 //
 // Scales: K's and V's exponents by quads of four positions (8-bit caches:
 // scales by position).  K's multiply the scores, V's go into the
-// probabilities, over O's unit in the row (vrun, next_unit).  A quad of positions whose magnitudes are unlike gets
-// an exponent for each, counted in its tile's scores and probabilities: so what
-// a row does not see takes none of its accuracy.  (On one card in turns, 32 q
-// heads, 8 KV heads, head_dim 128, 8192 tokens: 6% more time than exponents by
-// quad and one unit for all rows; by position throughout 10 to 20% more.)
+// probabilities, over O's unit in the row (vrun, next_unit).  A quad with a
+// position 2^4 times smaller than another gets an exponent for each, counted in
+// its tile's scores and probabilities: so what a row does not see takes no more
+// of its accuracy than that.  (On one card in turns, 32 q heads, 8 KV heads,
+// head_dim 128, 8192 tokens: 6% more time than exponents by quad and one unit
+// for all rows; by position throughout 10 to 20% more.)
 //
 // The running maximum is a reference that moves only when a score exceeds it
 // by more than 2^8 (then O and the sum are rescaled): probabilities are
@@ -59,7 +60,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = kWideWaves * kWave;
 constexpr int kOrdinary = 50;  // fp32 values of 2^-50 .. 2^50: no probability times factors over O's unit overflows
-constexpr unsigned kUnlike = 12;  // binary orders between positions of a quad from which each has an exponent of its own
+constexpr unsigned kUnlike = 4;  // binary orders between positions of a quad from which each has an exponent of its own
 
 template <int HD, bool Q8>
 struct WideShared {

@@ -16,10 +16,10 @@ def _needs_gpu(hip_device):
     return hip_device
 
 
-# The bound of one output element.  Writing y for the rotated row of q, N_t for
-# sum_i |y_i| |k_ti| / sqrt(hd) with every factor that is not 0 raised by 2^-14 of its row's
-# largest (elements of q, k and v are held to 2^-22 of themselves, or 2^-36 of
-# that largest, which is 2^-22 * 2^-14 of it):
+# The bound of one output element.  Elements of q, k and v are held to 2^-22 of
+# themselves or 2^-34 of their row's largest.  Writing y for the rotated row of
+# q, N_t for sum_i |y_i| |k_ti| / sqrt(hd) with every factor that is not 0
+# raised by 2^-12 of its row's largest (2^-34 = 2^-22 * 2^-12):
 #   a score is off by at most E = 2^-18 max N_t: 3 * 2^-22 for q, k and the
 #     product of the low halves, under 2^-22 for the rotation, 8 * 2^-22 for
 #     fp32 sums of 3 * 128 products in chains of at most 24 instructions,
@@ -28,17 +28,16 @@ def _needs_gpu(hip_device):
 #     E < 2^-6 here: 5% more), so by 2.1 E sum_t p_t |v_t| in any case;
 #   values, probabilities, products and sums: 2^-20 sum_t p_t |v_t| (2^-22
 #     twice, 2^-22 for the low halves, fp32 sums and the rounding of records);
-#   values far below their row's largest m_t: 2^-36 sum_t p_t m_t;
+#   values far below their row's largest m_t: 2^-34 sum_t p_t m_t;
 #   weighted values p_t m_t far below the row of q's largest: each to 2^-30 of
-#     that (2^-31 in a chunk and wave, and again where these are added up), and
-#     never by more than itself.
+#     that, and never by more than itself.
 def reference(m, q, at, kr, vr, see, tight=False):
     """Outputs and bounds of the rows q (rotated at `at`) over the cache rows kr and vr [rows][kv_dim], see[row][cache row]."""
     nh, nkv, hd = m.nh, m.nkv, m.hd
     n, group = len(q), nh // nkv
     y = rotated(m, q.astype(np.float64), at).reshape(n, nh, hd)
     out, bound = np.empty((n, nh, hd)), np.empty((n, nh, hd))
-    floor = lambda x: np.where(x == 0, 0, np.abs(x) + 2.0 ** -14 * np.abs(x).max(axis=1, keepdims=True))  # noqa: E731
+    floor = lambda x: np.where(x == 0, 0, np.abs(x) + 2.0 ** -12 * np.abs(x).max(axis=1, keepdims=True))  # noqa: E731
     for h in range(nh):
         k, v = (x.reshape(-1, nkv, hd)[:, h // group] for x in (kr, vr))
         s = np.where(see, y[:, h] @ k.T / np.sqrt(hd), -np.inf)
@@ -53,7 +52,7 @@ def reference(m, q, at, kr, vr, see, tight=False):
             moved = 1.05 * np.stack([p[r] @ np.abs(v - out[r, h]) for r in range(n)])
         else:
             moved = 2.1 * mass
-        bound[:, h] = (e * moved + 2.0 ** -20 * mass + 2.0 ** -36 * (p @ top)[:, None]
+        bound[:, h] = (e * moved + 2.0 ** -20 * mass + 2.0 ** -34 * (p @ top)[:, None]
                        + np.minimum(p * top, see * 2.0 ** -30 * (p * top).max(axis=1, keepdims=True))
                        @ (np.abs(v) / np.maximum(top, 1e-300)[:, None]))
     return out.reshape(n, -1), bound.reshape(n, -1)
@@ -174,6 +173,56 @@ def test_values_at_the_ends_of_fp32(kind, size):
 
 
 F32 = [k for k in KINDS if k[3] == "f32"]
+
+
+@pytest.mark.parametrize("score", [30, 100])
+@pytest.mark.parametrize("kind", F32)
+def test_values_beside_a_larger_row(kind, score):
+    """Three value rows with small elements beside one of 2^11 or 2^4 times
+    their size that is masked: each element as exact as by itself.  (score: of
+    a row's own key, which has nearly all the weight, or all that fp32 holds.)"""
+    for ratio in (2.0 ** 11, 2.0 ** 3.9):
+        run = Run(*kind, key=int(ratio))
+        with run.m.h:
+            m, T = run.m, run.cached + run.n
+            k = m.rng.standard_normal((T, m.nkv, m.hd))
+            v = m.rng.standard_normal((T, m.nkv, m.hd))
+            first = [t for t in range((run.cached + 3) // 4 * 4, T - 4, max(4, run.n // 5 // 4 * 4))]
+            y = np.zeros((run.n, m.nh, m.hd))
+            rows = []
+            for t in first:
+                v[t:t + 3, :, m.hd // 4:] *= 1e-4
+                v[t + 3] *= ratio
+                for j in (t, t + 1, t + 2):
+                    y[j - run.cached] = np.repeat(score / np.sqrt(m.hd) * k[j], m.nh // m.nkv, axis=0)
+                    rows.append(j - run.cached)
+            run.check(y.reshape(run.n, -1), k.reshape(T, -1), v.reshape(T, -1), rows, tight=True)
+
+
+@pytest.mark.parametrize("kind", F32)
+def test_keys_beside_a_larger_row(kind):
+    """Scores that come from the small elements of three keys, beside a masked
+    key of 2^11 times their size."""
+    run = Run(*kind)
+    with run.m.h:
+        m, T = run.m, run.cached + run.n
+        k = m.rng.standard_normal((T, m.nkv, m.hd))
+        v = m.rng.standard_normal((T, m.nkv, m.hd))
+        k[:, :, -2:] *= 2.0 ** -13
+        first = [t for t in range((run.cached + 3) // 4 * 4, T - 4, max(4, run.n // 5 // 4 * 4))]
+        y = np.zeros((run.n, m.nh, m.hd))
+        rows = []
+        for t in first:
+            # the last pair of both: q 20 sqrt(hd) along that of the keys, which are alike
+            k[t:t + 3, :, -2:] = k[t, :, -2:] * (1 + 0.01 * m.rng.standard_normal((3, m.nkv, 2)))
+            k[t + 3] *= 2.0 ** 11
+            k[t + 3, :, -2:] = 0  # (to later rows no more than others)
+            for j in (t + 1, t + 2):
+                pair = k[t, :, -2:]
+                y[j - run.cached, :, -2:] = np.repeat(20 * np.sqrt(m.hd) * pair / (pair ** 2).sum(axis=1, keepdims=True),
+                                                      m.nh // m.nkv, axis=0)
+                rows.append(j - run.cached)
+        run.check(y.reshape(run.n, -1), k.reshape(T, -1), v.reshape(T, -1), rows, tight=True)
 
 
 # ---- bad nodes, bad bounds ---------------------------------------------------
