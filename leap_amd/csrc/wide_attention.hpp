@@ -78,11 +78,10 @@ struct WideShared {
     };
     float qf[kWideWaves][32];             // factors of Q's rows
     // factors of K's and V's positions, by lane half: position 8 (j / 4) + 4
-    // half + j % 4; fp32: of quads, and for positions of unlike quads vfac in
-    // place of theirs, kfac on top of theirs
+    // half + j % 4; fp32: of quads, and of positions only in unlike quads
     float kfac[4][2][16], vfac[4][2][16], kquad[4][2][4], vquad[4][2][4];
-    // by the wave that brought them: positions that are not finite (bits
-    // 0-7), quads of unlike positions (bits 8-9); any: of a tile so far
+    // fp32, by the wave that brought them: positions that are not finite
+    // (bits 0-7), quads of unlike positions (bits 8-9); any: of a tile so far
     int odd[4][kWideWaves], any_odd;
     int any_extreme;  // fp32 values so far outside 2^-50 .. 2^50
     uint64_t sees[kTreeMax], bad;  // tree_lane of each node, and the bad ones
@@ -299,28 +298,21 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                 const int e = V && most == 0 ? 0 : tile_exp(most);
                 stage_sc[t] = exp2_int(13 - e);
                 if constexpr (V) extreme |= (unsigned)(e + kOrdinary) > 2u * kOrdinary;
+                // (every lane writes the same: no branch)
+                (V ? sh.vquad : sh.kquad)[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
                 if (__builtin_expect(unlike, 0)) {
                     // positions far below their neighbours: each by its own exponent
 #pragma unroll
                     for (int j = 0; j < Y; j++) {
                         const unsigned top = V ? wave_max_bits(__float_as_uint(y[j])) : dpp_max16(__float_as_uint(y[j]));
-                        const int by = top == 0 ? 0 : min(e - tile_exp(top), 126);
-                        if constexpr (V) extreme |= e - by < -kOrdinary;
-                        const float up = exp2_int(by);
+                        const int own = top == 0 ? e : tile_exp(top);
+                        if constexpr (V) extreme |= own < -kOrdinary;
 #pragma unroll
-                        for (int u = j; u < N; u += Y) x[u] *= up;
-                        if constexpr (V)
-                            sh.vfac[i & 3][quad & 1][4 * (quad >> 1) + j] = exp2_int(e - by - 13);
-                        else
-                            sh.kfac[i & 3][quad & 1][4 * (quad >> 1) + (ln >> 4)] = exp2_int(-by);
+                        for (int u = j; u < N; u += Y) x[u] = __builtin_amdgcn_ldexpf(x[u], e - own);
+                        (V ? sh.vfac : sh.kfac)[i & 3][quad & 1][4 * (quad >> 1) + (V ? j : ln >> 4)] = exp2_int(own - 13);
                     }
                     oddbits |= 256 << t;
                 }
-                // (every lane writes the same: no branch)
-                if constexpr (V)
-                    sh.vquad[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
-                else
-                    sh.kquad[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
             }
         }
         sh.odd[i & 3][wave] = oddbits;
@@ -547,11 +539,22 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // fp32: V's factor of a position of a tile that may have unlike quads
-    auto v_factor = [&](int i, int half, int r) LEAP_INLINE {
-        const int quad = 2 * (r >> 2) + half;
-        const bool own = (sh.odd[i & 3][quad & 3] >> (8 + (quad >> 2))) & 1;
-        return own ? sh.vfac[i & 3][half][r] : sh.vquad[i & 3][half][r >> 2];
+    // fp32: s times the factors of a tile that may have unlike quads, times f
+    // (quad 2 t + half of the tile came with wave quad % 4)
+    auto by_factors = [&](auto role, int i, int half, f32x16 &s, float f) LEAP_INLINE {
+        constexpr bool V = decltype(role)::value;
+        const int *bits = &sh.odd[i & 3][V ? half : 4 + half];
+        const float *own = (V ? sh.vfac : sh.kfac)[i & 3][half], *all = (V ? sh.vquad : sh.kquad)[i & 3][half];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const bool unlike = (bits[2 * (t & 1)] >> (8 + (t >> 1))) & 1;
+            const float4 x = *reinterpret_cast<const float4 *>(own + 4 * t);
+            const float y = all[t];
+            s[4 * t] *= (unlike ? x.x : y) * f;
+            s[4 * t + 1] *= (unlike ? x.y : y) * f;
+            s[4 * t + 2] *= (unlike ? x.z : y) * f;
+            s[4 * t + 3] *= (unlike ? x.w : y) * f;
+        }
     };
     auto softmax = [&](int i) LEAP_INLINE {
         constexpr int F = Q8 ? 16 : 4, P = 16 / F;  // factors of a lane, scores of each
@@ -565,25 +568,30 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] *= kf[r];
         }
-        bool odd = false, extreme = false;
+        int odd = 0;
+        bool extreme = false;
         if (!Q8 && __builtin_expect(__builtin_amdgcn_readfirstlane(sh.any_odd), 0)) {
             extreme = __builtin_amdgcn_readfirstlane(sh.any_extreme);
-            int bits = 0;
 #pragma unroll
-            for (int x = 0; x < kWideWaves; x++) bits |= sh.odd[i & 3][x];
-            odd = __builtin_amdgcn_readfirstlane(bits) != 0;
+            for (int x = 0; x < kWideWaves; x++) odd |= sh.odd[i & 3][x];
+            odd = __builtin_amdgcn_readfirstlane(odd);
         }
         if (!Q8 && __builtin_expect(odd, 0)) {
-            int gg = lane;
-            asm volatile("" : "+v"(gg));  // (formed anew, for the registers' sake, here and below)
-            gg >>= 5;
+            int half = lane;
+            asm volatile("" : "+v"(half));  // (formed anew, for the registers' sake, here and below)
+            half >>= 5;
+            // each position by its own factor, and not by one that a position
+            // the row does not see has a part in: that may be infinite
+            by_factors(std::false_type{}, i, half, s, qf);
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int quad = 2 * (r >> 2) + gg;  // waves quad & 3 brought it, V and K
-                const int fk = sh.odd[i & 3][4 + (quad & 3)], both = sh.odd[i & 3][quad & 3] | fk;
-                if ((fk >> (8 + (quad >> 2))) & 1) s[r] *= sh.kfac[i & 3][gg][r];
-                if ((both >> (4 * (quad >> 2) + (r & 3))) & 1) s[r] = __uint_as_float(0x7fc00000u);
-            }
+            for (int t = 0; t < F; t++) kf[t] = 1.0f;
+            if (__builtin_expect(odd & 255, 0))
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int quad = 2 * (r >> 2) + half;  // waves quad & 3 brought it, V and K
+                    const int both = sh.odd[i & 3][quad & 3] | sh.odd[i & 3][4 + (quad & 3)];
+                    if ((both >> (4 * (quad >> 2) + (r & 3))) & 1) s[r] = __uint_as_float(0x7fc00000u);
+                }
         }
         if (__builtin_expect(key0 + kTileKeys > c1 || key0 + kTileKeys - 1 > all_see, 0)) {
             // visible: positions up to `limit`, and of a tree's nodes those of `sees`
@@ -643,8 +651,18 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         const bool plain = Q8 || extreme;
         const float vmul = plain ? exp2_int(-kRoom) : inverse(vrun);
         float vf[F];
+        bool check = moves || extreme;  // of the products against fp16's range and precision
+        if constexpr (Q8) {
 #pragma unroll
-        for (int t = 0; t < F; t++) vf[t] = Q8 ? fmaxf(vfs[t], 0.0f) * vmul : odd ? 1.0f : vfs[t] * vmul;
+            for (int t = 0; t < F; t++) vf[t] = fmaxf(vfs[t], 0.0f) * vmul;
+        } else {
+            const float by = odd ? 0.0f : vmul, one = odd ? 1.0f : 0.0f;  // (an odd tile's factors follow below)
+#pragma unroll
+            for (int t = 0; t < F; t++) vf[t] = __builtin_fmaf(vfs[t], by, one);
+            // (no product is above the largest probability times the largest factor)
+            const float most = fmaxf(fmaxf(fmaxf(vf[0], vf[1]), vf[2]), vf[3]);
+            check |= !odd && __builtin_amdgcn_ballot_w64(mt + (float)__builtin_amdgcn_frexp_expf(most) > off + 16.0f) != 0;
+        }
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
             float x, y;
@@ -659,26 +677,29 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             s[r] = x * vf[r / P];
             s[r + 1] = y * vf[(r + 1) / P];
         }
-        if (!Q8 && __builtin_expect(odd, 0)) {
-            int gg = lane;
-            asm volatile("" : "+v"(gg)::"memory");
-            gg >>= 5;
+        auto largest = [&]() LEAP_INLINE {
+            float x[5];
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] *= v_factor(i, gg, r) * vmul;
+            for (int r = 0; r < 5; r++) x[r] = fmaxf(fmaxf(s[3 * r], s[3 * r + 1]), s[3 * r + 2]);
+            return fmaxf(fmaxf(fmaxf(fmaxf(x[0], x[1]), x[2]), fmaxf(x[3], x[4])), s[15]);
+        };
+        if (!Q8 && __builtin_expect(odd, 0)) {
+            int half = lane;
+            asm volatile("" : "+v"(half)::"memory");
+            half >>= 5;
+            by_factors(std::true_type{}, i, half, s, vmul);
+            check |= __builtin_amdgcn_ballot_w64(largest() > 0x1p15f) != 0;
         }
         Half8 h[2], l[2];
         auto split = [&]() LEAP_INLINE {
 #pragma unroll
             for (int r = 0; r < 16; r += 2) split2(s[r], s[r + 1], h[r >> 3].h[(r & 7) / 2], l[r >> 3].h[(r & 7) / 2]);
         };
-        if constexpr (!Q8) split();  // (as it nearly always stays; the check below would be waited for)
-        float top3[5];
-#pragma unroll
-        for (int r = 0; r < 5; r++) top3[r] = fmaxf(fmaxf(s[3 * r], s[3 * r + 1]), s[3 * r + 2]);
-        float top = fmaxf(fmaxf(fmaxf(fmaxf(top3[0], top3[1]), top3[2]), fmaxf(top3[3], top3[4])), s[15]);
-        if (__builtin_expect(moves || extreme || __builtin_amdgcn_ballot_w64(top > (plain ? 0.5f * vrun : 0x1p15f)) != 0, 0)) {
+        if constexpr (!Q8) split();
+        if constexpr (Q8) check |= __builtin_amdgcn_ballot_w64(largest() > 0.5f * vrun) != 0;
+        if (__builtin_expect(check, 0)) {
             const int was = (int)(__float_as_uint(vrun) >> 23) - 127;
-            const int now = next_unit(was, half_max(top), plain ? kRoom - was : 0, up);
+            const int now = next_unit(was, half_max(largest()), plain ? kRoom - was : 0, up);
             const float os = fast_exp2((float)(was - now) - up);
             vrun = exp2_int(now);
 #pragma unroll

@@ -225,6 +225,21 @@ def test_keys_beside_a_larger_row(kind):
         run.check(y.reshape(run.n, -1), k.reshape(T, -1), v.reshape(T, -1), rows, tight=True)
 
 
+@pytest.mark.parametrize("key,value,bad", [(1e-20, 1.0, 1e30), (2.0 ** -40, 1.0, 2.0 ** 126), (1.0, 2.0 ** -30, 2.0 ** 126)])
+@pytest.mark.parametrize("kind", F32)
+def test_small_rows_ahead_of_a_huge_masked_one(kind, key, value, bad):
+    """Small keys under large queries, or small values, and a later token up to
+    2^166 times as large in the same four positions."""
+    run = Run(*kind, key=int(np.log2(bad)))
+    with run.m.h:
+        m, T = run.m, run.cached + run.n
+        k, v = (x * m.rng.standard_normal((T, m.nkv * m.hd)) for x in (key, value))
+        y = 2.0 / key * m.rng.standard_normal((run.n, m.nh * m.hd))
+        late = T // 4 * 4 - 1
+        (k if key != 1 else v)[late] = bad * m.rng.choice([-0.4, 0.4], m.nkv * m.hd)
+        run.check(y, k, v, slice(0, late - run.cached))
+
+
 # ---- bad nodes, bad bounds ---------------------------------------------------
 
 # (heads, KV heads, head_dim, tokens, cached rows, rows of a tile, one launch)
