@@ -240,6 +240,35 @@ def test_small_rows_ahead_of_a_huge_masked_one(kind, key, value, bad):
         run.check(y, k, v, slice(0, late - run.cached))
 
 
+@pytest.mark.parametrize("where,bad", [("k", 1e30), ("v", np.finfo(np.float32).max), ("k", np.nan), ("v", np.nan), ("v", np.inf)])
+@pytest.mark.parametrize("kind", [k for k in KINDS if not k[7]])
+def test_a_late_row_moves_nothing_ahead_of_it(kind, where, bad):
+    """Huge elements, or one that is not finite, in a late token: every row
+    ahead of it keeps its accuracy, and exactly the rows and heads that see a
+    row that is not finite are NaN."""
+    run = Run(*kind, key=17)
+    with run.m.h:
+        m, n = run.m, run.n
+        late = n - 3
+        y = 2.0 * m.rng.standard_normal((n, m.nh * m.hd))
+        k, v = (m.rng.standard_normal((run.cached + n, m.nkv * m.hd)) for _ in range(2))
+        if not np.isfinite(bad):
+            {"k": k, "v": v}[where][run.cached + late, m.hd + 5] = bad  # KV head 1
+            got, q, kr, vr = run.out(y, k, v)
+            group = m.nh // m.nkv
+            nan = np.isnan(got).reshape(n, m.nh, m.hd)
+            want = np.zeros((n, m.nh, m.hd), bool)
+            want[late:, group:2 * group] = True
+            assert np.array_equal(nan, want)
+        else:
+            {"k": k, "v": v}[where][run.cached + late, 3::13] = bad
+            got, q, kr, vr = run.out(y, k, v)
+        rows = slice(0, late)
+        kr, vr = (x[:run.cached + late] for x in (kr, vr))
+        want, bound = reference(m, q[rows], run.at[rows], kr, vr, run.see[rows, :run.cached + late])
+        within(got[rows], want, bound)
+
+
 # ---- bad nodes, bad bounds ---------------------------------------------------
 
 # (heads, KV heads, head_dim, tokens, cached rows, rows of a tile, one launch)
