@@ -91,9 +91,9 @@ __device__ __forceinline__ int wave_scan_add(int v)
 
 // Lane i's sequence base + i of the packed batch: its first token row, its
 // tokens (0 where there is none) and its first position.  A sequence is
-// skipped (n = -1) where its rows leave [0, n_tokens) or go backwards, as are
-// all after it, and where it has more than max_tokens tokens or positions
-// outside [0, max_pos].  *stop: the sequences behind these are skipped too.
+// skipped (n = -1) where its rows leave [0, n_tokens), where it has more than
+// max_tokens tokens or positions outside [0, max_pos], and from one whose rows
+// go backwards on.  *stop: the sequences behind these are skipped too.
 struct SeqLane {
     int first, n, p0;
 };
@@ -101,17 +101,17 @@ __device__ __forceinline__ SeqLane seq_lane(const ManyArgs &a, int base, int lan
 {
     const int i = base + lane;
     SeqLane s{0, 0, 0};
-    bool ok = true;
+    bool back = false;
     if (i < a.n_seq) {
         s.first = a.begin[i];
         const int end = a.begin[i + 1];
         s.p0 = a.pos[i];
-        ok = s.first >= 0 && end >= s.first && end <= a.n_tokens;
-        s.n = end - s.first;
+        back = end < s.first;
+        s.n = s.first >= 0 && end <= a.n_tokens ? end - s.first : -1;
     }
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(!ok);
-    *stop = bad != 0;
-    if (bad && lane >= __builtin_ctzll(bad)) s.n = i < a.n_seq ? -1 : 0;
+    const uint64_t backs = __builtin_amdgcn_ballot_w64(back);
+    *stop = backs != 0;
+    if (backs && lane >= __builtin_ctzll(backs)) s.n = i < a.n_seq ? -1 : 0;
     if (s.n > 0 && (s.n > a.max_tokens || s.p0 < 0 || s.p0 > a.max_pos + 1 - s.n)) s.n = -1;
     return s;
 }

@@ -316,3 +316,40 @@ def test_what_is_stored_below_a_bad_node(nh, nkv, hd, lens, cached, rows, fused,
         assert np.isnan(got[bad]).all()
         assert np.abs(got[~bad] - want[~bad]).max() <= 1e-5 * np.abs(want[~bad]).max()
         m.check_cache([a + n for a, n in zip(cached, lens)])
+
+
+def _nine_rows(cache):
+    """Three sequences of 20 cached rows, nine rows of tokens on the device, a call and what the caches held."""
+    import torch
+    m = Model(8, 2, 128, 128, 3, cache)
+    for i in range(3):
+        m.fill(i, 20)
+    before = [m.h.kv_download(i, 0, 0, 128) for i in range(3)]
+    tokens = m.tokens(9)
+    d = [torch.from_numpy(x).cuda() for x in tokens]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def call(begin, max_tokens):
+        out, b, p = torch.full((9, 1024), 7.0, device="cuda"), i32(begin), i32([20, 20, 20])
+        m.h.prompt_async(0, 3, _ptr(b), _ptr(p), 9, max_tokens, 99, *map(_ptr, d), _ptr(out),
+                         torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return out.cpu().numpy()
+    return m, tokens, before, call
+
+
+def _untouched(m, i, before):
+    after = m.h.kv_download(i, 0, 0, 128)
+    assert np.array_equal(after[0], before[i][0]) and np.array_equal(after[1], before[i][1])
+
+
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+def test_a_begin_ahead_of_the_arrays(cache):
+    """A sequence whose rows begin below 0 comes back as NaN, the others are served."""
+    m, (q, k, v), before, call = _nine_rows(cache)
+    with m.h:
+        got = call([-4, 3, 5, 8], 8)
+        assert np.isnan(got[:3]).all() and (got[8:] == 7).all()
+        want = m.want([3, 3, 5, 8], [20, 20, 20], q, k, v)
+        assert np.abs(got[3:8] - want[3:8]).max() <= 1e-5 * np.abs(want[3:8]).max()
+        _untouched(m, 0, before)
