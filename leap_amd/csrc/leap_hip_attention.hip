@@ -884,7 +884,11 @@ int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, c
     if (int rc = many_reserve(h, stream)) return rc;
     const size_t li = (size_t)(layer - h->cfg.layer_begin);
     const size_t loff = li * h->layer_floats;
-    const ManyPlan p = many_plan(h, !begin, n_seq, n_tokens, max_tokens, max_pos);
+    ManyPlan p{};
+    if (max_tokens > 0)
+        p = many_plan(h, !begin, n_seq, n_tokens, max_tokens, max_pos);
+    else
+        p.fn.append = pick_many(h->cfg.head_dim, kManySmall, h->q8kv).append;  // (NaN for whoever has tokens all the same)
     leap::ManyArgs a{};
     a.q = q;
     a.k_new = k;
@@ -925,12 +929,13 @@ int launch_many(leap_hip_attention *h, int layer, int n_seq, const int *begin, c
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)h->cfg.head_dim));
     a.by_group = leap::make_fastdiv((uint32_t)h->group);
     a.by_kv_heads = leap::make_fastdiv((uint32_t)h->cfg.n_kv_heads);
-    a.by_splits = leap::make_fastdiv((uint32_t)p.splits);
+    a.by_splits = leap::make_fastdiv((uint32_t)std::max(p.splits, 1));
     if (p.wgs > 0x7fffffffLL) return set_err(h, -EINVAL, "%lld workgroups in one launch", p.wgs);
-    if (!p.fn.attention) return set_err(h, -EINVAL, "unsupported head_dim %d", h->cfg.head_dim);
+    if (!p.fn.append) return set_err(h, -EINVAL, "unsupported head_dim %d", h->cfg.head_dim);
     if (!p.fused)
         HIP_TRY(h, launch_k(p.fn.append, dim3((unsigned)((n_tokens + leap::kAppendWaves - 1) / leap::kAppendWaves)),
                             dim3(leap::kAppendWaves * leap::kWave), stream, a));
+    if (max_tokens == 0) return 0;
     HIP_TRY(h, launch_k(p.fn.attention, dim3((unsigned)p.wgs), dim3((unsigned)(p.fn.waves * leap::kWave)), stream, a));
     if (p.spread) {
         const int many = p.fn.merge[1] && p.groups * p.fn.rows / leap::kMergeRows[1] >= 4 * h->n_cu;
@@ -2113,7 +2118,7 @@ static int many_async(leap_hip_attention *h, int layer, int n_seq, const int *be
     if (max_tokens > max_pos + 1)
         return set_err(h, -EINVAL, "max_tokens %d do not fit positions up to %d", max_tokens, max_pos);
     if (!begin || !pos || (tree && !parent)) return set_err(h, -EINVAL, "NULL buffer");
-    if (max_tokens == 0) return 0;
+    if (n_tokens == 0) return 0;
     if (!q || !k_new || !v_new || !out) return set_err(h, -EINVAL, "NULL buffer");
     if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(out) || !aligned4(begin) || !aligned4(pos) ||
         !aligned4(parent))

@@ -353,3 +353,14 @@ def test_a_begin_ahead_of_the_arrays(cache):
         want = m.want([3, 3, 5, 8], [20, 20, 20], q, k, v)
         assert np.abs(got[3:8] - want[3:8]).max() <= 1e-5 * np.abs(want[3:8]).max()
         _untouched(m, 0, before)
+
+
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+def test_a_bound_of_no_tokens(cache):
+    """Sequences with tokens under a bound of none come back as NaN."""
+    m, _, before, call = _nine_rows(cache)
+    with m.h:
+        got = call([0, 2, 2, 5], 0)
+        assert np.isnan(got[:5]).all() and (got[5:] == 7).all()
+        for i in range(3):
+            _untouched(m, i, before)
