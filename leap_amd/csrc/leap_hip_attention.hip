@@ -782,6 +782,8 @@ hipError_t load_many_table(int head_dim)
 // longer chunks.
 constexpr size_t kManyRecords = 65536;
 constexpr size_t kManyCounters = 4096;
+// fp32 rows of an 8-bit cache that a host transfer stages at a time.
+constexpr size_t kStagingBytes = size_t(8) << 20;
 
 // What a call is cut into.
 struct ManyPlan {
@@ -970,6 +972,31 @@ int launch_rows_q8(leap_hip_attention *h, int seq, int layer, int pos_begin, int
     const long long words = (long long)n * h->kv_dim / 4;
     const unsigned grid = (unsigned)std::min<long long>((words + 255) / 256, 8ll * h->n_cu);
     HIP_TRY(h, launch_k(k_in || v_in ? fn.write : fn.read, dim3(grid, 2), dim3(256), stream, a));
+    return 0;
+}
+
+// Rows [pos_begin, pos_end) of an 8-bit cache from (k_in, v_in) or to (k_out,
+// v_out) fp32 rows in host memory, either of each pair NULL or not: staged in
+// pieces, so that the handle keeps no more than one.
+int transfer_q8(leap_hip_attention *h, int seq, int layer, int pos_begin, int pos_end, const float *k_in, const float *v_in,
+                float *k_out, float *v_out)
+{
+    const int piece = (int)std::max<size_t>(1, kStagingBytes / (2 * (size_t)h->kv_dim * sizeof(float)));
+    const size_t most = (size_t)std::min(piece, pos_end - pos_begin) * h->kv_dim;
+    if (int rc = many_staging(h, 2 * most * sizeof(float))) return rc;
+    float *kd = reinterpret_cast<float *>(h->many_in), *vd = kd + most;
+    for (int at = pos_begin; at < pos_end; at += piece) {
+        const int rows = std::min(piece, pos_end - at);
+        const size_t off = (size_t)(at - pos_begin) * h->kv_dim, bytes = (size_t)rows * h->kv_dim * sizeof(float);
+        if (k_in) HIP_TRY(h, hipMemcpyAsync(kd, k_in + off, bytes, hipMemcpyHostToDevice, h->stream));
+        if (v_in) HIP_TRY(h, hipMemcpyAsync(vd, v_in + off, bytes, hipMemcpyHostToDevice, h->stream));
+        if (int rc = launch_rows_q8(h, seq, layer, at, rows, k_in ? kd : nullptr, v_in ? vd : nullptr, k_out ? kd : nullptr,
+                                    v_out ? vd : nullptr, h->stream))
+            return rc;
+        if (k_out) HIP_TRY(h, hipMemcpyAsync(k_out + off, kd, bytes, hipMemcpyDeviceToHost, h->stream));
+        if (v_out) HIP_TRY(h, hipMemcpyAsync(v_out + off, vd, bytes, hipMemcpyDeviceToHost, h->stream));
+    }
+    HIP_TRY(h, hipStreamSynchronize(h->stream));
     return 0;
 }
 
@@ -1863,18 +1890,7 @@ int leap_hip_attention_kv_upload(leap_hip_attention *h, int seq, int layer, int 
     if (int rc = kv_range(h, seq, layer, pos_begin, pos_end, &off, &n)) return rc;
     HIP_TRY(h, hipSetDevice(h->cfg.device));
     if (n == 0) return 0;
-    if (h->q8kv) {
-        if (!k && !v) return 0;
-        if (int rc = many_staging(h, 2 * n * sizeof(float))) return rc;
-        float *kd = reinterpret_cast<float *>(h->many_in), *vd = kd + n;
-        if (k) HIP_TRY(h, hipMemcpyAsync(kd, k, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
-        if (v) HIP_TRY(h, hipMemcpyAsync(vd, v, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
-        if (int rc = launch_rows_q8(h, seq, layer, pos_begin, pos_end - pos_begin, k ? kd : nullptr, v ? vd : nullptr,
-                                    nullptr, nullptr, h->stream))
-            return rc;
-        HIP_TRY(h, hipStreamSynchronize(h->stream));
-        return 0;
-    }
+    if (h->q8kv) return k || v ? transfer_q8(h, seq, layer, pos_begin, pos_end, k, v, nullptr, nullptr) : 0;
     if (k) HIP_TRY(h, hipMemcpyAsync(h->k_cache + off, k, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
     if (v) HIP_TRY(h, hipMemcpyAsync(h->v_cache + off, v, n * sizeof(float), hipMemcpyHostToDevice, h->stream));
     HIP_TRY(h, hipStreamSynchronize(h->stream));
@@ -1888,18 +1904,7 @@ int leap_hip_attention_kv_download(leap_hip_attention *h, int seq, int layer, in
     if (int rc = kv_range(h, seq, layer, pos_begin, pos_end, &off, &n)) return rc;
     HIP_TRY(h, hipSetDevice(h->cfg.device));
     if (n == 0) return 0;
-    if (h->q8kv) {
-        if (!k && !v) return 0;
-        if (int rc = many_staging(h, 2 * n * sizeof(float))) return rc;
-        float *kd = reinterpret_cast<float *>(h->many_in), *vd = kd + n;
-        if (int rc = launch_rows_q8(h, seq, layer, pos_begin, pos_end - pos_begin, nullptr, nullptr, k ? kd : nullptr,
-                                    v ? vd : nullptr, h->stream))
-            return rc;
-        if (k) HIP_TRY(h, hipMemcpyAsync(k, kd, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
-        if (v) HIP_TRY(h, hipMemcpyAsync(v, vd, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
-        HIP_TRY(h, hipStreamSynchronize(h->stream));
-        return 0;
-    }
+    if (h->q8kv) return k || v ? transfer_q8(h, seq, layer, pos_begin, pos_end, nullptr, nullptr, k, v) : 0;
     if (k) HIP_TRY(h, hipMemcpyAsync(k, h->k_cache + off, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
     if (v) HIP_TRY(h, hipMemcpyAsync(v, h->v_cache + off, n * sizeof(float), hipMemcpyDeviceToHost, h->stream));
     HIP_TRY(h, hipStreamSynchronize(h->stream));

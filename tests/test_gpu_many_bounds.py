@@ -364,3 +364,23 @@ def test_a_bound_of_no_tokens(cache):
         assert np.isnan(got[:5]).all() and (got[5:] == 7).all()
         for i in range(3):
             _untouched(m, i, before)
+
+
+# ---- memory of transfers -----------------------------------------------------
+
+def test_transfers_of_an_8_bit_cache_keep_little_memory():
+    """A full slab up and down: the staging of fp32 rows stays a few MiB."""
+    import torch
+    rows, nkv, hd = 30000, 8, 128
+    m = Model(8, nkv, hd, rows, 1, "q8")
+    with m.h:
+        k, v = (m.rng.standard_normal((rows, nkv * hd)).astype(np.float32) for _ in range(2))
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info()[0]
+        m.h.kv_upload(0, 0, 0, k, v)
+        a, b = m.h.kv_download(0, 0, 0, rows)
+        assert free - torch.cuda.mem_get_info()[0] <= 64 << 20
+        np.testing.assert_allclose(a, m.held(k), rtol=2.0 ** -24, atol=0)
+        np.testing.assert_allclose(b, m.held(v), rtol=2.0 ** -24, atol=0)
+        a, _ = m.h.kv_download(0, 0, 12345, 12350)
+        np.testing.assert_allclose(a, m.held(k[12345:12350]), rtol=2.0 ** -24, atol=0)
