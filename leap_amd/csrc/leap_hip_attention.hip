@@ -767,12 +767,16 @@ int alloc_all(leap_hip_attention *h, std::initializer_list<std::pair<void **, si
     return 0;
 }
 
-// The kernels' table for prompts, trees and the 8-bit cache (see
-// load_kernel_tables), for a handle that launches them.
+// The kernels' tables for prompts, trees and the 8-bit cache (see
+// load_kernel_tables), for a handle that launches them: one by head_dim, and
+// the one that has tree_keep's.
 hipError_t load_many_table(int head_dim)
 {
     hipFuncAttributes attr;
-    return hipFuncGetAttributes(&attr, reinterpret_cast<const void *>(pick_many(head_dim, kManySmall, false).attention));
+    for (const void *f : {reinterpret_cast<const void *>(pick_many(head_dim, kManySmall, false).attention),
+                          reinterpret_cast<const void *>(pick_keep(false))})
+        if (hipError_t e = hipFuncGetAttributes(&attr, f); e != hipSuccess) return e;
+    return hipSuccess;
 }
 
 // ---- prompts, trees and the 8-bit cache ----------------------------------

@@ -384,3 +384,28 @@ def test_transfers_of_an_8_bit_cache_keep_little_memory():
         np.testing.assert_allclose(b, m.held(v), rtol=2.0 ** -24, atol=0)
         a, _ = m.h.kv_download(0, 0, 12345, 12350)
         np.testing.assert_allclose(a, m.held(k[12345:12350]), rtol=2.0 ** -24, atol=0)
+
+
+@pytest.mark.parametrize("hd,cache", [(64, "f32"), (128, "f32"), (64, "q8")])
+def test_keeping_a_path_allocates_nothing(hd, cache):
+    """tree_keep_async behind a handle's first tree call, in a process of its
+    own: the code it runs is on the device by then."""
+    import subprocess
+    import sys
+    code = f"""
+import torch
+from leap_amd.attention import HipAttention
+with HipAttention(8, 2, {hd}, 128, cache="{cache}") as h:
+    x, kv = torch.zeros(4, {8 * hd}, device="cuda"), torch.zeros(4, {2 * hd}, device="cuda")
+    b, z = torch.tensor([0, 4], dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    roots = z - 1
+    s = torch.cuda.current_stream().cuda_stream
+    h.tree_async(0, 1, b.data_ptr(), z.data_ptr(), roots.data_ptr(), 4, 4, 8, x.data_ptr(), kv.data_ptr(), kv.data_ptr(), x.data_ptr(), s)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    h.tree_keep_async(1, z.data_ptr(), z.data_ptr(), 2, s)
+    torch.cuda.synchronize()
+    print("took", free - torch.cuda.mem_get_info()[0])
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "took 0\n" in r.stdout, r.stdout + r.stderr
