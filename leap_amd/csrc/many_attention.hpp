@@ -50,6 +50,7 @@ constexpr int kManySplits = 64;                        // chunks of a tile, at m
 constexpr int kTreeMax = 64;                           // nodes of a sequence's tree
 constexpr float kProbBias = 7.0f, kProbRoom = 8.0f;    // probabilities are 2^(score - reference + 7) <= 2^15
 constexpr int kLeastUnit = -110;                       // the least exponent of O's unit
+constexpr float kNothing = -3.4028234664e38f;          // the softmax reference of a row that has seen nothing
 constexpr int kRoom = 16;                              // 2^16: probabilities times factors over that are finite
 constexpr float kAmaxFloor = 7.888609052210118e-31f;   // 2^-100: the least largest magnitude of an 8-bit head row
 
@@ -214,6 +215,13 @@ __device__ __forceinline__ void split2(float x, float y, half2v &h, half2v &l)
     h = half2v{(_Float16)x, (_Float16)y};
     asm("" : "+v"(h));  // (the packed pair is what the remainders are taken from)
     l = half2v{(_Float16)(x - (float)h.x), (_Float16)(y - (float)h.y)};
+}
+// The same of x * f and y * g, whose products are not rounded first.
+__device__ __forceinline__ void split2_by(float x, float y, float f, float g, half2v &h, half2v &l)
+{
+    h = half2v{(_Float16)(x * f), (_Float16)(y * g)};
+    asm("" : "+v"(h));
+    l = half2v{(_Float16)__builtin_fmaf(x, f, -(float)h.x), (_Float16)__builtin_fmaf(y, g, -(float)h.y)};
 }
 union Half8 {
     half8v v;
@@ -464,17 +472,26 @@ struct ManyShared {
     int last;
 };
 
-// The exponent of O's unit in a row, whose largest probability times factor
-// in a tile is top 2^scale of the units it had.  The unit is a power of two
-// such that these products, whose halves are held to 2^-25 at least, stay in
-// fp16 and are not small where they are all that the row is made of: with
-// products of 2^15 and more it goes up, to where they are near 2^6, and where
-// the softmax reference has moved (up by `up`, which took 2^-up off O) and
-// they are below 2^5, it goes down as far; but not by over 2^60 more than O
-// has lost, which then outweighs them.
-__device__ __forceinline__ int next_unit(int unit, float top, int scale, float up)
+// O's unit in a row is a power of two, and a probability times its value row's
+// factor over it goes into fp16 halves, which hold 2^-25 at least and 2^15 with
+// room.  Whether a tile leaves it, and the reference of the softmax, as they
+// are: mt is the largest score, and the exponent of `most` at least that of any
+// factor over the unit (of positions seen or not; NaN or infinite: it does not).
+__device__ __forceinline__ bool fits_unit(float mt, float ref, float most)
 {
-    const int e = (int)(__float_as_uint(top) >> 23) - 127 + scale;
+    // mt <= ref + 8, and mt - ref + 7 + (e - 127) <= 15
+    const float e = (float)max((int)(__float_as_uint(most) >> 23), 127);
+    return __builtin_fmaf(most, 0.0f, mt) + e <= ref + (kProbRoom + 127.0f);
+}
+// And where it does not, the unit's exponent: top 2^16 is the row's largest
+// product in the tile, `up` by how much the reference moved, which takes 2^-up
+// off what O holds.  With products of 2^15 units and more it goes up, to where
+// they are near 2^6.  With less than 2^5 after the reference moved (so that
+// they may be all that the row is made of) it goes down as far; but not by over
+// 2^60 more than O loses, which then outweighs them.
+__device__ __forceinline__ int next_unit(int unit, float top, float up)
+{
+    const int e = (int)(__float_as_uint(top) >> 23) - 127 + kRoom - unit;
     if (e < 15 && (up == 0.0f || e >= 5)) return unit;
     return min(max(unit + e - 6, max(kLeastUnit, unit - (int)fminf(up + 60.0f, 300.0f))), 126);
 }
@@ -849,7 +866,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
     const float qf = sh.qf[m];
 
     f32x4 o[VB];
-    float mrun = -__builtin_inff(), lrun = 0.0f;
+    float mrun = kNothing, lrun = 0.0f;
 #pragma unroll
     for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
     int erun = 0;  // O's unit in the lane's row is 2^(erun - 12) (8 bits: 2^erun, and values are 2^-9 times theirs)
@@ -1000,8 +1017,9 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
             }
         }
         // The reference, a whole number, moves only when a score exceeds it by
-        // more than 2^8: most tiles leave O and the sum as they are, and need
-        // no maximum over the row's lanes.
+        // more than 2^8, and O's unit where a product passes 2^15 of it: most
+        // tiles leave both, O and the sum as they are, and need no maximum over
+        // the row's lanes.
         auto largest = [&]() {
             return fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
         };
@@ -1010,11 +1028,11 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         if (moves) {
             mt = rows4<true>(mt);
             const float now = mt > mrun + kProbRoom ? ceilf(mt) : mrun;
-            if (now != mrun) up = now - mrun;  // (infinite from nothing)
+            up = now - mrun;
             lrun *= fast_exp2(-up);
             mrun = now;
         }
-        const float off = (mrun == -__builtin_inff() ? 0.0f : mrun) - kProbBias;  // (a row that has seen nothing yet)
+        const float off = mrun - kProbBias;
         // Probabilities times their value rows' factors (2^-16 of them: these
         // products are finite, and as small as fp32 holds).
 #pragma unroll
@@ -1025,7 +1043,7 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         }
         float top = largest();
         if (moves || __builtin_amdgcn_ballot_w64(top > exp2_int(erun - kRoom + 15))) {
-            const int now = next_unit(erun, rows4<true>(top), kRoom - erun, up);
+            const int now = next_unit(erun, rows4<true>(top), up);
             const float os = fast_exp2((float)(erun - now) - up);
             erun = now;
 #pragma unroll
@@ -1091,7 +1109,6 @@ __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_atte
         float top = sh.m[0][row];
 #pragma unroll
         for (int w = 1; w < W; w++) top = fmaxf(top, sh.m[w][row]);
-        if (top == -__builtin_inff()) top = 0.0f;
         float f[W], total = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) {

@@ -33,9 +33,10 @@
 // head_dim 128, 8192 tokens: 6% more time than exponents by quad and one unit
 // for all rows; by position throughout 10 to 20% more.)
 //
-// The running maximum is a reference that moves only when a score exceeds it
-// by more than 2^8 (then O and the sum are rescaled): probabilities are
-// 2^(s - ref + 7) <= 2^15.
+// The softmax reference moves only when a score exceeds it by more than 2^8,
+// and O's unit only when a product could pass fp16's range (fits_unit, asked
+// of the tile's largest score and factor): such a tile is taken once more, by
+// its products.
 //
 // Measured, heads/KV heads/head_dim: 8192 tokens 32/8/128 in fp32 1676 us, 328
 // TFLOP/s of useful work (984 of fp16 products), the card at 1.6 to 2.0 GHz
@@ -59,7 +60,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = kWideWaves * kWave;
-constexpr int kOrdinary = 50;  // fp32 values of 2^-50 .. 2^50: no probability times factors over O's unit overflows
 constexpr unsigned kUnlike = 4;  // binary orders between positions of a quad from which each has an exponent of its own
 
 template <int HD, bool Q8>
@@ -83,7 +83,6 @@ struct WideShared {
     // fp32, by the wave that brought them: positions that are not finite
     // (bits 0-7), quads of unlike positions (bits 8-9); any: of a tile so far
     int odd[4][kWideWaves], any_odd;
-    int any_extreme;  // fp32 values so far outside 2^-50 .. 2^50
     uint64_t sees[kTreeMax], bad;  // tree_lane of each node, and the bad ones
 };
 
@@ -144,7 +143,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
     const int c0 = split * a.chunk, c1 = min(kv_end, c0 + a.chunk);
     if (c0 >= kv_end) return;
     const int n_tiles = (c1 - c0 + kTileKeys - 1) / kTileKeys;
-    if (tid == 0) sh.any_odd = sh.any_extreme = 0;
+    if (tid == 0) sh.any_odd = 0;
     __syncthreads();
     auto tile_key = [&](int i) LEAP_INLINE { return c0 + kTileKeys * i; };
 
@@ -244,7 +243,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
         constexpr bool V = decltype(role)::value;
         if (Q8 || i >= n_tiles) return;
         int oddbits = 0, ln = lane;
-        bool extreme = false;
         asm volatile("" : "+v"(ln));  // (addresses formed anew, for the registers' sake)
         if constexpr (!Q8) {
 #pragma unroll
@@ -295,9 +293,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                         if (__builtin_amdgcn_ballot_w64((bits >> b) & 1)) oddbits |= 1 << (4 * t + b);
                     look();
                 }
-                const int e = V && most == 0 ? 0 : tile_exp(most);
+                const int e = tile_exp(most);
                 stage_sc[t] = exp2_int(13 - e);
-                if constexpr (V) extreme |= (unsigned)(e + kOrdinary) > 2u * kOrdinary;
                 // (every lane writes the same: no branch)
                 (V ? sh.vquad : sh.kquad)[i & 3][quad & 1][quad >> 1] = exp2_int(e - 13);
                 if (__builtin_expect(unlike, 0)) {
@@ -306,7 +303,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
                     for (int j = 0; j < Y; j++) {
                         const unsigned top = V ? wave_max_bits(__float_as_uint(y[j])) : dpp_max16(__float_as_uint(y[j]));
                         const int own = top == 0 ? e : tile_exp(top);
-                        if constexpr (V) extreme |= own < -kOrdinary;
 #pragma unroll
                         for (int u = j; u < N; u += Y) x[u] = __builtin_amdgcn_ldexpf(x[u], e - own);
                         (V ? sh.vfac : sh.kfac)[i & 3][quad & 1][4 * (quad >> 1) + (V ? j : ln >> 4)] = exp2_int(own - 13);
@@ -316,10 +312,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             }
         }
         sh.odd[i & 3][wave] = oddbits;
-        if (__builtin_expect(oddbits != 0 || extreme, 0)) {
-            if (extreme) sh.any_extreme = 1;
-            sh.any_odd = 1;
-        }
+        if (__builtin_expect(oddbits != 0, 0)) sh.any_odd = 1;
     };
     unsigned hi[2], lo[2];
     constexpr int P = WideShared<HD, Q8>::P;
@@ -475,7 +468,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
         for (int r = 0; r < 16; r++) o[v][r] = 0.0f;
     half8v ph[2], pl[2];
-    float ref = -__builtin_inff(), sum = 0.0f, vrun = 1.0f;  // (vrun: O's unit in the lane's row)
+    float ref = kNothing, sum = 0.0f, vrun = 1.0f;  // (vrun: O's unit in the lane's row)
 
     // (a lane's pieces: K piece 2 t + g of position n, V piece 2 u + g of dim
     // 32 v + n; the swizzles leave t and u as an exclusive or on the first's
@@ -569,9 +562,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
             for (int r = 0; r < 16; r++) s[r] *= kf[r];
         }
         int odd = 0;
-        bool extreme = false;
         if (!Q8 && __builtin_expect(__builtin_amdgcn_readfirstlane(sh.any_odd), 0)) {
-            extreme = __builtin_amdgcn_readfirstlane(sh.any_extreme);
 #pragma unroll
             for (int x = 0; x < kWideWaves; x++) odd |= sh.odd[i & 3][x];
             odd = __builtin_amdgcn_readfirstlane(odd);
@@ -624,99 +615,70 @@ __global__ __launch_bounds__(kWideThreads, 2) void wide_attention_kernel(ManyArg
 #pragma unroll
             for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[r]);
         }
-        // The reference, a whole number, moves only when a score exceeds it by
-        // more than 2^8: most tiles leave O and the sum as they are, and need
-        // no maximum over both lanes of a row.
-        const bool moves = __builtin_amdgcn_ballot_w64(mt > ref + kProbRoom) != 0;
-        float up = 0.0f;
-        if (__builtin_expect(moves, 0)) {
-            mt = half_max(mt);
-            const float now = mt > ref + kProbRoom ? ceilf(mt) : ref;
-            if (now != ref) up = now - ref;  // (infinite from nothing)
-            sum *= fast_exp2(-up);
-            ref = now;
-            if constexpr (!Q8) {
-                // (a first guess at O's unit, for values alike)
-                const float f = half_max(fmaxf(fmaxf(vfs[0], vfs[1]), fmaxf(vfs[2], vfs[3])));
-                if (up == __builtin_inff()) vrun = 0.5f * f;
-            }
-        }
-        const float off = (ref == -__builtin_inff() ? 0.0f : ref) - kProbBias;
-        if constexpr (Q8) asm volatile("" ::: "memory");  // (sixteen factors are read again rather than kept)
-        // Probabilities times their value rows' factors: in O's unit, or (8
-        // bits, and once there were fp32 values of extreme sizes) times 2^-16,
-        // which is finite and as small as fp32 holds.  0 for a scale of NaN,
-        // which a masked probability may meet.
+        // (the reference and O's unit move as in many_attention.hpp: most
+        // tiles leave both, and need no maximum over both lanes of a row)
         auto inverse = [](float x) LEAP_INLINE { return __uint_as_float(0x7f000000u - __float_as_uint(x)); };  // (of powers of two)
-        const bool plain = Q8 || extreme;
-        const float vmul = plain ? exp2_int(-kRoom) : inverse(vrun);
-        float vf[F];
-        bool check = moves || extreme;  // of the products against fp16's range and precision
-        if constexpr (Q8) {
+        const float vinv = inverse(vrun);
+        float most = vfs[0];
 #pragma unroll
-            for (int t = 0; t < F; t++) vf[t] = fmaxf(vfs[t], 0.0f) * vmul;
-        } else {
-            const float by = odd ? 0.0f : vmul, one = odd ? 1.0f : 0.0f;  // (an odd tile's factors follow below)
-#pragma unroll
-            for (int t = 0; t < F; t++) vf[t] = __builtin_fmaf(vfs[t], by, one);
-            // (no product is above the largest probability times the largest factor)
-            const float most = fmaxf(fmaxf(fmaxf(vf[0], vf[1]), vf[2]), vf[3]);
-            check |= !odd && __builtin_amdgcn_ballot_w64(mt + (float)__builtin_amdgcn_frexp_expf(most) > off + 16.0f) != 0;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-            float x, y;
-            if constexpr (!Q8) {
-                x = fast_exp2(__builtin_fmaf(s[r], kf[r / P], -off));
-                y = fast_exp2(__builtin_fmaf(s[r + 1], kf[r / P], -off));
-            } else {
-                x = fast_exp2(s[r] - off);
-                y = fast_exp2(s[r + 1] - off);
-            }
-            sum += x + y;
-            s[r] = x * vf[r / P];
-            s[r + 1] = y * vf[(r + 1) / P];
-        }
-        auto largest = [&]() LEAP_INLINE {
-            float x[5];
-#pragma unroll
-            for (int r = 0; r < 5; r++) x[r] = fmaxf(fmaxf(s[3 * r], s[3 * r + 1]), s[3 * r + 2]);
-            return fmaxf(fmaxf(fmaxf(fmaxf(x[0], x[1]), x[2]), fmaxf(x[3], x[4])), s[15]);
+        for (int t = 1; t < F; t++) most = fmaxf(most, vfs[t]);
+        if constexpr (Q8) asm volatile("" ::: "memory");  // (sixteen factors are read again rather than kept)
+        Half8 h[2], l[2];
+        auto split = [&](int r, float x, float y, float f, float g) LEAP_INLINE {
+            split2_by(x, y, f, g, h[r >> 3].h[(r & 7) / 2], l[r >> 3].h[(r & 7) / 2]);
         };
-        if (!Q8 && __builtin_expect(odd, 0)) {
+        auto prob = [&](int r, float off) LEAP_INLINE { return fast_exp2(Q8 ? s[r] - off : __builtin_fmaf(s[r], kf[r / P], -off)); };
+        // (scales of 8 bits are no powers of two: the next)
+        const bool fits = __builtin_amdgcn_ballot_w64(!fits_unit(mt, ref, (Q8 ? 2.0f : 1.0f) * most * vinv)) == 0;
+        float total = sum;
+        {
+            const float off = ref - kProbBias;
+            float vf[F];  // (0 for a scale of NaN, which a masked probability may meet)
+#pragma unroll
+            for (int t = 0; t < F; t++) vf[t] = Q8 ? fmaxf(vfs[t] * vinv, 0.0f) : vfs[t] * vinv;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float x = prob(r, off), y = prob(r + 1, off);
+                total += x + y;
+                split(r, x, y, vf[r / P], vf[(r + 1) / P]);
+            }
+        }
+        if (__builtin_expect(!fits || odd, 0)) {
+            // all of that again
+            mt = half_max(mt);
+            const float now = mt > ref + kProbRoom ? ceilf(mt) : ref, up = now - ref, off = now - kProbBias;
+            ref = now;
+            total = sum * fast_exp2(-up);
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[r] = prob(r, off);
+                total += s[r];
+            }
             int half = lane;
             asm volatile("" : "+v"(half)::"memory");
             half >>= 5;
-            by_factors(std::true_type{}, i, half, s, vmul);
-            check |= __builtin_amdgcn_ballot_w64(largest() > 0x1p15f) != 0;
-        }
-        Half8 h[2], l[2];
-        auto split = [&]() LEAP_INLINE {
+            if constexpr (Q8) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) split2(s[r], s[r + 1], h[r >> 3].h[(r & 7) / 2], l[r >> 3].h[(r & 7) / 2]);
-        };
-        if constexpr (!Q8) split();
-        if constexpr (Q8) check |= __builtin_amdgcn_ballot_w64(largest() > 0.5f * vrun) != 0;
-        if (__builtin_expect(check, 0)) {
-            const int was = (int)(__float_as_uint(vrun) >> 23) - 127;
-            const int now = next_unit(was, half_max(largest()), plain ? kRoom - was : 0, up);
-            const float os = fast_exp2((float)(was - now) - up);
-            vrun = exp2_int(now);
+                for (int r = 0; r < 16; r++) s[r] *= fmaxf(sh.vfac[i & 3][half][r], 0.0f) * exp2_int(-kRoom);
+            } else if (odd) {
+                by_factors(std::true_type{}, i, half, s, exp2_int(-kRoom));
+            } else {
 #pragma unroll
-            for (int v = 0; v < VB; v++) o[v] *= os;
-            if (!Q8 && __builtin_expect(extreme || __builtin_amdgcn_ballot_w64(now != was) != 0, 0)) {
-                const float by = exp2_int(extreme ? kRoom - now : was - now);
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] *= by;
-                split();
+                for (int r = 0; r < 16; r++) s[r] *= sh.vquad[i & 3][half][r >> 2] * exp2_int(-kRoom);
             }
-        }
-        if constexpr (Q8) {
-            const float by = inverse(vrun) * exp2_int(kRoom);
+            float top = fmaxf(s[0], s[1]);
 #pragma unroll
-            for (int r = 0; r < 16; r++) s[r] *= by;
-            split();
+            for (int r = 2; r < 16; r += 2) top = fmaxf(fmaxf(top, s[r]), s[r + 1]);
+            const int was = (int)(__float_as_uint(vrun) >> 23) - 127, unit = next_unit(was, half_max(top), up);
+            const float os = fast_exp2((float)(was - unit) - up), by = exp2_int(kRoom - unit);
+            vrun = exp2_int(unit);
+            if (__builtin_amdgcn_ballot_w64(os != 1.0f))
+#pragma unroll
+                for (int v = 0; v < VB; v++) o[v] *= os;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) split(r, s[r], s[r + 1], by, by);
         }
+        sum = total;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             ph[u] = h[u].v;
