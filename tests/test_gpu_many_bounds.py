@@ -268,6 +268,52 @@ def test_a_late_row_moves_nothing_ahead_of_it(kind, where, bad):
         want, bound = reference(m, q[rows], run.at[rows], kr, vr, run.see[rows, :run.cached + late])
         within(got[rows], want, bound)
 
+# Every form that a call is cut into, over both caches and in both head_dims:
+# heads, KV heads, head_dim, new tokens and cached rows of the sequences, rows
+# of a tile, one launch or two, more chunks than one, spread over the XCDs.
+FORMS = [
+    ("q8", 32, 8, 128, (8,), (300,), 16, True, False, False), ("f32", 3, 1, 64, (2,) * 100, (10,) * 100, 16, True, False, False),
+    ("f32", 32, 8, 128, (33,), (30,), 16, False, False, False), ("q8", 32, 8, 128, (40,) * 9, (100,) * 9, 16, False, False, False),
+    ("f32", 32, 8, 128, (8,), (300,), 16, True, True, False), ("q8", 32, 4, 64, (8,), (3000,), 16, True, True, False),
+    ("f32", 3, 1, 64, (33,), (3000,), 16, False, True, False), ("q8", 32, 8, 128, (33,), (3000,), 16, False, True, False),
+    ("f32", 3, 1, 64, (8,), (30000,), 16, True, True, True), ("q8", 8, 1, 128, (1,), (60000,), 16, True, True, True),
+    ("f32", 32, 8, 128, (64,) * 40, (50,) * 40, 256, False, False, False), ("q8", 64, 8, 128, (700,), (0,), 256, False, False, False),
+    ("f32", 8, 1, 128, (700,), (0,), 256, False, True, True), ("q8", 64, 8, 128, (64,) * 8, (1000,) * 8, 256, False, True, True),
+    ("f32", 32, 4, 64, (64,), (12000,), 256, True, True, True), ("q8", 32, 8, 128, (64,) * 8, (2000,) * 8, 256, True, True, True),
+    ("f32", 64, 4, 64, (33, 5, 64), (900, 2000, 0), 256, True, True, True),
+]
+
+
+@pytest.mark.parametrize("cache,nh,nkv,hd,lens,cached,rows,fused,split,spread,tree",
+                         [f + (t,) for f in FORMS for t in (False, True) if not t or max(f[4]) <= 64])
+def test_every_form_of_a_call(cache, nh, nkv, hd, lens, cached, rows, fused, split, spread, tree):
+    p = plan(nh, nkv, hd, cache, lens, cached)
+    assert (p.rows, p.fused, p.splits > 1, p.spread) == (rows, fused, split, spread), p
+    m = Model(nh, nkv, hd, max(a + b for a, b in zip(lens, cached)), len(lens), cache, key=sum(lens) + tree)
+    with m.h:
+        for i, c in enumerate(cached):
+            m.fill(i, c)
+        begin = _begin(lens)
+        parent = np.concatenate([[max(-1, j - int(m.rng.integers(1, 5))) for j in range(n)] for n in lens]).astype(np.int32)
+        q, k, v = m.tokens(begin[-1])
+        got = m.h.tree(0, begin, cached, parent, q, k, v) if tree else m.h.prompt(0, begin, cached, q, k, v)
+        for i, (n, c) in enumerate(zip(lens, cached)):
+            among = np.tril(np.ones((n, n), bool))
+            if tree:
+                among[:] = np.eye(n, dtype=bool)
+                for j in range(n):
+                    if parent[begin[i] + j] >= 0:
+                        among[j] |= among[parent[begin[i] + j]]
+            see = np.concatenate([np.ones((n, c), bool), among], axis=1)
+            at = c + among.sum(axis=1) - 1
+            for j in range(n):
+                m.k[i, c + j] = m.held(rope_f32(k[begin[i] + j], m.cos[at[j]], m.sin[at[j]]))
+                m.v[i, c + j] = m.held(v[begin[i] + j])
+            rr = slice(begin[i], begin[i] + n)
+            want, bound = reference(m, q[rr], at, m.k[i, :c + n], m.v[i, :c + n], see)
+            within(got[rr], want, bound)
+        m.check_cache([a + b for a, b in zip(lens, cached)])
+
 
 # ---- bad nodes, bad bounds ---------------------------------------------------
 
