@@ -186,9 +186,9 @@ int leap_hip_attention_step_noalloc(const leap_hip_attention_config *cfg, int po
  * 2^-22 of themselves or 2^-34 of their head row's largest element, whichever
  * is more (rows of less than 2^-100: to 2^-138), a weight times its value row's
  * largest element to 2^-22 of itself or 2^-30 of the largest such product of
- * the output row, sums are fp32.  An output row that attends to a key or value
- * row with an infinity or a NaN is NaN; what a row does not attend to does not
- * affect it further, whatever its size.
+ * the output row, sums are fp32.  Nothing that a row does not attend to moves
+ * it beyond that, whatever its size.  An output row that attends to a key or
+ * value row with an infinity or a NaN is NaN.
  * Host pointers: begin [n_seq+1] ascending from >= 0, pos [n_seq]; returns
  * when `out` is written.  -EINVAL, with nothing changed, if a sequence's
  * positions leave [0, seq_len). */
