@@ -612,14 +612,14 @@ __device__ __forceinline__ void merge_rows(const ManyArgs &a, Merge &sh, int gi,
 //
 // Short calls are latency: the launch, the rows of q, a pass or two of W x 32
 // positions, the records (3 us).  A pass is bound by its vector instructions,
-// about 480 a wave at head_dim 128 over 8 bits (900 in fp32) beside 32 (48)
+// about 500 a wave at head_dim 128 over 8 bits (900 in fp32) beside 32 (48)
 // products, half of them making fp16 operands of what comes from memory; 16
 // rows share them.  Eight waves for 8 bits, whose passes are short (one
 // workgroup a CU then holds 64 KB of rows on their way), four in fp32.
-// Measured under graph replay, heads/KV heads/head_dim, us: 8-bit step 32/4/64
-// at 256 5.2, 32/8/128 at 4096 10.7 and at 65536 30.5 (4.5 TB/s), 32 sequences
-// at 4096 51.4 (5.2 TB/s); fp32 tree of 8 at 258 32/4/64 10.0, of 31 at 1024
-// 32/8/128 20.5.
+// Measured under graph replay over several layers, heads/KV heads/head_dim, us:
+// 8-bit step 32/4/64 at 256 5.7, 32/8/128 at 4096 11.2 and at 65536 36.5 (3.8
+// TB/s), 32 sequences at 4096 63 (4.3 TB/s; one layer again and again 52);
+// fp32 tree of 8 at 258 32/4/64 10.6, of 31 at 1024 32/8/128 23.0.
 template <int HD, int W, bool Q8, bool STEP>
 __global__ __launch_bounds__(W * kWave, HD == 128 && !Q8 ? 1 : 2) void many_attention_kernel(ManyArgs a)
 {

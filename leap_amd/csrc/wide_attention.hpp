@@ -6,7 +6,7 @@
 //
 // Per wave and tile of 32 positions at head_dim 128: 48 32x32x16 MFMAs (three
 // products of S^T = K Q^T and of O^T = V^T P^T), 1536 cycles of the matrix
-// core, and about 300 vector instructions: 250 of the vector phase (the
+// core, and about 340 vector instructions: 260 of the vector phase (the
 // scores' scaling, maximum and 16 exponentials, the split of P, the largest
 // magnitudes of a share of the next tile) and that share's split, which fills
 // the waits between the products of the matrix phase (in the vector phase it
@@ -38,11 +38,11 @@
 // of the tile's largest score and factor): such a tile is taken once more, by
 // its products.
 //
-// Measured, heads/KV heads/head_dim: 8192 tokens 32/8/128 in fp32 1676 us, 328
-// TFLOP/s of useful work (984 of fp16 products), the card at 1.6 to 2.0 GHz
-// under it; 500 tokens at 7000 64/8/128 371 us (298 TFLOP/s); 4096 tokens over
-// an 8-bit cache 313 us (439 TFLOP/s).  A workgroup's start (its rows of Q) is
-// about 10 us, its results 2 to 3.
+// Measured, heads/KV heads/head_dim: 8192 tokens 32/8/128 in fp32 1671 us with
+// their append, 329 TFLOP/s of useful work (987 of fp16 products), the card at
+// 1.6 to 2.0 GHz under it; 500 tokens after 6800 64/8/128 374 us (309 TFLOP/s);
+// 4096 tokens over an 8-bit cache 310 us (443 TFLOP/s).  A workgroup's start
+// (its rows of Q) is about 10 us, its results 2 to 3.
 //
 // A call of few tokens (fused) has its new rows rotated, quantised and stored
 // here, ahead of the first tile.
