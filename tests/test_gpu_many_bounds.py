@@ -171,6 +171,23 @@ def test_values_at_the_ends_of_fp32(kind, size):
         shape = (run.cached + run.n, run.m.nkv * run.m.hd)
         run.check(y, keys(score), size * run.m.rng.uniform(1, 3, shape) * run.m.rng.choice([-1, 1], shape))
 
+@pytest.mark.parametrize("what", ["values", "the first values", "every other value", "keys", "queries"])
+@pytest.mark.parametrize("kind", KINDS)
+def test_zeros(kind, what):
+    """Rows of zeros, whose exponents mean nothing, alone and beside others."""
+    run = Run(*kind, key=len(what))
+    with run.m.h:
+        m, T = run.m, run.cached + run.n
+        y = 2.0 * m.rng.standard_normal((run.n, m.nh * m.hd))
+        k, v = (m.rng.standard_normal((T, m.nkv * m.hd)) for _ in range(2))
+        if what == "queries":
+            y[:] = 0
+        elif what == "keys":
+            k[::3] = 0
+        else:
+            v[{"values": slice(None), "the first values": slice(0, run.cached), "every other value": slice(0, T, 2)}[what]] = 0
+        run.check(y, k, v)
+
 
 F32 = [k for k in KINDS if k[3] == "f32"]
 
