@@ -280,6 +280,172 @@ int leap_hip_attention_kv_read_async(leap_hip_attention *h, int seq, int layer, 
 int leap_hip_attention_kv_q8_device_ptr(leap_hip_attention *h, int seq, int layer, int8_t **k8,
                                         float **ks, int8_t **v8, float **vs);
 
+/* ---- Caches of pages ------------------------------------------------------- */
+
+/* A cache whose rows lie in pages of a common pool, for batches whose lengths
+ * are not known beforehand and sequences that share rows (a common prompt,
+ * several samples, beams).  A handle of its own, with the conventions above.
+ *
+ * A page holds page_rows rows of every KV head in every held layer.  Sequence
+ * i (0 <= i < max_batch) has row i of the table, [max_batch][width] page
+ * numbers in the order of its rows, -1 where it has none; width is seq_len /
+ * page_rows rounded up.  refs[p] is the number of places that name page p; a
+ * page is free where that is 0, and a sequence's own where it is 1.  The
+ * calls below change the table: reserve before rows are written, fork to
+ * share, cut back and free, compact.  Page numbers follow from the calls
+ * alone, not from timing: the lowest free page goes first to the first
+ * sequence's first row.  Entry points that take n_seq work on the sequences
+ * 0..n_seq-1. */
+typedef struct leap_hip_attention_pages leap_hip_attention_pages;
+
+typedef struct leap_hip_attention_pages_config {
+    leap_hip_attention_config model; /* seq_len: rows of a sequence at most
+                                        (the RoPE table's); max_batch:
+                                        sequences                              */
+    int page_rows; /* rows of a page: 16, 32, 64 or 128                         */
+    int n_pages;   /* pages of the pool                                         */
+    int q8;        /* 0: fp32 rows; 1: int8 values and a scale per row and KV
+                      head, as leap_hip_attention_create_q8kv                   */
+    int bounds;    /* 1: keeps the bounds of each page's keys, which
+                      pages_step_sparse needs; 0: does not                      */
+} leap_hip_attention_pages_config;
+
+/* The pool is zeroed and every table empty.  -EINVAL for a model that
+ * leap_hip_attention_create refuses but for the size of a sequence's rows
+ * (here seq_len <= 2^24), a page size or a flag other than the above, n_pages
+ * outside [1, 2^26] and, with bounds, more than 16384 pages a sequence. */
+int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, leap_hip_attention_pages **out);
+int leap_hip_attention_pages_destroy(leap_hip_attention_pages *p);
+/* As leap_hip_attention_last_error; NULL: of the last pages_create here. */
+const char *leap_hip_attention_pages_last_error(const leap_hip_attention_pages *p);
+
+/* Rows [begin[i], end[i]) of sequence i will be written: afterwards it has
+ * pages for them, and they are its own.  A missing page is a free one (it
+ * holds what it held), a shared one is replaced by a copy, in all held layers;
+ * where all who share a page ask for it in one call, the last of them keeps
+ * it.  -ENOMEM, with nothing changed, if the pool has too few free pages.
+ * Host pointers; -EINVAL, with nothing changed, for a range outside
+ * [0, seq_len]. */
+int leap_hip_attention_pages_reserve(leap_hip_attention_pages *p, int n_seq, const int *begin, const int *end);
+/* The same with device pointers, enqueued on `stream`.  A sequence whose range
+ * is bad is left out.  status [n_seq] (or NULL) gets 0, -EINVAL for a sequence
+ * left out, or, of every other one, -ENOMEM: nothing changed for any. */
+int leap_hip_attention_pages_reserve_async(leap_hip_attention_pages *p, int n_seq, const int *begin, const int *end,
+                                           int *status, void *stream);
+
+/* Sequence i takes the pages of the first rows[i] rows of sequence parent[i]
+ * (any of the handle's), as all tables were before the call: shared, nothing
+ * is copied.  parent NULL: each its own, so that it is cut back to rows[i]
+ * rows, 0 to free it.  Pages that no one names any more are free.  (A beam
+ * search's reordering is one fork with the chosen parents; then reserve the
+ * next row.)  A parent's missing pages stay missing.  Host pointers; -EINVAL,
+ * with nothing changed, for a parent outside [0, max_batch) or rows outside
+ * [0, seq_len]. */
+int leap_hip_attention_pages_fork(leap_hip_attention_pages *p, int n_seq, const int *parent, const int *rows);
+/* The same with device pointers, enqueued on `stream`; a sequence whose parent
+ * or rows are out of range stays as it is. */
+int leap_hip_attention_pages_fork_async(leap_hip_attention_pages *p, int n_seq, const int *parent, const int *rows,
+                                        void *stream);
+
+/* Moves pages down until those in use are the first `used` ones: the i-th page
+ * in use from number `used` on goes to the i-th free page below it, in every
+ * layer, and the tables follow.  *used (or NULL) gets their number. */
+int leap_hip_attention_pages_compact(leap_hip_attention_pages *p, int *used);
+/* The same, enqueued on `stream`; used: a device pointer or NULL. */
+int leap_hip_attention_pages_compact_async(leap_hip_attention_pages *p, int *used, void *stream);
+
+/* leap_hip_attention_step_batched over pages: one token of each of the
+ * sequences 0..n_seq-1 at one layer, at position pos[i], whose row must be
+ * reserved.  A sequence whose position is out of range, that has no page for
+ * one of the rows [0, pos[i]], or whose page of row pos[i] is not its own,
+ * writes nothing and gets an output row of NaN.  fp32: products and sums in
+ * fp32.  8 bits: of q and of the weights times the value rows' scales, what
+ * lies below 2^-30 of their largest (of a head row; of 64 positions) is
+ * rounded away, products are exact and sums of 64 positions fp32's; q holds
+ * what is above 2^-119.  Host pointers. */
+int leap_hip_attention_pages_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, const float *q,
+                                  const float *k_new, const float *v_new, float *out);
+/* As leap_hip_attention_step_batched_async, over pages. */
+int leap_hip_attention_pages_step_async(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, int max_pos,
+                                        long long total_rows, const float *q, const float *k_new, const float *v_new,
+                                        float *out, void *stream);
+
+/* The same, attending, for each KV head, to at most `keep` pages: the page of
+ * row pos[i] and the keep - 1 with the largest scores of those before it; of
+ * equal scores the earlier page.  A page's score is the sum over the KV head's
+ * q heads of sum_j max(q_j lo_j, q_j hi_j): the most that q . k can be for
+ * keys between the page's bounds lo and hi, the least and largest of each
+ * element of its keys; q is rotated in fp32 (rounded as keys are), the sum is
+ * in 64 bits.  A score that is not a number comes first.  Bounds are those of
+ * a page's rows as they were when a step last wrote its last row, or
+ * pages_write a row of it: after a sequence is cut back, its rows are written
+ * again in order.  picked [n_seq][n_kv_heads][keep] (or NULL) gets the pages
+ * attended to, as places in the sequence's row of the table, ascending, -1
+ * behind the last.  Needs bounds (pages_create); keep >= 1. */
+int leap_hip_attention_pages_step_sparse(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, int keep,
+                                         const float *q, const float *k_new, const float *v_new, float *out,
+                                         int *picked);
+int leap_hip_attention_pages_step_sparse_async(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos,
+                                               int max_pos, int keep, const float *q, const float *k_new,
+                                               const float *v_new, float *out, int *picked, void *stream);
+
+/* Rows [pos_begin, pos_end) of (seq, layer) between fp32 rows in device memory
+ * ([pos][kv_dim], 16-byte aligned; either may be NULL) and the pages, on
+ * `stream`: k as it is stored, after rotation.  A row whose page is not the
+ * sequence's own is not written, one without a page is read as NaN. */
+int leap_hip_attention_pages_write_async(leap_hip_attention_pages *p, int seq, int layer, int pos_begin, int pos_end,
+                                         const float *k, const float *v, void *stream);
+int leap_hip_attention_pages_read_async(leap_hip_attention_pages *p, int seq, int layer, int pos_begin, int pos_end,
+                                        float *k, float *v, void *stream);
+/* The same with host pointers; write: -EINVAL, with nothing written, if a page
+ * is not the sequence's own. */
+int leap_hip_attention_pages_write(leap_hip_attention_pages *p, int seq, int layer, int pos_begin, int pos_end,
+                                   const float *k, const float *v);
+int leap_hip_attention_pages_read(leap_hip_attention_pages *p, int seq, int layer, int pos_begin, int pos_end, float *k,
+                                  float *v);
+
+/* Empties every table and zeroes the pool (and the arrival counters). */
+int leap_hip_attention_pages_clear(leap_hip_attention_pages *p);
+
+/* The table [max_batch][width] and refs [n_pages] in host memory; either may
+ * be NULL. */
+int leap_hip_attention_pages_state(leap_hip_attention_pages *p, int *table, int *refs);
+
+/* Device addresses, valid until destroy; to be read only, but for the pool's
+ * contents.  k, v, ks, vs and bounds are of the layer, and layers follow one
+ * another: with G KV heads of HD elements, pages of R rows, fp32 k and v
+ * [page][G][R][HD]; 8 bits k [page][G][R][HD], v [page][G][R / 16][HD][16] (16
+ * rows, element by element), scales ks and vs [page][G][R]; bounds
+ * [page][G][2][HD], least and largest. */
+typedef struct leap_hip_attention_pages_arrays {
+    const int *table, *refs;
+    int width;
+    void *k, *v;
+    float *ks, *vs, *bounds; /* NULL where there are none */
+} leap_hip_attention_pages_arrays;
+int leap_hip_attention_pages_view(leap_hip_attention_pages *p, int layer, leap_hip_attention_pages_arrays *out);
+
+/* The selection of a beam search.  For each of n_groups groups of `beams`
+ * beams (row r = group * beams + beam; n_groups * beams <= max_batch), of all
+ * continuations (r, t) of its beams by the tokens t < vocab the `beams` best by
+ * score[r] + logits[r][t] - log sum_u exp(logits[r][u]), best first: parent
+ * (r, as fork takes it), token (t) and best (their new score).  Totals are
+ * compared in 64 bits; of equal ones the lower beam comes first, within a beam
+ * the larger logit, then the lower token.  Logits may be -inf (a token that is
+ * not allowed).  Every continuation counts -inf of a row with a NaN or +inf
+ * among its logits or none above -inf, and of one whose score is not finite
+ * (a search starts with scores 0, -inf, -inf, ...); these have the lowest
+ * tokens.  Rows lie `stride` floats apart.  1 <= beams <= 16, beams <= vocab
+ * <= 262144.  Device pointers, 4-byte aligned, enqueued on `stream`; parent,
+ * token, best [n_groups * beams], best may be score.  A handle's first call
+ * allocates its workspace; -EINVAL if that one is under stream capture. */
+int leap_hip_attention_pages_beam_select_async(leap_hip_attention_pages *p, int n_groups, int beams, int vocab,
+                                               const float *logits, long long stride, const float *score, int *parent,
+                                               int *token, float *best, void *stream);
+/* The same with host pointers (logits [n_groups * beams][vocab]). */
+int leap_hip_attention_pages_beam_select(leap_hip_attention_pages *p, int n_groups, int beams, int vocab,
+                                         const float *logits, const float *score, int *parent, int *token, float *best);
+
 /* ---- The attention sub-block of run_layer on the device ----------------- */
 
 /* Weights of one held layer for leap_hip_attention_block, copied from host

@@ -45,6 +45,14 @@ EXPORTS = (
     "leap_hip_attention_tree", "leap_hip_attention_tree_async", "leap_hip_attention_tree_keep",
     "leap_hip_attention_tree_keep_async", "leap_hip_attention_kv_write_async", "leap_hip_attention_kv_read_async",
     "leap_hip_attention_kv_q8_device_ptr",
+    "leap_hip_attention_pages_create", "leap_hip_attention_pages_destroy", "leap_hip_attention_pages_last_error",
+    "leap_hip_attention_pages_reserve", "leap_hip_attention_pages_reserve_async", "leap_hip_attention_pages_fork",
+    "leap_hip_attention_pages_fork_async", "leap_hip_attention_pages_compact", "leap_hip_attention_pages_compact_async",
+    "leap_hip_attention_pages_step", "leap_hip_attention_pages_step_async", "leap_hip_attention_pages_step_sparse",
+    "leap_hip_attention_pages_step_sparse_async", "leap_hip_attention_pages_write", "leap_hip_attention_pages_write_async",
+    "leap_hip_attention_pages_read", "leap_hip_attention_pages_read_async", "leap_hip_attention_pages_clear",
+    "leap_hip_attention_pages_state", "leap_hip_attention_pages_view", "leap_hip_attention_pages_beam_select",
+    "leap_hip_attention_pages_beam_select_async",
 )
 
 PACKET_HEADER_BYTES = 8
@@ -77,6 +85,15 @@ class Config(ctypes.Structure):
         ("n_kv_heads", _I), ("head_dim", _I), ("seq_len", _I), ("rope_theta", ctypes.c_float),
         ("max_batch", _I), ("device", _I),
     ]
+
+
+class PagesConfig(ctypes.Structure):
+    _fields_ = [("model", Config), ("page_rows", _I), ("n_pages", _I), ("q8", _I), ("bounds", _I)]
+
+
+class PagesArrays(ctypes.Structure):
+    """leap_hip_attention_pages_arrays: device addresses of a layer's pages and of the table."""
+    _fields_ = [("table", _P), ("refs", _P), ("width", _I)] + [(n, _P) for n in ("k", "v", "ks", "vs", "bounds")]
 
 
 _lib = None
@@ -150,9 +167,27 @@ def _open(path: str):
     L.leap_hip_attention_kv_read_async.argtypes = [H, _I, _I, _I, _I, _P, _P, _P]
     L.leap_hip_attention_kv_q8_device_ptr.argtypes = [H, _I, _I] + [ctypes.POINTER(_P)] * 4
     L.leap_hip_attention_timeline.argtypes = [_P, ctypes.c_size_t, ctypes.POINTER(ctypes.c_longlong)]
+    pages = {
+        "create": [ctypes.POINTER(PagesConfig), ctypes.POINTER(H)], "destroy": [H], "last_error": [H], "clear": [H],
+        "reserve": [H, _I, _IP, _IP], "reserve_async": [H, _I, _P, _P, _P, _P],
+        "fork": [H, _I, _IP, _IP], "fork_async": [H, _I, _P, _P, _P],
+        "compact": [H, _IP], "compact_async": [H, _P, _P],
+        "step": [H, _I, _I, _IP, _F, _F, _F, _F],
+        "step_async": [H, _I, _I, _P, _I, ctypes.c_longlong] + [_P] * 5,
+        "step_sparse": [H, _I, _I, _IP, _I, _F, _F, _F, _F, _IP],
+        "step_sparse_async": [H, _I, _I, _P, _I, _I] + [_P] * 6,
+        "write": [H, _I, _I, _I, _I, _F, _F], "write_async": [H, _I, _I, _I, _I, _P, _P, _P],
+        "read": [H, _I, _I, _I, _I, _F, _F], "read_async": [H, _I, _I, _I, _I, _P, _P, _P],
+        "state": [H, _IP, _IP], "view": [H, _I, ctypes.POINTER(PagesArrays)],
+        "beam_select": [H, _I, _I, _I, _F, _F, _IP, _IP, _F],
+        "beam_select_async": [H, _I, _I, _I, _P, ctypes.c_longlong] + [_P] * 5,
+    }
+    for name, types in pages.items():
+        getattr(L, "leap_hip_attention_pages_" + name).argtypes = types
+    L.leap_hip_attention_pages_last_error.restype = ctypes.c_char_p
     for name in EXPORTS:
         fn = getattr(L, name)
-        if name != "leap_hip_attention_last_error":
+        if not name.endswith("_last_error"):
             fn.restype = _I
     return L
 
@@ -485,3 +520,165 @@ class HipAttention:
         self._check(self.lib.leap_hip_attention_kv_device_ptr(self.h, seq, layer,
                                                               ctypes.byref(k), ctypes.byref(v)))
         return k.value, v.value
+
+
+class PagedAttention:
+    """One handle of a cache of pages (see the C header): sequences 0..max_batch-1 whose
+    rows lie in pages of page_rows rows of a pool of n_pages.
+    cache: "f32" or "q8"; bounds: keep what step_sparse chooses pages by."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, seq_len, n_pages, page_rows=16, n_layers=1, layer_begin=0,
+                 layer_end=None, rope_theta=500000.0, max_batch=1, device=0, cache="f32", bounds=False):
+        if cache not in ("f32", "q8"):
+            raise ValueError(f"cache {cache!r} is not 'f32' or 'q8'")
+        self.lib = load_library()
+        model = Config(n_layers, layer_begin, n_layers if layer_end is None else layer_end, n_heads, n_kv_heads, head_dim,
+                       seq_len, rope_theta, max_batch, device)
+        self.cfg = PagesConfig(model, page_rows, n_pages, cache == "q8", bool(bounds))
+        self.n_kv_heads, self.max_batch, self.n_pages, self.seq_len = n_kv_heads, max_batch, n_pages, seq_len
+        self.q_dim, self.kv_dim = n_heads * head_dim, n_kv_heads * head_dim
+        self.width = -(-seq_len // page_rows) if page_rows > 0 else 0
+        h = _P()
+        rc = self.lib.leap_hip_attention_pages_create(ctypes.byref(self.cfg), ctypes.byref(h))
+        if rc != 0:
+            raise LeapError(rc, self.lib.leap_hip_attention_pages_last_error(None).decode())
+        self.h = h
+
+    def close(self):
+        if getattr(self, "h", None):
+            self.lib.leap_hip_attention_pages_destroy(self.h)
+            self.h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _call(self, name, *args):
+        rc = getattr(self.lib, "leap_hip_attention_pages_" + name)(self.h, *args)
+        if rc != 0:
+            raise LeapError(rc, self.lib.leap_hip_attention_pages_last_error(self.h).decode())
+
+    @staticmethod
+    def _pair(a, b, what):
+        a, b = _i32(a), _i32(b)
+        if a.size != b.size:
+            raise ValueError(f"{what}: {a.size} and {b.size} values")
+        return a, b
+
+    # -- pages ----------------------------------------------------------------
+    def reserve(self, begin, end):
+        """Pages of its own for rows [begin[i], end[i]) of each sequence."""
+        begin, end = self._pair(begin, end, "begin and end")
+        self._call("reserve", begin.size, _ip(begin), _ip(end))
+
+    def reserve_async(self, n_seq, begin_ptr, end_ptr, status_ptr=0, stream=0):
+        self._call("reserve_async", n_seq, begin_ptr, end_ptr, status_ptr, stream)
+
+    def fork(self, parent, rows):
+        """Sequence i takes the pages of the first rows[i] rows of parent[i] (None: each its own)."""
+        if parent is None:
+            rows = _i32(rows)
+            self._call("fork", rows.size, None, _ip(rows))
+        else:
+            parent, rows = self._pair(parent, rows, "parent and rows")
+            self._call("fork", rows.size, _ip(parent), _ip(rows))
+
+    def fork_async(self, n_seq, parent_ptr, rows_ptr, stream=0):
+        self._call("fork_async", n_seq, parent_ptr, rows_ptr, stream)
+
+    def compact(self):
+        """The pages in use moved to the pool's front; how many they are."""
+        used = _I()
+        self._call("compact", ctypes.byref(used))
+        return used.value
+
+    def compact_async(self, used_ptr=0, stream=0):
+        self._call("compact_async", used_ptr, stream)
+
+    def state(self):
+        """The table [max_batch][width] and the pages' numbers of references."""
+        table, refs = np.empty((self.max_batch, self.width), np.int32), np.empty(self.n_pages, np.int32)
+        self._call("state", _ip(table), _ip(refs))
+        return table, refs
+
+    def view(self, layer) -> dict:
+        """Device addresses of the table, the references and a layer's pages (None where there are none)."""
+        a = PagesArrays()
+        self._call("view", layer, ctypes.byref(a))
+        return {n: getattr(a, n) for n, _ in PagesArrays._fields_}
+
+    def clear(self):
+        self._call("clear")
+
+    # -- the step ---------------------------------------------------------------
+    def _step_in(self, pos, q, k_new, v_new):
+        pos = _i32(pos)
+        n = pos.size
+        return pos, n, _f32(q, n * self.q_dim), _f32(k_new, n * self.kv_dim), _f32(v_new, n * self.kv_dim)
+
+    def step(self, layer, pos, q, k_new, v_new):
+        pos, n, q, k, v = self._step_in(pos, q, k_new, v_new)
+        out = np.empty((n, self.q_dim), np.float32)
+        self._call("step", layer, n, _ip(pos), _fp(q), _fp(k), _fp(v), _fp(out))
+        return out
+
+    def step_async(self, layer, n_seq, pos_ptr, max_pos, q_ptr, k_ptr, v_ptr, out_ptr, stream=0, total_rows=0):
+        """total_rows: sum of pos[i] + 1 if known on the host (sizes the split), else 0."""
+        self._call("step_async", layer, n_seq, pos_ptr, max_pos, total_rows, q_ptr, k_ptr, v_ptr, out_ptr, stream)
+
+    def step_sparse(self, layer, pos, keep, q, k_new, v_new):
+        """The step over at most `keep` pages a KV head; also returns which, [n_seq][n_kv_heads][keep]."""
+        pos, n, q, k, v = self._step_in(pos, q, k_new, v_new)
+        out = np.empty((n, self.q_dim), np.float32)
+        picked = np.empty((n, self.n_kv_heads, max(keep, 1)), np.int32)
+        self._call("step_sparse", layer, n, _ip(pos), keep, _fp(q), _fp(k), _fp(v), _fp(out), _ip(picked))
+        return out, picked
+
+    def step_sparse_async(self, layer, n_seq, pos_ptr, max_pos, keep, q_ptr, k_ptr, v_ptr, out_ptr, picked_ptr=0, stream=0):
+        self._call("step_sparse_async", layer, n_seq, pos_ptr, max_pos, keep, q_ptr, k_ptr, v_ptr, out_ptr, picked_ptr, stream)
+
+    # -- rows -------------------------------------------------------------------
+    def write(self, seq, layer, pos_begin, k=None, v=None):
+        k, v = (None if x is None else _f32(x) for x in (k, v))
+        rows = {x.size // self.kv_dim for x in (k, v) if x is not None}
+        if len(rows) > 1:
+            raise ValueError("k and v have different rows")
+        if rows:
+            self._call("write", seq, layer, pos_begin, pos_begin + rows.pop(), _fp(k), _fp(v))
+
+    def write_async(self, seq, layer, pos_begin, pos_end, k_ptr, v_ptr, stream=0):
+        self._call("write_async", seq, layer, pos_begin, pos_end, k_ptr, v_ptr, stream)
+
+    def read(self, seq, layer, pos_begin, pos_end):
+        k = np.empty((max(0, pos_end - pos_begin), self.kv_dim), np.float32)
+        v = np.empty_like(k)
+        self._call("read", seq, layer, pos_begin, pos_end, _fp(k), _fp(v))
+        return k, v
+
+    def read_async(self, seq, layer, pos_begin, pos_end, k_ptr, v_ptr, stream=0):
+        self._call("read_async", seq, layer, pos_begin, pos_end, k_ptr, v_ptr, stream)
+
+    # -- beams ------------------------------------------------------------------
+    def beam_select(self, n_groups, beams, logits, score):
+        """The best continuations of each group of beams: parent, token and score."""
+        n = n_groups * beams
+        logits = _f32(logits)
+        vocab = logits.size // max(1, n)
+        if logits.size != n * vocab:
+            raise ValueError(f"{logits.size} logits of {n} beams")
+        score = _f32(score, n)
+        parent, token, best = np.empty(n, np.int32), np.empty(n, np.int32), np.empty(n, np.float32)
+        self._call("beam_select", n_groups, beams, vocab, _fp(logits), _fp(score), _ip(parent), _ip(token), _fp(best))
+        return parent, token, best
+
+    def beam_select_async(self, n_groups, beams, vocab, logits_ptr, stride, score_ptr, parent_ptr, token_ptr, best_ptr, stream=0):
+        self._call("beam_select_async", n_groups, beams, vocab, logits_ptr, stride, score_ptr, parent_ptr, token_ptr, best_ptr,
+                   stream)

@@ -7,7 +7,8 @@
 //   - kernels_gemv.hip: the fp32 projection GEMVs by model width;
 //   - kernels_q8.hip: the int8 W8A8 projection GEMVs by width, group size,
 //     rows per workgroup and input kind;
-//   - kernels_many_{64,128}.hip: prompts, trees and the 8-bit cache by head_dim.
+//   - kernels_many_{64,128}.hip: prompts, trees and the 8-bit cache by head_dim;
+//   - kernels_paged_{64,128}.hip: caches of pages by head_dim.
 // leap_hip_attention.hip holds the host side and picks kernels through these
 // functions only.
 #pragma once
@@ -16,6 +17,9 @@
 #include "gemv.hpp"
 #include "gemv_q8.hpp"
 #include "many_attention.hpp"
+#include "page_rows.hpp"
+#include "page_select.hpp"
+#include "paged_attention.hpp"
 
 namespace leap_kernels {
 
@@ -140,5 +144,21 @@ inline RowsKernels pick_rows(int hd) { return hd == 64 ? pick_rows_hd<64>() : pi
 // The accepted paths' rows moved together, in an fp32 or 8-bit cache.
 using KeepFn = void (*)(leap::KeepArgs);
 KeepFn pick_keep(bool q8);
+
+// Caches of pages: the step over them by workgroups of 4 and 8 waves, the sum
+// of a spread launch's records, rows in and out, and the choice of pages.
+using PagedFn = void (*)(leap::PagedArgs);
+using PageRowsFn = void (*)(leap::PageRowsArgs);
+using SelectFn = void (*)(leap::SelectArgs);
+struct PagedKernels {
+    PagedFn attention[2], merge;
+    PageRowsFn write, read, bounds;
+    SelectFn select;
+};
+template <int HD>
+PagedKernels pick_paged_hd(bool q8);
+extern template PagedKernels pick_paged_hd<64>(bool);
+extern template PagedKernels pick_paged_hd<128>(bool);
+inline PagedKernels pick_paged(int hd, bool q8) { return hd == 64 ? pick_paged_hd<64>(q8) : pick_paged_hd<128>(q8); }
 
 }  // namespace leap_kernels

@@ -1,0 +1,6 @@
+// Caches of pages at head_dim 128 (see kernels.hpp).
+#include "kernels_paged_table.hpp"
+
+namespace leap_kernels {
+template PagedKernels pick_paged_hd<128>(bool);
+}  // namespace leap_kernels

@@ -27,6 +27,7 @@
 
 #include "aux_kernels.hpp"
 #include "checkpoint.hpp"
+#include "host_util.hpp"
 #include "kernels.hpp"
 
 extern "C" void leap_rope_table_host(int seq_len, int head_size, float theta, float *cos_tab,
@@ -130,19 +131,7 @@ int set_err(leap_hip_attention *h, int code, const char *fmt, ...)
         }                                                                                      \
     } while (0)
 
-template <typename T>
-struct same_type {
-    using type = T;
-};
-
-// Enqueue fn<<<grid, block, 0, stream>>>(args...) and return that launch's
-// own status (not the thread's sticky last error, which may be older).
-template <typename... P>
-hipError_t launch_k(void (*fn)(P...), dim3 grid, dim3 block, hipStream_t stream, typename same_type<P>::type... args)
-{
-    void *kargs[] = {static_cast<void *>(&args)...};
-    return hipLaunchKernel(reinterpret_cast<const void *>(fn), grid, block, kargs, 0, stream);
-}
+using leap_host::launch_k;
 
 // How launches see a head shape: 16 q heads per KV head run as two groups
 // of 8 per cache head (the decode kernel's kv_split), so that no kernel
@@ -1229,6 +1218,13 @@ int check_placement(leap_hip_attention *h, int device, int n_wg)
 }
 
 }  // namespace
+
+int leap_host::check_placement(int device, int n_wg, std::string *why)
+{
+    const int rc = ::check_placement(nullptr, device, n_wg);
+    if (rc) *why = g_create_error;
+    return rc;
+}
 
 extern "C" {
 

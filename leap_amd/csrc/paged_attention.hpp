@@ -1,0 +1,796 @@
+// Attention of one new token of each sequence over a cache kept in pages, of
+// fp32 or of 8-bit values.
+//
+// A page holds R rows (16, 32, 64 or 128) of every KV head of one layer; a
+// sequence's pages are named by its row of a table.  Per layer the arrays are
+//   fp32    k, v    [page][kv_head][R][HD]
+//   8 bits  k8      [page][kv_head][R][HD]
+//           v8      [page][kv_head][R / 16][HD][16]  (16 rows, dim by dim)
+//           ks, vs  [page][kv_head][R]
+// so that a KV head's rows of a page lie together, and the operands of both
+// products are read from memory as the matrix instructions take them.
+//
+// A workgroup takes one (sequence, KV head) and one run of tiles of positions;
+// its waves take tiles in turn, each with an online softmax of its own, and
+// their results are combined in LDS.  The runs of one group leave records
+// (output, log2 of the sum) that the last one to arrive adds up, or, where a
+// group's runs are spread over the XCDs, a second launch.  A launch attends
+// either to all pages of a sequence or to a list of them for each KV head
+// (ascending, the new row's page last): the rows are then numbered along the
+// list, and only the last page may be partly filled, as without a list.
+//
+// Products, m = lane % 16, g = lane / 16.  S^T = K Q^T: a lane holds K's row m
+// of a block of 16 and q head m, and gets the scores of positions 4 g + i for
+// head m.  O^T = V^T P^T takes those registers as its B operand as they are:
+// slot (g, i) of its contraction is position 4 g + i.  No score leaves its
+// lane, and a row's maximum and sum need two lane swaps.
+//   fp32: v_mfma_f32_16x16x4_f32, the dims of a load instruction's 64 (K) and
+//     256 (V) bytes of a row in the order in which the lanes get them.
+//   8 bits: v_mfma_i32_16x16x64_i8 on the cache's bytes as they are.  The
+//     other operand, q or the probabilities times the value rows' scales, is
+//     a 30-bit fixed-point number over a power of two just above the largest
+//     of its head row (q) or of its tile (probabilities), as four signed
+//     digits of 8 bits; the four integer sums are exact and are put together
+//     in fp32.  What is lost is 2^-30 of that largest element.
+#pragma once
+
+#include "many_attention.hpp"
+
+namespace leap {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kPagedSplits = 64;     // runs of a group, at most: a lane each in the merge
+constexpr int kPagedHeads = 16;      // q heads of a KV head, at most
+// Probabilities are 2^(score - reference - kPagedBias), and the reference
+// moves when a score exceeds it by more than kPagedMargin: sums of up to 2^16
+// probabilities stay below 1, and weighted values below the largest value.
+constexpr float kPagedMargin = 4.0f, kPagedBias = 20.0f;
+
+// One launch over one layer.
+struct PagedArgs {
+    const float *q, *k_new, *v_new;  // rows of [n_heads*HD], [n_kv_heads*HD]
+    float *out;
+    void *k, *v;                     // the layer's pages
+    float *ks, *vs;                  // 8 bits: their scales
+    float *bounds;                   // the layer's [page][kv_head][2][HD], or NULL
+    const float4 *rope;
+    const int *pos;
+    const int *table;                // [sequence][width]
+    const int *refs;                 // [page]
+    const int *lists;                // [group][keep] pages (keep 0: none, all pages of the table)
+    float *ws_o, *ws_lse;            // records: [group][split][q head][HD], [group][split][q head]
+    int *counters;                   // [group], zero between launches
+    int width, keep, n_pages;
+    int n_seq, max_pos, n_heads, n_kv_heads, group;
+    int rows_log2;                   // R = 1 << rows_log2
+    int chunk, splits;               // tiles of a run at least, runs of a group at most
+    int spread;                      // a group's runs lie on all XCDs, and paged_merge_kernel adds up their records
+    float scale_log2;
+    FastDiv by_kv_heads, by_splits;
+};
+
+// What a group (sequence, KV head) attends to.
+struct PagedPlace {
+    int seq, kvh, pos;   // seq < 0: nothing (a skipped position)
+    const int *list;     // page numbers
+    int n_list, rows;    // pages, and rows along the list with the new one
+};
+__device__ __forceinline__ PagedPlace paged_place(const PagedArgs &a, int gi)
+{
+    PagedPlace p;
+    p.seq = (int)fast_div((uint32_t)gi, a.by_kv_heads);
+    p.kvh = gi - p.seq * a.n_kv_heads;
+    p.pos = a.pos[p.seq];
+    const int at = p.pos >> a.rows_log2;
+    p.n_list = a.keep ? min(a.keep, at + 1) : at + 1;
+    p.list = a.keep ? a.lists + (size_t)gi * a.keep : a.table + (size_t)p.seq * a.width;
+    p.rows = ((p.n_list - 1) << a.rows_log2) + (p.pos & ((1 << a.rows_log2) - 1)) + 1;
+    if (p.pos < 0 || p.pos > a.max_pos) p.seq = -1 - p.seq;
+    return p;
+}
+// Its runs: of `chunk` tiles each, the tiles dealt evenly.
+struct PagedRuns {
+    int n, per, more;  // runs, tiles of each, and how many have one more
+};
+__device__ __forceinline__ PagedRuns paged_runs(const PagedArgs &a, int tiles)
+{
+    PagedRuns r;
+    r.n = min(a.splits, (tiles + a.chunk - 1) / a.chunk);
+    r.per = tiles / r.n;
+    r.more = tiles - r.per * r.n;
+    return r;
+}
+
+template <int HD, int W>
+struct PagedShared {
+    union {
+        float o[W][kPagedHeads][HD + 4];  // the waves' outputs
+        struct {
+            float w[kPagedHeads][kPagedSplits + 1];  // the merge: weights of a head's records
+            float4 part[W * kWave];                  // and partial sums of them
+        } merge;
+    };
+    float m[W][kPagedHeads], l[W][kPagedHeads];
+    alignas(16) int fresh[2][HD / 4];     // 8 bits: the new token's K and V rows
+    float fresh_scale[2];
+    int last;
+};
+
+__device__ __forceinline__ float lanes_max(float x)
+{
+    x = fmaxf(x, dpp<0x121>(x));
+    x = fmaxf(x, dpp<0x122>(x));
+    x = fmaxf(x, dpp<0x124>(x));
+    x = fmaxf(x, dpp<0x128>(x));
+    return rows4<true>(x);
+}
+__device__ __forceinline__ float lanes_sum(float x)
+{
+    x += dpp<0x121>(x);
+    x += dpp<0x122>(x);
+    x += dpp<0x124>(x);
+    x += dpp<0x128>(x);
+    return rows4<false>(x);
+}
+
+// The sum of a group's records by T threads: record s of head h counts
+// 2^(lse_s - max lse) / their sum.
+template <int HD, int T, typename Merge>
+__device__ __forceinline__ void paged_merge(const PagedArgs &a, Merge &sh, int gi, int n_split, const PagedPlace &p, int tid)
+{
+    constexpr int LR = HD / 4;
+    const int lane = tid & (kWave - 1), items = a.group * LR;
+    const size_t rec0 = (size_t)gi * a.splits * a.group;
+    int parts = 1;
+    while (2 * parts * items <= T) parts *= 2;
+    const int part = parts > 1 ? tid / items : 0;
+    const auto wr = make_rsrc(a.ws_o + rec0 * HD, (uint32_t)(n_split * items) * 16u);
+    float4 x[8];
+    auto load = [&](int i, int s) {  // (past the last record: 0)
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = buf_load4<kSc1>(wr, (uint32_t)((s + k * parts) * items + i) * 16u);
+    };
+    load(tid - part * items, part);  // on their way while the weights are formed
+    const auto lr = make_rsrc(a.ws_lse + rec0, (uint32_t)(n_split * a.group) * 4u);
+    for (int head = tid / kWave; head < a.group; head += T / kWave) {
+        float y = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (lane * a.group + head) * 4, 0, kSc1));
+        if (lane >= n_split) y = -__builtin_inff();
+        y = fast_exp2(y - lanes_max(y));
+        sh.w[head][lane] = y * (1.0f / lanes_sum(y));
+    }
+    __syncthreads();
+    float4 *out = reinterpret_cast<float4 *>(a.out) + ((size_t)p.seq * a.n_heads + p.kvh * a.group) * LR;
+    for (int i0 = 0; i0 < items; i0 += T) {
+        const int i = i0 + tid - part * items, head = i / LR;
+        const bool mine = i < items && part < parts;
+        float4 acc = make_float4(0, 0, 0, 0);
+        for (int s = part; s < n_split; s += 8 * parts) {
+            if (i0 > 0 || s != part) load(i, s);
+            if (mine)
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (s + k * parts < n_split) fma4(acc, sh.w[head][s + k * parts], x[k]);
+        }
+        if (parts > 1) {
+            sh.part[tid] = acc;
+            __syncthreads();
+            if (part == 0 && mine)
+                for (int t = 1; t < parts; t++) fma4(acc, 1.0f, sh.part[t * items + i]);
+        }
+        if (part == 0 && mine) out[i] = acc;
+    }
+}
+
+// ---- fixed-point digits ---------------------------------------------------------
+
+// x of magnitude under 2^30 (already scaled) as four signed digits of 8 bits,
+// least first, in the bytes of a word.
+__device__ __forceinline__ unsigned digits_of(float x)
+{
+    return ((unsigned)(int)rintf(x) + 0x80808080u) ^ 0x80808080u;
+}
+// Digit j of four words, in order: d[j] holds the bytes j of w0..w3.
+__device__ __forceinline__ void digits4(unsigned w0, unsigned w1, unsigned w2, unsigned w3, unsigned d[4])
+{
+    const unsigned a = __builtin_amdgcn_perm(w1, w0, 0x05010400u), b = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
+    const unsigned c = __builtin_amdgcn_perm(w1, w0, 0x07030602u), e = __builtin_amdgcn_perm(w3, w2, 0x07030602u);
+    d[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    d[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    d[2] = __builtin_amdgcn_perm(e, c, 0x05040100u);
+    d[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
+}
+// The exponent of a largest magnitude `bits`, at least -90: what is scaled by
+// 2^(29 - e) is below 2^30.
+__device__ __forceinline__ int fixed_exp(unsigned bits) { return max((int)(bits >> 23), 37) - 127; }
+// The four digits' sums together.
+__device__ __forceinline__ float digits_sum(int d0, int d1, int d2, int d3)
+{
+    return __builtin_fmaf((float)((int)((unsigned)d3 << 8) + d2), 65536.0f, (float)((int)((unsigned)d1 << 8) + d0));
+}
+__device__ __forceinline__ i32x4 mfma8(u32x4 a, u32x4 b, i32x4 c)
+{
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma32(float a, float b, f32x4 c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// The smaller / larger; NaN if either is.
+__device__ __forceinline__ float4 min4(float4 a, float4 b)
+{
+    return make_float4(__builtin_elementwise_minimum(a.x, b.x), __builtin_elementwise_minimum(a.y, b.y),
+                       __builtin_elementwise_minimum(a.z, b.z), __builtin_elementwise_minimum(a.w, b.w));
+}
+__device__ __forceinline__ float4 max4(float4 a, float4 b)
+{
+    return make_float4(__builtin_elementwise_maximum(a.x, b.x), __builtin_elementwise_maximum(a.y, b.y),
+                       __builtin_elementwise_maximum(a.z, b.z), __builtin_elementwise_maximum(a.w, b.w));
+}
+__device__ __forceinline__ float4 shfl_xor4(float4 x, int by)
+{
+    return make_float4(__shfl_xor(x.x, by), __shfl_xor(x.y, by), __shfl_xor(x.z, by), __shfl_xor(x.w, by));
+}
+// Four int8 values of a word times a scale.
+__device__ __forceinline__ float4 bytes4(int q, float s)
+{
+    return make_float4((float)(int8_t)q * s, (float)(int8_t)(q >> 8) * s, (float)(int8_t)(q >> 16) * s, (float)(q >> 24) * s);
+}
+
+// The least and the largest of each element over a page's keys of one KV head,
+// by one wave, LR lanes a row: rows [0, n) from memory, and x (the lane's
+// float4 of the row behind them) where more is set.
+template <int HD, bool Q8>
+__device__ __forceinline__ void page_bounds(const void *k, const float *ks, float *to, int n, float4 x, bool more, int lane)
+{
+    constexpr int LR = HD / 4, PER = kWave / LR;
+    const int c = lane & (LR - 1);
+    const float inf = __builtin_inff();
+    float4 lo = make_float4(inf, inf, inf, inf), hi = make_float4(-inf, -inf, -inf, -inf);
+    if (more) lo = hi = x;
+#pragma unroll 4
+    for (int r = lane / LR; r < n; r += PER) {
+        float4 y;
+        if constexpr (Q8)
+            y = bytes4(reinterpret_cast<const int *>(k)[r * LR + c], ks[r]);
+        else
+            y = reinterpret_cast<const float4 *>(k)[r * LR + c];
+        lo = min4(lo, y);
+        hi = max4(hi, y);
+    }
+    for (int by = LR; by < kWave; by *= 2) {
+        lo = min4(lo, shfl_xor4(lo, by));
+        hi = max4(hi, shfl_xor4(hi, by));
+    }
+    if (lane < LR) {
+        reinterpret_cast<float4 *>(to)[c] = lo;
+        reinterpret_cast<float4 *>(to)[LR + c] = hi;
+    }
+}
+
+// Positions of a wave's tile, 16 KiB of fp32 rows and 16 (8 at head_dim 64) of
+// 8-bit ones.
+__host__ __device__ constexpr int paged_tile(int hd, bool q8) { return q8 ? 64 : 2048 / hd; }
+
+// W waves.
+template <int HD, int W, bool Q8>
+__global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_kernel(PagedArgs a)
+{
+    constexpr int TK = paged_tile(HD, Q8), NB = TK / 16, LR = HD / 4, VB = HD / 16, kThreads = W * kWave;
+    __shared__ PagedShared<HD, W> sh;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int m = lane & 15, g = lane >> 4;
+
+    // the group and its run: a group's runs on one XCD, or (spread) on all
+    const int n_groups = a.n_seq * a.n_kv_heads;
+    int gi, split;
+    if (a.spread) {
+        split = blockIdx.x / n_groups;
+        gi = blockIdx.x - split * n_groups;
+    } else {
+        const int local = blockIdx.x / kXcds, gl = (int)fast_div((uint32_t)local, a.by_splits);
+        split = local - gl * a.splits;
+        gi = gl * kXcds + (blockIdx.x & (kXcds - 1));
+    }
+    if (gi >= n_groups) return;
+    PagedPlace p = paged_place(a, gi);
+    if (p.seq < 0) {
+        if (split == 0)
+            fill_nan<HD>(a.out, ((size_t)(-1 - p.seq) * a.n_heads + p.kvh * a.group) * LR, a.group * LR, tid, kThreads);
+        return;
+    }
+    const int tiles = (p.rows + TK - 1) / TK;
+    const PagedRuns runs = paged_runs(a, tiles);
+    if (split >= runs.n) return;
+    const int t0 = split * runs.per + min(split, runs.more), t1 = t0 + runs.per + (split < runs.more);
+
+    const int blocks_log2 = a.rows_log2 - 4;  // blocks of 16 rows of a page
+    auto row0_of = [&](int page, int block) {  // a block's first row among the KV heads' rows of the layer
+        return (((size_t)page * a.n_kv_heads + p.kvh) << a.rows_log2) + ((block & ((1 << blocks_log2) - 1)) << 4);
+    };
+    const int n_blocks = (p.rows + 15) >> 4;
+    bool bad = false;  // a page is missing, or the new row's is shared
+
+    // ---- this wave's rows of q, and the new token's if it has the last tile ----
+    int t = t0 + wave;
+    const bool has_new = t1 == tiles && (tiles - 1 - t0) % W == wave;  // (t0 + wave <= tiles - 1 then)
+    const int new_row = (p.rows - 1) & (TK - 1);                       // its row of the last tile
+    const int own = has_new ? p.list[p.n_list - 1] : 0;
+    const bool keeps = has_new && (unsigned)own < (unsigned)a.n_pages && a.refs[own] == 1;  // its page is its own
+    if (has_new && !keeps) bad = true;
+    const float *q_at = a.q + ((size_t)p.seq * a.n_heads + p.kvh * a.group + m) * HD;
+    const size_t new_at = ((size_t)p.seq * a.n_kv_heads + p.kvh) * HD;
+    const float4 *turn_at = a.rope + (size_t)p.pos * LR;
+
+    f32x4 o[VB];
+#pragma unroll
+    for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
+    float mrun = kNothing, lrun = 0.0f;
+
+    if constexpr (!Q8) {
+        constexpr int KF = HD / 16, VF = HD / 64;
+        const float *kp = static_cast<const float *>(a.k), *vp = static_cast<const float *>(a.v);
+        float4 kraw[NB][KF], vraw[NB][4][VF];
+        // a tile's pages, uniform over the wave: loaded a tile ahead
+        int pages[NB];
+        auto look = [&](int at) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const int block = min(at * NB + b, n_blocks - 1);
+                pages[b] = p.list[block >> blocks_log2];
+            }
+        };
+        // (rows from the new one on read as zero)
+        auto rows_at = [&](const float *base, int at, int b) {
+            const int block = at * NB + b, page = pages[b];
+            const bool ok = (unsigned)page < (unsigned)a.n_pages;
+            if (block < n_blocks && !ok) bad = true;
+            const int n = ok ? max(0, min(16, p.rows - 1 - 16 * block)) : 0;
+            return make_rsrc(base + row0_of(ok ? page : 0, block) * HD, (uint32_t)(n * HD * 4));
+        };
+        auto load_k = [&](int at) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const auto r = rows_at(kp, at, b);
+#pragma unroll
+                for (int f = 0; f < KF; f++) kraw[b][f] = buf_load4<kNt>(r, (uint32_t)(m * HD + 16 * f + 4 * g) * 4u);
+            }
+        };
+        auto load_v = [&](int at) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const auto r = rows_at(vp, at, b);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int f = 0; f < VF; f++)
+                        vraw[b][i][f] = buf_load4<kNt>(r, (uint32_t)((4 * g + i) * HD + 64 * f + 4 * m) * 4u);
+            }
+        };
+        float4 q[KF];
+        {
+            float4 turn[KF];
+#pragma unroll
+            for (int f = 0; f < KF; f++) {
+                q[f] = m < a.group ? *reinterpret_cast<const float4 *>(q_at + 16 * f + 4 * g) : make_float4(0, 0, 0, 0);
+                turn[f] = turn_at[4 * f + g];
+            }
+            if (t < t1) {
+                look(t);
+                load_k(t);
+                load_v(t);
+                look(t + W);
+            }
+#pragma unroll
+            for (int f = 0; f < KF; f++) q[f] = rope4(q[f], turn[f]);
+        }
+        for (; t < t1; t += W) {
+            const bool newest = has_new && t == tiles - 1;
+            if (newest) {
+                // the new key in place of what was read, and into the cache
+                const int b_new = new_row >> 4, r_new = new_row & 15;
+                float *to = static_cast<float *>(a.k) + (row0_of(own, t * NB + b_new) + r_new) * HD;
+#pragma unroll
+                for (int f = 0; f < KF; f++) {
+                    const float4 x = rope4(*reinterpret_cast<const float4 *>(a.k_new + new_at + 16 * f + 4 * g), turn_at[4 * f + g]);
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+                        if (b == b_new && m == r_new) kraw[b][f] = x;
+                    if (keeps && m == 0) *reinterpret_cast<float4 *>(to + 16 * f + 4 * g) = x;
+                }
+            }
+            // ---- scores ----
+            f32x4 s[NB], s2[NB];
+#pragma unroll
+            for (int b = 0; b < NB; b++) s[b] = s2[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int f = 0; f < KF; f++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    s[b] = mfma32(kraw[b][f].x, q[f].x, s[b]);
+                    s2[b] = mfma32(kraw[b][f].y, q[f].y, s2[b]);
+                    s[b] = mfma32(kraw[b][f].z, q[f].z, s[b]);
+                    s2[b] = mfma32(kraw[b][f].w, q[f].w, s2[b]);
+                }
+            const bool next = t + W < t1;
+            if (next) load_k(t + W);
+            // ---- softmax ----
+            float x[NB][4], mt = -__builtin_inff();
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[b][i] = (s[b][i] + s2[b][i]) * a.scale_log2;
+            if (t == tiles - 1)
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (16 * b + 4 * g + i > new_row) x[b][i] = -__builtin_inff();
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
+            if (__builtin_amdgcn_ballot_w64(mt > mrun + kPagedMargin) != 0) {
+                mt = rows4<true>(mt);
+                const float now = mt > mrun + kPagedMargin ? mt : mrun, f = fast_exp2(mrun - now);
+                mrun = now;
+                lrun *= f;
+#pragma unroll
+                for (int v = 0; v < VB; v++) o[v] *= f;
+            }
+            const float off = mrun + kPagedBias;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[b][i] = fast_exp2(x[b][i] - off);
+                    lrun += x[b][i];
+                }
+            if (newest) {
+                const int b_new = new_row >> 4, r_new = new_row & 15;
+                float *to = static_cast<float *>(a.v) + (row0_of(own, t * NB + b_new) + r_new) * HD;
+#pragma unroll
+                for (int f = 0; f < VF; f++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(a.v_new + new_at + 64 * f + 4 * m);
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (b == b_new && 4 * g + i == r_new) vraw[b][i][f] = y;
+                    if (keeps && g == 0) *reinterpret_cast<float4 *>(to + 64 * f + 4 * m) = y;
+                }
+            }
+            // ---- weighted values ----
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int f = 0; f < VF; f++) {
+                        o[4 * f] = mfma32(vraw[b][i][f].x, x[b][i], o[4 * f]);
+                        o[4 * f + 1] = mfma32(vraw[b][i][f].y, x[b][i], o[4 * f + 1]);
+                        o[4 * f + 2] = mfma32(vraw[b][i][f].z, x[b][i], o[4 * f + 2]);
+                        o[4 * f + 3] = mfma32(vraw[b][i][f].w, x[b][i], o[4 * f + 3]);
+                    }
+            if (next) {
+                load_v(t + W);
+                look(t + 2 * W);
+            }
+        }
+        if (has_new && keeps && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
+            // the page is complete: the bounds of its keys
+            const size_t head = (size_t)own * a.n_kv_heads + p.kvh;
+            const int c = lane & (LR - 1);
+            const float4 x = rope4(reinterpret_cast<const float4 *>(a.k_new + new_at)[c], turn_at[c]);
+            page_bounds<HD, false>(kp + (head << a.rows_log2) * HD, nullptr, a.bounds + head * 2 * HD, (1 << a.rows_log2) - 1, x,
+                                   true, lane);
+        }
+    } else {
+        constexpr int KS = HD / 64;
+        const int8_t *kp = static_cast<const int8_t *>(a.k), *vp = static_cast<const int8_t *>(a.v);
+        u32x4 kraw[NB][KS], vraw[VB];
+        float4 ksc[NB], vsc[NB];
+        // A tile is 4 blocks of 16 rows.  K's row m of product block b is row
+        // 4 b + m % 4 of block m / 4, so that the scores of a lane, 4 for
+        // each b, are the 16 rows of block g in order: the 16 bytes of V that
+        // it loads.
+        int page_k = 0, page_v = 0;  // the pages of blocks m / 4 and g, a tile ahead
+        auto look = [&](int at) {
+            page_k = p.list[min(4 * at + (m >> 2), n_blocks - 1) >> blocks_log2];
+            page_v = p.list[min(4 * at + g, n_blocks - 1) >> blocks_log2];
+        };
+        const int8_t *k_at, *v_at;
+        const float *ks_at, *vs_at;
+        auto point = [&](int at) {
+            // (blocks behind the last: its rows once more; their scores are masked)
+            const int bk = min(4 * at + (m >> 2), n_blocks - 1), bv = min(4 * at + g, n_blocks - 1);
+            bad |= (unsigned)page_v >= (unsigned)a.n_pages;
+            const size_t rk = row0_of((unsigned)page_k < (unsigned)a.n_pages ? page_k : 0, bk);
+            const size_t rv = row0_of((unsigned)page_v < (unsigned)a.n_pages ? page_v : 0, bv);
+            k_at = kp + (rk + (m & 3)) * HD + 16 * g;
+            v_at = vp + rv * HD + 16 * m;
+            ks_at = a.ks + rv;
+            vs_at = a.vs + rv;
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+                    kraw[b][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(k_at + 4 * b * HD + 64 * s));
+                ksc[b] = *reinterpret_cast<const float4 *>(ks_at + 4 * b);
+            }
+        };
+        auto load_v = [&]() {
+#pragma unroll
+            for (int v = 0; v < VB; v++) vraw[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(v_at + 256 * v));
+#pragma unroll
+            for (int b = 0; b < NB; b++) vsc[b] = *reinterpret_cast<const float4 *>(vs_at + 4 * b);
+        };
+        // q's digits, and the unit of its head row over the score's scale
+        u32x4 qd[KS][4];
+        float qf;
+        {
+            float4 x[KS][4], turn[KS][4];
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    x[s][c] = m < a.group ? *reinterpret_cast<const float4 *>(q_at + 64 * s + 16 * g + 4 * c) : make_float4(0, 0, 0, 0);
+                    turn[s][c] = turn_at[16 * s + 4 * g + c];
+                }
+            if (t < t1) {
+                look(t);
+                point(t);
+                load_k();
+            }
+            unsigned top = 0;
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    x[s][c] = rope4(x[s][c], turn[s][c]);
+                    top = max4_bits(top, x[s][c]);
+                }
+            top = rows4_bits(top);
+            const bool good = finite_bits(top);
+            const int e = fixed_exp(good ? top : 0u);
+            const float up = good ? exp2_int(29 - e) : 0.0f;
+            qf = good ? exp2_int(e - 29) * a.scale_log2 : __uint_as_float(0x7fc00000u);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    unsigned d[4];
+                    digits4(digits_of(x[s][c].x * up), digits_of(x[s][c].y * up), digits_of(x[s][c].z * up),
+                            digits_of(x[s][c].w * up), d);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) qd[s][j][c] = d[j];
+                }
+            if (t < t1) {  // (behind the digits, whose registers it takes)
+                load_v();
+                look(t + W);
+            }
+        }
+        // the new row as the cache holds it, into the cache and for the loop
+        if (has_new) {
+            const size_t row = row0_of(own, n_blocks - 1) + (new_row & 15);
+            const int c = lane & (LR - 1);
+            float sc[2];
+            int w[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float4 y = reinterpret_cast<const float4 *>((u ? a.v_new : a.k_new) + new_at)[c];
+                if (!u) y = rope4(y, turn_at[c]);
+                w[u] = quantize_row<HD>(y, &sc[u]);
+            }
+            if (lane < LR) {
+                sh.fresh[0][c] = w[0];
+                sh.fresh[1][c] = w[1];
+                sh.fresh_scale[0] = sc[0];
+                sh.fresh_scale[1] = sc[1];
+                if (keeps) {
+                    reinterpret_cast<int *>(a.k)[row * LR + c] = w[0];
+                    int8_t *to = static_cast<int8_t *>(a.v) + (row - (new_row & 15)) * HD + 64 * c + (new_row & 15);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) to[16 * i] = (int8_t)(w[1] >> (8 * i));
+                    if (c == 0) {
+                        a.ks[row] = sc[0];
+                        a.vs[row] = sc[1];
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        }
+        for (; t < t1; t += W) {
+            const bool newest = has_new && t == tiles - 1;
+            const int b_new = new_row >> 4, r_new = new_row & 15;  // its block of the tile, and row of that
+            if (newest) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    if (4 * b + (m & 3) == r_new && (m >> 2) == b_new)
+#pragma unroll
+                        for (int s = 0; s < KS; s++) kraw[b][s] = *reinterpret_cast<const u32x4 *>(&sh.fresh[0][16 * s + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (g == b_new && 4 * b + i == r_new) {
+                            (&ksc[b].x)[i] = sh.fresh_scale[0];
+                            (&vsc[b].x)[i] = sh.fresh_scale[1];
+                        }
+                }
+            }
+            // ---- scores ----
+            float x[NB][4];
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                i32x4 d[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    d[j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < KS; s++) d[j] = mfma8(kraw[b][s], qd[s][j], d[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[b][i] = digits_sum(d[0][i], d[1][i], d[2][i], d[3][i]) * ((&ksc[b].x)[i] * qf);
+                // (put together here: all sums of a tile at once would not fit the registers)
+                asm volatile("" : "+v"(x[b][0]), "+v"(x[b][1]), "+v"(x[b][2]), "+v"(x[b][3]));
+            }
+            const bool next = t + W < t1;
+            if (newest) {
+                // the new value's byte of each dim's 16
+                const int sh8 = 8 * (r_new & 3);
+                const int8_t *y = reinterpret_cast<const int8_t *>(sh.fresh[1]);
+#pragma unroll
+                for (int v = 0; v < VB; v++) {
+                    const unsigned w = (unsigned)(uint8_t)y[16 * v + m] << sh8;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (g == b_new && c == (r_new >> 2)) vraw[v][c] = (vraw[v][c] & ~(255u << sh8)) | w;
+                }
+            }
+            // ---- softmax ----
+            float mt = -__builtin_inff();
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[b][i] += 0.0f * (&vsc[b].x)[i];  // (NaN in a value row's scale marks the row)
+                    if (t == tiles - 1 && 16 * g + 4 * b + i > new_row) x[b][i] = -__builtin_inff();
+                    mt = fmaxf(mt, x[b][i]);
+                }
+            if (__builtin_amdgcn_ballot_w64(mt > mrun + kPagedMargin) != 0) {
+                mt = rows4<true>(mt);
+                const float now = mt > mrun + kPagedMargin ? mt : mrun, f = fast_exp2(mrun - now);
+                mrun = now;
+                lrun *= f;
+#pragma unroll
+                for (int v = 0; v < VB; v++) o[v] *= f;
+            }
+            const float off = mrun + kPagedBias;
+            float wt = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float y = fast_exp2(x[b][i] - off);
+                    lrun += y;
+                    x[b][i] = y * fmaxf((&vsc[b].x)[i], 0.0f);
+                    wt = fmaxf(wt, x[b][i]);
+                }
+            if (next) {
+                point(t + W);
+                load_k();
+            }
+            // ---- weighted values ----
+            const int e = fixed_exp(__float_as_uint(rows4<true>(wt)));
+            const float up = exp2_int(29 - e), down = exp2_int(e - 29);
+            u32x4 pd[4];
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                unsigned d[4];
+                digits4(digits_of(x[b][0] * up), digits_of(x[b][1] * up), digits_of(x[b][2] * up), digits_of(x[b][3] * up), d);
+#pragma unroll
+                for (int j = 0; j < 4; j++) pd[j][b] = d[j];
+            }
+#pragma unroll
+            for (int v = 0; v < VB; v++) {
+                i32x4 d[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) d[j] = mfma8(vraw[v], pd[j], i32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[v][i] = __builtin_fmaf(digits_sum(d[0][i], d[1][i], d[2][i], d[3][i]), down, o[v][i]);
+                asm volatile("" : "+v"(o[v]));
+            }
+            if (next) {
+                load_v();
+                look(t + 2 * W);
+            }
+        }
+        if (has_new && keeps && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
+            const size_t head = (size_t)own * a.n_kv_heads + p.kvh;
+            const int c = lane & (LR - 1);
+            page_bounds<HD, true>(kp + (head << a.rows_log2) * HD, a.ks + (head << a.rows_log2), a.bounds + head * 2 * HD,
+                                  (1 << a.rows_log2) - 1, bytes4(sh.fresh[0][c], sh.fresh_scale[0]), true, lane);
+        }
+    }
+
+    // ---- the waves' results together ----
+    lrun = rows4<false>(lrun);
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) lrun = __uint_as_float(0x7fc00000u);
+    if (g == 0) {
+        sh.m[wave][m] = mrun;
+        sh.l[wave][m] = lrun;
+    }
+    // register i of block v: dim (8 bits) 16 v + 4 g + i, or 64 (v / 4) + 16 g + 4 i + v % 4
+    if (m < a.group) {
+        if constexpr (Q8) {
+#pragma unroll
+            for (int v = 0; v < VB; v++)
+                *reinterpret_cast<float4 *>(&sh.o[wave][m][16 * v + 4 * g]) = make_float4(o[v][0], o[v][1], o[v][2], o[v][3]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VB; v += 4)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(&sh.o[wave][m][16 * v + 16 * g + 4 * i]) =
+                        make_float4(o[v][i], o[v + 1][i], o[v + 2][i], o[v + 3][i]);
+        }
+    }
+    __syncthreads();
+    const size_t rec = ((size_t)gi * a.splits + split) * a.group;
+    for (int i = tid; i < a.group * LR; i += kThreads) {
+        const int head = i / LR, d = (i - head * LR) * 4;
+        float top = sh.m[0][head];
+#pragma unroll
+        for (int w = 1; w < W; w++) top = fmaxf(top, sh.m[w][head]);
+        float f[W], total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            f[w] = fast_exp2(sh.m[w][head] - top);
+            total += f[w] * sh.l[w][head];
+        }
+        float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < W; w++) fma4(acc, f[w], *reinterpret_cast<const float4 *>(&sh.o[w][head][d]));
+        // (no weight at all, every score -inf: as a record nothing, as a result NaN)
+        if (runs.n == 1) {
+            scale4(acc, 1.0f / total);
+            *reinterpret_cast<float4 *>(a.out + ((size_t)p.seq * a.n_heads + p.kvh * a.group + head) * HD + d) = acc;
+        } else {
+            scale4(acc, total == 0.0f ? 0.0f : 1.0f / total);
+            *reinterpret_cast<float4 *>(a.ws_o + (rec + head) * HD + d) = acc;
+            if (d == 0) a.ws_lse[rec + head] = total == 0.0f ? -__builtin_inff() : top + log2f(total);
+        }
+    }
+    if (runs.n == 1 || a.spread) return;
+
+    // ---- the last run to arrive adds up the records ----
+    // (all in one XCD's L2: the stores have drained to it, the counter is an
+    // L2 atomic, and the loads miss in L1)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        const int before = __hip_atomic_fetch_add(a.counters + gi, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.last = before == runs.n - 1;
+        if (before == runs.n - 1) __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (sh.last) paged_merge<HD, kThreads>(a, sh.merge, gi, runs.n, p, tid);
+}
+
+// The records of a spread launch's groups added up, a workgroup each.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a)
+{
+    __shared__ struct {
+        float w[kPagedHeads][kPagedSplits + 1];
+        float4 part[256];
+    } sh;
+    const PagedPlace p = paged_place(a, blockIdx.x);
+    if (p.seq < 0) return;
+    const PagedRuns runs = paged_runs(a, (p.rows + paged_tile(HD, Q8) - 1) / paged_tile(HD, Q8));
+    if (runs.n > 1) paged_merge<HD, 256>(a, sh, blockIdx.x, runs.n, p, threadIdx.x);
+}
+
+}  // namespace leap
