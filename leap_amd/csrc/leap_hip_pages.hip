@@ -199,10 +199,12 @@ int launch_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *po
     a.rows_log2 = p->rows_log2;
     a.chunk = s.chunk;
     a.splits = s.splits;
+    a.blocks = (longest + 15) / 16;
     a.spread = s.spread;
     a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)m.head_dim));
     a.by_kv_heads = leap::make_fastdiv((uint32_t)m.n_kv_heads);
     a.by_splits = leap::make_fastdiv((uint32_t)s.splits);
+    a.by_chunk = leap::make_fastdiv((uint32_t)s.chunk);
     if (s.wgs > 0x7fffffffLL) return set_err(p, -EINVAL, "%lld workgroups in one launch", s.wgs);
     HIP_TRY(p, launch_k(fn.attention[s.waves == 8], dim3((unsigned)s.wgs), dim3((unsigned)(s.waves * leap::kWave)), stream, a));
     if (s.spread) HIP_TRY(p, launch_k(fn.merge, dim3((unsigned)(n_seq * m.n_kv_heads)), dim3(256), stream, a));

@@ -64,47 +64,58 @@ struct PagedArgs {
     int width, keep, n_pages;
     int n_seq, max_pos, n_heads, n_kv_heads, group;
     int rows_log2;                   // R = 1 << rows_log2
-    int chunk, splits;               // tiles of a run at least, runs of a group at most
+    int chunk, splits;               // tiles of a run, runs of the longest group
+    int blocks;                      // blocks of 16 rows of the longest group
     int spread;                      // a group's runs lie on all XCDs, and paged_merge_kernel adds up their records
     float scale_log2;
-    FastDiv by_kv_heads, by_splits;
+    FastDiv by_kv_heads, by_splits, by_chunk;
 };
+
+// A word that the kernel does not write, at an address that is the same in all
+// lanes: by way of the scalar cache, so that the wait for it is not one for
+// the rows that are on their way.
+__device__ __forceinline__ int uniform_load(const int *p)
+{
+    typedef __attribute__((address_space(4))) const int ConstInt;
+    return *(ConstInt *)(uintptr_t)p;
+}
 
 // What a group (sequence, KV head) attends to.
 struct PagedPlace {
-    int seq, kvh, pos;   // seq < 0: nothing (a skipped position)
+    int seq, kvh, pos;
     const int *list;     // page numbers
     int n_list, rows;    // pages, and rows along the list with the new one
+    bool skip;           // a position out of range
 };
 __device__ __forceinline__ PagedPlace paged_place(const PagedArgs &a, int gi)
 {
     PagedPlace p;
     p.seq = (int)fast_div((uint32_t)gi, a.by_kv_heads);
     p.kvh = gi - p.seq * a.n_kv_heads;
-    p.pos = a.pos[p.seq];
-    const int at = p.pos >> a.rows_log2;
-    p.n_list = a.keep ? min(a.keep, at + 1) : at + 1;
     p.list = a.keep ? a.lists + (size_t)gi * a.keep : a.table + (size_t)p.seq * a.width;
-    p.rows = ((p.n_list - 1) << a.rows_log2) + (p.pos & ((1 << a.rows_log2) - 1)) + 1;
-    if (p.pos < 0 || p.pos > a.max_pos) p.seq = -1 - p.seq;
     return p;
 }
-// Its runs: of `chunk` tiles each, the tiles dealt evenly.
-struct PagedRuns {
-    int n, per, more;  // runs, tiles of each, and how many have one more
-};
-__device__ __forceinline__ PagedRuns paged_runs(const PagedArgs &a, int tiles)
+// (its position known)
+__device__ __forceinline__ void paged_rows(const PagedArgs &a, PagedPlace &p)
 {
-    PagedRuns r;
-    r.n = min(a.splits, (tiles + a.chunk - 1) / a.chunk);
-    r.per = tiles / r.n;
-    r.more = tiles - r.per * r.n;
-    return r;
+    const int at = p.pos >> a.rows_log2;
+    p.n_list = a.keep ? min(a.keep, at + 1) : at + 1;
+    p.rows = ((p.n_list - 1) << a.rows_log2) + (p.pos & ((1 << a.rows_log2) - 1)) + 1;
+    p.skip = p.pos < 0 || p.pos > a.max_pos;
 }
+// The runs of a group of so many tiles (run i: tiles [i chunk, (i + 1) chunk)).
+__device__ __forceinline__ int paged_runs(const PagedArgs &a, int tiles) { return (int)fast_div((uint32_t)(tiles + a.chunk - 1), a.by_chunk); }
 
-template <int HD, int W>
+template <int HD, int W, bool Q8>
 struct PagedShared {
     union {
+        struct {
+            // q as the products take it, a lane's word after the other: float4 of
+            // dims 16 f + 4 g (8 bits: the digits j of dims 64 s + 16 g, [s][j])
+            u32x4 q[HD / 16][kWave];
+            alignas(16) float k_new[HD], v_new[HD];  // the new rows (8 bits: of bytes)
+            float new_scale[2], q_unit[kPagedHeads];
+        };
         float o[W][kPagedHeads][HD + 4];  // the waves' outputs
         struct {
             float w[kPagedHeads][kPagedSplits + 1];  // the merge: weights of a head's records
@@ -112,8 +123,6 @@ struct PagedShared {
         } merge;
     };
     float m[W][kPagedHeads], l[W][kPagedHeads];
-    alignas(16) int fresh[2][HD / 4];     // 8 bits: the new token's K and V rows
-    float fresh_scale[2];
     int last;
 };
 
@@ -273,12 +282,28 @@ __device__ __forceinline__ void page_bounds(const void *k, const float *ks, floa
 // 8-bit ones.
 __host__ __device__ constexpr int paged_tile(int hd, bool q8) { return q8 ? 64 : 2048 / hd; }
 
-// W waves.
+// A row's value of lane j of each row of 16 lanes (DPP row_newbcast).
+template <int J>
+__device__ __forceinline__ float row_lane(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xF, 0xF, true));
+}
+template <int I, int N, class F>
+__device__ __forceinline__ void unroll(F f)
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        unroll<I + 1, N>(f);
+    }
+}
+
+// W waves.  Loads go out before the position is known: a run's tiles, and
+// their pages, do not depend on it.
 template <int HD, int W, bool Q8>
-__global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_kernel(PagedArgs a)
+__global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_kernel(PagedArgs a)
 {
     constexpr int TK = paged_tile(HD, Q8), NB = TK / 16, LR = HD / 4, VB = HD / 16, kThreads = W * kWave;
-    __shared__ PagedShared<HD, W> sh;
+    __shared__ PagedShared<HD, W, Q8> sh;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, g = lane >> 4;
 
@@ -295,150 +320,258 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
     }
     if (gi >= n_groups) return;
     PagedPlace p = paged_place(a, gi);
-    if (p.seq < 0) {
-        if (split == 0)
-            fill_nan<HD>(a.out, ((size_t)(-1 - p.seq) * a.n_heads + p.kvh * a.group) * LR, a.group * LR, tid, kThreads);
-        return;
-    }
-    const int tiles = (p.rows + TK - 1) / TK;
-    const PagedRuns runs = paged_runs(a, tiles);
-    if (split >= runs.n) return;
-    const int t0 = split * runs.per + min(split, runs.more), t1 = t0 + runs.per + (split < runs.more);
-
     const int blocks_log2 = a.rows_log2 - 4;  // blocks of 16 rows of a page
     auto row0_of = [&](int page, int block) {  // a block's first row among the KV heads' rows of the layer
         return (((size_t)page * a.n_kv_heads + p.kvh) << a.rows_log2) + ((block & ((1 << blocks_log2) - 1)) << 4);
     };
-    const int n_blocks = (p.rows + 15) >> 4;
-    bool bad = false;  // a page is missing, or the new row's is shared
-
-    // ---- this wave's rows of q, and the new token's if it has the last tile ----
+    auto there = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
+    const int t0 = split * a.chunk;
     int t = t0 + wave;
-    const bool has_new = t1 == tiles && (tiles - 1 - t0) % W == wave;  // (t0 + wave <= tiles - 1 then)
-    const int new_row = (p.rows - 1) & (TK - 1);                       // its row of the last tile
-    const int own = has_new ? p.list[p.n_list - 1] : 0;
-    const bool keeps = has_new && (unsigned)own < (unsigned)a.n_pages && a.refs[own] == 1;  // its page is its own
-    if (has_new && !keeps) bad = true;
-    const float *q_at = a.q + ((size_t)p.seq * a.n_heads + p.kvh * a.group + m) * HD;
-    const size_t new_at = ((size_t)p.seq * a.n_kv_heads + p.kvh) * HD;
-    const float4 *turn_at = a.rope + (size_t)p.pos * LR;
 
-    f32x4 o[VB];
+    // ---- a tile's loads ----
+    // (always made, on or not, so that the waits for them count exactly: an
+    // empty range reads nothing)
+    // (blocks behind a sequence's last: page 0 or another's rows, which are masked)
+    constexpr int KF = Q8 ? HD / 64 : HD / 16, VF = HD / 64;
+    float4 kraw[Q8 ? 1 : NB][KF], vraw[Q8 ? 1 : NB][4][VF];  // fp32
+    u32x4 k8[Q8 ? NB : 1][KF], v8[Q8 ? VB : 1];               // 8 bits
+    float ksc = 0.0f, vsc = 0.0f;                             // and the scales of position 16 g + m
+    // Its pages, a tile ahead.  fp32: of each block, the same in all lanes.  8
+    // bits: of blocks m / 4 and g: K's row m of product block b is row 4 b + m
+    // % 4 of block m / 4, so that the scores of a lane, 4 for each b, are the
+    // 16 rows of block g in order, which are the 16 bytes of V that it loads.
+    int pages[Q8 ? 2 : NB];
+    auto look = [&](int at) {
+        if constexpr (Q8) {
+            int here = lane;
+            asm volatile("" : "+v"(here));
+            pages[0] = p.list[min(4 * at + ((here & 15) >> 2), a.blocks - 1) >> blocks_log2];
+            pages[1] = p.list[min(4 * at + (here >> 4), a.blocks - 1) >> blocks_log2];
+        } else {
 #pragma unroll
-    for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
-    float mrun = kNothing, lrun = 0.0f;
-
-    if constexpr (!Q8) {
-        constexpr int KF = HD / 16, VF = HD / 64;
-        const float *kp = static_cast<const float *>(a.k), *vp = static_cast<const float *>(a.v);
-        float4 kraw[NB][KF], vraw[NB][4][VF];
-        // a tile's pages, uniform over the wave: loaded a tile ahead
-        int pages[NB];
-        auto look = [&](int at) {
+            for (int b = 0; b < NB; b++) pages[b] = uniform_load(p.list + (min(at * NB + b, a.blocks - 1) >> blocks_log2));
+        }
+    };
+    const int8_t *v8_at = nullptr;
+    const float *vs_at = nullptr;
+    int used[Q8 ? 1 : NB];  // the pages of the tile that is loaded (8 bits: V's)
+    auto load_k = [&](int at, bool on) {
+        if constexpr (Q8) {
+            used[0] = pages[1];
+            int here = on ? lane : 0;  // (not on: all lanes the same line)
+            asm volatile("" : "+v"(here));  // (addresses formed here: kept, their parts would take the registers of a load)
+            const int m = here & 15, g = here >> 4;
+            const size_t rk = row0_of(on && there(pages[0]) ? pages[0] : 0, 4 * at + (m >> 2)) + (m & 3);
+            const size_t rv = row0_of(on && there(pages[1]) ? pages[1] : 0, 4 * at + g);
+            const int8_t *from = static_cast<const int8_t *>(a.k) + rk * HD + 16 * g;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int s = 0; s < KF; s++)
+                    k8[b][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + 4 * b * HD + 64 * s));
+            ksc = a.ks[rv + m];
+            v8_at = static_cast<const int8_t *>(a.v) + rv * HD + 16 * m;
+            vs_at = a.vs + rv + m;
+        } else {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const int block = min(at * NB + b, n_blocks - 1);
-                pages[b] = p.list[block >> blocks_log2];
-            }
-        };
-        // (rows from the new one on read as zero)
-        auto rows_at = [&](const float *base, int at, int b) {
-            const int block = at * NB + b, page = pages[b];
-            const bool ok = (unsigned)page < (unsigned)a.n_pages;
-            if (block < n_blocks && !ok) bad = true;
-            const int n = ok ? max(0, min(16, p.rows - 1 - 16 * block)) : 0;
-            return make_rsrc(base + row0_of(ok ? page : 0, block) * HD, (uint32_t)(n * HD * 4));
-        };
-        auto load_k = [&](int at) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const auto r = rows_at(kp, at, b);
+                used[b] = pages[b];
+                const bool ok = on && there(pages[b]);
+                const auto r = make_rsrc(static_cast<const float *>(a.k) + row0_of(ok ? pages[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
 #pragma unroll
                 for (int f = 0; f < KF; f++) kraw[b][f] = buf_load4<kNt>(r, (uint32_t)(m * HD + 16 * f + 4 * g) * 4u);
             }
-        };
-        auto load_v = [&](int at) {
+        }
+    };
+    auto load_v = [&](int at, bool on) {
+        if constexpr (Q8) {
+#pragma unroll
+            for (int v = 0; v < VB; v++) v8[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(v8_at + 256 * v));
+            vsc = *vs_at;
+        } else {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const auto r = rows_at(vp, at, b);
+                const bool ok = on && there(used[b]);
+                const auto r = make_rsrc(static_cast<const float *>(a.v) + row0_of(ok ? used[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int f = 0; f < VF; f++)
                         vraw[b][i][f] = buf_load4<kNt>(r, (uint32_t)((4 * g + i) * HD + 64 * f + 4 * m) * 4u);
             }
-        };
-        float4 q[KF];
-        {
-            float4 turn[KF];
-#pragma unroll
-            for (int f = 0; f < KF; f++) {
-                q[f] = m < a.group ? *reinterpret_cast<const float4 *>(q_at + 16 * f + 4 * g) : make_float4(0, 0, 0, 0);
-                turn[f] = turn_at[4 * f + g];
-            }
-            if (t < t1) {
-                look(t);
-                load_k(t);
-                load_v(t);
-                look(t + W);
-            }
-#pragma unroll
-            for (int f = 0; f < KF; f++) q[f] = rope4(q[f], turn[f]);
         }
-        for (; t < t1; t += W) {
-            const bool newest = has_new && t == tiles - 1;
-            if (newest) {
-                // the new key in place of what was read, and into the cache
-                const int b_new = new_row >> 4, r_new = new_row & 15;
-                float *to = static_cast<float *>(a.k) + (row0_of(own, t * NB + b_new) + r_new) * HD;
+    };
+    // ---- rows of q, and the new token's ----
+    // LR threads a row; a head that a group of fewer than 16 leaves out is
+    // zero.  These loads, the position's and the first pages' go out together.
+    const int c = tid & (LR - 1);
+    constexpr int kJobs = kThreads / LR, kRows = (kPagedHeads + kJobs - 1) / kJobs;
+    const size_t new_at = ((size_t)p.seq * a.n_kv_heads + p.kvh) * LR;
+    float4 row[kRows];
+    const auto q_rows = make_rsrc(a.q + ((size_t)p.seq * a.n_heads + p.kvh * a.group) * HD, (uint32_t)(a.group * HD) * 4u);
 #pragma unroll
-                for (int f = 0; f < KF; f++) {
-                    const float4 x = rope4(*reinterpret_cast<const float4 *>(a.k_new + new_at + 16 * f + 4 * g), turn_at[4 * f + g]);
+    for (int u = 0; u < kRows; u++) row[u] = buf_load4(q_rows, (uint32_t)((tid / LR + u * kJobs) * LR + c) * 16u);
+    const float4 k_row = reinterpret_cast<const float4 *>(a.k_new)[new_at + c];
+    const float4 v_row = reinterpret_cast<const float4 *>(a.v_new)[new_at + c];
+    look(t);
+    p.pos = uniform_load(a.pos + p.seq);
+    if constexpr (!Q8) asm volatile("" ::"s"(p.pos), "s"(pages[0]), "s"(pages[NB - 1]));  // (one wait for them all)
+    __builtin_amdgcn_sched_barrier(0);
+    paged_rows(a, p);
+    if (p.skip) {
+        if (split == 0) fill_nan<HD>(a.out, ((size_t)p.seq * a.n_heads + p.kvh * a.group) * LR, a.group * LR, tid, kThreads);
+        return;
+    }
+    const int tiles = (p.rows + TK - 1) / TK;
+    if (t0 >= tiles) return;
+    const int t1 = min(t0 + a.chunk, tiles), n_runs = paged_runs(a, tiles), n_blocks = (p.rows + 15) >> 4;
+    const bool newest_run = t1 == tiles;
+    const float4 turn = a.rope[(size_t)p.pos * LR + c];
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(t, t < t1);
+    load_v(t, t < t1);
+    look(t + W);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
-                        if (b == b_new && m == r_new) kraw[b][f] = x;
-                    if (keeps && m == 0) *reinterpret_cast<float4 *>(to + 16 * f + 4 * g) = x;
+    for (int u = 0; u < kRows; u++) {
+        const int job = tid / LR + u * kJobs;
+        if (kPagedHeads % kJobs && job >= kPagedHeads) break;
+        const float4 x = rope4(row[u], turn);
+        if constexpr (Q8) {
+            unsigned top = dpp_max16(max4_bits(0u, x));
+            if constexpr (HD == 128) top = max(top, (unsigned)__shfl_xor((int)top, 16));
+            const bool good = finite_bits(top);
+            const int e = fixed_exp(good ? top : 0u);
+            const float up = good ? exp2_int(29 - e) : 0.0f;
+            unsigned d[4];
+            digits4(digits_of(x.x * up), digits_of(x.y * up), digits_of(x.z * up), digits_of(x.w * up), d);
+            // dims 4 c: s = c / 16, g = c / 4 % 4, word c % 4
+#pragma unroll
+            for (int j = 0; j < 4; j++) reinterpret_cast<unsigned *>(&sh.q[4 * (c >> 4) + j][16 * ((c >> 2) & 3) + job])[c & 3] = d[j];
+            if (c == 0) sh.q_unit[job] = good ? exp2_int(e - 29) * a.scale_log2 : __uint_as_float(0x7fc00000u);
+        } else {
+            // dims 4 c: f = c / 4, g = c % 4
+            sh.q[c >> 2][16 * (c & 3) + job] = u32x4{__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
+        }
+    }
+    if (newest_run && wave == W - 1) {
+        const float4 x[2] = {rope4(k_row, turn), v_row};
+#pragma unroll
+        for (int value = 0; value < 2; value++) {
+            float *to = value ? sh.v_new : sh.k_new;
+            if constexpr (Q8) {
+                float sc;
+                const int w = quantize_row<HD>(x[value], &sc);
+                reinterpret_cast<int *>(to)[c] = w;
+                if (c == 0) sh.new_scale[value] = sc;
+            } else {
+                reinterpret_cast<float4 *>(to)[c] = x[value];
+            }
+        }
+    }
+    __syncthreads();
+    const float qf = Q8 ? sh.q_unit[m] : a.scale_log2;
+
+    // ---- the new rows into the cache, by the wave that has the last tile ----
+    const bool has_new = newest_run && (tiles - 1 - t0) % W == wave;
+    const int new_row = (p.rows - 1) & (TK - 1);                       // its row of the last tile
+    const int b_new = new_row >> 4, r_new = new_row & 15;              // its block of that, and row of the block
+    bool bad = false;  // a page is missing, or the new row's is shared
+    if (has_new) {
+        const int own = uniform_load(p.list + p.n_list - 1);
+        bad = !there(own) || uniform_load(a.refs + (there(own) ? own : 0)) != 1;
+        if (!bad && lane < LR) {
+            const size_t to = row0_of(own, n_blocks - 1) + r_new;
+            if constexpr (Q8) {
+                const int w = reinterpret_cast<const int *>(sh.v_new)[lane];
+                reinterpret_cast<int *>(a.k)[to * LR + lane] = reinterpret_cast<const int *>(sh.k_new)[lane];
+                int8_t *bytes = static_cast<int8_t *>(a.v) + (to - r_new) * HD + 64 * lane + r_new;
+#pragma unroll
+                for (int i = 0; i < 4; i++) bytes[16 * i] = (int8_t)(w >> (8 * i));
+                if (lane == 0) {
+                    a.ks[to] = sh.new_scale[0];
+                    a.vs[to] = sh.new_scale[1];
                 }
+            } else {
+                reinterpret_cast<float4 *>(a.k)[to * LR + lane] = reinterpret_cast<const float4 *>(sh.k_new)[lane];
+                reinterpret_cast<float4 *>(a.v)[to * LR + lane] = reinterpret_cast<const float4 *>(sh.v_new)[lane];
+            }
+        }
+        if (!bad && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
+            // the page is complete: the bounds of its keys
+            const size_t head = (size_t)own * a.n_kv_heads + p.kvh;
+            const int d = lane & (LR - 1);
+            const float4 x = Q8 ? bytes4(reinterpret_cast<const int *>(sh.k_new)[d], sh.new_scale[0])
+                                : reinterpret_cast<const float4 *>(sh.k_new)[d];
+            page_bounds<HD, Q8>(static_cast<const char *>(a.k) + (head << a.rows_log2) * HD * (Q8 ? 1 : 4),
+                                Q8 ? a.ks + (head << a.rows_log2) : nullptr, a.bounds + head * 2 * HD, (1 << a.rows_log2) - 1, x, true,
+                                lane);
+        }
+    }
+
+    f32x4 o[VB];
+#pragma unroll
+    for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
+    float mrun = kNothing, lrun = 0.0f;
+    // The scores' maximum mt of a tile: the reference moved, and what was summed with it.
+    auto follow = [&](float mt) {
+        if (__builtin_amdgcn_ballot_w64(mt > mrun + kPagedMargin) != 0) {
+            mt = rows4<true>(mt);
+            const float now = mt > mrun + kPagedMargin ? mt : mrun, f = fast_exp2(mrun - now);
+            mrun = now;
+            lrun *= f;
+#pragma unroll
+            for (int v = 0; v < VB; v++) o[v] *= f;
+        }
+        return mrun + kPagedBias;
+    };
+    for (; t < t1; t += W) {
+        const bool last = t == tiles - 1, next = t + W < t1;
+        int zero = 0;
+        asm volatile("" : "+v"(zero));  // (q is read from LDS for each tile: kept, it would take a quarter of the registers)
+        const u32x4 *qs = &sh.q[0][lane + zero];
+        float x[NB][4], mt = -__builtin_inff();
+        if constexpr (!Q8) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) bad |= t * NB + b < n_blocks && !there(used[b]);
+            if (last) {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    if (b == b_new && m == r_new)
+#pragma unroll
+                        for (int f = 0; f < KF; f++) kraw[b][f] = *reinterpret_cast<const float4 *>(&sh.k_new[16 * f + 4 * g]);
             }
             // ---- scores ----
             f32x4 s[NB], s2[NB];
 #pragma unroll
             for (int b = 0; b < NB; b++) s[b] = s2[b] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int f = 0; f < KF; f++)
+            for (int f = 0; f < KF; f++) {
+                const f32x4 q = __builtin_bit_cast(f32x4, qs[f * kWave]);
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    s[b] = mfma32(kraw[b][f].x, q[f].x, s[b]);
-                    s2[b] = mfma32(kraw[b][f].y, q[f].y, s2[b]);
-                    s[b] = mfma32(kraw[b][f].z, q[f].z, s[b]);
-                    s2[b] = mfma32(kraw[b][f].w, q[f].w, s2[b]);
+                    s[b] = mfma32(kraw[b][f].x, q.x, s[b]);
+                    s2[b] = mfma32(kraw[b][f].y, q.y, s2[b]);
+                    s[b] = mfma32(kraw[b][f].z, q.z, s[b]);
+                    s2[b] = mfma32(kraw[b][f].w, q.w, s2[b]);
                 }
-            const bool next = t + W < t1;
-            if (next) load_k(t + W);
+            }
+            load_k(t + W, next);
             // ---- softmax ----
-            float x[NB][4], mt = -__builtin_inff();
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[b][i] = (s[b][i] + s2[b][i]) * a.scale_log2;
-            if (t == tiles - 1)
+                for (int i = 0; i < 4; i++) x[b][i] = (s[b][i] + s2[b][i]) * qf;
+            if (last) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         if (16 * b + 4 * g + i > new_row) x[b][i] = -__builtin_inff();
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
-            if (__builtin_amdgcn_ballot_w64(mt > mrun + kPagedMargin) != 0) {
-                mt = rows4<true>(mt);
-                const float now = mt > mrun + kPagedMargin ? mt : mrun, f = fast_exp2(mrun - now);
-                mrun = now;
-                lrun *= f;
-#pragma unroll
-                for (int v = 0; v < VB; v++) o[v] *= f;
             }
-            const float off = mrun + kPagedBias;
+#pragma unroll
+            for (int b = 0; b < NB; b++) mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
+            const float off = follow(mt);
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -446,19 +579,19 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
                     x[b][i] = fast_exp2(x[b][i] - off);
                     lrun += x[b][i];
                 }
-            if (newest) {
-                const int b_new = new_row >> 4, r_new = new_row & 15;
-                float *to = static_cast<float *>(a.v) + (row0_of(own, t * NB + b_new) + r_new) * HD;
+            if (last) {
+                // the new value, and zeros behind it
 #pragma unroll
-                for (int f = 0; f < VF; f++) {
-                    const float4 y = *reinterpret_cast<const float4 *>(a.v_new + new_at + 64 * f + 4 * m);
+                for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
+                    for (int i = 0; i < 4; i++) {
+                        const int r = 16 * b + 4 * g + i;
+                        if (r >= new_row)
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (b == b_new && 4 * g + i == r_new) vraw[b][i][f] = y;
-                    if (keeps && g == 0) *reinterpret_cast<float4 *>(to + 64 * f + 4 * m) = y;
-                }
+                            for (int f = 0; f < VF; f++)
+                                vraw[b][i][f] = r == new_row ? *reinterpret_cast<const float4 *>(&sh.v_new[64 * f + 4 * m])
+                                                             : make_float4(0, 0, 0, 0);
+                    }
             }
             // ---- weighted values ----
 #pragma unroll
@@ -472,156 +605,23 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
                         o[4 * f + 2] = mfma32(vraw[b][i][f].z, x[b][i], o[4 * f + 2]);
                         o[4 * f + 3] = mfma32(vraw[b][i][f].w, x[b][i], o[4 * f + 3]);
                     }
-            if (next) {
-                load_v(t + W);
-                look(t + 2 * W);
-            }
-        }
-        if (has_new && keeps && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
-            // the page is complete: the bounds of its keys
-            const size_t head = (size_t)own * a.n_kv_heads + p.kvh;
-            const int c = lane & (LR - 1);
-            const float4 x = rope4(reinterpret_cast<const float4 *>(a.k_new + new_at)[c], turn_at[c]);
-            page_bounds<HD, false>(kp + (head << a.rows_log2) * HD, nullptr, a.bounds + head * 2 * HD, (1 << a.rows_log2) - 1, x,
-                                   true, lane);
-        }
-    } else {
-        constexpr int KS = HD / 64;
-        const int8_t *kp = static_cast<const int8_t *>(a.k), *vp = static_cast<const int8_t *>(a.v);
-        u32x4 kraw[NB][KS], vraw[VB];
-        float4 ksc[NB], vsc[NB];
-        // A tile is 4 blocks of 16 rows.  K's row m of product block b is row
-        // 4 b + m % 4 of block m / 4, so that the scores of a lane, 4 for
-        // each b, are the 16 rows of block g in order: the 16 bytes of V that
-        // it loads.
-        int page_k = 0, page_v = 0;  // the pages of blocks m / 4 and g, a tile ahead
-        auto look = [&](int at) {
-            page_k = p.list[min(4 * at + (m >> 2), n_blocks - 1) >> blocks_log2];
-            page_v = p.list[min(4 * at + g, n_blocks - 1) >> blocks_log2];
-        };
-        const int8_t *k_at, *v_at;
-        const float *ks_at, *vs_at;
-        auto point = [&](int at) {
-            // (blocks behind the last: its rows once more; their scores are masked)
-            const int bk = min(4 * at + (m >> 2), n_blocks - 1), bv = min(4 * at + g, n_blocks - 1);
-            bad |= (unsigned)page_v >= (unsigned)a.n_pages;
-            const size_t rk = row0_of((unsigned)page_k < (unsigned)a.n_pages ? page_k : 0, bk);
-            const size_t rv = row0_of((unsigned)page_v < (unsigned)a.n_pages ? page_v : 0, bv);
-            k_at = kp + (rk + (m & 3)) * HD + 16 * g;
-            v_at = vp + rv * HD + 16 * m;
-            ks_at = a.ks + rv;
-            vs_at = a.vs + rv;
-        };
-        auto load_k = [&]() {
+        } else {
+            bad |= 4 * t + g < n_blocks && !there(used[0]);
+            if (last) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-                    kraw[b][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(k_at + 4 * b * HD + 64 * s));
-                ksc[b] = *reinterpret_cast<const float4 *>(ks_at + 4 * b);
-            }
-        };
-        auto load_v = [&]() {
-#pragma unroll
-            for (int v = 0; v < VB; v++) vraw[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(v_at + 256 * v));
-#pragma unroll
-            for (int b = 0; b < NB; b++) vsc[b] = *reinterpret_cast<const float4 *>(vs_at + 4 * b);
-        };
-        // q's digits, and the unit of its head row over the score's scale
-        u32x4 qd[KS][4];
-        float qf;
-        {
-            float4 x[KS][4], turn[KS][4];
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    x[s][c] = m < a.group ? *reinterpret_cast<const float4 *>(q_at + 64 * s + 16 * g + 4 * c) : make_float4(0, 0, 0, 0);
-                    turn[s][c] = turn_at[16 * s + 4 * g + c];
-                }
-            if (t < t1) {
-                look(t);
-                point(t);
-                load_k();
-            }
-            unsigned top = 0;
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    x[s][c] = rope4(x[s][c], turn[s][c]);
-                    top = max4_bits(top, x[s][c]);
-                }
-            top = rows4_bits(top);
-            const bool good = finite_bits(top);
-            const int e = fixed_exp(good ? top : 0u);
-            const float up = good ? exp2_int(29 - e) : 0.0f;
-            qf = good ? exp2_int(e - 29) * a.scale_log2 : __uint_as_float(0x7fc00000u);
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    unsigned d[4];
-                    digits4(digits_of(x[s][c].x * up), digits_of(x[s][c].y * up), digits_of(x[s][c].z * up),
-                            digits_of(x[s][c].w * up), d);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) qd[s][j][c] = d[j];
-                }
-            if (t < t1) {  // (behind the digits, whose registers it takes)
-                load_v();
-                look(t + W);
-            }
-        }
-        // the new row as the cache holds it, into the cache and for the loop
-        if (has_new) {
-            const size_t row = row0_of(own, n_blocks - 1) + (new_row & 15);
-            const int c = lane & (LR - 1);
-            float sc[2];
-            int w[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                float4 y = reinterpret_cast<const float4 *>((u ? a.v_new : a.k_new) + new_at)[c];
-                if (!u) y = rope4(y, turn_at[c]);
-                w[u] = quantize_row<HD>(y, &sc[u]);
-            }
-            if (lane < LR) {
-                sh.fresh[0][c] = w[0];
-                sh.fresh[1][c] = w[1];
-                sh.fresh_scale[0] = sc[0];
-                sh.fresh_scale[1] = sc[1];
-                if (keeps) {
-                    reinterpret_cast<int *>(a.k)[row * LR + c] = w[0];
-                    int8_t *to = static_cast<int8_t *>(a.v) + (row - (new_row & 15)) * HD + 64 * c + (new_row & 15);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) to[16 * i] = (int8_t)(w[1] >> (8 * i));
-                    if (c == 0) {
-                        a.ks[row] = sc[0];
-                        a.vs[row] = sc[1];
-                    }
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        }
-        for (; t < t1; t += W) {
-            const bool newest = has_new && t == tiles - 1;
-            const int b_new = new_row >> 4, r_new = new_row & 15;  // its block of the tile, and row of that
-            if (newest) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
+                for (int b = 0; b < NB; b++)
                     if (4 * b + (m & 3) == r_new && (m >> 2) == b_new)
 #pragma unroll
-                        for (int s = 0; s < KS; s++) kraw[b][s] = *reinterpret_cast<const u32x4 *>(&sh.fresh[0][16 * s + 4 * g]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (g == b_new && 4 * b + i == r_new) {
-                            (&ksc[b].x)[i] = sh.fresh_scale[0];
-                            (&vsc[b].x)[i] = sh.fresh_scale[1];
-                        }
+                        for (int s = 0; s < KF; s++)
+                            k8[b][s] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const int8_t *>(sh.k_new) + 64 * s + 16 * g);
+                if (g == b_new && m == r_new) {
+                    ksc = sh.new_scale[0];
+                    vsc = sh.new_scale[1];
                 }
             }
             // ---- scores ----
-            float x[NB][4];
+            // (NaN in either of a row's scales marks it)
+            const float sc = ksc + 0.0f * vsc;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 i32x4 d[4];
@@ -629,59 +629,43 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
                 for (int j = 0; j < 4; j++) {
                     d[j] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int s = 0; s < KS; s++) d[j] = mfma8(kraw[b][s], qd[s][j], d[j]);
+                    for (int s = 0; s < KF; s++) d[j] = mfma8(k8[b][s], qs[(4 * s + j) * kWave], d[j]);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[b][i] = digits_sum(d[0][i], d[1][i], d[2][i], d[3][i]) * ((&ksc[b].x)[i] * qf);
+                for (int i = 0; i < 4; i++) x[b][i] = digits_sum(d[0][i], d[1][i], d[2][i], d[3][i]) * qf;
                 // (put together here: all sums of a tile at once would not fit the registers)
                 asm volatile("" : "+v"(x[b][0]), "+v"(x[b][1]), "+v"(x[b][2]), "+v"(x[b][3]));
             }
-            const bool next = t + W < t1;
-            if (newest) {
+            unroll<0, 16>([&](auto j) { x[j / 4][j % 4] *= row_lane<j>(sc); });
+            if (last) {
                 // the new value's byte of each dim's 16
                 const int sh8 = 8 * (r_new & 3);
-                const int8_t *y = reinterpret_cast<const int8_t *>(sh.fresh[1]);
+                const uint8_t *y = reinterpret_cast<const uint8_t *>(sh.v_new);
 #pragma unroll
                 for (int v = 0; v < VB; v++) {
-                    const unsigned w = (unsigned)(uint8_t)y[16 * v + m] << sh8;
+                    const unsigned w = (unsigned)y[16 * v + m] << sh8;
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        if (g == b_new && c == (r_new >> 2)) vraw[v][c] = (vraw[v][c] & ~(255u << sh8)) | w;
+                    for (int i = 0; i < 4; i++)
+                        if (g == b_new && i == (r_new >> 2)) v8[v][i] = (v8[v][i] & ~(255u << sh8)) | w;
                 }
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (16 * g + 4 * b + i > new_row) x[b][i] = -__builtin_inff();
             }
             // ---- softmax ----
-            float mt = -__builtin_inff();
 #pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[b][i] += 0.0f * (&vsc[b].x)[i];  // (NaN in a value row's scale marks the row)
-                    if (t == tiles - 1 && 16 * g + 4 * b + i > new_row) x[b][i] = -__builtin_inff();
-                    mt = fmaxf(mt, x[b][i]);
-                }
-            if (__builtin_amdgcn_ballot_w64(mt > mrun + kPagedMargin) != 0) {
-                mt = rows4<true>(mt);
-                const float now = mt > mrun + kPagedMargin ? mt : mrun, f = fast_exp2(mrun - now);
-                mrun = now;
-                lrun *= f;
-#pragma unroll
-                for (int v = 0; v < VB; v++) o[v] *= f;
-            }
-            const float off = mrun + kPagedBias;
+            for (int b = 0; b < NB; b++) mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
+            const float off = follow(mt), vs = fmaxf(vsc, 0.0f);
             float wt = 0.0f;
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float y = fast_exp2(x[b][i] - off);
-                    lrun += y;
-                    x[b][i] = y * fmaxf((&vsc[b].x)[i], 0.0f);
-                    wt = fmaxf(wt, x[b][i]);
-                }
-            if (next) {
-                point(t + W);
-                load_k();
-            }
+            unroll<0, 16>([&](auto j) {
+                const float y = fast_exp2(x[j / 4][j % 4] - off);
+                lrun += y;
+                x[j / 4][j % 4] = y * row_lane<j>(vs);
+                wt = fmaxf(wt, x[j / 4][j % 4]);
+            });
+            load_k(t + W, next);
             // ---- weighted values ----
             const int e = fixed_exp(__float_as_uint(rows4<true>(wt)));
             const float up = exp2_int(29 - e), down = exp2_int(e - 29);
@@ -697,26 +681,20 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
             for (int v = 0; v < VB; v++) {
                 i32x4 d[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) d[j] = mfma8(vraw[v], pd[j], i32x4{0, 0, 0, 0});
+                for (int j = 0; j < 4; j++) d[j] = mfma8(v8[v], pd[j], i32x4{0, 0, 0, 0});
 #pragma unroll
                 for (int i = 0; i < 4; i++) o[v][i] = __builtin_fmaf(digits_sum(d[0][i], d[1][i], d[2][i], d[3][i]), down, o[v][i]);
                 asm volatile("" : "+v"(o[v]));
-            }
-            if (next) {
-                load_v();
-                look(t + 2 * W);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (has_new && keeps && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
-            const size_t head = (size_t)own * a.n_kv_heads + p.kvh;
-            const int c = lane & (LR - 1);
-            page_bounds<HD, true>(kp + (head << a.rows_log2) * HD, a.ks + (head << a.rows_log2), a.bounds + head * 2 * HD,
-                                  (1 << a.rows_log2) - 1, bytes4(sh.fresh[0][c], sh.fresh_scale[0]), true, lane);
-        }
+        load_v(t + W, next);
+        look(t + 2 * W);
     }
 
     // ---- the waves' results together ----
     lrun = rows4<false>(lrun);
+    __syncthreads();  // (q is read; its memory takes the outputs)
     if (__builtin_amdgcn_ballot_w64(bad) != 0) lrun = __uint_as_float(0x7fc00000u);
     if (g == 0) {
         sh.m[wave][m] = mrun;
@@ -754,7 +732,7 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
 #pragma unroll
         for (int w = 0; w < W; w++) fma4(acc, f[w], *reinterpret_cast<const float4 *>(&sh.o[w][head][d]));
         // (no weight at all, every score -inf: as a record nothing, as a result NaN)
-        if (runs.n == 1) {
+        if (n_runs == 1) {
             scale4(acc, 1.0f / total);
             *reinterpret_cast<float4 *>(a.out + ((size_t)p.seq * a.n_heads + p.kvh * a.group + head) * HD + d) = acc;
         } else {
@@ -763,7 +741,7 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
             if (d == 0) a.ws_lse[rec + head] = total == 0.0f ? -__builtin_inff() : top + log2f(total);
         }
     }
-    if (runs.n == 1 || a.spread) return;
+    if (n_runs == 1 || a.spread) return;
 
     // ---- the last run to arrive adds up the records ----
     // (all in one XCD's L2: the stores have drained to it, the counter is an
@@ -772,11 +750,11 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 2 : 1) void paged_attention_ker
     __syncthreads();
     if (tid == 0) {
         const int before = __hip_atomic_fetch_add(a.counters + gi, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh.last = before == runs.n - 1;
-        if (before == runs.n - 1) __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.last = before == n_runs - 1;
+        if (before == n_runs - 1) __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (sh.last) paged_merge<HD, kThreads>(a, sh.merge, gi, runs.n, p, tid);
+    if (sh.last) paged_merge<HD, kThreads>(a, sh.merge, gi, n_runs, p, tid);
 }
 
 // The records of a spread launch's groups added up, a workgroup each.
@@ -787,10 +765,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a)
         float w[kPagedHeads][kPagedSplits + 1];
         float4 part[256];
     } sh;
-    const PagedPlace p = paged_place(a, blockIdx.x);
-    if (p.seq < 0) return;
-    const PagedRuns runs = paged_runs(a, (p.rows + paged_tile(HD, Q8) - 1) / paged_tile(HD, Q8));
-    if (runs.n > 1) paged_merge<HD, 256>(a, sh, blockIdx.x, runs.n, p, threadIdx.x);
+    PagedPlace p = paged_place(a, blockIdx.x);
+    p.pos = a.pos[p.seq];
+    paged_rows(a, p);
+    if (p.skip) return;
+    const int n_runs = paged_runs(a, (p.rows + paged_tile(HD, Q8) - 1) / paged_tile(HD, Q8));
+    if (n_runs > 1) paged_merge<HD, 256>(a, sh, blockIdx.x, n_runs, p, threadIdx.x);
 }
 
 }  // namespace leap
