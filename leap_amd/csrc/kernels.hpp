@@ -156,9 +156,9 @@ struct PagedKernels {
     SelectFn select;
 };
 template <int HD>
-PagedKernels pick_paged_hd(bool q8);
-extern template PagedKernels pick_paged_hd<64>(bool);
-extern template PagedKernels pick_paged_hd<128>(bool);
-inline PagedKernels pick_paged(int hd, bool q8) { return hd == 64 ? pick_paged_hd<64>(q8) : pick_paged_hd<128>(q8); }
+PagedKernels pick_paged_hd(int group, bool q8);
+extern template PagedKernels pick_paged_hd<64>(int, bool);
+extern template PagedKernels pick_paged_hd<128>(int, bool);
+inline PagedKernels pick_paged(int hd, int group, bool q8) { return hd == 64 ? pick_paged_hd<64>(group, q8) : pick_paged_hd<128>(group, q8); }
 
 }  // namespace leap_kernels

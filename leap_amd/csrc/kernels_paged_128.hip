@@ -2,5 +2,5 @@
 #include "kernels_paged_table.hpp"
 
 namespace leap_kernels {
-template PagedKernels pick_paged_hd<128>(bool);
+template PagedKernels pick_paged_hd<128>(int, bool);
 }  // namespace leap_kernels

@@ -2,5 +2,5 @@
 #include "kernels_paged_table.hpp"
 
 namespace leap_kernels {
-template PagedKernels pick_paged_hd<64>(bool);
+template PagedKernels pick_paged_hd<64>(int, bool);
 }  // namespace leap_kernels

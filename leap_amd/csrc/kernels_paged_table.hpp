@@ -6,10 +6,10 @@
 
 namespace leap_kernels {
 
-template <int HD, bool Q8>
+template <int HD, int NQ, bool Q8>
 PagedKernels paged_table()
 {
-    return {{leap::paged_attention_kernel<HD, 4, Q8>, leap::paged_attention_kernel<HD, 8, Q8>},
+    return {{leap::paged_attention_kernel<HD, 4, NQ, Q8>, leap::paged_attention_kernel<HD, 8, NQ, Q8>},
             leap::paged_merge_kernel<HD, Q8>,
             leap::page_write_kernel<HD, Q8>,
             leap::page_read_kernel<HD, Q8>,
@@ -17,9 +17,10 @@ PagedKernels paged_table()
             leap::page_select_kernel<HD>};
 }
 template <int HD>
-PagedKernels pick_paged_hd(bool q8)
+PagedKernels pick_paged_hd(int group, bool q8)
 {
-    return q8 ? paged_table<HD, true>() : paged_table<HD, false>();
+    if (q8) return paged_table<HD, 4, true>();
+    return group <= 4 ? paged_table<HD, 1, false>() : group == 8 ? paged_table<HD, 2, false>() : paged_table<HD, 4, false>();
 }
 
 }  // namespace leap_kernels

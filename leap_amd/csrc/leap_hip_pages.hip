@@ -167,7 +167,7 @@ int launch_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *po
     const auto &m = p->cfg.model;
     const int longest = keep ? std::min(max_pos + 1, keep << p->rows_log2) : max_pos + 1;
     const StepPlan s = step_plan(p, n_seq, longest, keep ? (long long)n_seq * longest : total);
-    const PagedKernels fn = pick_paged(m.head_dim, p->q8);
+    const PagedKernels fn = pick_paged(m.head_dim, p->group, p->q8);
     leap::PagedArgs a{};
     a.q = q;
     a.k_new = k;
@@ -245,7 +245,7 @@ int launch_select(leap_hip_attention_pages *p, int layer, int n_seq, const int *
     a.by_units = leap::make_fastdiv((uint32_t)a.units);
     const long long wgs = (groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * a.units;
     if (wgs > 0x7fffffffLL) return set_err(p, -EINVAL, "%lld workgroups in one launch", wgs);
-    HIP_TRY(p, launch_k(pick_paged(m.head_dim, p->q8).select, dim3((unsigned)wgs), dim3(leap::kSelectThreads), stream, a));
+    HIP_TRY(p, launch_k(pick_paged(m.head_dim, p->group, p->q8).select, dim3((unsigned)wgs), dim3(leap::kSelectThreads), stream, a));
     return 0;
 }
 
@@ -350,7 +350,7 @@ int clear_all(leap_hip_attention_pages *p)
     }
     for (int k = 0; k < 5; k++)
         if (p->pool[k]) HIP_TRY(p, hipMemsetAsync(p->pool[k], 0, p->page_bytes[k] * n * p->n_local, p->stream));
-    HIP_TRY(p, hipMemsetAsync(p->counters, 0, kCounters * sizeof(int), p->stream));
+    HIP_TRY(p, hipMemsetAsync(p->counters, 0, kCounters * leap::kCtrStride * sizeof(int), p->stream));
     if (p->select_counters)
         HIP_TRY(p, hipMemsetAsync(p->select_counters, 0, (size_t)p->cfg.model.max_batch * p->cfg.model.n_kv_heads * sizeof(int), p->stream));
     HIP_TRY(p, hipStreamSynchronize(p->stream));
@@ -389,7 +389,7 @@ int launch_rows(leap_hip_attention_pages *p, int seq, int layer, int pos_begin, 
     a.rows_log2 = p->rows_log2;
     a.row0 = pos_begin;
     a.n = n;
-    const PagedKernels fn = pick_paged(p->cfg.model.head_dim, p->q8);
+    const PagedKernels fn = pick_paged(p->cfg.model.head_dim, p->group, p->q8);
     const long long words = (long long)n * p->kv_dim / 4;
     const unsigned grid = (unsigned)std::min<long long>((words + 255) / 256, 16ll * p->n_cu);
     HIP_TRY(p, launch_k(k_in || v_in ? fn.write : fn.read, dim3(grid, 2), dim3(256), stream, a));
@@ -578,7 +578,7 @@ int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, 
     CREATE_TRY(hipStreamCreate(&p->stream));
     if ((rc = leap_host::check_placement(m.device, 2 * p->n_cu, &p->err)) != 0) return fail(rc);
     // the kernels' code (a launch that loads it cannot be captured)
-    for (const void *f : {reinterpret_cast<const void *>(pick_paged(m.head_dim, p->q8).merge),
+    for (const void *f : {reinterpret_cast<const void *>(pick_paged(m.head_dim, p->group, p->q8).merge),
                           reinterpret_cast<const void *>(&leap::reserve_kernel)}) {
         hipFuncAttributes attr;
         CREATE_TRY(hipFuncGetAttributes(&attr, f));
@@ -598,7 +598,7 @@ int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, 
     CREATE_TRY(hipMalloc(&p->n_copies, 2 * sizeof(int)));
     CREATE_TRY(hipMalloc(&p->ws_o, kRecords * m.head_dim * sizeof(float)));
     CREATE_TRY(hipMalloc(&p->ws_lse, kRecords * sizeof(float)));
-    CREATE_TRY(hipMalloc(&p->counters, kCounters * sizeof(int)));
+    CREATE_TRY(hipMalloc(&p->counters, kCounters * leap::kCtrStride * sizeof(int)));
     if (c.bounds) {
         CREATE_TRY(hipMalloc(&p->keys, groups * width * sizeof(uint64_t)));
         CREATE_TRY(hipMalloc(&p->lists, groups * width * sizeof(int)));

@@ -19,19 +19,22 @@
 // (ascending, the new row's page last): the rows are then numbered along the
 // list, and only the last page may be partly filled, as without a list.
 //
-// Products, m = lane % 16, g = lane / 16.  S^T = K Q^T: a lane holds K's row m
-// of a block of 16 and q head m, and gets the scores of positions 4 g + i for
-// head m.  O^T = V^T P^T takes those registers as its B operand as they are:
-// slot (g, i) of its contraction is position 4 g + i.  No score leaves its
-// lane, and a row's maximum and sum need two lane swaps.
-//   fp32: v_mfma_f32_16x16x4_f32, the dims of a load instruction's 64 (K) and
-//     256 (V) bytes of a row in the order in which the lanes get them.
-//   8 bits: v_mfma_i32_16x16x64_i8 on the cache's bytes as they are.  The
-//     other operand, q or the probabilities times the value rows' scales, is
-//     a 30-bit fixed-point number over a power of two just above the largest
-//     of its head row (q) or of its tile (probabilities), as four signed
-//     digits of 8 bits; the four integer sums are exact and are put together
-//     in fp32.  What is lost is 2^-30 of that largest element.
+// Products, m = lane % 16, g = lane / 16.
+//   fp32: v_mfma_f32_4x4x1_16b_f32, 4 q heads (a quad) by 4 rows and blocks of
+//     16: a lane's K is row m of 16, dims 16 f + 4 g.., and after the sum over
+//     the four g it has the score of head g of the quad at position m: every
+//     lane one, whatever the scores' number.  A V load is whole rows, 4 dims a
+//     lane, whose weights of the quad come through LDS.  16x16x4 products,
+//     which have no use for 12 of 16 columns with 4 heads, take four times as
+//     long (eight tiles a CU at once: 1.9 us for 0.5).
+//   8 bits: v_mfma_i32_16x16x64_i8 on the cache's bytes as they are.  S^T = K
+//     Q^T: a lane holds K's row m and q head m, and gets the scores of 4
+//     positions for head m; O^T = V^T P^T takes those registers as its B
+//     operand.  The other operand, q or the probabilities times the value
+//     rows' scales, is a 30-bit fixed-point number over a power of two just
+//     above the largest of its head row (q) or of its tile (probabilities), as
+//     four signed digits of 8 bits; the four integer sums are exact and are put
+//     together in fp32.  What is lost is 2^-30 of that largest element.
 #pragma once
 
 #include "many_attention.hpp"
@@ -60,7 +63,7 @@ struct PagedArgs {
     const int *refs;                 // [page]
     const int *lists;                // [group][keep] pages (keep 0: none, all pages of the table)
     float *ws_o, *ws_lse;            // records: [group][split][q head][HD], [group][split][q head]
-    int *counters;                   // [group], zero between launches
+    int *counters;                   // [group], kCtrStride apart, zero between launches
     int width, keep, n_pages;
     int n_seq, max_pos, n_heads, n_kv_heads, group;
     int rows_log2;                   // R = 1 << rows_log2
@@ -106,17 +109,20 @@ __device__ __forceinline__ void paged_rows(const PagedArgs &a, PagedPlace &p)
 // The runs of a group of so many tiles (run i: tiles [i chunk, (i + 1) chunk)).
 __device__ __forceinline__ int paged_runs(const PagedArgs &a, int tiles) { return (int)fast_div((uint32_t)(tiles + a.chunk - 1), a.by_chunk); }
 
-template <int HD, int W, bool Q8>
+template <int HD, int W, int NQ, bool Q8>
 struct PagedShared {
+    static constexpr int kHeads = Q8 ? kPagedHeads : 4 * NQ;
     union {
         struct {
-            // q as the products take it, a lane's word after the other: float4 of
-            // dims 16 f + 4 g (8 bits: the digits j of dims 64 s + 16 g, [s][j])
-            u32x4 q[HD / 16][kWave];
+            // q as the products take it: fp32 [quad][f] float4 of dims 16 f + 4 g
+            // of head 4 quad + i at 4 g + i; 8 bits [s][j] digits j of dims 64 s +
+            // 16 g of head m at 16 g + m
+            u32x4 q[Q8 ? HD / 16 * kWave : NQ * (HD / 16) * 16];
             alignas(16) float k_new[HD], v_new[HD];  // the new rows (8 bits: of bytes)
             float new_scale[2], q_unit[kPagedHeads];
+            float p[Q8 ? 1 : W][Q8 ? 1 : NQ][32][4];  // fp32: a tile's probabilities, by position and head of a quad
         };
-        float o[W][kPagedHeads][HD + 4];  // the waves' outputs
+        float o[W][kHeads][HD + 4];  // the waves' outputs
         struct {
             float w[kPagedHeads][kPagedSplits + 1];  // the merge: weights of a head's records
             float4 part[W * kWave];                  // and partial sums of them
@@ -126,22 +132,23 @@ struct PagedShared {
     int last;
 };
 
-__device__ __forceinline__ float lanes_max(float x)
+// Over the 16 lanes of a row, and over a wave; the result in every lane.
+__device__ __forceinline__ float row_max(float x)
 {
     x = fmaxf(x, dpp<0x121>(x));
     x = fmaxf(x, dpp<0x122>(x));
     x = fmaxf(x, dpp<0x124>(x));
-    x = fmaxf(x, dpp<0x128>(x));
-    return rows4<true>(x);
+    return fmaxf(x, dpp<0x128>(x));
 }
-__device__ __forceinline__ float lanes_sum(float x)
+__device__ __forceinline__ float row_sum(float x)
 {
     x += dpp<0x121>(x);
     x += dpp<0x122>(x);
     x += dpp<0x124>(x);
-    x += dpp<0x128>(x);
-    return rows4<false>(x);
+    return x + dpp<0x128>(x);
 }
+__device__ __forceinline__ float lanes_max(float x) { return rows4<true>(row_max(x)); }
+__device__ __forceinline__ float lanes_sum(float x) { return rows4<false>(row_sum(x)); }
 
 // The sum of a group's records by T threads: record s of head h counts
 // 2^(lse_s - max lse) / their sum.
@@ -221,10 +228,6 @@ __device__ __forceinline__ i32x4 mfma8(u32x4 a, u32x4 b, i32x4 c)
 {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mfma32(float a, float b, f32x4 c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
 
 // The smaller / larger; NaN if either is.
 __device__ __forceinline__ float4 min4(float4 a, float4 b)
@@ -299,11 +302,11 @@ __device__ __forceinline__ void unroll(F f)
 
 // W waves.  Loads go out before the position is known: a run's tiles, and
 // their pages, do not depend on it.
-template <int HD, int W, bool Q8>
-__global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_kernel(PagedArgs a)
+template <int HD, int W, int NQ, bool Q8>
+__global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2 ? 3 : 2) : 2) void paged_attention_kernel(PagedArgs a)
 {
     constexpr int TK = paged_tile(HD, Q8), NB = TK / 16, LR = HD / 4, VB = HD / 16, kThreads = W * kWave;
-    __shared__ PagedShared<HD, W, Q8> sh;
+    __shared__ PagedShared<HD, W, NQ, Q8> sh;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, g = lane >> 4;
 
@@ -332,8 +335,8 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
     // (always made, on or not, so that the waits for them count exactly: an
     // empty range reads nothing)
     // (blocks behind a sequence's last: page 0 or another's rows, which are masked)
-    constexpr int KF = Q8 ? HD / 64 : HD / 16, VF = HD / 64;
-    float4 kraw[Q8 ? 1 : NB][KF], vraw[Q8 ? 1 : NB][4][VF];  // fp32
+    constexpr int KF = Q8 ? HD / 64 : HD / 16, VR = kWave / LR, VS = 16 / VR;  // (rows of a V load, and loads of a block)
+    float4 kraw[Q8 ? 1 : NB][KF], vraw[Q8 ? 1 : NB][Q8 ? 1 : VS];  // fp32
     u32x4 k8[Q8 ? NB : 1][KF], v8[Q8 ? VB : 1];               // 8 bits
     float ksc = 0.0f, vsc = 0.0f;                             // and the scales of position 16 g + m
     // Its pages, a tile ahead.  fp32: of each block, the same in all lanes.  8
@@ -394,10 +397,7 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
                 const bool ok = on && there(used[b]);
                 const auto r = make_rsrc(static_cast<const float *>(a.v) + row0_of(ok ? used[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int f = 0; f < VF; f++)
-                        vraw[b][i][f] = buf_load4<kNt>(r, (uint32_t)((4 * g + i) * HD + 64 * f + 4 * m) * 4u);
+                for (int v = 0; v < VS; v++) vraw[b][v] = buf_load4<kNt>(r, (uint32_t)(v * VR * HD + 4 * lane) * 4u);
             }
         }
     };
@@ -447,11 +447,12 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
             digits4(digits_of(x.x * up), digits_of(x.y * up), digits_of(x.z * up), digits_of(x.w * up), d);
             // dims 4 c: s = c / 16, g = c / 4 % 4, word c % 4
 #pragma unroll
-            for (int j = 0; j < 4; j++) reinterpret_cast<unsigned *>(&sh.q[4 * (c >> 4) + j][16 * ((c >> 2) & 3) + job])[c & 3] = d[j];
+            for (int j = 0; j < 4; j++) reinterpret_cast<unsigned *>(&sh.q[(4 * (c >> 4) + j) * kWave + 16 * ((c >> 2) & 3) + job])[c & 3] = d[j];
             if (c == 0) sh.q_unit[job] = good ? exp2_int(e - 29) * a.scale_log2 : __uint_as_float(0x7fc00000u);
         } else {
             // dims 4 c: f = c / 4, g = c % 4
-            sh.q[c >> 2][16 * (c & 3) + job] = u32x4{__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
+            if (job < 4 * NQ)
+                sh.q[((job >> 2) * (HD / 16) + (c >> 2)) * 16 + 4 * (c & 3) + (job & 3)] = u32x4{__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
         }
     }
     if (newest_run && wave == W - 1) {
@@ -509,28 +510,23 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
         }
     }
 
-    f32x4 o[VB];
+    // fp32: o[4 quad + e] has dims 4 (lane % LR) + e of the quad's heads, over
+    // the rows lane / LR of each V load; a lane's sums are of head 4 quad + g.
+    // 8 bits: o[v] has dims 16 v + 4 g + i of head m, and the sums are of head m.
+    constexpr int kAcc = Q8 ? VB : 4 * NQ, kSums = Q8 ? 1 : NQ;
+    f32x4 o[kAcc];
 #pragma unroll
-    for (int v = 0; v < VB; v++) o[v] = f32x4{0, 0, 0, 0};
-    float mrun = kNothing, lrun = 0.0f;
-    // The scores' maximum mt of a tile: the reference moved, and what was summed with it.
-    auto follow = [&](float mt) {
-        if (__builtin_amdgcn_ballot_w64(mt > mrun + kPagedMargin) != 0) {
-            mt = rows4<true>(mt);
-            const float now = mt > mrun + kPagedMargin ? mt : mrun, f = fast_exp2(mrun - now);
-            mrun = now;
-            lrun *= f;
+    for (int v = 0; v < kAcc; v++) o[v] = f32x4{0, 0, 0, 0};
+    float mrun[kSums], lrun[kSums];
 #pragma unroll
-            for (int v = 0; v < VB; v++) o[v] *= f;
-        }
-        return mrun + kPagedBias;
-    };
+    for (int k = 0; k < kSums; k++) {
+        mrun[k] = kNothing;
+        lrun[k] = 0.0f;
+    }
     for (; t < t1; t += W) {
         const bool last = t == tiles - 1, next = t + W < t1;
         int zero = 0;
         asm volatile("" : "+v"(zero));  // (q is read from LDS for each tile: kept, it would take a quarter of the registers)
-        const u32x4 *qs = &sh.q[0][lane + zero];
-        float x[NB][4], mt = -__builtin_inff();
         if constexpr (!Q8) {
 #pragma unroll
             for (int b = 0; b < NB; b++) bad |= t * NB + b < n_blocks && !there(used[b]);
@@ -542,70 +538,90 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
                         for (int f = 0; f < KF; f++) kraw[b][f] = *reinterpret_cast<const float4 *>(&sh.k_new[16 * f + 4 * g]);
             }
             // ---- scores ----
-            f32x4 s[NB], s2[NB];
+            const u32x4 *qs = &sh.q[4 * g + (m & 3) + zero];
+            float x[NQ][NB];  // of head 4 quad + g at position 16 b + m
+            f32x4 s[NQ][NB][2];
 #pragma unroll
-            for (int b = 0; b < NB; b++) s[b] = s2[b] = f32x4{0, 0, 0, 0};
+            for (int k = 0; k < NQ; k++)
 #pragma unroll
-            for (int f = 0; f < KF; f++) {
-                const f32x4 q = __builtin_bit_cast(f32x4, qs[f * kWave]);
+                for (int b = 0; b < NB; b++) s[k][b][0] = s[k][b][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    s[b] = mfma32(kraw[b][f].x, q.x, s[b]);
-                    s2[b] = mfma32(kraw[b][f].y, q.y, s2[b]);
-                    s[b] = mfma32(kraw[b][f].z, q.z, s[b]);
-                    s2[b] = mfma32(kraw[b][f].w, q.w, s2[b]);
+            for (int f = 0; f < KF; f++)
+#pragma unroll
+                for (int k = 0; k < NQ; k++) {
+                    const f32x4 q = __builtin_bit_cast(f32x4, qs[(k * KF + f) * 16]);
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        s[k][b][0] = __builtin_amdgcn_mfma_f32_4x4x1f32(q.x, kraw[b][f].x, s[k][b][0], 0, 0, 0);
+                        s[k][b][1] = __builtin_amdgcn_mfma_f32_4x4x1f32(q.y, kraw[b][f].y, s[k][b][1], 0, 0, 0);
+                        s[k][b][0] = __builtin_amdgcn_mfma_f32_4x4x1f32(q.z, kraw[b][f].z, s[k][b][0], 0, 0, 0);
+                        s[k][b][1] = __builtin_amdgcn_mfma_f32_4x4x1f32(q.w, kraw[b][f].w, s[k][b][1], 0, 0, 0);
+                    }
                 }
-            }
             load_k(t + W, next);
             // ---- softmax ----
+            float up = -__builtin_inff();
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int k = 0; k < NQ; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[b][i] = (s[b][i] + s2[b][i]) * qf;
-            if (last) {
+                for (int b = 0; b < NB; b++) {
+                    const f32x4 y = s[k][b][0] + s[k][b][1];
+                    x[k][b] = halves_sum2(rows_sum2(y[0], y[1]), rows_sum2(y[2], y[3])) * a.scale_log2;
+                    if (last && 16 * b + m > new_row) x[k][b] = -__builtin_inff();
+                    up = fmaxf(up, x[k][b] - mrun[k]);
+                }
+            if (__builtin_amdgcn_ballot_w64(up > kPagedMargin) != 0) {
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                for (int k = 0; k < NQ; k++) {
+                    float mt = x[k][0];
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (16 * b + 4 * g + i > new_row) x[b][i] = -__builtin_inff();
+                    for (int b = 1; b < NB; b++) mt = fmaxf(mt, x[k][b]);
+                    mt = row_max(mt);
+                    const float now = mt > mrun[k] + kPagedMargin ? mt : mrun[k], f = fast_exp2(mrun[k] - now);
+                    mrun[k] = now;
+                    lrun[k] *= f;
+                    const f32x4 by = {lane_value(f, 0), lane_value(f, 16), lane_value(f, 32), lane_value(f, 48)};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[4 * k + e] *= by;
+                }
             }
 #pragma unroll
-            for (int b = 0; b < NB; b++) mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
-            const float off = follow(mt);
+            for (int k = 0; k < NQ; k++)
 #pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[b][i] = fast_exp2(x[b][i] - off);
-                    lrun += x[b][i];
+                for (int b = 0; b < NB; b++) {
+                    x[k][b] = fast_exp2(x[k][b] - (mrun[k] + kPagedBias));
+                    lrun[k] += x[k][b];
+                    sh.p[wave][k][16 * b + m][g] = x[k][b];
                 }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             if (last) {
                 // the new value, and zeros behind it
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = 16 * b + 4 * g + i;
+                    for (int v = 0; v < VS; v++) {
+                        const int r = 16 * b + VR * v + lane / LR;
                         if (r >= new_row)
-#pragma unroll
-                            for (int f = 0; f < VF; f++)
-                                vraw[b][i][f] = r == new_row ? *reinterpret_cast<const float4 *>(&sh.v_new[64 * f + 4 * m])
-                                                             : make_float4(0, 0, 0, 0);
+                            vraw[b][v] = r == new_row ? *reinterpret_cast<const float4 *>(&sh.v_new[4 * (lane & (LR - 1))])
+                                                      : make_float4(0, 0, 0, 0);
                     }
             }
             // ---- weighted values ----
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int k = 0; k < NQ; k++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int f = 0; f < VF; f++) {
-                        o[4 * f] = mfma32(vraw[b][i][f].x, x[b][i], o[4 * f]);
-                        o[4 * f + 1] = mfma32(vraw[b][i][f].y, x[b][i], o[4 * f + 1]);
-                        o[4 * f + 2] = mfma32(vraw[b][i][f].z, x[b][i], o[4 * f + 2]);
-                        o[4 * f + 3] = mfma32(vraw[b][i][f].w, x[b][i], o[4 * f + 3]);
+                    for (int v = 0; v < VS; v++) {
+                        const float w = sh.p[wave][k][16 * b + VR * v + lane / LR][lane & 3];
+                        o[4 * k] = __builtin_amdgcn_mfma_f32_4x4x1f32(w, vraw[b][v].x, o[4 * k], 0, 0, 0);
+                        o[4 * k + 1] = __builtin_amdgcn_mfma_f32_4x4x1f32(w, vraw[b][v].y, o[4 * k + 1], 0, 0, 0);
+                        o[4 * k + 2] = __builtin_amdgcn_mfma_f32_4x4x1f32(w, vraw[b][v].z, o[4 * k + 2], 0, 0, 0);
+                        o[4 * k + 3] = __builtin_amdgcn_mfma_f32_4x4x1f32(w, vraw[b][v].w, o[4 * k + 3], 0, 0, 0);
                     }
         } else {
+            const u32x4 *qs = &sh.q[lane + zero];
+            float x[NB][4], mt = -__builtin_inff();
             bad |= 4 * t + g < n_blocks && !there(used[0]);
             if (last) {
 #pragma unroll
@@ -657,11 +673,19 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
             // ---- softmax ----
 #pragma unroll
             for (int b = 0; b < NB; b++) mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
-            const float off = follow(mt), vs = fmaxf(vsc, 0.0f);
+            if (__builtin_amdgcn_ballot_w64(mt > mrun[0] + kPagedMargin) != 0) {
+                mt = rows4<true>(mt);
+                const float now = mt > mrun[0] + kPagedMargin ? mt : mrun[0], f = fast_exp2(mrun[0] - now);
+                mrun[0] = now;
+                lrun[0] *= f;
+#pragma unroll
+                for (int v = 0; v < VB; v++) o[v] *= f;
+            }
+            const float off = mrun[0] + kPagedBias, vs = fmaxf(vsc, 0.0f);
             float wt = 0.0f;
             unroll<0, 16>([&](auto j) {
                 const float y = fast_exp2(x[j / 4][j % 4] - off);
-                lrun += y;
+                lrun[0] += y;
                 x[j / 4][j % 4] = y * row_lane<j>(vs);
                 wt = fmaxf(wt, x[j / 4][j % 4]);
             });
@@ -693,27 +717,35 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
     }
 
     // ---- the waves' results together ----
-    lrun = rows4<false>(lrun);
     __syncthreads();  // (q is read; its memory takes the outputs)
-    if (__builtin_amdgcn_ballot_w64(bad) != 0) lrun = __uint_as_float(0x7fc00000u);
-    if (g == 0) {
-        sh.m[wave][m] = mrun;
-        sh.l[wave][m] = lrun;
-    }
-    // register i of block v: dim (8 bits) 16 v + 4 g + i, or 64 (v / 4) + 16 g + 4 i + v % 4
-    if (m < a.group) {
-        if constexpr (Q8) {
+    const bool missing = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if constexpr (Q8) {
+        const float l = rows4<false>(lrun[0]);
+        if (g == 0) {
+            sh.m[wave][m] = mrun[0];
+            sh.l[wave][m] = missing ? __uint_as_float(0x7fc00000u) : l;
+        }
+        if (m < a.group)
 #pragma unroll
             for (int v = 0; v < VB; v++)
                 *reinterpret_cast<float4 *>(&sh.o[wave][m][16 * v + 4 * g]) = make_float4(o[v][0], o[v][1], o[v][2], o[v][3]);
-        } else {
+    } else {
 #pragma unroll
-            for (int v = 0; v < VB; v += 4)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<float4 *>(&sh.o[wave][m][16 * v + 16 * g + 4 * i]) =
-                        make_float4(o[v][i], o[v + 1][i], o[v + 2][i], o[v + 3][i]);
+        for (int k = 0; k < NQ; k++) {
+            const float l = row_sum(lrun[k]);
+            if (m == 0) {
+                sh.m[wave][4 * k + g] = mrun[k];
+                sh.l[wave][4 * k + g] = missing ? __uint_as_float(0x7fc00000u) : l;
+            }
         }
+        f32x4 acc[NQ][4];
+#pragma unroll
+        for (int k = 0; k < NQ; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[k][e] = o[4 * k + e];
+        slot_sums<HD, 4 * NQ>(acc, lane, [&](int, int head, float4 y) {
+            *reinterpret_cast<float4 *>(&sh.o[wave][head][4 * (lane & (LR - 1))]) = y;
+        });
     }
     __syncthreads();
     const size_t rec = ((size_t)gi * a.splits + split) * a.group;
@@ -749,9 +781,9 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? 3 : 2) void paged_attention_ker
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
-        const int before = __hip_atomic_fetch_add(a.counters + gi, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int before = __hip_atomic_fetch_add(a.counters + (size_t)gi * kCtrStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         sh.last = before == n_runs - 1;
-        if (before == n_runs - 1) __hip_atomic_store(a.counters + gi, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == n_runs - 1) __hip_atomic_store(a.counters + (size_t)gi * kCtrStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (sh.last) paged_merge<HD, kThreads>(a, sh.merge, gi, n_runs, p, tid);
