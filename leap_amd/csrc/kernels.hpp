@@ -145,13 +145,13 @@ inline RowsKernels pick_rows(int hd) { return hd == 64 ? pick_rows_hd<64>() : pi
 using KeepFn = void (*)(leap::KeepArgs);
 KeepFn pick_keep(bool q8);
 
-// Caches of pages: the step over them by workgroups of 4 and 8 waves, the sum
+// Caches of pages: the step over them in uniform and in flat launches, the sum
 // of a spread launch's records, rows in and out, and the choice of pages.
 using PagedFn = void (*)(leap::PagedArgs);
 using PageRowsFn = void (*)(leap::PageRowsArgs);
 using SelectFn = void (*)(leap::SelectArgs);
 struct PagedKernels {
-    PagedFn attention[2], merge;
+    PagedFn attention, flat, merge;
     PageRowsFn write, read, bounds;
     SelectFn select;
 };

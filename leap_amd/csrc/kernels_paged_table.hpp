@@ -9,7 +9,8 @@ namespace leap_kernels {
 template <int HD, int NQ, bool Q8>
 PagedKernels paged_table()
 {
-    return {{leap::paged_attention_kernel<HD, 4, NQ, Q8>, leap::paged_attention_kernel<HD, 8, NQ, Q8>},
+    return {leap::paged_attention_kernel<HD, NQ, Q8>,
+            leap::paged_flat_kernel<HD, NQ, Q8>,
             leap::paged_merge_kernel<HD, Q8>,
             leap::page_write_kernel<HD, Q8>,
             leap::page_read_kernel<HD, Q8>,

@@ -95,6 +95,7 @@ constexpr size_t kStagingBytes = size_t(8) << 20;
 // than XCDs.
 constexpr long long kSpreadBytes = 4ll << 20;
 
+long long round_up(long long x, int q) { return (x + q - 1) / q * q; }
 bool aligned(const void *p, unsigned by) { return reinterpret_cast<uintptr_t>(p) % by == 0; }
 
 int check_layer(leap_hip_attention_pages *p, int layer)
@@ -131,32 +132,65 @@ int staging(leap_hip_attention_pages *p, size_t bytes)
 // ---- the step ------------------------------------------------------------------
 
 struct StepPlan {
-    int waves, chunk, splits, spread;
+    int chunk, splits;
+    bool spread, flat;
     long long wgs;
 };
 // total: rows of all sequences; longest: of one, both along what is attended to.
+//
+// Uniform launches cut every group into runs of the same length.  Their time,
+// past a constant, is near the larger of what memory and a run take, and the
+// merge: a tile of a wave takes 1.65 us (8 bits 2.4) from its loads to its
+// products, four waves at a time, tiles come in at 6.8 TB/s over the card (8
+// bits: an eighth slower with one workgroup a CU; fp32 a tenth over long runs
+// of one sequence), 1 us of them within the constant, and records take 2 us
+// and 0.03 for each.  (us, 32/8/128 in fp32,
+// the chosen number of runs and its neighbours; 512 rows 4: 8.4, 8: 6.8; 4096
+// 16: 13.6, 22: 12.3, 32: 11.2, 64: 13.0; 16384 32: 26.9, 64: 27.8; 8 bits at
+// 16384 22: 17.8, 32: 15.3, 64: 16.7, at 131072 32: 61.8, 64: 58.5.)
+// Batches of unequal lengths, or whose groups and runs do not divide over the
+// CUs, run flat once they have 16 tiles a CU (uniform : flat; 32/8/128 fp32, 8
+// sequences of up to 500 9.8 : 11.3, 16 of up to 1000 22.5 : 21.0, 32 of up to
+// 7300 180 : 163, 64/8/128 16 of up to 7300 124 : 108; 8 bits, 32 of up to
+// 8192 73 : 68).  Two workgroups a CU: 8 bits need both (one: 84), fp32 takes
+// as long with one.
 StepPlan step_plan(const leap_hip_attention_pages *p, int n_seq, int longest, long long total)
 {
     const int n_kv = p->cfg.model.n_kv_heads, hd = p->cfg.model.head_dim, tk = leap::paged_tile(hd, p->q8);
-    const long long groups = (long long)n_seq * n_kv;
+    const long long groups = (long long)n_seq * n_kv, items = (groups + leap::kXcds - 1) / leap::kXcds;
     const long long mean = (total + n_seq - 1) / n_seq;
     const long long tiles_mean = (mean + tk - 1) / tk, tiles_max = (longest + tk - 1) / tk;
     const long long group_bytes = mean * (p->q8 ? 2ll * (hd + 4) : 8ll * hd);
+    const bool few = groups < leap::kXcds && group_bytes < kSpreadBytes;  // on as many XCDs as groups
+    const double cus = few ? p->n_cu * groups / (double)leap::kXcds : p->n_cu;
+    const double tile_us = (p->q8 ? hd / 128.0 : 1.0) * 0.0024, run_us = p->q8 ? 2.4 : 1.65;
     StepPlan s{};
-    const bool few = groups < leap::kXcds && group_bytes < kSpreadBytes;
-    const long long cus = few ? p->n_cu * groups / leap::kXcds : p->n_cu;
-    s.waves = groups * ((tiles_max + 7) / 8) <= 2 * cus ? 8 : 4;
-    const long long want = std::max<long long>(1, cus * (s.waves == 8 ? 1 : 4) / groups);
-    long long chunk = std::max<long long>(s.waves, (tiles_mean + want - 1) / want);
-    chunk = std::max(chunk, (tiles_max + leap::kPagedSplits - 1) / leap::kPagedSplits);
-    s.splits = (int)((tiles_max + chunk - 1) / chunk);
-    while (s.splits > 1 && ((size_t)groups * s.splits * p->group > kRecords || (size_t)groups > kCounters)) {
-        chunk *= 2;
-        s.splits = (int)((tiles_max + chunk - 1) / chunk);
+    double best = 0;
+    for (int n = 1; n <= leap::kPagedSplits && n <= tiles_max; n++) {
+        // (a tile for every wave, or as many)
+        const long long chunk = n == 1 ? tiles_max : round_up((tiles_max + n - 1) / n, leap::kPagedWaves);
+        if (n > 1 && (chunk == s.chunk || (size_t)groups * n * p->group > kRecords || (size_t)groups > kCounters)) continue;
+        const double wgs = groups * std::ceil((double)tiles_mean / chunk);
+        const double rate = wgs < cus ? 0.9 : wgs > cus ? 1.0 : p->q8 ? 1.125 : 1.03;
+        const double memory = std::ceil(wgs / cus) * chunk * tile_us * p->n_cu * rate - 1.0;
+        const double run = std::ceil(chunk / (double)leap::kPagedWaves) * run_us;
+        const double us = std::max(memory, run) + (n > 1 ? 2.0 + 0.03 * n : 0.0);
+        if (n == 1 || us < best) {
+            best = us;
+            s.chunk = (int)chunk;
+            s.splits = (int)((tiles_max + chunk - 1) / chunk);
+        }
     }
-    s.chunk = (int)chunk;
+    const long long flat_wgs = 2ll * p->n_cu;
+    const double tiles = (double)groups * tiles_mean / p->n_cu;
+    if (n_seq > 1 && tiles >= 16 && items <= leap::kWave && (size_t)(leap::kXcds * items + flat_wgs) * p->group <= kRecords &&
+        (size_t)groups <= kCounters && flat_wgs <= (long long)leap::kXcds * leap::kPagedSplits) {
+        const bool equal = total == (long long)n_seq * longest;
+        const double us = (tiles + leap::kPagedStart * (2.0 + (double)groups / p->n_cu)) * p->n_cu * tile_us + 3.0;
+        if (!equal || us < best) return StepPlan{1, (int)items, false, true, flat_wgs};
+    }
     s.spread = s.splits > 1 && groups < leap::kXcds && !few;
-    s.wgs = s.spread ? groups * s.splits : (groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * s.splits;
+    s.wgs = s.spread ? groups * s.splits : items * leap::kXcds * s.splits;
     return s;
 }
 
@@ -205,8 +239,9 @@ int launch_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *po
     a.by_kv_heads = leap::make_fastdiv((uint32_t)m.n_kv_heads);
     a.by_splits = leap::make_fastdiv((uint32_t)s.splits);
     a.by_chunk = leap::make_fastdiv((uint32_t)s.chunk);
+    a.by_groups = leap::make_fastdiv((uint32_t)(n_seq * m.n_kv_heads));
     if (s.wgs > 0x7fffffffLL) return set_err(p, -EINVAL, "%lld workgroups in one launch", s.wgs);
-    HIP_TRY(p, launch_k(fn.attention[s.waves == 8], dim3((unsigned)s.wgs), dim3((unsigned)(s.waves * leap::kWave)), stream, a));
+    HIP_TRY(p, launch_k(s.flat ? fn.flat : fn.attention, dim3((unsigned)s.wgs), dim3(leap::kPagedWaves * leap::kWave), stream, a));
     if (s.spread) HIP_TRY(p, launch_k(fn.merge, dim3((unsigned)(n_seq * m.n_kv_heads)), dim3(256), stream, a));
     return 0;
 }

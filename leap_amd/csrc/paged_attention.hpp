@@ -43,6 +43,7 @@ namespace leap {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kPagedWaves = 4;       // waves of a workgroup
 constexpr int kPagedSplits = 64;     // runs of a group, at most: a lane each in the merge
 constexpr int kPagedHeads = 16;      // q heads of a KV head, at most
 // Probabilities are 2^(score - reference - kPagedBias), and the reference
@@ -67,11 +68,11 @@ struct PagedArgs {
     int width, keep, n_pages;
     int n_seq, max_pos, n_heads, n_kv_heads, group;
     int rows_log2;                   // R = 1 << rows_log2
-    int chunk, splits;               // tiles of a run, runs of the longest group
+    int chunk, splits;               // tiles of a run, runs of the longest group (flat: most groups of an XCD)
     int blocks;                      // blocks of 16 rows of the longest group
     int spread;                      // a group's runs lie on all XCDs, and paged_merge_kernel adds up their records
     float scale_log2;
-    FastDiv by_kv_heads, by_splits, by_chunk;
+    FastDiv by_kv_heads, by_splits, by_chunk, by_groups;
 };
 
 // A word that the kernel does not write, at an address that is the same in all
@@ -106,11 +107,18 @@ __device__ __forceinline__ void paged_rows(const PagedArgs &a, PagedPlace &p)
     p.rows = ((p.n_list - 1) << a.rows_log2) + (p.pos & ((1 << a.rows_log2) - 1)) + 1;
     p.skip = p.pos < 0 || p.pos > a.max_pos;
 }
+// NaN into a skipped sequence's output row, by `step` threads.
+template <int HD>
+__device__ __forceinline__ void paged_skip(const PagedArgs &a, const PagedPlace &p, int i0, int step = kPagedWaves * kWave)
+{
+    fill_nan<HD>(a.out, ((size_t)p.seq * a.n_heads + p.kvh * a.group) * (HD / 4), a.group * (HD / 4), i0, step);
+}
 // The runs of a group of so many tiles (run i: tiles [i chunk, (i + 1) chunk)).
 __device__ __forceinline__ int paged_runs(const PagedArgs &a, int tiles) { return (int)fast_div((uint32_t)(tiles + a.chunk - 1), a.by_chunk); }
 
-template <int HD, int W, int NQ, bool Q8>
+template <int HD, int NQ, bool Q8>
 struct PagedShared {
+    static constexpr int W = kPagedWaves;
     static constexpr int kHeads = Q8 ? kPagedHeads : 4 * NQ;
     union {
         struct {
@@ -153,11 +161,11 @@ __device__ __forceinline__ float lanes_sum(float x) { return rows4<false>(row_su
 // The sum of a group's records by T threads: record s of head h counts
 // 2^(lse_s - max lse) / their sum.
 template <int HD, int T, typename Merge>
-__device__ __forceinline__ void paged_merge(const PagedArgs &a, Merge &sh, int gi, int n_split, const PagedPlace &p, int tid)
+__device__ __forceinline__ void paged_merge(const PagedArgs &a, Merge &sh, size_t first, int n_split, const PagedPlace &p, int tid)
 {
     constexpr int LR = HD / 4;
     const int lane = tid & (kWave - 1), items = a.group * LR;
-    const size_t rec0 = (size_t)gi * a.splits * a.group;
+    const size_t rec0 = first * a.group;
     int parts = 1;
     while (2 * parts * items <= T) parts *= 2;
     const int part = parts > 1 ? tid / items : 0;
@@ -300,35 +308,28 @@ __device__ __forceinline__ void unroll(F f)
     }
 }
 
-// W waves.  Loads go out before the position is known: a run's tiles, and
-// their pages, do not depend on it.
-template <int HD, int W, int NQ, bool Q8>
-__global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2 ? 3 : 2) : 2) void paged_attention_kernel(PagedArgs a)
+// A run of a group's tiles: [t0, t1) of group gi, run `run` of n, whose
+// records start at rec0.  FLAT: all known; else t0 is, and t1 and n follow from
+// the position.
+struct PagedRun {
+    int gi, t0, t1, run, n;
+    size_t rec0;
+};
+// Loads go out before the position is known where that is possible: a run's
+// pages do not depend on it.
+template <int HD, int NQ, bool Q8, bool FLAT>
+__device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ, Q8> &sh, const PagedRun &r, int pos)
 {
-    constexpr int TK = paged_tile(HD, Q8), NB = TK / 16, LR = HD / 4, VB = HD / 16, kThreads = W * kWave;
-    __shared__ PagedShared<HD, W, NQ, Q8> sh;
+    constexpr int TK = paged_tile(HD, Q8), NB = TK / 16, LR = HD / 4, VB = HD / 16, W = kPagedWaves, kThreads = W * kWave;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int m = lane & 15, g = lane >> 4;
-
-    // the group and its run: a group's runs on one XCD, or (spread) on all
-    const int n_groups = a.n_seq * a.n_kv_heads;
-    int gi, split;
-    if (a.spread) {
-        split = blockIdx.x / n_groups;
-        gi = blockIdx.x - split * n_groups;
-    } else {
-        const int local = blockIdx.x / kXcds, gl = (int)fast_div((uint32_t)local, a.by_splits);
-        split = local - gl * a.splits;
-        gi = gl * kXcds + (blockIdx.x & (kXcds - 1));
-    }
-    if (gi >= n_groups) return;
-    PagedPlace p = paged_place(a, gi);
+    PagedPlace p = paged_place(a, r.gi);
     const int blocks_log2 = a.rows_log2 - 4;  // blocks of 16 rows of a page
     auto row0_of = [&](int page, int block) {  // a block's first row among the KV heads' rows of the layer
         return (((size_t)page * a.n_kv_heads + p.kvh) << a.rows_log2) + ((block & ((1 << blocks_log2) - 1)) << 4);
     };
     auto there = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
-    const int t0 = split * a.chunk;
+    const int t0 = r.t0;
     int t = t0 + wave;
 
     // ---- a tile's loads ----
@@ -380,9 +381,9 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
             for (int b = 0; b < NB; b++) {
                 used[b] = pages[b];
                 const bool ok = on && there(pages[b]);
-                const auto r = make_rsrc(static_cast<const float *>(a.k) + row0_of(ok ? pages[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
+                const auto rows = make_rsrc(static_cast<const float *>(a.k) + row0_of(ok ? pages[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
 #pragma unroll
-                for (int f = 0; f < KF; f++) kraw[b][f] = buf_load4<kNt>(r, (uint32_t)(m * HD + 16 * f + 4 * g) * 4u);
+                for (int f = 0; f < KF; f++) kraw[b][f] = buf_load4<kNt>(rows, (uint32_t)(m * HD + 16 * f + 4 * g) * 4u);
             }
         }
     };
@@ -395,48 +396,53 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const bool ok = on && there(used[b]);
-                const auto r = make_rsrc(static_cast<const float *>(a.v) + row0_of(ok ? used[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
+                const auto rows = make_rsrc(static_cast<const float *>(a.v) + row0_of(ok ? used[b] : 0, at * NB + b) * HD, ok ? 64u * HD : 0u);
 #pragma unroll
-                for (int v = 0; v < VS; v++) vraw[b][v] = buf_load4<kNt>(r, (uint32_t)(v * VR * HD + 4 * lane) * 4u);
+                for (int v = 0; v < VS; v++) vraw[b][v] = buf_load4<kNt>(rows, (uint32_t)(v * VR * HD + 4 * lane) * 4u);
             }
         }
     };
     // ---- rows of q, and the new token's ----
-    // LR threads a row; a head that a group of fewer than 16 leaves out is
-    // zero.  These loads, the position's and the first pages' go out together.
-    const int c = tid & (LR - 1);
-    constexpr int kJobs = kThreads / LR, kRows = (kPagedHeads + kJobs - 1) / kJobs;
+    // LR lanes a row, by the first waves alone: a CU's loads come back in the
+    // order in which its waves made them, and everyone waits for q.  These
+    // loads, the position's and the first pages' go out together.  (A head
+    // that the group leaves out is zero.)
+    const int c = lane & (LR - 1);
+    constexpr int kPer = kWave / LR, kHeads = Q8 ? kPagedHeads : 4 * NQ;       // rows of a wave at a time, and of q
+    constexpr int kRows = (kHeads + W * kPer - 1) / (W * kPer);
+    constexpr int kRowWaves = (kHeads + kRows * kPer - 1) / (kRows * kPer);    // waves that have some
+    static_assert(kHeads % (kRows * kPer) == 0 || kRowWaves == 1, "rows of q");
+    const int head0 = wave * kRows * kPer + lane / LR;
     const size_t new_at = ((size_t)p.seq * a.n_kv_heads + p.kvh) * LR;
+    const bool has_rows = wave < kRowWaves && wave * kRows * kPer < a.group;
+    if (has_rows) __builtin_amdgcn_s_setprio(3);
     float4 row[kRows];
-    const auto q_rows = make_rsrc(a.q + ((size_t)p.seq * a.n_heads + p.kvh * a.group) * HD, (uint32_t)(a.group * HD) * 4u);
+    const auto q_rows = make_rsrc(a.q + ((size_t)p.seq * a.n_heads + p.kvh * a.group) * HD, has_rows ? (uint32_t)(a.group * HD) * 4u : 0u);
 #pragma unroll
-    for (int u = 0; u < kRows; u++) row[u] = buf_load4(q_rows, (uint32_t)((tid / LR + u * kJobs) * LR + c) * 16u);
-    const float4 k_row = reinterpret_cast<const float4 *>(a.k_new)[new_at + c];
-    const float4 v_row = reinterpret_cast<const float4 *>(a.v_new)[new_at + c];
+    for (int u = 0; u < kRows; u++) row[u] = buf_load4(q_rows, (uint32_t)((head0 + u * kPer) * LR + c) * 16u);
+    const uint32_t new_bytes = wave == 0 ? HD * 4u : 0u;
+    const float4 k_row = buf_load4(make_rsrc(a.k_new + new_at * 4, new_bytes), c * 16u);
+    const float4 v_row = buf_load4(make_rsrc(a.v_new + new_at * 4, new_bytes), c * 16u);
     look(t);
-    p.pos = uniform_load(a.pos + p.seq);
+    p.pos = FLAT ? pos : uniform_load(a.pos + p.seq);
     if constexpr (!Q8) asm volatile("" ::"s"(p.pos), "s"(pages[0]), "s"(pages[NB - 1]));  // (one wait for them all)
     __builtin_amdgcn_sched_barrier(0);
     paged_rows(a, p);
-    if (p.skip) {
-        if (split == 0) fill_nan<HD>(a.out, ((size_t)p.seq * a.n_heads + p.kvh * a.group) * LR, a.group * LR, tid, kThreads);
+    if (!FLAT && p.skip) {
+        if (r.run == 0) paged_skip<HD>(a, p, tid);
         return;
     }
     const int tiles = (p.rows + TK - 1) / TK;
-    if (t0 >= tiles) return;
-    const int t1 = min(t0 + a.chunk, tiles), n_runs = paged_runs(a, tiles), n_blocks = (p.rows + 15) >> 4;
+    if (!FLAT && t0 >= tiles) return;
+    const int t1 = FLAT ? r.t1 : min(t0 + a.chunk, tiles), n_runs = FLAT ? r.n : paged_runs(a, tiles), n_blocks = (p.rows + 15) >> 4;
     const bool newest_run = t1 == tiles;
-    const float4 turn = a.rope[(size_t)p.pos * LR + c];
+    const float4 turn = buf_load4(make_rsrc(a.rope + (size_t)p.pos * LR, has_rows ? HD * 4u : 0u), c * 16u);
     __builtin_amdgcn_sched_barrier(0);
     load_k(t, t < t1);
     load_v(t, t < t1);
     look(t + W);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int u = 0; u < kRows; u++) {
-        const int job = tid / LR + u * kJobs;
-        if (kPagedHeads % kJobs && job >= kPagedHeads) break;
-        const float4 x = rope4(row[u], turn);
+    auto put_row = [&](int job, float4 x) {
         if constexpr (Q8) {
             unsigned top = dpp_max16(max4_bits(0u, x));
             if constexpr (HD == 128) top = max(top, (unsigned)__shfl_xor((int)top, 16));
@@ -451,11 +457,17 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
             if (c == 0) sh.q_unit[job] = good ? exp2_int(e - 29) * a.scale_log2 : __uint_as_float(0x7fc00000u);
         } else {
             // dims 4 c: f = c / 4, g = c % 4
-            if (job < 4 * NQ)
-                sh.q[((job >> 2) * (HD / 16) + (c >> 2)) * 16 + 4 * (c & 3) + (job & 3)] = u32x4{__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
+            sh.q[((job >> 2) * (HD / 16) + (c >> 2)) * 16 + 4 * (c & 3) + (job & 3)] = u32x4{__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
         }
+    };
+    if (has_rows) {
+#pragma unroll
+        for (int u = 0; u < kRows; u++) put_row(head0 + u * kPer, rope4(row[u], turn));
+    } else if (wave < kRowWaves) {
+#pragma unroll
+        for (int u = 0; u < kRows; u++) put_row(head0 + u * kPer, make_float4(0, 0, 0, 0));
     }
-    if (newest_run && wave == W - 1) {
+    if (newest_run && wave == 0) {
         const float4 x[2] = {rope4(k_row, turn), v_row};
 #pragma unroll
         for (int value = 0; value < 2; value++) {
@@ -470,6 +482,7 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
             }
         }
     }
+    if (has_rows) __builtin_amdgcn_s_setprio(0);
     __syncthreads();
     const float qf = Q8 ? sh.q_unit[m] : a.scale_log2;
 
@@ -600,9 +613,9 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int v = 0; v < VS; v++) {
-                        const int r = 16 * b + VR * v + lane / LR;
-                        if (r >= new_row)
-                            vraw[b][v] = r == new_row ? *reinterpret_cast<const float4 *>(&sh.v_new[4 * (lane & (LR - 1))])
+                        const int row = 16 * b + VR * v + lane / LR;
+                        if (row >= new_row)
+                            vraw[b][v] = row == new_row ? *reinterpret_cast<const float4 *>(&sh.v_new[4 * (lane & (LR - 1))])
                                                       : make_float4(0, 0, 0, 0);
                     }
             }
@@ -748,7 +761,7 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
         });
     }
     __syncthreads();
-    const size_t rec = ((size_t)gi * a.splits + split) * a.group;
+    const size_t rec = (r.rec0 + r.run) * a.group;
     for (int i = tid; i < a.group * LR; i += kThreads) {
         const int head = i / LR, d = (i - head * LR) * 4;
         float top = sh.m[0][head];
@@ -781,12 +794,80 @@ __global__ __launch_bounds__(W * kWave, W == 4 ? (Q8 ? 3 : NQ == 1 ? 4 : NQ == 2
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
-        const int before = __hip_atomic_fetch_add(a.counters + (size_t)gi * kCtrStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int before = __hip_atomic_fetch_add(a.counters + (size_t)r.gi * kCtrStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         sh.last = before == n_runs - 1;
-        if (before == n_runs - 1) __hip_atomic_store(a.counters + (size_t)gi * kCtrStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == n_runs - 1) __hip_atomic_store(a.counters + (size_t)r.gi * kCtrStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (sh.last) paged_merge<HD, kThreads>(a, sh.merge, gi, n_runs, p, tid);
+    if (sh.last) paged_merge<HD, kThreads>(a, sh.merge, r.rec0, n_runs, p, tid);
+}
+
+// (waves a SIMD: fp32 rows on their way in as many as the registers allow)
+__host__ __device__ constexpr int paged_occupancy(int nq, bool q8) { return q8 ? 3 : nq == 1 ? 4 : nq == 2 ? 3 : 2; }
+
+// Runs of equal length, the same number for every group, which short ones do
+// not use up.
+template <int HD, int NQ, bool Q8>
+__global__ __launch_bounds__(kPagedWaves *kWave, paged_occupancy(NQ, Q8)) void paged_attention_kernel(PagedArgs a)
+{
+    __shared__ PagedShared<HD, NQ, Q8> sh;
+    // the group and its run: a group's runs on one XCD, or (spread) on all
+    const int n_groups = a.n_seq * a.n_kv_heads;
+    int gi, run;
+    if (a.spread) {
+        run = (int)fast_div(blockIdx.x, a.by_groups);
+        gi = blockIdx.x - run * n_groups;
+    } else {
+        const int local = blockIdx.x / kXcds, gl = (int)fast_div((uint32_t)local, a.by_splits);
+        run = local - gl * a.splits;
+        gi = gl * kXcds + (blockIdx.x & (kXcds - 1));
+    }
+    if (gi >= n_groups) return;
+    paged_run<HD, NQ, Q8, false>(a, sh, PagedRun{gi, run * a.chunk, 0, run, 0, (size_t)gi * a.splits}, 0);
+}
+
+// A batch whose groups do not cut evenly: an XCD's groups (i kXcds + its
+// number) laid end to end and cut into runs of equal length, one a workgroup,
+// which may end one group and begin the next.  A beginning counts as
+// kPagedStart tiles.  Records: run w's of group i is w + i of the XCD's (one of
+// the two grows from each to the next, so a group's lie together).
+constexpr int kPagedStart = 4;
+template <int HD, int NQ, bool Q8>
+__global__ __launch_bounds__(kPagedWaves *kWave, NQ == 4 && HD == 64 && !Q8 ? 1 : 2) void paged_flat_kernel(PagedArgs a)
+{
+    __shared__ PagedShared<HD, NQ, Q8> sh;
+    constexpr int TK = paged_tile(HD, Q8);
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int xcd = blockIdx.x & (kXcds - 1), w = blockIdx.x / kXcds, n_wg = gridDim.x / kXcds;
+    const int n_groups = a.n_seq * a.n_kv_heads, items = (n_groups - xcd + kXcds - 1) / kXcds;
+    // lane i: item i's tiles
+    int len = 0, pos = 0;
+    if (lane < items) {
+        PagedPlace p = paged_place(a, lane * kXcds + xcd);
+        p.pos = pos = a.pos[p.seq];
+        paged_rows(a, p);
+        if (!p.skip)
+            len = (p.rows + TK - 1) / TK + kPagedStart;
+        else if (w == 0 && tid < kWave)
+            paged_skip<HD>(a, p, 0, 1);
+    }
+    const int upto = wave_scan_add(len);
+    const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    const int length = max(kPagedWaves, (total + n_wg - 1) / n_wg), stop = min((w + 1) * length, total);
+    bool again = false;
+    for (int at = w * length; at < stop;) {
+        const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
+        const int end = __builtin_amdgcn_readlane(upto, l), row0 = end - __builtin_amdgcn_readlane(len, l) + kPagedStart;
+        const int t0 = max(at, row0) - row0, t1 = min(stop, end) - row0, first = row0 / length;
+        if (t1 > t0) {
+            if (again) __syncthreads();  // (the last group's outputs are read)
+            again = true;
+            paged_run<HD, NQ, Q8, true>(a, sh, PagedRun{l * kXcds + xcd, t0, t1, w - first, (end - 1) / length - first + 1,
+                                                        (size_t)xcd * (n_wg + a.splits) + first + l},
+                                        __builtin_amdgcn_readlane(pos, l));
+        }
+        at = end;
+    }
 }
 
 // The records of a spread launch's groups added up, a workgroup each.
@@ -802,7 +883,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a)
     paged_rows(a, p);
     if (p.skip) return;
     const int n_runs = paged_runs(a, (p.rows + paged_tile(HD, Q8) - 1) / paged_tile(HD, Q8));
-    if (n_runs > 1) paged_merge<HD, 256>(a, sh, blockIdx.x, n_runs, p, threadIdx.x);
+    if (n_runs > 1) paged_merge<HD, 256>(a, sh, (size_t)blockIdx.x * a.splits, n_runs, p, threadIdx.x);
 }
 
 }  // namespace leap
