@@ -2,12 +2,16 @@
 // group of beams, the best by score[beam] + log_softmax(logits[beam])[token].
 //
 // Two launches.  beam_rows_kernel reads the logits once: a wave takes up to
-// 4096 of a row, keeps them in registers, and leaves the row's maximum and sum
-// of exponentials over them and their `beams` best, in order.  The k-th
-// largest of the lanes' maxima bounds the k-th largest of all from below, so
-// that few values are looked at one by one.  beam_best_kernel joins a group's
-// records: a wave a row, then all rows' best against each other, in 64 bits.
-// Bound by the logits' bytes, or for few rows by latency.
+// 4096 of a row, all loads in flight at once, keeps them in registers, and
+// leaves the row's maximum and sum of exponentials over them and their `beams`
+// best, in order.  The k-th largest of the lanes' maxima bounds the k-th
+// largest of all from below, so that little more than k values are looked at
+// one by one.  beam_best_kernel joins a group's records: a wave a row, then all
+// rows' best against each other, in 64 bits.
+//
+// Bound by the logits' bytes (192 rows of 128256: 98.5 MB in 19.7 us, 5.0 TB/s,
+// 8 us of it also spent on instructions, 13 a value), or for few rows by two
+// launches' latency (4 rows of 32000: 4.1 and 4.7 us).
 //
 // Order: a larger total first; of one beam's equal totals the larger logit,
 // then the lower token; of several beams' the lower beam.
@@ -46,8 +50,6 @@ __device__ __forceinline__ float beam_value(uint64_t key)
 }
 __device__ __forceinline__ int beam_place(uint64_t key) { return (int)~(unsigned)key; }
 
-__device__ __forceinline__ unsigned wave_max_u32(unsigned x) { return rows4_bits(dpp_max16(x)); }
-
 // The k-th largest of the lanes' values (as ordered bits).
 __device__ __forceinline__ unsigned kth_largest(unsigned mine, int k)
 {
@@ -62,24 +64,20 @@ __device__ __forceinline__ unsigned kth_largest(unsigned mine, int k)
     return top;
 }
 
-// The first k of n keys in LDS, best first, into to[0 .. k) (0: none).
-__device__ __forceinline__ void best_keys(const uint64_t *list, int n, int k, uint64_t *to, int lane)
-{
-    for (int i0 = 0; i0 < n; i0 += kWave) {
-        const uint64_t mine = i0 + lane < n ? list[i0 + lane] : 0;
-        int rank = 0;
-        for (int j = 0; j < n; j++) rank += list[j] > mine;
-        if (i0 + lane < n && rank < k) to[rank] = mine;
-    }
-    for (int i = n + lane; i < k; i += kWave) to[i] = 0;
-}
-
 // U words of four logits a lane.
 template <int U>
-__global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs a)
+__global__ __launch_bounds__(256, U == 16 ? 5 : 8) void beam_rows_kernel(BeamArgs a)
 {
-    constexpr int kList = (kBeamMax - 1) * 4 * U + kBeamMax;  // values above the bound (in at most k - 1 lanes), and k at it
-    __shared__ uint64_t lists[4][kList];
+    // (values and places apart: 6 bytes)
+    constexpr int kList = (kBeamMax - 1) * 4 * U;  // values above the bound: in at most k - 1 lanes
+    union BeamList {
+        uint64_t keys[kWave];
+        struct {
+            float value[kList];
+            uint16_t place[kList], tie[kBeamMax];
+        } apart;
+    };
+    __shared__ BeamList lists[4];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const long long at = (long long)blockIdx.x * 4 + wave;
     const int row = (int)(at / a.units), unit = (int)(at - (long long)row * a.units);
@@ -88,158 +86,209 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs a)
     const int first = unit * (U * 4 * kWave);
     const float ninf = -__builtin_inff();
     float x[U][4];
+    // (loads without branches between them: all in flight at once)
+    if (first + U * 4 * kWave <= a.vocab) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int i = first + (u * kWave + lane) * 4;
-        if (i + 4 <= a.vocab) {
+        for (int u = 0; u < U; u++) {
             f32x4 y;
-            __builtin_memcpy(&y, x_at + i, 16);  // (rows need not be aligned)
+            __builtin_memcpy(&y, x_at + first + (u * kWave + lane) * 4, 16);  // (rows need not be aligned)
 #pragma unroll
             for (int e = 0; e < 4; e++) x[u][e] = y[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[u][e] = i + e < a.vocab ? x_at[i + e] : ninf;
         }
+    } else {
+        const int left = a.vocab - first;
+        const auto r = make_rsrc(x_at + first, (uint32_t)left * 4u);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = (u * kWave + lane) * 4 + e;
+                const float y = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, i * 4, 0, 0));
+                x[u][e] = i < left ? y : ninf;
+            }
     }
     float top = ninf;
-    bool odd = false;  // NaN or +inf
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            odd |= !(x[u][e] < __builtin_inff());
-            top = fmaxf(top, x[u][e]);
-        }
-    odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    for (int u = 0; u < U; u++) top = fmaxf(fmaxf(top, fmaxf(x[u][0], x[u][1])), fmaxf(x[u][2], x[u][3]));
     const unsigned mine = (unsigned)(beam_key(top, 0) >> 32);
     const float all = lanes_max(top);
+    // a NaN or +inf makes the sum NaN; the maxima pass over a NaN
     float sum = 0.0f;
-    if (all > ninf && !odd) {
+    if (all > ninf) {
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int e = 0; e < 4; e++) sum += fast_exp2((x[u][e] - all) * 1.44269504088896341f);
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum += x[u][e] != x[u][e] ? x[u][e] : 0.0f;
     }
     sum = lanes_sum(sum);
-    if (lane == 0) a.sums[at] = make_float2(odd ? __uint_as_float(0x7fc00000u) : all, sum);
+    const bool odd = sum != sum;
+    if (lane == 0) a.sums[at] = make_float2(odd ? sum : all, sum);
     uint64_t *to = a.keys + at * a.beams;
     if (odd) return;  // (its row has no distribution: beam_best_kernel does not look at these)
-    // the values above the bound, and in order of their places the first k at it
     const unsigned b = kth_largest(mine, a.beams);
     const float bound = beam_value((uint64_t)b << 32);
-    uint64_t *list = lists[wave];
-    int n = 0, ties = 0;
+    constexpr int H = (4 * U + 31) / 32;
+    unsigned hits[H];  // the lane's values from the bound on
+    int n = 0;
 #pragma unroll
+    for (int h = 0; h < H; h++) {
+        hits[h] = 0;
+#pragma unroll
+        for (int j = min(31, 4 * U - 1); j >= 0; j--) hits[h] = hits[h] + hits[h] + (x[8 * h + j / 4][j % 4] >= bound);
+        n += __popc(hits[h]);
+    }
+    const int upto = wave_scan_add(n), all_hits = __builtin_amdgcn_readlane(upto, kWave - 1);
+    BeamList &list = lists[wave];
+    if (all_hits <= kWave) {
+        // as a rule: little more than k.  One a lane, and each one's rank is its place in the record
+        int at = upto - n;
+#pragma unroll
+        for (int h = 0; h < H; h++)
+            while (hits[h]) {
+                const int j = 32 * h + __builtin_ctz(hits[h]), i = first + (j / 4 * kWave + lane) * 4 + j % 4;
+                hits[h] &= hits[h] - 1;
+                list.keys[at++] = beam_key(i < a.vocab ? x_at[i] : ninf, i);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint64_t key = lane < all_hits ? list.keys[lane] : 0;
+        int rank = 0;
+        for (int j = 0; j < all_hits; j++) rank += list.keys[j] > key;
+        if (lane < all_hits && rank < a.beams) to[rank] = key;
+        return;
+    }
+    // many equal values, or a few lanes with large ones: the values above the
+    // bound, and in order of their places the first k at it
+    n = 0;
+    int ties = 0;
     for (int u = 0; u < U; u++) {
-        const int i = first + (u * kWave + lane) * 4;
-        const float w = fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3]));
-        if (__builtin_amdgcn_ballot_w64(w >= bound) == 0) continue;
+        const int i = (u * kWave + lane) * 4;
         uint64_t eq[4];
+        int rank = ties;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const uint64_t gt = __builtin_amdgcn_ballot_w64(x[u][e] > bound);
-            eq[e] = __builtin_amdgcn_ballot_w64(x[u][e] == bound);
-            if (x[u][e] > bound) list[n + (int)__popcll(gt & ((1ull << lane) - 1))] = beam_key(x[u][e], i + e);
+            const float y = first + i + e < a.vocab ? x_at[first + i + e] : ninf;
+            const uint64_t gt = __builtin_amdgcn_ballot_w64(y > bound), below = (1ull << lane) - 1;
+            eq[e] = __builtin_amdgcn_ballot_w64(y == bound);
+            if (y > bound) {
+                const int at = n + (int)__popcll(gt & below);
+                list.apart.value[at] = y;
+                list.apart.place[at] = (uint16_t)(i + e);
+            }
             n += (int)__popcll(gt);
+            rank += (int)__popcll(eq[e] & below);
         }
-        if (ties < a.beams) {
-            int rank = ties;
 #pragma unroll
-            for (int e = 0; e < 4; e++) rank += (int)__popcll(eq[e] & ((1ull << lane) - 1));
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (x[u][e] == bound) {
-                    if (rank < a.beams) list[kList - 1 - rank] = beam_key(x[u][e], i + e);
-                    rank++;
-                }
-#pragma unroll
-            for (int e = 0; e < 4; e++) ties += (int)__popcll(eq[e]);
+        for (int e = 0; e < 4; e++) {
+            if (eq[e] >> lane & 1) {
+                if (rank < a.beams) list.apart.tie[rank] = (uint16_t)(i + e);
+                rank++;
+            }
+            ties += (int)__popcll(eq[e]);
         }
+        ties = min(ties, a.beams);
     }
-    ties = min(ties, a.beams);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    // (together: the ties behind the others)
-    uint64_t tie = 0;
-    if (lane < ties) tie = list[kList - 1 - lane];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (lane < ties) list[n + lane] = tie;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    best_keys(list, n + ties, a.beams, to, lane);
+    for (int i0 = 0; i0 < n; i0 += kWave) {
+        const int i = min(i0 + lane, n - 1);
+        const uint64_t key = beam_key(list.apart.value[i], list.apart.place[i]);
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += beam_key(list.apart.value[j], list.apart.place[j]) > key;
+        if (i0 + lane < n && rank < a.beams) to[rank] = beam_key(list.apart.value[i], first + list.apart.place[i]);
+    }
+    if (n + lane < a.beams) to[n + lane] = lane < ties ? beam_key(bound, first + list.apart.tie[lane]) : 0;
 }
 
-// A workgroup a group, a wave a beam.
-__global__ __launch_bounds__(kBeamMax *kWave) void beam_best_kernel(BeamArgs a)
+// A workgroup a group, a wave a beam.  A row's records are sorted lists, one a
+// lane: its k best are k times the largest of the lanes' heads.  K: beams, at most.
+template <int K>
+__global__ __launch_bounds__(K *kWave) void beam_best_kernel(BeamArgs a)
 {
-    __shared__ uint64_t lists[kBeamMax][kBeamMax * kBeamMax];  // (k - 1 lanes' kBeamMax keys, and k)
-    __shared__ uint64_t best[kBeamMax][kBeamMax];
-    __shared__ double lse[kBeamMax], total[kBeamMax * kBeamMax];
+    __shared__ uint64_t lists[K][K * kBeamUnits];
+    __shared__ double total[K * K];
+    __shared__ int ranks[K * K];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int k = a.beams, row = blockIdx.x * k + wave;
-    const double ninf = -__builtin_inf();
-    if (wave < k) {
-        // the row's distribution (units: a lane each)
-        const float2 s = lane < a.units ? a.sums[(size_t)row * a.units + lane] : make_float2(-__builtin_inff(), 0.0f);
-        const bool odd = __builtin_amdgcn_ballot_w64(s.x != s.x) != 0;
-        const float top = lanes_max(s.x), score = a.scores[row];
-        double part = s.y > 0.0f ? (double)s.y * exp((double)s.x - (double)top) : 0.0;
-        for (int by = 1; by < kWave; by *= 2) part += __shfl_xor(part, by);
-        // (no distribution, or a score that is not finite: every continuation counts -inf)
-        const bool ok = !odd && top > -__builtin_inff() && finite_bits(abs_bits(score));
-        if (lane == 0) lse[wave] = ok ? (double)top + log(part) : __builtin_inf();
-        // its k best
-        if (ok) {
-            const int n = a.units * k;
-            const uint64_t *keys = a.keys + (size_t)row * n;
-            uint64_t mine[kBeamMax], most = 0;
+    const int k = a.beams, row = blockIdx.x * k + wave, n = a.units * k;
+    // (every load at once)
+    const auto keys = make_rsrc(a.keys + (size_t)row * n, (uint32_t)n * 8u);
+    u32x2 words[K];
+    const float2 s = lane < a.units ? a.sums[(size_t)row * a.units + lane] : make_float2(-__builtin_inff(), 0.0f);
+    const float score = a.scores[row];
 #pragma unroll
-            for (int i = 0; i < kBeamMax; i++) {
-                const int at = i * kWave + lane;
-                mine[i] = at < n ? keys[at] : 0;
-                if (beam_place(mine[i]) >= a.vocab) mine[i] = 0;  // (none, or behind the row's end)
-                most = mine[i] > most ? mine[i] : most;
-            }
-            // those of values above the bound, in at most k - 1 lanes, and the first k at it
-            const unsigned bound = kth_largest((unsigned)(most >> 32), k);
-            int count = 0;
+    for (int i = 0; i < K; i++)
+        if (i < k) words[i] = __builtin_amdgcn_raw_buffer_load_b64(keys, (i * kWave + lane) * 8, 0, 0);
 #pragma unroll
-            for (int pass = 0; pass < 2; pass++) {
-                const int end = pass ? count + k : kBeamMax * kBeamMax;
-#pragma unroll
-                for (int i = 0; i < kBeamMax; i++) {
-                    const unsigned v = (unsigned)(mine[i] >> 32);
-                    const bool in = mine[i] != 0 && (pass ? v == bound : v > bound);
-                    const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-                    const int to = count + (int)__popcll(who & ((1ull << lane) - 1));
-                    if (in && to < end) lists[wave][to] = mine[i];
-                    count = min(count + (int)__popcll(who), end);
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            best_keys(lists[wave], count, k, best[wave], lane);
-        } else if (lane < k) {
-            best[wave][lane] = beam_key(-__builtin_inff(), lane);
+    for (int i = 0; i < K; i++)
+        if (i < k) {
+            const uint64_t key = (uint64_t)words[i].y << 32 | words[i].x;
+            lists[wave][i * kWave + lane] = beam_place(key) < a.vocab ? key : 0;  // (none, or behind the row's end)
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (lane < k) {
-            const uint64_t key = best[wave][lane];
-            // (key 0: the row has no k tokens; behind everything)
-            total[wave * k + lane] = key == 0 ? __builtin_nan("") : ok ? (double)beam_value(key) - lse[wave] + (double)score : ninf;
+    if (lane < k) ranks[wave * k + lane] = 0;
+    // the row's distribution (units: a lane each)
+    const bool odd = __builtin_amdgcn_ballot_w64(s.x != s.x) != 0;
+    const float top = lanes_max(s.x);
+    double part = s.y > 0.0f ? (double)s.y * exp((double)s.x - (double)top) : 0.0;
+    for (int by = 1; by < kWave; by *= 2) part += __shfl_xor(part, by);
+    // (no distribution, or a score that is not finite: every continuation counts -inf)
+    const bool ok = !odd && top > -__builtin_inff() && finite_bits(abs_bits(score));
+    const double lse = (double)top + log(part);
+    uint64_t mine = 0;  // lane i: the row's i-th best
+    if (ok) {
+        const uint64_t *list = lists[wave] + lane * k;
+        int at = 1;
+        uint64_t head = lane < a.units ? list[0] : 0, next = lane < a.units && k > 1 ? list[1] : 0;
+        for (int i = 0; i < k; i++) {
+            const unsigned high = wave_max_u32((unsigned)(head >> 32));
+            bool won = (unsigned)(head >> 32) == high;
+            const uint64_t who = __builtin_amdgcn_ballot_w64(won);
+            if (who & (who - 1)) {  // (equal values: the lowest token)
+                const unsigned low = wave_max_u32(won ? (unsigned)head : 0u);
+                won = won && (unsigned)head == low;
+            }
+            const int winner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(won));
+            const unsigned first = (unsigned)__builtin_amdgcn_readlane((int)head, winner);
+            if (lane == i) mine = (uint64_t)high << 32 | first;
+            if (lane == winner) {
+                head = next;
+                at++;
+                next = at < k ? list[at] : 0;
+            }
         }
+    } else if (lane < k) {
+        mine = beam_key(-__builtin_inff(), lane);
+    }
+    if (lane < k) {
+        // (key 0: the row has no k tokens; behind everything)
+        total[wave * k + lane] = mine == 0 ? __builtin_nan("") : ok ? (double)beam_value(mine) - lse + (double)score : -__builtin_inf();
     }
     __syncthreads();
-    for (int i = tid; i < k * k; i += blockDim.x) {
-        const double mine = total[i];
-        if (mine != mine) continue;
+    // each total's rank among the group's: against the wave's row's
+    double row_total[K];
+#pragma unroll
+    for (int j = 0; j < K; j++)
+        if (j < k) row_total[j] = total[wave * k + j];
+    for (int i = lane; i < k * k; i += kWave) {
+        const double x = total[i];
         int rank = 0;
-        for (int j = 0; j < k * k; j++) {
-            const double y = total[j];
-            rank += y > mine || (y == mine && j < i);
-        }
-        if (rank < k) {
+#pragma unroll
+        for (int j = 0; j < K; j++)
+            if (j < k) rank += row_total[j] > x || (row_total[j] == x && wave * k + j < i);
+        if (rank) atomicAdd(&ranks[i], rank);
+    }
+    __syncthreads();
+    const int i = wave * k + lane;
+    if (lane < k) {
+        const double x = total[i];
+        const int rank = ranks[i];
+        if (x == x && rank < k) {
             const int to = blockIdx.x * k + rank;
-            a.parent[to] = blockIdx.x * k + i / k;
-            a.token[to] = beam_place(best[i / k][i % k]);
-            a.best[to] = (float)mine;
+            a.parent[to] = row;
+            a.token[to] = beam_place(mine);
+            a.best[to] = (float)x;
         }
     }
 }

@@ -246,6 +246,15 @@ int launch_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *po
     return 0;
 }
 
+// A counter for each group, and one for each part of the groups' workgroups:
+// two workgroups a CU at most where a group has more than one.
+size_t select_counters(const leap_hip_attention_pages *p)
+{
+    const long long groups = (long long)p->cfg.model.max_batch * p->cfg.model.n_kv_heads;
+    const long long parts = 2ll * p->n_cu / leap::kSelectPart + p->n_cu;
+    return (size_t)(round_up(groups, leap::kCtrStride) + parts * leap::kCtrStride);
+}
+
 int launch_select(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, int max_pos, int keep, int picked_keep,
                   const float *q, int *picked, hipStream_t stream)
 {
@@ -262,6 +271,7 @@ int launch_select(leap_hip_attention_pages *p, int layer, int n_seq, const int *
     a.lists = p->lists;
     a.picked = picked;
     a.counters = p->select_counters;
+    a.part_counters = p->select_counters + round_up((long long)p->cfg.model.max_batch * m.n_kv_heads, leap::kCtrStride);
     a.width = p->width;
     a.keep = keep;
     a.picked_keep = picked_keep;
@@ -276,6 +286,7 @@ int launch_select(leap_hip_attention_pages *p, int layer, int n_seq, const int *
     const long long most = std::max<long long>(1, 2ll * p->n_cu / groups);
     const long long step = leap::kSelectWaves * leap::kPagesAStep;
     a.units = (int)std::max<long long>(1, std::min(most, (pages + step - 1) / step));
+    a.parts = (a.units + leap::kSelectPart - 1) / leap::kSelectPart;
     a.by_kv_heads = leap::make_fastdiv((uint32_t)m.n_kv_heads);
     a.by_units = leap::make_fastdiv((uint32_t)a.units);
     const long long wgs = (groups + leap::kXcds - 1) / leap::kXcds * leap::kXcds * a.units;
@@ -387,7 +398,7 @@ int clear_all(leap_hip_attention_pages *p)
         if (p->pool[k]) HIP_TRY(p, hipMemsetAsync(p->pool[k], 0, p->page_bytes[k] * n * p->n_local, p->stream));
     HIP_TRY(p, hipMemsetAsync(p->counters, 0, kCounters * leap::kCtrStride * sizeof(int), p->stream));
     if (p->select_counters)
-        HIP_TRY(p, hipMemsetAsync(p->select_counters, 0, (size_t)p->cfg.model.max_batch * p->cfg.model.n_kv_heads * sizeof(int), p->stream));
+        HIP_TRY(p, hipMemsetAsync(p->select_counters, 0, select_counters(p) * sizeof(int), p->stream));
     HIP_TRY(p, hipStreamSynchronize(p->stream));
     return 0;
 }
@@ -530,18 +541,22 @@ int launch_beam(leap_hip_attention_pages *p, int n_groups, int beams, int vocab,
     a.vocab = vocab;
     a.beams = beams;
     a.rows = n_groups * beams;
-    // 4 words a lane while that fits the records and leaves few waves, else 16
-    const int small = 4 * 4 * leap::kWave, large = leap::kBeamWords * 4 * leap::kWave;
-    const bool few = (vocab + small - 1) / small <= leap::kBeamUnits && (long long)a.rows * ((vocab + small - 1) / small) <= 8 * p->n_cu;
-    a.units = few ? (vocab + small - 1) / small : (vocab + large - 1) / large;
+    // 4 words a lane while that fits the records and leaves up to 16 waves a
+    // CU, else 16 (4 rows of 32000: 7.5 us and with 16 words 9.8; 128 rows: 9.8
+    // and 10.6; 128 rows of 65536, 32 waves a CU: 14.6 and 13.4)
+    const auto units = [&](int words) { return (vocab + words * 4 * leap::kWave - 1) / (words * 4 * leap::kWave); };
+    const int words = units(4) <= leap::kBeamUnits && (long long)a.rows * units(4) <= 16 * p->n_cu ? 4 : leap::kBeamWords;
+    a.units = units(words);
     a.keys = p->beam_keys;
     a.sums = p->beam_sums;
     a.parent = parent;
     a.token = token;
     a.best = best;
     const unsigned grid = (unsigned)(((long long)a.rows * a.units + 3) / 4);
-    HIP_TRY(p, launch_k(few ? leap::beam_rows_kernel<4> : leap::beam_rows_kernel<leap::kBeamWords>, dim3(grid), dim3(256), stream, a));
-    HIP_TRY(p, launch_k(leap::beam_best_kernel, dim3((unsigned)n_groups), dim3((unsigned)(beams * leap::kWave)), stream, a));
+    const auto rows = words == 4 ? leap::beam_rows_kernel<4> : leap::beam_rows_kernel<leap::kBeamWords>;
+    HIP_TRY(p, launch_k(rows, dim3(grid), dim3(256), stream, a));
+    const auto join = beams <= 4 ? leap::beam_best_kernel<4> : beams <= 8 ? leap::beam_best_kernel<8> : leap::beam_best_kernel<leap::kBeamMax>;
+    HIP_TRY(p, launch_k(join, dim3((unsigned)n_groups), dim3((unsigned)(beams * leap::kWave)), stream, a));
     return 0;
 }
 
@@ -637,7 +652,7 @@ int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, 
     if (c.bounds) {
         CREATE_TRY(hipMalloc(&p->keys, groups * width * sizeof(uint64_t)));
         CREATE_TRY(hipMalloc(&p->lists, groups * width * sizeof(int)));
-        CREATE_TRY(hipMalloc(&p->select_counters, groups * sizeof(int)));
+        CREATE_TRY(hipMalloc(&p->select_counters, select_counters(p) * sizeof(int)));
     }
     const size_t rope_n = (size_t)m.seq_len * (m.head_dim / 2);
     std::vector<float> packed;

@@ -16,12 +16,54 @@ struct PageRowsArgs {
     const int *table, *refs;   // the sequence's row of the table
     int n_pages, n_kv_heads, rows_log2, row0, n;
 };
+// 8-bit values: a workgroup turns 16 rows of a KV head to their layout in LDS,
+// and writes them 16 bytes a lane; at the range's ends, the range's bytes.
+// (8192 rows of 8 KV heads of 128, with the keys: 18.8 us; byte by byte, 50.2)
+template <int HD>
+__device__ __forceinline__ void page_write_v8(const PageRowsArgs &a)
+{
+    constexpr int LR = HD / 4, kRows = 256 / LR;  // rows of a pass
+    __shared__ alignas(16) int8_t turned[HD][16];
+    const int tid = threadIdx.x, c = tid & (LR - 1), end = a.row0 + a.n;
+    const int first = a.row0 >> 4, blocks = ((end + 15) >> 4) - first;
+    const long long items = (long long)blocks * a.n_kv_heads;
+    for (long long i = blockIdx.x; i < items; i += gridDim.x) {
+        const int b = (int)(i / a.n_kv_heads), head = (int)(i - (long long)b * a.n_kv_heads), r0 = (first + b) * 16;
+        const int page = a.table[r0 >> a.rows_log2];
+        if ((unsigned)page >= (unsigned)a.n_pages || a.refs[page] != 1) continue;  // (the same for the workgroup)
+        const size_t at = (((size_t)page * a.n_kv_heads + head) << a.rows_log2) + (r0 & ((1 << a.rows_log2) - 1));
+        __syncthreads();
+#pragma unroll
+        for (int r = tid / LR; r < 16; r += kRows) {
+            const int row = r0 + r;
+            const bool in = row >= a.row0 && row < end;
+            const float4 x = in ? reinterpret_cast<const float4 *>(a.v_in)[((long long)(row - a.row0) * a.n_kv_heads + head) * LR + c]
+                                : make_float4(0, 0, 0, 0);
+            float sc;
+            const int q = quantize_row<HD>(x, &sc);
+#pragma unroll
+            for (int e = 0; e < 4; e++) turned[4 * c + e][r] = (int8_t)(q >> (8 * e));
+            if (in && c == 0) a.vs[at + r] = sc;
+        }
+        __syncthreads();
+        int8_t *to = static_cast<int8_t *>(a.v) + at * HD + 16 * tid;
+        if (tid < HD) {
+            if (r0 >= a.row0 && r0 + 16 <= end) {
+                *reinterpret_cast<i32x4 *>(to) = *reinterpret_cast<const i32x4 *>(turned[tid]);
+            } else {
+                for (int r = max(0, a.row0 - r0); r < min(16, end - r0); r++) to[r] = turned[tid][r];
+            }
+        }
+    }
+}
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256) void page_write_kernel(PageRowsArgs a)
 {
     constexpr int LR = HD / 4;
     const float *in = blockIdx.y ? a.v_in : a.k_in;
     if (!in) return;
+    if constexpr (Q8)
+        if (blockIdx.y) return page_write_v8<HD>(a);
     const long long per_row = (long long)a.n_kv_heads * LR, total = a.n * per_row;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const int r = (int)(i / per_row), w = (int)(i - r * per_row), head = w / LR, c = w & (LR - 1);
@@ -34,14 +76,8 @@ __global__ __launch_bounds__(256) void page_write_kernel(PageRowsArgs a)
         if constexpr (!Q8) {
             reinterpret_cast<float4 *>(blockIdx.y ? a.v : a.k)[at * LR + c] = x;
         } else {
-            if (!blockIdx.y) {
-                reinterpret_cast<int *>(a.k)[at * LR + c] = q;
-            } else {
-                int8_t *to = static_cast<int8_t *>(a.v) + (at & ~(size_t)15) * HD + 64 * c + (at & 15);
-#pragma unroll
-                for (int e = 0; e < 4; e++) to[16 * e] = (int8_t)(q >> (8 * e));
-            }
-            if (c == 0) (blockIdx.y ? a.vs : a.ks)[at] = sc;
+            reinterpret_cast<int *>(a.k)[at * LR + c] = q;
+            if (c == 0) a.ks[at] = sc;
         }
     }
 }

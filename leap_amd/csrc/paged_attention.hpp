@@ -156,6 +156,7 @@ __device__ __forceinline__ float row_sum(float x)
     return x + dpp<0x128>(x);
 }
 __device__ __forceinline__ float lanes_max(float x) { return rows4<true>(row_max(x)); }
+__device__ __forceinline__ unsigned wave_max_u32(unsigned x) { return rows4_bits(dpp_max16(x)); }
 __device__ __forceinline__ float lanes_sum(float x) { return rows4<false>(row_sum(x)); }
 
 // The sum of a group's records by T threads: record s of head h counts
