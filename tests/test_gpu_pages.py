@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from leap_amd.attention import LeapError, PagedAttention
-from tests.helpers import rng_for
+from tests.helpers import attention_f64, rng_for, rope_f32
 from tests.pages_model import Model
 
 pytestmark = pytest.mark.gpu
@@ -672,3 +672,149 @@ def test_a_create_that_does_not_fit_frees_everything():
     with PagedAttention(32, 8, 128, 4096, 10):
         pass
     assert torch.cuda.mem_get_info()[0] >= free - (64 << 20)
+
+
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+@pytest.mark.parametrize("nh,nkv,hd,n_seq", [(32, 8, 128, 24), (8, 8, 128, 20), (64, 8, 128, 21), (32, 8, 64, 33), (8, 8, 64, 24), (128, 8, 64, 24),
+                                             (16, 8, 64, 70)])
+def test_unequal_batches(nh, nkv, hd, n_seq, cache):
+    """Enough rows for a launch that shares the tiles out over the chip, and (70 sequences) too many sequences for it:
+    lengths from one row on, positions out of range, shared and missing pages among them."""
+    import torch
+    m = Model(nh, nkv, hd, 1500, n_seq, cache, 16, key=n_seq)
+    with m.h:
+        pos = m.rng.integers(300, 1400, n_seq)
+        pos[[0, 3, 5, 11, 12, 13]] = [0, 1, 15, 16, 1450, 63]
+        pos[n_seq - 1] = 2
+        m.fill(pos)
+        m.fork(list(range(n_seq - 2)) + [4], [int(x) for x in pos[:-2]] + [20])   # the last but one shares a page with 4
+        m.reserve(pos, [int(p) + 1 if i not in (6, n_seq - 2) else int(p) for i, p in enumerate(pos)])
+        pos[n_seq - 2] = 7
+        m.fork(None, [0 if i == 7 else int(p) + 1 for i, p in enumerate(pos)])    # 7 has no pages
+        pos[8], pos[9] = -5, 1453
+        m.reserve([0] * 6 + [int(pos[6])], [0] * 6 + [int(pos[6]) + 1])
+        q, k, v = m.tokens(n_seq)
+        d, out = _dev(q, k, v), torch.full((n_seq + 1, nh * hd), 3.0, device="cuda")
+        at = _i32(pos)
+        bad = [7, 8, 9, n_seq - 2]
+        good = [i for i in range(n_seq) if i not in bad]
+        # (the model stores the rows of those that are served)
+        want = np.zeros((n_seq, nh * hd))
+        for i in good:
+            row = m.p.row(0, i, pos[i])
+            row[0], row[1] = m.held(rope_f32(k[i], m.cos[pos[i]], m.sin[pos[i]])), m.held(v[i])
+        for i in good:
+            want[i] = attention_f64(m.turned(q[i], pos[i]), *m.p.of(0, i, int(pos[i]) + 1), nh, nkv, hd)
+        for total in (0, int(np.maximum(pos, 0).sum()) + n_seq):
+            out.fill_(3.0)
+            m.h.step_async(0, n_seq, _ptr(at), 1450, *map(_ptr, d), _ptr(out), torch.cuda.current_stream().cuda_stream, total_rows=total)
+            torch.cuda.synchronize()
+            got = out.cpu().numpy()
+            assert np.isnan(got[bad]).all() and (got[n_seq] == 3.0).all()
+            _close(got[good], want[good])
+
+
+@pytest.mark.parametrize("n_seq,rows", [(1100, 17), (3, 9000), (1024, 16), (1025, 16)])
+def test_more_pages_at_once_than_one_pass_takes(n_seq, rows):
+    """Reservations of more than 1024 pages or sequences, missing and shared ones."""
+    m = Model(1, 1, 64, rows + 16, n_seq, "q8", 16, spare=5, n_pages=n_seq * (rows // 16 + 1) + 30)
+    with m.h:
+        m.reserve([0] * n_seq, [rows - 1] * n_seq)
+        m.check_state()
+        parent = m.rng.integers(0, n_seq, n_seq).tolist()
+        m.fork(parent, [rows - 1] * n_seq)
+        m.check_state()
+        last = m.rng.random(n_seq) < 0.9
+        m.reserve([rows - 1 if x else 0 for x in last], [rows if x else 0 for x in last])
+        m.check_state()
+        begin = [0 if i < 900 else rows for i in range(n_seq)]
+        m.reserve(begin, [rows] * n_seq)
+        m.check_state()
+
+
+@pytest.mark.parametrize("pages", [2048, 2049, 4096, 4097])
+def test_sparse_around_a_threads_number_of_pages(pages):
+    m = Model(2, 1, 64, 16 * 4200, 1, "f32", 16, bounds=True, spare=0, key=pages)
+    with m.h:
+        pos = 16 * pages + 3
+        m.fill([pos])
+        m.reserve([pos], [pos + 1])
+        for keep in (2, 65, pages):
+            q, k, v = m.tokens(1)
+            got, picked = m.h.step_sparse(0, [pos], keep, q, k, v)
+            want, chosen = m.want_sparse(0, [pos], keep, q, k, v)
+            assert np.array_equal(picked, chosen)
+            _close(got, want)
+
+
+def test_two_graphs_of_a_handle_take_turns():
+    """They share the handle's workspace; each replay leaves it as it was."""
+    import torch
+    nh, nkv, hd = 16, 4, 128
+    m = Model(nh, nkv, hd, 3000, 12, "f32", 16, layers=1, bounds=True)
+    with m.h:
+        pos = [2900] + [700 + 130 * i for i in range(11)]
+        m.fill(pos)
+        m.reserve(pos, [p + 1 for p in pos])
+        at = _i32(pos)
+        tok = m.tokens(12)
+        d = _dev(*tok)
+        stream = torch.cuda.Stream()
+        outs = [torch.zeros(12, nh * hd, device="cuda") for _ in range(3)]
+        picked = _i32(np.zeros((12, nkv, 40)))
+
+        def call(i):
+            s = stream.cuda_stream
+            if i == 0:
+                m.h.step_async(0, 1, _ptr(at), 2999, *map(_ptr, d), _ptr(outs[0]), s)
+            elif i == 1:
+                m.h.step_async(0, 12, _ptr(at), 2999, *map(_ptr, d), _ptr(outs[1]), s)
+            else:
+                m.h.step_sparse_async(0, 12, _ptr(at), 2999, 40, *map(_ptr, d), _ptr(outs[2]), _ptr(picked), s)
+        graphs = []
+        torch.cuda.synchronize()
+        for i in range(3):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                call(i)
+        want = m.want(0, pos, *tok)
+        sparse, pages = m.want_sparse(0, pos, 40, *tok)
+        for i in (0, 1, 2, 1, 0, 2, 2, 0, 1, 1):
+            for o in outs:
+                o.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graphs[i].replay()
+            torch.cuda.synchronize()
+            if i == 2:
+                assert np.array_equal(picked.cpu().numpy(), pages)
+                _close(outs[2].cpu().numpy(), sparse)
+            else:
+                n = (1, 12)[i]
+                _close(outs[i][:n].cpu().numpy(), want[:n])
+                assert not outs[i][n:].any()
+
+
+def test_two_handles_on_two_streams():
+    import torch
+    ms = [Model(32, 8, 128, 4096, 2, c, 32, key=i) for i, c in enumerate(("f32", "q8"))]
+    try:
+        jobs = []
+        for m in ms:
+            pos = [4000, 1234]
+            m.fill(pos)
+            m.reserve(pos, [p + 1 for p in pos])
+            tok = m.tokens(2)
+            jobs.append((m, pos, tok, _dev(*tok), _i32(pos), torch.zeros(8, 2, 32 * 128, device="cuda"), torch.cuda.Stream()))
+        torch.cuda.synchronize()
+        for i in range(8):
+            for m, pos, tok, d, at, out, s in jobs:
+                m.h.step_async(0, 2, _ptr(at), 4095, *map(_ptr, d), _ptr(out[i]), s.cuda_stream)
+        torch.cuda.synchronize()
+        for m, pos, tok, d, at, out, s in jobs:
+            want = m.want(0, pos, *tok)
+            for i in range(8):
+                _close(out[i].cpu().numpy(), want)
+    finally:
+        for m in ms:
+            m.h.close()
