@@ -684,6 +684,8 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
                     for (int i = 0; i < 4; i++)
                         if (16 * g + 4 * b + i > new_row) x[b][i] = -__builtin_inff();
             }
+            load_k(t + W, next);
+            __builtin_amdgcn_sched_barrier(0);
             // ---- softmax ----
 #pragma unroll
             for (int b = 0; b < NB; b++) mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
@@ -703,7 +705,6 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
                 x[j / 4][j % 4] = y * row_lane<j>(vs);
                 wt = fmaxf(wt, x[j / 4][j % 4]);
             });
-            load_k(t + W, next);
             // ---- weighted values ----
             const int e = fixed_exp(__float_as_uint(rows4<true>(wt)));
             const float up = exp2_int(29 - e), down = exp2_int(e - 29);
@@ -722,11 +723,13 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
                 for (int j = 0; j < 4; j++) d[j] = mfma8(v8[v], pd[j], i32x4{0, 0, 0, 0});
 #pragma unroll
                 for (int i = 0; i < 4; i++) o[v][i] = __builtin_fmaf(digits_sum(d[0][i], d[1][i], d[2][i], d[3][i]), down, o[v][i]);
+                v8[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(v8_at + 256 * v));  // (the next tile's)
                 asm volatile("" : "+v"(o[v]));
                 __builtin_amdgcn_sched_barrier(0);
             }
+            vsc = *vs_at;
         }
-        load_v(t + W, next);
+        if constexpr (!Q8) load_v(t + W, next);
         look(t + 2 * W);
     }
 
