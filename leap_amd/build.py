@@ -4,7 +4,7 @@
 
 The RoPE table TU is compiled by the host C++ compiler with the reference's
 release flags, the checkpoint reader by the host compiler, and the HIP TUs
-(the host side and the three kernel tables, see csrc/kernels.hpp) by hipcc
+(the host sides and the kernel tables, see csrc/kernels.hpp) by hipcc
 for gfx950 only, in parallel.  Packed-fp32 VALU instructions are disabled for
 device code (``-packed-fp32-ops``).
 """

@@ -7,7 +7,8 @@ namespace leap {
 
 // Rows [row0, row0 + n) of one sequence and layer, [row][kv_head][HD] outside.
 // A row is written only into a page of the sequence's own, and read as NaN
-// where it has none.
+// where it has none.  Bound by memory: 8192 rows of 8 heads of 128 in 21 us each
+// way (fp32, 134 MB: 6.3 TB/s), 8 bits 19 us in and 27 out (bytes gathered).
 struct PageRowsArgs {
     const float *k_in, *v_in;  // (write: either may be NULL)
     float *k_out, *v_out;      // (read)

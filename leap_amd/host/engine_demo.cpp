@@ -34,6 +34,14 @@
 // master's layers, the packet sent, an int32 that says whether the worker
 // forwarded, the packet it forwarded and the master's x after the reply
 // (zeros where nothing was forwarded).
+//
+//   engine_demo ... out_dir pages BEAMS
+//
+// decodes BEAMS beams of one group over a cache of pages: each token, every
+// layer's step for all beams, then the selection over synthetic logits of
+// kVocab tokens, and the fork of the caches to the chosen parents.  The trace
+// holds, per token, each layer's q, k, v and xb of all beams, the logits, and
+// the chosen parents, tokens (int32) and scores.
 // Exit status: 0 success, 2 bad usage, 3 shim error.
 #include <hip/hip_runtime_api.h>
 
@@ -136,6 +144,42 @@ int run_pipeline(int n_layers, int n_heads, int n_kv, int head_dim, int seq_len,
     return 0;
 }
 
+constexpr int kVocab = 1000;
+
+// A beam search over a cache of pages (see the header).
+int run_pages(int n_layers, int n_heads, int n_kv, int head_dim, int seq_len, int n_tokens, int beams, std::FILE *f)
+{
+    const int page_rows = 16, width = (seq_len + page_rows - 1) / page_rows;
+    leap::HipPages cache({{n_layers, 0, n_layers, n_heads, n_kv, head_dim, seq_len, 500000.0f, beams}, beams * width, page_rows});
+    const size_t dim = (size_t)n_heads * head_dim, kv_dim = (size_t)n_kv * head_dim;
+    std::vector<float> q(beams * dim), k(beams * kv_dim), v(beams * kv_dim), xb(beams * dim), logits((size_t)beams * kVocab), score(beams), best(beams);
+    std::vector<int> pos(beams), next(beams), parent(beams), token(beams);
+    const float scale = 1.0f / std::sqrt((float)head_dim);
+    Rng rng{0x4C454150};
+    std::fill(score.begin() + 1, score.end(), -INFINITY);  // one prompt: the first beam's continuations
+    for (int t = 0; t < n_tokens; t++) {
+        std::fill(pos.begin(), pos.end(), t);
+        std::fill(next.begin(), next.end(), t + 1);
+        if (!cache.reserve(pos, next)) throw std::runtime_error("the pool has too few pages");
+        for (int l = 0; l < n_layers; l++) {
+            for (auto *x : {&q, &k, &v})
+                for (float &e : *x) e = rng.next(scale);
+            cache.step(l, pos, q, k, v, xb);
+            for (auto *x : {&q, &k, &v, &xb}) std::fwrite(x->data(), 4, x->size(), f);
+        }
+        for (float &e : logits) e = rng.next(8.0f);
+        cache.beam_select(beams, logits, score, parent, token, best);
+        std::fwrite(logits.data(), 4, logits.size(), f);
+        std::fwrite(parent.data(), 4, parent.size(), f);
+        std::fwrite(token.data(), 4, token.size(), f);
+        std::fwrite(best.data(), 4, best.size(), f);
+        cache.fork(parent, next);
+        score = best;
+    }
+    std::printf("engine_demo: %d tokens x %d beams, %d of %d pages in use\n", n_tokens, beams, cache.compact(), beams * width);
+    return 0;
+}
+
 }  // namespace
 
 int main(int argc, char **argv)
@@ -143,10 +187,11 @@ int main(int argc, char **argv)
     const bool block = argc == 9 && std::string(argv[8]) == "block";
     const bool ckpt = argc == 10 && std::string(argv[8]) == "ckpt";
     const bool pipeline = argc == 11 && std::string(argv[8]) == "pipeline";
-    if (argc != 8 && !block && !ckpt && !pipeline) {
+    const bool pages = argc == 10 && std::string(argv[8]) == "pages";
+    if (argc != 8 && !block && !ckpt && !pipeline && !pages) {
         std::fprintf(stderr,
                      "usage: %s n_layers n_heads n_kv_heads head_dim seq_len n_tokens out_dir "
-                     "[block | ckpt PATH | pipeline PATH SPLIT]\n",
+                     "[block | ckpt PATH | pipeline PATH SPLIT | pages BEAMS]\n",
                      argv[0]);
         return 2;
     }
@@ -170,6 +215,21 @@ int main(int argc, char **argv)
                 return 2;
             }
             const int rc = run_pipeline(n_layers, n_heads, n_kv, head_dim, seq_len, n_tokens, argv[9], split, f);
+            std::fclose(f);
+            return rc;
+        }
+        if (pages) {
+            const int beams = std::atoi(argv[9]);
+            if (beams < 1 || beams > 16) {
+                std::fprintf(stderr, "BEAMS must be in [1, 16]\n");
+                return 2;
+            }
+            std::FILE *f = std::fopen((out_dir + "/trace.bin").c_str(), "wb");
+            if (!f) {
+                std::fprintf(stderr, "cannot write %s/trace.bin\n", out_dir.c_str());
+                return 2;
+            }
+            const int rc = run_pages(n_layers, n_heads, n_kv, head_dim, seq_len, n_tokens, beams, f);
             std::fclose(f);
             return rc;
         }

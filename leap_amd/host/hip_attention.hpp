@@ -8,6 +8,7 @@
 // one call.
 #pragma once
 
+#include <cerrno>
 #include <cstddef>
 #include <cstdint>
 #include <optional>
@@ -215,6 +216,135 @@ private:
 
     leap_hip_attention *h_ = nullptr;
     int q_dim_ = 0, kv_dim_ = 0;
+};
+
+// A cache of pages (leap_hip_attention_pages): sequences of a batch that share
+// rows and hold no more memory than they use.
+class HipPages {
+public:
+    struct Dims {
+        HipAttention::Dims model;  // (cache_q8: pages of 8-bit rows)
+        int n_pages;
+        int page_rows = 16;   // 16, 32, 64 or 128
+        bool bounds = false;  // step_sparse needs them
+    };
+
+    explicit HipPages(const Dims &d)
+    {
+        const HipAttention::Dims &m = d.model;
+        const leap_hip_attention_pages_config c{{m.n_layers, m.layer_begin, m.layer_end, m.n_heads, m.n_kv_heads, m.head_dim,
+                                                 m.seq_len, m.rope_theta, m.max_batch, m.device},
+                                                d.page_rows, d.n_pages, m.cache_q8, d.bounds};
+        check(leap_hip_attention_pages_create(&c, &p_), nullptr);
+        q_dim_ = m.n_heads * m.head_dim;
+        kv_dim_ = m.n_kv_heads * m.head_dim;
+        n_kv_heads_ = m.n_kv_heads;
+    }
+    HipPages(const HipPages &) = delete;
+    HipPages &operator=(const HipPages &) = delete;
+    HipPages(HipPages &&o) noexcept
+        : p_(std::exchange(o.p_, nullptr)), q_dim_(o.q_dim_), kv_dim_(o.kv_dim_), n_kv_heads_(o.n_kv_heads_)
+    {
+    }
+    ~HipPages() { leap_hip_attention_pages_destroy(p_); }
+
+    // Pages of its own for rows [begin[i], end[i]) of each sequence; false, with
+    // nothing changed, where the pool has too few.
+    bool reserve(std::span<const int> begin, std::span<const int> end)
+    {
+        same(begin.size(), end.size(), "reserve: begin and end");
+        const int rc = leap_hip_attention_pages_reserve(p_, (int)begin.size(), begin.data(), end.data());
+        if (rc == -ENOMEM) return false;
+        check(rc, p_);
+        return true;
+    }
+    // Sequence i takes the pages of the first rows[i] rows of parent[i] (empty: its own).
+    void fork(std::span<const int> parent, std::span<const int> rows)
+    {
+        if (!parent.empty()) same(parent.size(), rows.size(), "fork: parent and rows");
+        check(leap_hip_attention_pages_fork(p_, (int)rows.size(), parent.empty() ? nullptr : parent.data(), rows.data()), p_);
+    }
+    // The pages in use to the front of the pool; how many there are.
+    int compact()
+    {
+        int used = 0;
+        check(leap_hip_attention_pages_compact(p_, &used), p_);
+        return used;
+    }
+
+    // One token of each sequence, at pos[i], whose row is reserved.
+    void step(int layer, std::span<const int> pos, std::span<const float> q, std::span<const float> k_new,
+              std::span<const float> v_new, std::span<float> out)
+    {
+        check_rows(pos, q, k_new, v_new, out);
+        check(leap_hip_attention_pages_step(p_, layer, (int)pos.size(), pos.data(), q.data(), k_new.data(), v_new.data(), out.data()), p_);
+    }
+    // The same over at most `keep` pages for each KV head; picked: empty, or [pos.size()][n_kv_heads][keep].
+    void step_sparse(int layer, std::span<const int> pos, int keep, std::span<const float> q, std::span<const float> k_new,
+                     std::span<const float> v_new, std::span<float> out, std::span<int> picked = {})
+    {
+        check_rows(pos, q, k_new, v_new, out);
+        if (!picked.empty()) same(picked.size(), pos.size() * (size_t)n_kv_heads_ * (size_t)(keep > 0 ? keep : 0), "step_sparse: picked");
+        check(leap_hip_attention_pages_step_sparse(p_, layer, (int)pos.size(), pos.data(), keep, q.data(), k_new.data(), v_new.data(),
+                                                   out.data(), picked.empty() ? nullptr : picked.data()),
+              p_);
+    }
+
+    // Rows [begin, begin + k.size() / kv_dim) of a sequence, k as it is stored (after rotation).
+    void write(int seq, int layer, int begin, std::span<const float> k, std::span<const float> v)
+    {
+        check_kv(k.size(), v.size(), "write");
+        check(leap_hip_attention_pages_write(p_, seq, layer, begin, begin + (int)(k.size() / (size_t)kv_dim_), k.data(), v.data()), p_);
+    }
+    void read(int seq, int layer, int begin, std::span<float> k, std::span<float> v)
+    {
+        check_kv(k.size(), v.size(), "read");
+        check(leap_hip_attention_pages_read(p_, seq, layer, begin, begin + (int)(k.size() / (size_t)kv_dim_), k.data(), v.data()), p_);
+    }
+
+    // The `beams` best continuations of each group of beams: logits [score.size()][vocab].
+    void beam_select(int beams, std::span<const float> logits, std::span<const float> score, std::span<int> parent,
+                     std::span<int> token, std::span<float> best)
+    {
+        const size_t n = score.size();
+        same(parent.size(), n, "beam_select: parent");
+        same(token.size(), n, "beam_select: token");
+        same(best.size(), n, "beam_select: best");
+        if (n == 0 || beams <= 0 || n % (size_t)beams || logits.size() % n)
+            throw std::invalid_argument("HipPages::beam_select: sizes are no groups of beams");
+        check(leap_hip_attention_pages_beam_select(p_, (int)(n / (size_t)beams), beams, (int)(logits.size() / n), logits.data(),
+                                                   score.data(), parent.data(), token.data(), best.data()),
+              p_);
+    }
+
+    void clear() { check(leap_hip_attention_pages_clear(p_), p_); }
+    leap_hip_attention_pages *handle() { return p_; }
+
+private:
+    static void same(size_t a, size_t b, const char *what)
+    {
+        if (a != b) throw std::invalid_argument(std::string("HipPages::") + what + ": sizes differ");
+    }
+    void check_kv(size_t k, size_t v, const char *what) const
+    {
+        same(k, v, what);
+        same(k % (size_t)kv_dim_, 0, what);
+    }
+    void check_rows(std::span<const int> pos, std::span<const float> q, std::span<const float> k, std::span<const float> v,
+                    std::span<const float> out) const
+    {
+        same(q.size(), pos.size() * (size_t)q_dim_, "step: q");
+        same(out.size(), q.size(), "step: out");
+        same(k.size(), pos.size() * (size_t)kv_dim_, "step: k_new");
+        same(v.size(), k.size(), "step: v_new");
+    }
+    static void check(int rc, leap_hip_attention_pages *p)
+    {
+        if (rc != 0) throw std::runtime_error(std::string("leap_hip_attention_pages: ") + leap_hip_attention_pages_last_error(p));
+    }
+
+    leap_hip_attention_pages *p_ = nullptr;
+    int q_dim_ = 0, kv_dim_ = 0, n_kv_heads_ = 0;
 };
 
 }  // namespace leap
