@@ -587,6 +587,9 @@ int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, 
     if ((c.q8 != 0 && c.q8 != 1) || (c.bounds != 0 && c.bounds != 1))
         return set_err(nullptr, -EINVAL, "q8 %d and bounds %d must be 0 or 1", c.q8, c.bounds);
     const int width = (m.seq_len + c.page_rows - 1) / c.page_rows;
+    // (a reservation counts the pages asked for in 32 bits)
+    if ((long long)m.max_batch * width > 0x7fffffff)
+        return set_err(nullptr, -EINVAL, "a table of %d sequences of %d pages is too large", m.max_batch, width);
     if (c.bounds && width > leap::kSelectPages)
         return set_err(nullptr, -EINVAL, "%d pages a sequence: with bounds at most %d", width, leap::kSelectPages);
     // (rows of a page and KV head are 32-bit offsets, records of a group 32-bit bytes)

@@ -8,8 +8,8 @@
 // timing: the lowest free page first, to the first sequence's first page first.
 //
 // All are bound by latency (a few dependent passes over a few KB: fork's two
-// launches 2.4 us each for 4 sequences and 4.6 for 64, compact's plan 7.0 for
-// 1600 pages); what copies pages is bound by memory (507 MB moved in 104 us, 4.9
+// launches 2.4 us each for 4 sequences and 4.6 for 64, compact's plan 7.0 for a
+// pool of 489 pages); what copies pages is bound by memory (507 MB moved in 104 us, 4.9
 // TB/s, where a large copy reaches 5.2).
 #pragma once
 

@@ -48,6 +48,7 @@ def test_a_missing_handle_is_refused(lib):
     (dict(page_rows=256), "page_rows"), (dict(n_pages=0), "n_pages"), (dict(n_pages=(1 << 26) + 1), "n_pages"),
     (dict(q8=2), "q8"), (dict(bounds=-1), "bounds"), (dict(bounds=1, seq_len=16 * 16384 + 1), "pages a sequence"),
     (dict(n_heads=65536, n_kv_heads=65536, page_rows=16), "too large"),
+    (dict(max_batch=2048, seq_len=1 << 24), "a table of 2048"), (dict(max_batch=65535, seq_len=1 << 24, page_rows=128), "a table of 65535"),
 ])
 def test_create_refuses(lib, change, fragment):
     kw = dict(n_layers=1, layer_begin=0, layer_end=1, n_heads=8, n_kv_heads=2, head_dim=128, seq_len=64, rope_theta=0.0, max_batch=1,
