@@ -228,6 +228,7 @@ __global__ __launch_bounds__(K *kWave) void beam_best_kernel(BeamArgs a)
             lists[wave][i * kWave + lane] = beam_place(key) < a.vocab ? key : 0;  // (none, or behind the row's end)
         }
     if (lane < k) ranks[wave * k + lane] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // the row's distribution (units: a lane each)
     const bool odd = __builtin_amdgcn_ballot_w64(s.x != s.x) != 0;
     const float top = lanes_max(s.x);

@@ -214,8 +214,8 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int 
         }
         items += total;
     }
+    __syncthreads();  // (few.first: either way the next wave's is read)
     if (in_lds && items <= kPlanThreads) {
-        __syncthreads();
         reserve_few(a, few, sh, &copies, items, tid, e_nomem);
         return;
     }

@@ -714,7 +714,27 @@ def test_unequal_batches(nh, nkv, hd, n_seq, cache):
             _close(got[good], want[good])
 
 
-@pytest.mark.parametrize("n_seq,rows", [(1100, 17), (3, 9000), (1024, 16), (1025, 16)])
+@pytest.mark.parametrize("cache", ["f32", "q8"])
+@pytest.mark.parametrize("nkv,pos,page_rows", [(1, [70000, 100, 30000, 65000, 0], 128), (2, [40000, 16, 33333], 64), (3, [30000, 29999, 1], 64),
+                                               (8, [30000], 32)])
+def test_unequal_batches_of_few_kv_heads(nkv, pos, page_rows, cache):
+    """Fewer groups than XCDs, and one sequence far below the bound of its position."""
+    import torch
+    m = Model(4 * nkv, nkv, 64, 75000, len(pos), cache, page_rows, spare=0)
+    with m.h:
+        m.fill(pos)
+        m.reserve(pos, [p + 1 for p in pos])
+        q, k, v = m.tokens(len(pos))
+        d, at = _dev(q, k, v), _i32(pos)
+        want = m.want(0, pos, q, k, v)
+        for total in (0, sum(pos) + len(pos)):
+            out = torch.full((len(pos), 4 * nkv * 64), 3.0, device="cuda")
+            m.h.step_async(0, len(pos), _ptr(at), 74999, *map(_ptr, d), _ptr(out), torch.cuda.current_stream().cuda_stream, total_rows=total)
+            torch.cuda.synchronize()
+            _close(out.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("n_seq,rows", [(1100, 17), (3, 9000), (1024, 16), (1025, 16), (700, 30), (1024, 40)])
 def test_more_pages_at_once_than_one_pass_takes(n_seq, rows):
     """Reservations of more than 1024 pages or sequences, missing and shared ones."""
     m = Model(1, 1, 64, rows + 16, n_seq, "q8", 16, spare=5, n_pages=n_seq * (rows // 16 + 1) + 30)
