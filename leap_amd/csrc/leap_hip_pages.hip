@@ -144,15 +144,14 @@ struct StepPlan {
 // products, four waves at a time, tiles come in at 6.8 TB/s over the card (8
 // bits: an eighth slower with one workgroup a CU; fp32 a tenth over long runs
 // of one sequence), 1 us of them within the constant, and records take 2 us
-// and 0.03 for each.  (us, 32/8/128 in fp32,
-// the chosen number of runs and its neighbours; 512 rows 4: 8.4, 8: 6.8; 4096
-// 16: 13.6, 22: 12.3, 32: 11.2, 64: 13.0; 16384 32: 26.9, 64: 27.8; 8 bits at
-// 16384 22: 17.8, 32: 15.3, 64: 16.7, at 131072 32: 61.8, 64: 58.5.)
-// Batches of unequal lengths, or whose groups and runs do not divide over the
-// CUs, run flat once they have 16 tiles a CU (uniform : flat; 32/8/128 fp32, 8
-// sequences of up to 500 9.8 : 11.3, 16 of up to 1000 22.5 : 21.0, 32 of up to
-// 7300 180 : 163, 64/8/128 16 of up to 7300 124 : 108; 8 bits, 32 of up to
-// 8192 73 : 68).  Two workgroups a CU: 8 bits need both (one: 84), fp32 takes
+// and 0.03 for each.  (us, 32/8/128, runs of 4, 8, 16, 32 tiles: fp32, one
+// sequence of 4096 11.2, 11.2, 13.6, 19.9, of 8192 -, 17.8, 16.7, 22.6; 12 of
+// 4096 -, 73, 72, 64.6; 8 bits, one of 4096 10.4, 13.2, of 16384 16.5, 15.3.)
+// Batches of unequal lengths with a group for every XCD run flat once they have
+// 16 tiles a CU (uniform : flat; 32/8/128 fp32, 8 sequences of up to 500 9.8 :
+// 11.3, 16 of up to 1000 22.5 : 21.0, 32 of up to 7300 180 : 163, 64/8/128 16
+// of up to 7300 124 : 108; 8 bits, 32 of up to 8192 73 : 68; equal lengths, 16
+// of 8192 160 : 162, 8 bits 32 of 8192 100 : 110).  Two workgroups a CU: 8 bits need both (one: 84), fp32 takes
 // as long with one.
 StepPlan step_plan(const leap_hip_attention_pages *p, int n_seq, int longest, long long total)
 {
@@ -182,13 +181,10 @@ StepPlan step_plan(const leap_hip_attention_pages *p, int n_seq, int longest, lo
         }
     }
     const long long flat_wgs = 2ll * p->n_cu;
-    const double tiles = (double)groups * tiles_mean / p->n_cu;
-    if (n_seq > 1 && tiles >= 16 && items <= leap::kWave && (size_t)(leap::kXcds * items + flat_wgs) * p->group <= kRecords &&
-        (size_t)groups <= kCounters && flat_wgs <= (long long)leap::kXcds * leap::kPagedSplits) {
-        const bool equal = total == (long long)n_seq * longest;
-        const double us = (tiles + leap::kPagedStart * (2.0 + (double)groups / p->n_cu)) * p->n_cu * tile_us + 3.0;
-        if (!equal || us < best) return StepPlan{1, (int)items, false, true, flat_wgs};
-    }
+    const bool equal = total == (long long)n_seq * longest;
+    if (n_seq > 1 && groups >= leap::kXcds && !equal && groups * tiles_mean >= 16ll * p->n_cu && items <= leap::kWave && (size_t)(leap::kXcds * items + flat_wgs) * p->group <= kRecords &&
+        (size_t)groups <= kCounters && flat_wgs <= (long long)leap::kXcds * leap::kPagedSplits)
+        return StepPlan{1, (int)items, false, true, flat_wgs};
     s.spread = s.splits > 1 && groups < leap::kXcds && !few;
     s.wgs = s.spread ? groups * s.splits : items * leap::kXcds * s.splits;
     return s;
