@@ -648,9 +648,10 @@ class PagedAttention:
     # -- rows -------------------------------------------------------------------
     def write(self, seq, layer, pos_begin, k=None, v=None):
         k, v = (None if x is None else _f32(x) for x in (k, v))
-        rows = {x.size // self.kv_dim for x in (k, v) if x is not None}
-        if len(rows) > 1:
-            raise ValueError("k and v have different rows")
+        sizes = {x.size for x in (k, v) if x is not None}
+        if len(sizes) > 1 or any(n % self.kv_dim for n in sizes):
+            raise ValueError(f"k and v: {sorted(sizes)} values are no equal numbers of rows of {self.kv_dim}")
+        rows = {n // self.kv_dim for n in sizes}
         if rows:
             self._call("write", seq, layer, pos_begin, pos_begin + rows.pop(), _fp(k), _fp(v))
 

@@ -615,6 +615,17 @@ def test_results_do_not_change_from_call_to_call():
             assert torch.equal(outs[i], outs[i % 2])
 
 
+def test_rows_that_are_not_whole():
+    m = Model(8, 2, 64, 64, 1)
+    with m.h:
+        m.reserve([0], [10])
+        x = np.zeros(3 * 128, np.float32)
+        for k, v in ((x[:-1], None), (x, x[:128]), (None, x[:5]), (x[:200], x[:200])):
+            with pytest.raises(ValueError):
+                m.h.write(0, 0, 0, k, v)
+        m.h.write(0, 0, 0, x, x)
+
+
 def test_refusals_of_a_handle():
     import torch
     m = Model(8, 2, 128, 64, 3, page_rows=16, layers=2)
