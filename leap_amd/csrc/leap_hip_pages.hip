@@ -537,11 +537,13 @@ int launch_beam(leap_hip_attention_pages *p, int n_groups, int beams, int vocab,
     a.vocab = vocab;
     a.beams = beams;
     a.rows = n_groups * beams;
-    // 4 words a lane while that fits the records and leaves up to 16 waves a
-    // CU, else 16 (4 rows of 32000: 7.5 us and with 16 words 9.8; 128 rows: 9.8
-    // and 10.6; 128 rows of 65536, 32 waves a CU: 14.6 and 13.4)
+    // 4 words a lane, or 8, while they fit the records and leave up to 16 waves
+    // a CU, else 16 (4 rows of 32000: with 4 words 7.5 us, with 16 9.8; 128 rows
+    // 9.8 and 10.6; 128 rows of 65536, 32 waves a CU: 14.6 and 13.4; of 128256,
+    // 8 words and 16: 1 row 6.4 and 7.6, 8 rows 10.5 and 11.6, 64 14.0 and 14.4)
     const auto units = [&](int words) { return (vocab + words * 4 * leap::kWave - 1) / (words * 4 * leap::kWave); };
-    const int words = units(4) <= leap::kBeamUnits && (long long)a.rows * units(4) <= 16 * p->n_cu ? 4 : leap::kBeamWords;
+    int words = 4;
+    while (words < leap::kBeamWords && (units(words) > leap::kBeamUnits || (long long)a.rows * units(words) > 16 * p->n_cu)) words *= 2;
     a.units = units(words);
     a.keys = p->beam_keys;
     a.sums = p->beam_sums;
@@ -549,7 +551,7 @@ int launch_beam(leap_hip_attention_pages *p, int n_groups, int beams, int vocab,
     a.token = token;
     a.best = best;
     const unsigned grid = (unsigned)(((long long)a.rows * a.units + 3) / 4);
-    const auto rows = words == 4 ? leap::beam_rows_kernel<4> : leap::beam_rows_kernel<leap::kBeamWords>;
+    const auto rows = words == 4 ? leap::beam_rows_kernel<4> : words == 8 ? leap::beam_rows_kernel<8> : leap::beam_rows_kernel<leap::kBeamWords>;
     HIP_TRY(p, launch_k(rows, dim3(grid), dim3(256), stream, a));
     const auto join = beams <= 4 ? leap::beam_best_kernel<4> : beams <= 8 ? leap::beam_best_kernel<8> : leap::beam_best_kernel<leap::kBeamMax>;
     HIP_TRY(p, launch_k(join, dim3((unsigned)n_groups), dim3((unsigned)(beams * leap::kWave)), stream, a));

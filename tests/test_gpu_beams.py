@@ -62,7 +62,8 @@ def h():
 
 @pytest.mark.parametrize("groups,beams,vocab", [
     (1, 1, 1), (1, 1, 2), (1, 4, 4), (1, 4, 5), (3, 5, 63), (2, 16, 16), (2, 16, 1000), (1, 4, 32000), (5, 3, 1023), (5, 3, 1024), (5, 3, 1025),
-    (4, 8, 4097), (7, 2, 50257), (2, 8, 128256), (1, 16, 262144), (40, 16, 300), (233, 3, 999), (600, 1, 2500),
+    (4, 8, 4097), (7, 2, 50257), (2, 8, 128256), (1, 16, 262144), (40, 16, 300), (233, 3, 999), (600, 1, 2500), (3, 4, 70001), (30, 8, 66000), (1, 2, 131072),
+    (1, 2, 131073),
 ])
 def test_selection_matches_64_bits(h, groups, beams, vocab):
     rng = rng_for(0x6265616D, groups, beams, vocab)
@@ -73,7 +74,7 @@ def test_selection_matches_64_bits(h, groups, beams, vocab):
     _check(h.beam_select(groups, beams, logits, score), logits, score, groups, beams)
 
 
-@pytest.mark.parametrize("beams,vocab", [(4, 50), (8, 5000), (16, 70000)])
+@pytest.mark.parametrize("beams,vocab", [(4, 50), (8, 5000), (16, 70000), (5, 200000)])
 def test_equal_logits(h, beams, vocab):
     """All equal; a few values only; and in blocks, so that a lane has most of the largest."""
     rng = rng_for(0x74696573, beams, vocab)
@@ -89,7 +90,7 @@ def test_equal_logits(h, beams, vocab):
         _check(h.beam_select(2, beams, logits, score), logits, score, 2, beams)
 
 
-@pytest.mark.parametrize("beams,vocab", [(1, 40), (4, 300), (5, 9000), (8, 40000)])
+@pytest.mark.parametrize("beams,vocab", [(1, 40), (4, 300), (5, 9000), (8, 40000), (3, 100000), (2, 150000)])
 def test_masks_and_rows_that_are_not_distributions(h, beams, vocab):
     rng = rng_for(0x6D61736B, beams, vocab)
     n = 6 * beams
