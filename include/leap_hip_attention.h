@@ -412,7 +412,7 @@ int leap_hip_attention_pages_clear(leap_hip_attention_pages *p);
 int leap_hip_attention_pages_state(leap_hip_attention_pages *p, int *table, int *refs);
 
 /* Device addresses, valid until destroy; to be read only, but for the pool's
- * contents.  k, v, ks, vs and bounds are of the layer, and layers follow one
+ * contents (who writes keys there writes their bounds too).  k, v, ks, vs and bounds are of the layer, and layers follow one
  * another: with G KV heads of HD elements, pages of R rows, fp32 k and v
  * [page][G][R][HD]; 8 bits k [page][G][R][HD], v [page][G][R / 16][HD][16] (16
  * rows, element by element), scales ks and vs [page][G][R]; bounds

@@ -99,7 +99,7 @@ __device__ __forceinline__ int list_pages(const unsigned *bits, bool want_free, 
 constexpr int kBadRange = (int)0x80000000u;
 constexpr int kAskedSlots = 2 * kPlanThreads;
 struct ReserveFew {
-    int first[kPlanThreads + 1];  // items ahead of each sequence's
+    int first[kPlanThreads];      // items ahead of each sequence's
     int base[kPlanThreads];       // a sequence's page of item f: base + f
     int ids[kPlanThreads];        // free pages, in order
     int page[kAskedSlots], asked[kAskedSlots], last[kAskedSlots];  // shared pages: how many ask, and the last of them
