@@ -34,7 +34,7 @@ struct leap_hip_attention_pages {
     float4 *rope = nullptr;
     int *table = nullptr, *refs = nullptr;
     unsigned *free_bits = nullptr;
-    int *asked = nullptr, *last = nullptr, *item = nullptr, *prefix = nullptr, *ids = nullptr, *n_copies = nullptr;
+    int *whole = nullptr, *asked = nullptr, *last = nullptr, *item = nullptr, *prefix = nullptr, *ids = nullptr, *n_copies = nullptr;
     int2 *copies = nullptr;
     // the step's records and counters; the sparse step's keys, lists and counters
     float *ws_o = nullptr, *ws_lse = nullptr;
@@ -214,6 +214,7 @@ int launch_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *po
     a.pos = pos;
     a.table = p->table;
     a.refs = p->refs;
+    a.whole = p->whole;
     a.lists = p->lists;
     a.ws_o = p->ws_o;
     a.ws_lse = p->ws_lse;
@@ -314,6 +315,7 @@ leap::PagesArgs pages_args(const leap_hip_attention_pages *p, int n_seq)
     a.table = p->table;
     a.refs = p->refs;
     a.free_bits = p->free_bits;
+    a.whole = p->whole;
     a.asked = p->asked;
     a.last = p->last;
     a.item = p->item;
@@ -382,6 +384,7 @@ int clear_all(leap_hip_attention_pages *p)
     const size_t entries = (size_t)p->cfg.model.max_batch * p->width, n = (size_t)p->cfg.n_pages;
     HIP_TRY(p, hipMemsetAsync(p->table, 0xff, entries * sizeof(int), p->stream));
     HIP_TRY(p, hipMemsetAsync(p->refs, 0, n * sizeof(int), p->stream));
+    HIP_TRY(p, hipMemsetAsync(p->whole, 0, (size_t)p->cfg.model.max_batch * sizeof(int), p->stream));
     HIP_TRY(p, hipMemsetAsync(p->asked, 0, n * sizeof(int), p->stream));
     HIP_TRY(p, hipMemsetAsync(p->last, 0xff, n * sizeof(int), p->stream));
     HIP_TRY(p, hipMemsetAsync(p->free_bits, 0xff, (n / 32) * sizeof(unsigned), p->stream));
@@ -640,6 +643,7 @@ int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, 
     CREATE_TRY(hipMalloc(&p->table, entries * sizeof(int)));
     CREATE_TRY(hipMalloc(&p->item, entries * sizeof(int)));
     CREATE_TRY(hipMalloc(&p->refs, n * sizeof(int)));
+    CREATE_TRY(hipMalloc(&p->whole, (size_t)m.max_batch * sizeof(int)));
     CREATE_TRY(hipMalloc(&p->asked, n * sizeof(int)));
     CREATE_TRY(hipMalloc(&p->last, n * sizeof(int)));
     CREATE_TRY(hipMalloc(&p->ids, n * sizeof(int)));
@@ -681,7 +685,7 @@ int leap_hip_attention_pages_destroy(leap_hip_attention_pages *p)
     if (!p) return 0;
     (void)hipSetDevice(p->cfg.model.device);
     if (p->stream) (void)hipStreamSynchronize(p->stream);
-    void *bufs[] = {p->pool[0], p->pool[1], p->pool[2], p->pool[3], p->pool[4], p->rope, p->table, p->item, p->refs, p->asked,
+    void *bufs[] = {p->pool[0], p->pool[1], p->pool[2], p->pool[3], p->pool[4], p->rope, p->table, p->item, p->refs, p->whole, p->asked,
                     p->last, p->ids, p->copies, p->free_bits, p->prefix, p->n_copies, p->ws_o, p->ws_lse, p->counters, p->keys,
                     p->lists, p->select_counters, p->beam_keys, p->beam_sums, p->staging};
     for (void *b : bufs)

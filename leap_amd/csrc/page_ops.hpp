@@ -2,8 +2,10 @@
 // references), and moving their contents.
 //
 // table [sequence][width] names a sequence's pages in order (-1: none),
-// refs [page] counts the tables that name a page, and bit p % 32 of
-// free_bits [p / 32] is set where refs is 0.  The calls below are the only
+// refs [page] counts the tables that name a page, bit p % 32 of
+// free_bits [p / 32] is set where refs is 0, and whole [sequence] counts a
+// sequence's pages ahead of the first that it lacks, so that a step learns
+// with its position whether a page is missing.  The calls below are the only
 // ones that change them.  Numbers are given by a rule that does not depend on
 // timing: the lowest free page first, to the first sequence's first page first.
 //
@@ -23,9 +25,10 @@ constexpr int kPlanWaves = kPlanThreads / kWave;
 struct PagesArgs {
     int *table, *refs;
     unsigned *free_bits;
+    int *whole;                   // [sequence]
     int *asked, *last;            // [page], 0 and -1 between launches
     int *item;                    // [sequence][width]: scratch (fork: the new tables)
-    int *prefix;                  // [sequence + 1]: scratch
+    int *prefix;                  // [sequence + 1]: scratch (fork: the new `whole`)
     int *ids;                     // [page]: scratch (free pages in order; compact: where a page went)
     int2 *copies;                 // [page]: from, to
     int *n_copies;                // [2]: how many copies; pages in use before compact
@@ -94,6 +97,33 @@ __device__ __forceinline__ int list_pages(const unsigned *bits, bool want_free, 
     return found;
 }
 
+// What reserve needs to bring `whole` up to date for a sequence that gets the
+// pages [first, end): loaded before the table changes, of entries that stay.
+struct Whole {
+    int seq, first, end, now, next;  // now: whole; next: the page behind the range (-1: none)
+};
+__device__ __forceinline__ Whole whole_load(const PagesArgs &a, int seq, int first, int end, int now)
+{
+    Whole w{seq, first, end, now, -1};
+    if (end > first && end < a.width) w.next = a.table[(size_t)seq * a.width + end];
+    return w;
+}
+// By all lanes of a wave.  Where the range closes a gap ahead of pages that
+// were there, the wave looks for the next one, 64 entries at a time.
+__device__ __forceinline__ void whole_store(const PagesArgs &a, const Whole &w, int lane)
+{
+    const bool grows = w.end > w.first && w.first <= w.now && w.now < w.end;
+    if (grows && w.next < 0) a.whole[w.seq] = w.end;
+    for (uint64_t left = __builtin_amdgcn_ballot_w64(grows && w.next >= 0); left; left &= left - 1) {
+        const int from = __builtin_ctzll(left), seq = __builtin_amdgcn_readlane(w.seq, from);
+        uint64_t gap = 0;
+        int at = __builtin_amdgcn_readlane(w.end, from);
+        for (; !gap; at += gap ? __builtin_ctzll(gap) : kWave)
+            gap = __builtin_amdgcn_ballot_w64(at + lane >= a.width || a.table[(size_t)seq * a.width + at + lane] < 0);
+        if (lane == 0) a.whole[seq] = at;
+    }
+}
+
 // reserve_kernel's way for up to 1024 sequences and items (a step's: one item a
 // sequence): LDS and registers, an item a thread.
 constexpr int kBadRange = (int)0x80000000u;
@@ -113,7 +143,7 @@ __device__ __forceinline__ int asked_slot(int *pages, int page, bool put)
         if (there == page || there == -1) return (int)at;
     }
 }
-__device__ __forceinline__ void reserve_few(const PagesArgs &a, ReserveFew &l, int *sh, int *copies, int items, int tid, int e_nomem)
+__device__ __forceinline__ void reserve_few(const PagesArgs &a, ReserveFew &l, int *sh, int *copies, int items, const Whole &whole, int tid, int e_nomem)
 {
     const unsigned word = word_of(a.free_bits, tid, a.n_pages);
     int seq = 0, page = -1, refs = 0;
@@ -151,10 +181,12 @@ __device__ __forceinline__ void reserve_few(const PagesArgs &a, ReserveFew &l, i
     }
     int need;
     const int rank = block_scan(take, sh, tid, &need) - 1;
+    bool granted = true;
     if (need > 0) {
         const int n_free = list_pages(a.free_bits, true, 0, a.n_pages, need, word, sh, tid, [&](int i, int page) { l.ids[i] = page; });
         __syncthreads();
-        if (n_free < need) {
+        granted = n_free >= need;
+        if (!granted) {
             if (a.status && tid < a.n_seq && l.base[tid] != kBadRange) a.status[tid] = e_nomem;
         } else if (take) {
             const int to = l.ids[rank];
@@ -167,6 +199,7 @@ __device__ __forceinline__ void reserve_few(const PagesArgs &a, ReserveFew &l, i
             a.table[at] = to;
         }
     }
+    if (granted) whole_store(a, whole, tid & (kWave - 1));
     __syncthreads();
     if (tid == 0) a.n_copies[0] = *copies;
 }
@@ -191,15 +224,19 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int 
     // items ahead of each sequence's
     int items = 0;
     const bool in_lds = a.n_seq <= kPlanThreads;
+    Whole whole{0, 0, 0, 0, -1};  // (of sequence tid: where all are in LDS)
     for (int i0 = 0; i0 < a.n_seq; i0 += kPlanThreads) {
         const int i = i0 + tid;
         int n = 0, b = 0;
         bool ok = false;
         if (i < a.n_seq) {
-            const int e = a.end[i];
+            const int e = a.end[i], now = a.whole[i];
             b = a.begin[i];
             ok = b >= 0 && b <= e && e <= a.seq_len;
-            if (ok && b < e) n = ((e + R - 1) >> a.rows_log2) - (b >> a.rows_log2);
+            if (ok && b < e) {
+                n = ((e + R - 1) >> a.rows_log2) - (b >> a.rows_log2);
+                if (in_lds) whole = whole_load(a, i, b >> a.rows_log2, (e + R - 1) >> a.rows_log2, now);
+            }
             if (a.status) a.status[i] = ok ? 0 : e_inval;
         }
         int total;
@@ -216,7 +253,7 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int 
     }
     __syncthreads();  // (few.first: either way the next wave's is read)
     if (in_lds && items <= kPlanThreads) {
-        reserve_few(a, few, sh, &copies, items, tid, e_nomem);
+        reserve_few(a, few, sh, &copies, items, whole, tid, e_nomem);
         return;
     }
     if (in_lds && tid < a.n_seq) store_now(a.prefix + tid + 1, tid + 1 < a.n_seq ? few.first[tid + 1] : items);
@@ -250,6 +287,7 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int 
     if (shared) plan_sync();
     // which items take a free page, and which of them in order
     int need = 0;
+    bool granted = true;
     for (int f0 = 0; f0 < items; f0 += kPlanThreads) {
         const int f = f0 + tid;
         bool take = false;
@@ -271,18 +309,18 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int 
         const int n_free = list_pages(a.free_bits, true, 0, a.n_pages, need, word_of(a.free_bits, tid, a.n_pages), sh, tid,
                                       [&](int i, int page) { store_now(a.ids + i, page); });
         plan_sync();
-        if (n_free < need) {
+        granted = n_free >= need;
+        if (!granted) {
             if (a.status)
                 for (int i = tid; i < a.n_seq; i += kPlanThreads)
                     if (a.begin[i] >= 0 && a.begin[i] <= a.end[i] && a.end[i] <= a.seq_len) a.status[i] = e_nomem;
-            need = 0;
         }
     }
     for (int f = tid; f < items; f += kPlanThreads) {
         int i;
         const size_t at = place(f, &i);
         const int page = a.table[at], rank = a.item[f];
-        if (need > 0 && rank >= 0) {
+        if (granted && rank >= 0) {
             const int to = load_now(a.ids + rank);
             if (page >= 0) {
                 __hip_atomic_fetch_add(a.refs + page, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -297,6 +335,18 @@ __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int 
             store_now(a.last + page, -1);
         }
     }
+    if (granted)
+        for (int i0 = 0; i0 < a.n_seq; i0 += kPlanThreads) {
+            const int i = i0 + tid;
+            if (!in_lds) {
+                whole = Whole{0, 0, 0, 0, -1};
+                if (i < a.n_seq) {
+                    const int b = a.begin[i], e = a.end[i];
+                    if (b >= 0 && b < e && e <= a.seq_len) whole = whole_load(a, i, b >> a.rows_log2, (e + R - 1) >> a.rows_log2, a.whole[i]);
+                }
+            }
+            whole_store(a, whole, tid & (kWave - 1));
+        }
     __syncthreads();
     if (tid == 0) a.n_copies[0] = copies;
 }
@@ -312,9 +362,11 @@ __global__ __launch_bounds__(256) void fork_gather_kernel(PagesArgs a)
     if (j >= a.width) return;
     const int from = a.parent ? a.parent[i] : i, rows = a.rows[i];
     const int old = a.table[(size_t)i * a.width + j];
+    const bool ok = from >= 0 && from < a.max_batch && rows >= 0 && rows <= a.seq_len;
+    const int whole = a.whole[ok ? from : i];
     int page = old;
-    if (from >= 0 && from < a.max_batch && rows >= 0 && rows <= a.seq_len)
-        page = (long long)j << a.rows_log2 < rows ? a.table[(size_t)from * a.width + j] : -1;
+    if (ok) page = (long long)j << a.rows_log2 < rows ? a.table[(size_t)from * a.width + j] : -1;
+    if (j == 0) a.prefix[i] = ok ? min(whole, (rows + (1 << a.rows_log2) - 1) >> a.rows_log2) : whole;
     a.item[(size_t)i * a.width + j] = page;
     if (page >= 0 && page != old) __hip_atomic_fetch_add(a.refs + page, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -323,7 +375,8 @@ __global__ __launch_bounds__(256) void fork_drop_kernel(PagesArgs a)
     const int i = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
     if (j >= a.width) return;
     const size_t at = (size_t)i * a.width + j;
-    const int old = a.table[at], page = a.item[at];
+    const int old = a.table[at], page = a.item[at], whole = a.prefix[i];
+    if (j == 0) a.whole[i] = whole;
     if (page == old) return;
     a.table[at] = page;
     if (old >= 0 && __hip_atomic_fetch_add(a.refs + old, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 1)

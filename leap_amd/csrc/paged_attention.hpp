@@ -69,6 +69,7 @@ struct PagedArgs {
     const int *pos;
     const int *table;                // [sequence][width]
     const int *refs;                 // [page]
+    const int *whole;                // [sequence]: its pages ahead of the first that is missing
     const int *lists;                // [group][keep] pages (keep 0: none, all pages of the table)
     float *ws_o, *ws_lse;            // records: [group][split][q head][HD], [group][split][q head]
     int *counters;                   // [group], kCtrStride apart, zero between launches
@@ -96,7 +97,7 @@ struct PagedPlace {
     int seq, kvh, pos;
     const int *list;     // page numbers
     int n_list, rows;    // pages, and rows along the list with the new one
-    bool skip;           // a position out of range
+    bool skip;           // a position out of range, or a page of its rows missing
 };
 __device__ __forceinline__ PagedPlace paged_place(const PagedArgs &a, int gi)
 {
@@ -106,13 +107,13 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedArgs &a, int gi)
     p.list = a.keep ? a.lists + (size_t)gi * a.keep : a.table + (size_t)p.seq * a.width;
     return p;
 }
-// (its position known)
-__device__ __forceinline__ void paged_rows(const PagedArgs &a, PagedPlace &p)
+// (its position known, and how many of its pages are there)
+__device__ __forceinline__ void paged_rows(const PagedArgs &a, PagedPlace &p, int whole)
 {
     const int at = p.pos >> a.rows_log2;
     p.n_list = a.keep ? min(a.keep, at + 1) : at + 1;
     p.rows = ((p.n_list - 1) << a.rows_log2) + (p.pos & ((1 << a.rows_log2) - 1)) + 1;
-    p.skip = p.pos < 0 || p.pos > a.max_pos;
+    p.skip = p.pos < 0 || p.pos > a.max_pos || at >= whole;
 }
 // NaN into a skipped sequence's output row, by `step` threads.
 template <int HD>
@@ -366,10 +367,9 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
     };
     const int8_t *v8_at = nullptr;
     const float *vs_at = nullptr;
-    int used[Q8 ? 1 : NB];  // the pages of the tile that is loaded (8 bits: V's)
+    int used[Q8 ? 1 : NB];  // fp32: the pages of the tile that is loaded
     auto load_k = [&](int at, bool on) {
         if constexpr (Q8) {
-            used[0] = pages[1];
             int here = on ? lane : 0;  // (not on: all lanes the same line)
             asm volatile("" : "+v"(here));  // (addresses formed here: kept, their parts would take the registers of a load)
             const int m = here & 15, g = here >> 4;
@@ -433,9 +433,10 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
     const float4 v_row = buf_load4(make_rsrc(a.v_new + new_at * 4, new_bytes), c * 16u);
     look(t);
     p.pos = FLAT ? pos : uniform_load(a.pos + p.seq);
-    if constexpr (!Q8) asm volatile("" ::"s"(p.pos), "s"(pages[0]), "s"(pages[NB - 1]));  // (one wait for them all)
+    const int whole = FLAT ? 0x7fffffff : uniform_load(a.whole + p.seq);
+    if constexpr (!Q8) asm volatile("" ::"s"(p.pos), "s"(whole), "s"(pages[0]), "s"(pages[NB - 1]));  // (one wait for them all)
     __builtin_amdgcn_sched_barrier(0);
-    paged_rows(a, p);
+    paged_rows(a, p, whole);
     if (!FLAT && p.skip) {
         if (r.run == 0) paged_skip<HD>(a, p, tid);
         return;
@@ -498,11 +499,11 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
     const bool has_new = newest_run && (tiles - 1 - t0) % W == wave;
     const int new_row = (p.rows - 1) & (TK - 1);                       // its row of the last tile
     const int b_new = new_row >> 4, r_new = new_row & 15;              // its block of that, and row of the block
-    bool bad = false;  // a page is missing, or the new row's is shared
+    bool shared = false;  // the new row's page is not the sequence's own
     if (has_new) {
         const int own = uniform_load(p.list + p.n_list - 1);
-        bad = !there(own) || uniform_load(a.refs + (there(own) ? own : 0)) != 1;
-        if (!bad && lane < LR) {
+        shared = !there(own) || uniform_load(a.refs + (there(own) ? own : 0)) != 1;
+        if (!shared && lane < LR) {
             const size_t to = row0_of(own, n_blocks - 1) + r_new;
             if constexpr (Q8) {
                 const int w = reinterpret_cast<const int *>(sh.v_new)[lane];
@@ -519,7 +520,7 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
                 reinterpret_cast<float4 *>(a.v)[to * LR + lane] = reinterpret_cast<const float4 *>(sh.v_new)[lane];
             }
         }
-        if (!bad && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
+        if (!shared && a.bounds && (p.pos & ((1 << a.rows_log2) - 1)) == (1 << a.rows_log2) - 1) {
             // the page is complete: the bounds of its keys
             const size_t head = (size_t)own * a.n_kv_heads + p.kvh;
             const int d = lane & (LR - 1);
@@ -549,8 +550,6 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
         int zero = 0;
         asm volatile("" : "+v"(zero));  // (q is read from LDS for each tile: kept, it would take a quarter of the registers)
         if constexpr (!Q8) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) bad |= t * NB + b < n_blocks && !there(used[b]);
             if (last) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
@@ -643,7 +642,6 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
         } else {
             const u32x4 *qs = &sh.q[lane + zero];
             float x[NB][4], mt = -__builtin_inff();
-            bad |= 4 * t + g < n_blocks && !there(used[0]);
             if (last) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
@@ -742,12 +740,11 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
 
     // ---- the waves' results together ----
     __syncthreads();  // (q is read; its memory takes the outputs)
-    const bool missing = __builtin_amdgcn_ballot_w64(bad) != 0;
     if constexpr (Q8) {
         const float l = rows4<false>(lrun[0]);
         if (g == 0) {
             sh.m[wave][m] = mrun[0];
-            sh.l[wave][m] = missing ? __uint_as_float(0x7fc00000u) : l;
+            sh.l[wave][m] = shared ? __uint_as_float(0x7fc00000u) : l;
         }
         if (m < a.group)
 #pragma unroll
@@ -759,7 +756,7 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
             const float l = row_sum(lrun[k]);
             if (m == 0) {
                 sh.m[wave][4 * k + g] = mrun[k];
-                sh.l[wave][4 * k + g] = missing ? __uint_as_float(0x7fc00000u) : l;
+                sh.l[wave][4 * k + g] = shared ? __uint_as_float(0x7fc00000u) : l;
             }
         }
         f32x4 acc[NQ][4];
@@ -856,7 +853,7 @@ __global__ __launch_bounds__(kPagedWaves *kWave, NQ == 4 && HD == 64 && !Q8 ? 1 
     if (lane < items) {
         PagedPlace p = paged_place(a, lane * kXcds + xcd);
         p.pos = pos = a.pos[p.seq];
-        paged_rows(a, p);
+        paged_rows(a, p, a.whole[p.seq]);
         if (!p.skip)
             len = (p.rows + TK - 1) / TK + kPagedStart;
         else if (w == 0 && tid < kWave)
@@ -891,7 +888,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a)
     } sh;
     PagedPlace p = paged_place(a, blockIdx.x);
     p.pos = a.pos[p.seq];
-    paged_rows(a, p);
+    paged_rows(a, p, a.whole[p.seq]);
     if (p.skip) return;
     const int n_runs = paged_runs(a, (p.rows + paged_tile(HD, Q8) - 1) / paged_tile(HD, Q8));
     if (n_runs > 1) paged_merge<HD, 256>(a, sh, (size_t)blockIdx.x * a.splits, n_runs, p, threadIdx.x);
