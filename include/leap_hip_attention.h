@@ -323,9 +323,9 @@ const char *leap_hip_attention_pages_last_error(const leap_hip_attention_pages *
  * pages for them, and they are its own.  A missing page is a free one (it
  * holds what it held), a shared one is replaced by a copy, in all held layers;
  * where all who share a page ask for it in one call, the last of them keeps
- * it.  -ENOMEM, with nothing changed, if the pool has too few free pages.
- * Host pointers; -EINVAL, with nothing changed, for a range outside
- * [0, seq_len]. */
+ * it.  -ENOMEM, with nothing changed, if the pool has too few free pages, and
+ * for nothing else (memory that HIP cannot get is -EIO).  Host pointers;
+ * -EINVAL, with nothing changed, for a range outside [0, seq_len]. */
 int leap_hip_attention_pages_reserve(leap_hip_attention_pages *p, int n_seq, const int *begin, const int *end);
 /* The same with device pointers, enqueued on `stream`.  A sequence whose range
  * is bad is left out.  status [n_seq] (or NULL) gets 0, -EINVAL for a sequence

@@ -44,7 +44,7 @@ struct leap_hip_attention_pages {
     // the beam selection's records (its first call)
     uint64_t *beam_keys = nullptr;
     float2 *beam_sums = nullptr;
-    // the host-pointer calls' staging (grown)
+    // the host-pointer calls' staging (the tables' calls' from the start, else grown)
     char *staging = nullptr;
     size_t staging_bytes = 0;
     hipStream_t stream = nullptr;
@@ -367,6 +367,21 @@ int launch_reserve(leap_hip_attention_pages *p, int n_seq, const int *begin, con
     return launch_copies(p, false, stream);
 }
 
+// (checked) ranges in host memory; *status: the device's answer.
+int reserve_host(leap_hip_attention_pages *p, int n_seq, const int *begin, const int *end, int *status)
+{
+    HIP_TRY(p, hipSetDevice(p->cfg.model.device));
+    const size_t bytes = (size_t)n_seq * sizeof(int);
+    if (int rc = staging(p, 3 * bytes)) return rc;
+    int *bd = reinterpret_cast<int *>(p->staging), *ed = bd + n_seq, *sd = ed + n_seq;
+    HIP_TRY(p, hipMemcpyAsync(bd, begin, bytes, hipMemcpyHostToDevice, p->stream));
+    HIP_TRY(p, hipMemcpyAsync(ed, end, bytes, hipMemcpyHostToDevice, p->stream));
+    if (int rc = launch_reserve(p, n_seq, bd, ed, sd, p->stream)) return rc;
+    HIP_TRY(p, hipMemcpyAsync(status, sd, sizeof *status, hipMemcpyDeviceToHost, p->stream));  // (one for all)
+    HIP_TRY(p, hipStreamSynchronize(p->stream));
+    return 0;
+}
+
 int launch_fork(leap_hip_attention_pages *p, int n_seq, const int *parent, const int *rows, hipStream_t stream)
 {
     leap::PagesArgs a = pages_args(p, n_seq);
@@ -654,6 +669,7 @@ int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, 
     CREATE_TRY(hipMalloc(&p->ws_o, kRecords * m.head_dim * sizeof(float)));
     CREATE_TRY(hipMalloc(&p->ws_lse, kRecords * sizeof(float)));
     CREATE_TRY(hipMalloc(&p->counters, kCounters * leap::kCtrStride * sizeof(int)));
+    if ((rc = staging(p, 3 * (size_t)m.max_batch * sizeof(int))) != 0) return fail(rc);
     if (c.bounds) {
         CREATE_TRY(hipMalloc(&p->keys, groups * width * sizeof(uint64_t)));
         CREATE_TRY(hipMalloc(&p->lists, groups * width * sizeof(int)));
@@ -748,15 +764,9 @@ int leap_hip_attention_pages_reserve(leap_hip_attention_pages *p, int n_seq, con
     for (int i = 0; i < n_seq; i++)
         if (begin[i] < 0 || begin[i] > end[i] || end[i] > p->cfg.model.seq_len)
             return set_err(p, -EINVAL, "sequence %d: rows [%d, %d) outside [0, %d)", i, begin[i], end[i], p->cfg.model.seq_len);
-    HIP_TRY(p, hipSetDevice(p->cfg.model.device));
-    const size_t bytes = (size_t)n_seq * sizeof(int);
-    if (int rc = staging(p, 3 * bytes)) return rc;
-    int *bd = reinterpret_cast<int *>(p->staging), *ed = bd + n_seq, *sd = ed + n_seq, status = 0;
-    HIP_TRY(p, hipMemcpyAsync(bd, begin, bytes, hipMemcpyHostToDevice, p->stream));
-    HIP_TRY(p, hipMemcpyAsync(ed, end, bytes, hipMemcpyHostToDevice, p->stream));
-    if (int rc = launch_reserve(p, n_seq, bd, ed, sd, p->stream)) return rc;
-    HIP_TRY(p, hipMemcpyAsync(&status, sd, sizeof status, hipMemcpyDeviceToHost, p->stream));  // (one for all)
-    HIP_TRY(p, hipStreamSynchronize(p->stream));
+    int status = 0;
+    // (-ENOMEM is the pool's alone: who gets it can free pages, or wait)
+    if (int rc = reserve_host(p, n_seq, begin, end, &status)) return rc == -ENOMEM ? -EIO : rc;
     return status ? set_err(p, status, "the pool of %d pages has too few free ones", p->cfg.n_pages) : 0;
 }
 
