@@ -134,12 +134,13 @@ struct ReserveFew {
     int ids[kPlanThreads];        // free pages, in order
     int page[kAskedSlots], asked[kAskedSlots], last[kAskedSlots];  // shared pages: how many ask, and the last of them
 };
-__device__ __forceinline__ int asked_slot(int *pages, int page, bool put)
+// The page's slot, put there if it is new.
+__device__ __forceinline__ int asked_slot(int *pages, int page)
 {
     unsigned at = ((unsigned)page * 2654435761u) >> 21;  // (of 2048; a page in 1024 at most: an empty slot is always left)
     static_assert(kAskedSlots == 2048, "slots");
     for (;; at = (at + 1) & (kAskedSlots - 1)) {
-        const int there = put ? atomicCAS(&pages[at], -1, page) : pages[at];
+        const int there = atomicCAS(&pages[at], -1, page);
         if (there == page || there == -1) return (int)at;
     }
 }
@@ -172,7 +173,7 @@ __device__ __forceinline__ void reserve_few(const PagesArgs &a, ReserveFew &l, i
         __syncthreads();
         int slot = 0;
         if (refs > 1) {
-            slot = asked_slot(l.page, page, true);
+            slot = asked_slot(l.page, page);
             atomicAdd(&l.asked[slot], 1);
             atomicMax(&l.last[slot], seq);
         }
