@@ -840,6 +840,23 @@ __global__ __launch_bounds__(kPagedWaves *kWave, paged_occupancy(NQ, Q8)) void p
 // kPagedStart tiles.  Records: run w's of group i is w + i of the XCD's (one of
 // the two grows from each to the next, so a group's lie together).
 constexpr int kPagedStart = 4;
+// Tiles and starts of a run, where an XCD's n_wg workgroups share `total`.
+__host__ __device__ inline int paged_length(int total, int n_wg)
+{
+    const int each = (total + n_wg - 1) / n_wg;
+    return each > kPagedWaves ? each : kPagedWaves;
+}
+// Run w's part [t0, t1) of the tiles of an XCD's item (empty: t1 <= t0), the
+// run's number among the item's n, and the XCD's record of the item's first.
+// The run covers [at, stop), and the item its last len of [0, end).
+struct PagedSegment {
+    int t0, t1, run, n, record;
+};
+__host__ __device__ inline PagedSegment paged_segment(int w, int length, int at, int stop, int item, int len, int end)
+{
+    const int row0 = end - len + kPagedStart, first = row0 / length;
+    return {(at > row0 ? at : row0) - row0, (stop < end ? stop : end) - row0, w - first, (end - 1) / length - first + 1, first + item};
+}
 template <int HD, int NQ, bool Q8>
 __global__ __launch_bounds__(kPagedWaves *kWave, NQ == 4 && HD == 64 && !Q8 ? 1 : 2) void paged_flat_kernel(PagedArgs a)
 {
@@ -861,17 +878,16 @@ __global__ __launch_bounds__(kPagedWaves *kWave, NQ == 4 && HD == 64 && !Q8 ? 1 
     }
     const int upto = wave_scan_add(len);
     const int total = __builtin_amdgcn_readlane(upto, kWave - 1);
-    const int length = max(kPagedWaves, (total + n_wg - 1) / n_wg), stop = min((w + 1) * length, total);
+    const int length = paged_length(total, n_wg), stop = min((w + 1) * length, total);
     bool again = false;
     for (int at = w * length; at < stop;) {
         const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
-        const int end = __builtin_amdgcn_readlane(upto, l), row0 = end - __builtin_amdgcn_readlane(len, l) + kPagedStart;
-        const int t0 = max(at, row0) - row0, t1 = min(stop, end) - row0, first = row0 / length;
-        if (t1 > t0) {
+        const int end = __builtin_amdgcn_readlane(upto, l);
+        const PagedSegment s = paged_segment(w, length, at, stop, l, __builtin_amdgcn_readlane(len, l), end);
+        if (s.t1 > s.t0) {
             if (again) __syncthreads();  // (the last group's outputs are read)
             again = true;
-            paged_run<HD, NQ, Q8, true>(a, sh, PagedRun{l * kXcds + xcd, t0, t1, w - first, (end - 1) / length - first + 1,
-                                                        (size_t)xcd * (n_wg + a.splits) + first + l},
+            paged_run<HD, NQ, Q8, true>(a, sh, PagedRun{l * kXcds + xcd, s.t0, s.t1, s.run, s.n, (size_t)xcd * (n_wg + a.splits) + s.record},
                                         __builtin_amdgcn_readlane(pos, l));
         }
         at = end;

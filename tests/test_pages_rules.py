@@ -31,6 +31,11 @@ def _program():
     return exe
 
 
+def test_every_launch_covers_its_work_inside_its_workspace():
+    r = subprocess.run([_program(), "launches"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 def test_tables_change_without_memory_and_a_full_pool_has_its_own_code():
     r = subprocess.run([_program(), "memory"], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
