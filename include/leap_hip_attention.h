@@ -359,10 +359,11 @@ int leap_hip_attention_pages_compact_async(leap_hip_attention_pages *p, int *use
  * reserved.  A sequence whose position is out of range, that has no page for
  * one of the rows [0, pos[i]], or whose page of row pos[i] is not its own,
  * writes nothing and gets an output row of NaN.  fp32: products and sums in
- * fp32.  8 bits: of q and of the weights times the value rows' scales, what
- * lies below 2^-30 of their largest (of a head row; of 64 positions) is
- * rounded away, products are exact and sums of 64 positions fp32's; q holds
- * what is above 2^-119.  Host pointers. */
+ * fp32, with weights of 2^-20 at the reference: values below 2^-106 lose bits.
+ * 8 bits: of q and of the weights (at most 1) times the value rows' scales,
+ * what lies below 2^-30 of their largest (of a head row; of 64 positions) is
+ * rounded away, and what lies below 2^-119 of q and 2^-126 of those; products
+ * are exact and sums of 64 positions fp32's.  Host pointers. */
 int leap_hip_attention_pages_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, const float *q,
                                   const float *k_new, const float *v_new, float *out);
 /* As leap_hip_attention_step_batched_async, over pages. */

@@ -41,7 +41,8 @@
 //     rows' scales, is a 30-bit fixed-point number over a power of two just
 //     above the largest of its head row (q) or of its tile (probabilities), as
 //     four signed digits of 8 bits; the four integer sums are exact and are put
-//     together in fp32.  What is lost is 2^-30 of that largest element.
+//     together in fp32.  What is lost is 2^-30 of that largest element.  O is
+//     held in units of a power of two of the weighted values' size.
 #pragma once
 
 #include "many_attention.hpp"
@@ -53,10 +54,17 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kPagedWaves = 4;       // waves of a workgroup
 constexpr int kPagedSplits = 64;     // runs of a group, at most: a lane each in the merge
 constexpr int kPagedHeads = 16;      // q heads of a KV head, at most
-// Probabilities are 2^(score - reference - kPagedBias), and the reference
-// moves when a score exceeds it by more than kPagedMargin: sums of up to 2^16
-// probabilities stay below 1, and weighted values below the largest value.
-constexpr float kPagedMargin = 4.0f, kPagedBias = 20.0f;
+// Probabilities are 2^(score - reference - bias), and the reference moves when
+// a score exceeds it by more than kPagedMargin.  fp32: with a bias of 20 sums
+// of up to 2^16 probabilities stay below 1, and weighted values below the
+// largest value.  8 bits: probabilities are at most 1, and the weighted values
+// are in units of a power of two of their size, O's unit, which moves up with
+// them and down where the reference leaves them behind (without one, values
+// below 1e-21 lost bits: 0.1% at 1e-25).  It costs 0.1 to 0.2 us of small steps
+// and nothing of large ones.
+constexpr float kPagedMargin = 4.0f;
+template <bool Q8>
+constexpr float kPagedBias = Q8 ? kPagedMargin : 20.0f;
 
 // One launch over one layer.
 struct PagedArgs {
@@ -144,7 +152,10 @@ struct PagedShared {
             float4 part[W * kWave];                  // and partial sums of them
         } merge;
     };
-    float m[W][kPagedHeads], l[W][kPagedHeads];
+    struct alignas(16) {
+        float m, l;
+        int unit;  // 8 bits: the exponent of O's unit
+    } sums[W][kPagedHeads];  // the waves' references and sums
     int last;
 };
 
@@ -233,14 +244,17 @@ __device__ __forceinline__ void digits4(unsigned w0, unsigned w1, unsigned w2, u
     d[2] = __builtin_amdgcn_perm(e, c, 0x05040100u);
     d[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
 }
-// The exponent of a largest magnitude `bits`, at least -90: what is scaled by
-// 2^(29 - e) is below 2^30.
-__device__ __forceinline__ int fixed_exp(unsigned bits) { return max((int)(bits >> 23), 37) - 127; }
+// The exponent of a largest magnitude `bits`, at least `least`: what is scaled
+// by 2^(29 - e) is below 2^30.
+constexpr int kLeastQ = -90, kLeastWeight = -97;  // (2^(29 - e) is a float)
+__device__ __forceinline__ int fixed_exp(unsigned bits, int least) { return max((int)(bits >> 23) - 127, least); }
 // The four digits' sums together.
 __device__ __forceinline__ float digits_sum(int d0, int d1, int d2, int d3)
 {
     return __builtin_fmaf((float)((int)((unsigned)d3 << 8) + d2), 65536.0f, (float)((int)((unsigned)d1 << 8) + d0));
 }
+// The integer at or below a difference of references.
+__device__ __forceinline__ int whole_part(float x) { return (int)floorf(fmaxf(x, -1000.0f)); }
 __device__ __forceinline__ i32x4 mfma8(u32x4 a, u32x4 b, i32x4 c)
 {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
@@ -456,7 +470,7 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
             unsigned top = dpp_max16(max4_bits(0u, x));
             if constexpr (HD == 128) top = max(top, (unsigned)__shfl_xor((int)top, 16));
             const bool good = finite_bits(top);
-            const int e = fixed_exp(good ? top : 0u);
+            const int e = fixed_exp(good ? top : 0u, kLeastQ);
             const float up = good ? exp2_int(29 - e) : 0.0f;
             unsigned d[4];
             digits4(digits_of(x.x * up), digits_of(x.y * up), digits_of(x.z * up), digits_of(x.w * up), d);
@@ -540,6 +554,7 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
 #pragma unroll
     for (int v = 0; v < kAcc; v++) o[v] = f32x4{0, 0, 0, 0};
     float mrun[kSums], lrun[kSums];
+    int unit = kLeastWeight;
 #pragma unroll
     for (int k = 0; k < kSums; k++) {
         mrun[k] = kNothing;
@@ -609,7 +624,7 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
             for (int k = 0; k < NQ; k++)
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    x[k][b] = fast_exp2(x[k][b] - (mrun[k] + kPagedBias));
+                    x[k][b] = fast_exp2(x[k][b] - (mrun[k] + kPagedBias<Q8>));
                     lrun[k] += x[k][b];
                     sh.p[wave][k][16 * b + m][g] = x[k][b];
                 }
@@ -641,6 +656,7 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
                     }
         } else {
             const u32x4 *qs = &sh.q[lane + zero];
+            const bool first = t == t0 + wave;  // (o is zero)
             float x[NB][4], mt = -__builtin_inff();
             if (last) {
 #pragma unroll
@@ -696,13 +712,17 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
             for (int b = 0; b < NB; b++) mt = fmaxf(mt, fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])));
             if (__builtin_amdgcn_ballot_w64(mt > mrun[0] + kPagedMargin) != 0) {
                 mt = rows4<true>(mt);
-                const float now = mt > mrun[0] + kPagedMargin ? mt : mrun[0], f = fast_exp2(mrun[0] - now);
+                const float now = mt > mrun[0] + kPagedMargin ? mt : mrun[0], d = mrun[0] - now;
+                const int down = max(unit + whole_part(d), kLeastWeight);  // (O's unit goes with its weights)
+                const float f = fast_exp2(d - (float)(down - unit));
                 mrun[0] = now;
-                lrun[0] *= f;
+                lrun[0] *= fast_exp2(d);
+                unit = down;
+                if (!first)
 #pragma unroll
-                for (int v = 0; v < VB; v++) o[v] *= f;
+                    for (int v = 0; v < VB; v++) o[v] *= f;
             }
-            const float off = mrun[0] + kPagedBias, vs = fmaxf(vsc, 0.0f);
+            const float off = mrun[0] + kPagedBias<Q8>, vs = fmaxf(vsc, 0.0f);
             float wt = 0.0f;
             unroll<0, 16>([&](auto j) {
                 const float y = fast_exp2(x[j / 4][j % 4] - off);
@@ -711,8 +731,16 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
                 wt = fmaxf(wt, x[j / 4][j % 4]);
             });
             // ---- weighted values ----
-            const int e = fixed_exp(__float_as_uint(rows4<true>(wt)));
-            const float up = exp2_int(29 - e), down = exp2_int(e - 29);
+            const int e = fixed_exp(__float_as_uint(rows4<true>(wt)), kLeastWeight);
+            if (__builtin_amdgcn_ballot_w64(e > unit) != 0) {
+                const int now = max(unit, min(e + 2, 127));
+                const float f = exp2_int(max(unit - now, -126));
+                unit = now;
+                if (!first)
+#pragma unroll
+                    for (int v = 0; v < VB; v++) o[v] *= f;
+            }
+            const float up = exp2_int(29 - e), down = exp2_int(max(e - unit - 29, -126));
             u32x4 pd[4];
 #pragma unroll
             for (int b = 0; b < NB; b++) {
@@ -743,8 +771,9 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
     if constexpr (Q8) {
         const float l = rows4<false>(lrun[0]);
         if (g == 0) {
-            sh.m[wave][m] = mrun[0];
-            sh.l[wave][m] = shared ? __uint_as_float(0x7fc00000u) : l;
+            sh.sums[wave][m].m = mrun[0];
+            sh.sums[wave][m].unit = unit;
+            sh.sums[wave][m].l = shared ? __uint_as_float(0x7fc00000u) : l;
         }
         if (m < a.group)
 #pragma unroll
@@ -755,8 +784,8 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
         for (int k = 0; k < NQ; k++) {
             const float l = row_sum(lrun[k]);
             if (m == 0) {
-                sh.m[wave][4 * k + g] = mrun[k];
-                sh.l[wave][4 * k + g] = shared ? __uint_as_float(0x7fc00000u) : l;
+                sh.sums[wave][4 * k + g].m = mrun[k];
+                sh.sums[wave][4 * k + g].l = shared ? __uint_as_float(0x7fc00000u) : l;
             }
         }
         f32x4 acc[NQ][4];
@@ -772,14 +801,27 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
     const size_t rec = (r.rec0 + r.run) * a.group;
     for (int i = tid; i < a.group * LR; i += kThreads) {
         const int head = i / LR, d = (i - head * LR) * 4;
-        float top = sh.m[0][head];
+        std::remove_reference_t<decltype(sh.sums[0][0])> part[W];
 #pragma unroll
-        for (int w = 1; w < W; w++) top = fmaxf(top, sh.m[w][head]);
+        for (int w = 0; w < W; w++) part[w] = sh.sums[w][head];
+        float top = part[0].m;
+#pragma unroll
+        for (int w = 1; w < W; w++) top = fmaxf(top, part[w].m);
         float f[W], total = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            f[w] = fast_exp2(sh.m[w][head] - top);
-            total += f[w] * sh.l[w][head];
+            f[w] = fast_exp2(part[w].m - top);
+            total += f[w] * part[w].l;
+        }
+        float o_unit = 1.0f;
+        if constexpr (Q8) {
+            // in the largest of the waves' units, as they count
+            int unit = kLeastWeight;
+#pragma unroll
+            for (int w = 0; w < W; w++) unit = max(unit, part[w].unit + whole_part(part[w].m - top));
+#pragma unroll
+            for (int w = 0; w < W; w++) f[w] = fast_exp2(part[w].m - top + (float)(part[w].unit - unit));
+            o_unit = exp2_int(unit);
         }
         float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
@@ -787,9 +829,11 @@ __device__ __forceinline__ void paged_run(const PagedArgs &a, PagedShared<HD, NQ
         // (no weight at all, every score -inf: as a record nothing, as a result NaN)
         if (n_runs == 1) {
             scale4(acc, 1.0f / total);
+            if constexpr (Q8) scale4(acc, o_unit);
             *reinterpret_cast<float4 *>(a.out + ((size_t)p.seq * a.n_heads + p.kvh * a.group + head) * HD + d) = acc;
         } else {
             scale4(acc, total == 0.0f ? 0.0f : 1.0f / total);
+            if constexpr (Q8) scale4(acc, o_unit);
             *reinterpret_cast<float4 *>(a.ws_o + (rec + head) * HD + d) = acc;
             if (d == 0) a.ws_lse[rec + head] = total == 0.0f ? -__builtin_inff() : top + log2f(total);
         }
