@@ -313,7 +313,9 @@ typedef struct leap_hip_attention_pages_config {
 /* The pool is zeroed and every table empty.  -EINVAL for a model that
  * leap_hip_attention_create refuses but for the size of a sequence's rows
  * (here seq_len <= 2^24), a page size or a flag other than the above, n_pages
- * outside [1, 2^26] and, with bounds, more than 16384 pages a sequence. */
+ * outside [1, 2^26], a table of 2^31 entries or more (max_batch * width), a
+ * page of 2^26 elements or more (page_rows * n_kv_heads * head_dim, of a
+ * layer's keys) and, with bounds, more than 16384 pages a sequence. */
 int leap_hip_attention_pages_create(const leap_hip_attention_pages_config *cfg, leap_hip_attention_pages **out);
 int leap_hip_attention_pages_destroy(leap_hip_attention_pages *p);
 /* As leap_hip_attention_last_error; NULL: of the last pages_create here. */
@@ -366,7 +368,11 @@ int leap_hip_attention_pages_compact_async(leap_hip_attention_pages *p, int *use
  * are exact and sums of 64 positions fp32's.  Host pointers. */
 int leap_hip_attention_pages_step(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, const float *q,
                                   const float *k_new, const float *v_new, float *out);
-/* As leap_hip_attention_step_batched_async, over pages. */
+/* As leap_hip_attention_step_batched_async, over pages.  total_rows also picks
+ * the launch: without it the lengths are taken as spread up to max_pos, and
+ * sequences that are all as long as that can take longer (32/8 heads of 128, 32
+ * sequences of 1000 rows 49 us for 45, 8 bits 26 for 21; 16 of 8192 164 for
+ * 165, 58 for 55).  Results do not depend on it beyond the order of sums. */
 int leap_hip_attention_pages_step_async(leap_hip_attention_pages *p, int layer, int n_seq, const int *pos, int max_pos,
                                         long long total_rows, const float *q, const float *k_new, const float *v_new,
                                         float *out, void *stream);
@@ -413,11 +419,11 @@ int leap_hip_attention_pages_clear(leap_hip_attention_pages *p);
 int leap_hip_attention_pages_state(leap_hip_attention_pages *p, int *table, int *refs);
 
 /* Device addresses, valid until destroy; to be read only, but for the pool's
- * contents (who writes keys there writes their bounds too).  k, v, ks, vs and bounds are of the layer, and layers follow one
- * another: with G KV heads of HD elements, pages of R rows, fp32 k and v
- * [page][G][R][HD]; 8 bits k [page][G][R][HD], v [page][G][R / 16][HD][16] (16
- * rows, element by element), scales ks and vs [page][G][R]; bounds
- * [page][G][2][HD], least and largest. */
+ * contents (who writes keys there writes their bounds too).  k, v, ks, vs and
+ * bounds are of the layer, and layers follow one another: with G KV heads of
+ * HD elements, pages of R rows, fp32 k and v [page][G][R][HD]; 8 bits k
+ * [page][G][R][HD], v [page][G][R / 16][HD][16] (16 rows, element by element),
+ * scales ks and vs [page][G][R]; bounds [page][G][2][HD], least and largest. */
 typedef struct leap_hip_attention_pages_arrays {
     const int *table, *refs;
     int width;
@@ -436,10 +442,13 @@ int leap_hip_attention_pages_view(leap_hip_attention_pages *p, int layer, leap_h
  * not allowed).  Every continuation counts -inf of a row with a NaN or +inf
  * among its logits or none above -inf, and of one whose score is not finite
  * (a search starts with scores 0, -inf, -inf, ...); these have the lowest
- * tokens.  Rows lie `stride` floats apart.  1 <= beams <= 16, beams <= vocab
- * <= 262144.  Device pointers, 4-byte aligned, enqueued on `stream`; parent,
- * token, best [n_groups * beams], best may be score.  A handle's first call
- * allocates its workspace; -EINVAL if that one is under stream capture. */
+ * tokens.  log sum exp is an fp32 sum of each 4096 logits, joined in 64 bits: up
+ * to 6e-6 off, so that beams whose totals are closer than twice that may come
+ * in either order (equal rows of equal scores are equal).  Rows lie `stride`
+ * floats apart.  1 <= beams <= 16, beams <= vocab <= 262144.  Device pointers,
+ * 4-byte aligned, enqueued on `stream`; parent, token, best [n_groups * beams],
+ * best may be score.  A handle's first call allocates its workspace; -EINVAL if
+ * that one is under stream capture. */
 int leap_hip_attention_pages_beam_select_async(leap_hip_attention_pages *p, int n_groups, int beams, int vocab,
                                                const float *logits, long long stride, const float *score, int *parent,
                                                int *token, float *best, void *stream);

@@ -631,7 +631,7 @@ class PagedAttention:
         return out
 
     def step_async(self, layer, n_seq, pos_ptr, max_pos, q_ptr, k_ptr, v_ptr, out_ptr, stream=0, total_rows=0):
-        """total_rows: sum of pos[i] + 1 if known on the host (sizes the split), else 0."""
+        """total_rows: sum of pos[i] + 1 if known on the host (sizes and picks the launch), else 0."""
         self._call("step_async", layer, n_seq, pos_ptr, max_pos, total_rows, q_ptr, k_ptr, v_ptr, out_ptr, stream)
 
     def step_sparse(self, layer, pos, keep, q, k_new, v_new):

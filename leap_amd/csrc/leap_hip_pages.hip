@@ -147,12 +147,20 @@ struct StepPlan {
 // and 0.03 for each.  (us, 32/8/128, runs of 4, 8, 16, 32 tiles: fp32, one
 // sequence of 4096 11.2, 11.2, 13.6, 19.9, of 8192 -, 17.8, 16.7, 22.6; 12 of
 // 4096 -, 73, 72, 64.6; 8 bits, one of 4096 10.4, 13.2, of 16384 16.5, 15.3.)
+// What it leaves out: a workgroup's start, and that rounds of workgroups
+// overlap.  So equal lengths whose groups do not divide by the CUs get the
+// shortest runs, which stream less: sequences of 4096, 32/8/128, fp32 32 166,
+// 33 210, 40 211, 45 281, 48 251; 8 bits 57, 70, 76, 91, 78.
+//
 // Batches of unequal lengths with a group for every XCD run flat once they have
 // 16 tiles a CU (uniform : flat; 32/8/128 fp32, 8 sequences of up to 500 9.8 :
 // 11.3, 16 of up to 1000 22.5 : 21.0, 32 of up to 7300 180 : 163, 64/8/128 16
 // of up to 7300 124 : 108; 8 bits, 32 of up to 8192 73 : 68; equal lengths, 16
-// of 8192 160 : 162, 8 bits 32 of 8192 100 : 110).  Two workgroups a CU: 8 bits need both (one: 84), fp32 takes
-// as long with one.
+// of 8192 160 : 162, 8 bits 32 of 8192 100 : 110).  Two workgroups a CU: 8 bits
+// need both (one: 84), fp32 takes as long with one.  A lane holds one group of
+// its XCD, so that more than 512 groups stay uniform: of up to 4096, 32/32/128,
+// 16 sequences (flat) 162, 17 213, 20 298; 8 bits 62, 86, 104.  Without a count
+// of rows the lengths are taken as unequal.
 StepPlan step_plan(const leap_hip_attention_pages *p, int n_seq, int longest, long long total)
 {
     const int n_kv = p->cfg.model.n_kv_heads, hd = p->cfg.model.head_dim, tk = leap::paged_tile(hd, p->q8);
@@ -182,8 +190,9 @@ StepPlan step_plan(const leap_hip_attention_pages *p, int n_seq, int longest, lo
     }
     const long long flat_wgs = 2ll * p->n_cu;
     const bool equal = total == (long long)n_seq * longest;
-    if (n_seq > 1 && groups >= leap::kXcds && !equal && groups * tiles_mean >= 16ll * p->n_cu && items <= leap::kWave && (size_t)(leap::kXcds * items + flat_wgs) * p->group <= kRecords &&
-        (size_t)groups <= kCounters && flat_wgs <= (long long)leap::kXcds * leap::kPagedSplits)
+    const bool fits = items <= leap::kWave && (size_t)(leap::kXcds * items + flat_wgs) * p->group <= kRecords &&
+                      (size_t)groups <= kCounters && flat_wgs <= (long long)leap::kXcds * leap::kPagedSplits;
+    if (n_seq > 1 && groups >= leap::kXcds && !equal && groups * tiles_mean >= 16ll * p->n_cu && fits)
         return StepPlan{1, (int)items, false, true, flat_wgs};
     s.spread = s.splits > 1 && groups < leap::kXcds && !few;
     s.wgs = s.spread ? groups * s.splits : items * leap::kXcds * s.splits;

@@ -10,7 +10,7 @@
 // timing: the lowest free page first, to the first sequence's first page first.
 //
 // All are bound by latency (a few dependent passes over a few KB: fork's two
-// launches 2.4 us each for 4 sequences and 4.6 for 64, compact's plan 7.0 for a
+// launches 2.3 and 2.6 us for 4 sequences and 4.6 for 64, compact's plan 7.0 for a
 // pool of 489 pages); what copies pages is bound by memory (507 MB moved in 104 us, 4.9
 // TB/s, where a large copy reaches 5.2).
 #pragma once
@@ -213,8 +213,10 @@ __device__ __forceinline__ void reserve_few(const PagesArgs &a, ReserveFew &l, i
 // out, -EINVAL.  Items: the (sequence, page) pairs asked for, in order.
 //
 // Bound by its chain of trips to memory: ranges, tables, counts, results.  With
-// up to 1024 items 7.4 us for 64 sequences that share pages and 4.1 for 4,
-// where the passes over memory below take 11.6 and 6.5.
+// up to 1024 items 7.8 us for 64 sequences that share pages and 4.4 for 4,
+// where the passes over memory below take 11.6 and 6.5.  Beyond that each item
+// looks for its sequence three times: 4 sequences of 512 pages 47 us, 32 254, 64
+// 500.
 __global__ __launch_bounds__(kPlanThreads) void reserve_kernel(PagesArgs a, int e_inval, int e_nomem)
 {
     __shared__ int sh[kPlanWaves];

@@ -22,7 +22,7 @@
 // Bound by memory in batches: 16 sequences of 411 to 7300 rows, 64/8 heads of
 // 128, 675 MB in 108 us (6.2 TB/s), 16 of 8192, 32/8 heads, in 160 us (6.7);
 // 8 bits, 32 of 8192, 555 MB in 100 us (5.5).  Small steps are bound by
-// latency: one sequence of 4096 11.2 us, of 256 rows with 4 KV heads of 64 5.6
+// latency: one sequence of 4096 11.6 us, of 256 rows with 4 KV heads of 64 6.9
 // (page numbers, rows, a tile, records).  Four waves a workgroup and one or two
 // workgroups a CU: more, shorter runs stream less (8 tiles each 200 us for 160).
 //
